@@ -10,6 +10,7 @@ and workspaces, ``torch.cuda.current_stream()`` for the stream handle).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from pathlib import Path
@@ -90,6 +91,11 @@ SIGNATURES = {
     "mtx_quant_fp8_weights_both": (_I, [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
     "mtx_fp8_chunks": (_I, [_P, _I64, _I64, _P, _I64, _P]),
     "mtx_quant_fp8_operands": (_I, [_I, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "mtx_linear_workspace_size": (_I64, [_I64, _I64, _I64]),
+    "mtx_linear": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
+    "mtx_linear_dx": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "mtx_linear_dw": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "mtx_linear_act_bwd": (_I, [_P, _P, _I, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
     "mtx_transpose_batched": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P]),
     "mtx_stream_copy": (_I, [_P, _P, _I64, _I, _I64, _P]),
 }
@@ -183,6 +189,13 @@ def stream(device: torch.device) -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _raw_stream(device.index)
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one, which is where a kernel is launched."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def plain_forward(*tensors) -> bool:

@@ -2,11 +2,12 @@
 
 The reference exports route, unroute, grouped_matmul, grouped_matmul_vjp and tgmm; this
 package adds route_topk (router top-k), grouped_matmul_swiglu (fused gate_up + SwiGLU),
-swiglu and the blockwise-fp8 entry points in ``fp8``.
+swiglu, the blockwise-fp8 entry points in ``fp8`` and linear (the dense product with its epilogue).
 """
 from .grouped_matmul import grouped_matmul, grouped_matmul_swiglu, grouped_matmul_vjp, swiglu, tgmm
+from .linear import linear
 from .moe_dispatch import _sort_with_vjp, route, unroute
 from .router import route_topk, update_expert_bias
 
 __all__ = ["route", "unroute", "grouped_matmul", "grouped_matmul_vjp", "tgmm", "route_topk",
-           "grouped_matmul_swiglu", "swiglu", "_sort_with_vjp", "update_expert_bias"]
+           "grouped_matmul_swiglu", "swiglu", "linear", "_sort_with_vjp", "update_expert_bias"]

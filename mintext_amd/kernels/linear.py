@@ -1,0 +1,119 @@
+"""Dense product with its epilogue: ``act(x @ weight + bias) + residual``, differentiable.
+
+The dense counterpart of ``grouped_matmul``, for the projections and MLPs around the experts (the reference's
+``Linear`` and ``MLP``, mintext/modules/linear.py:123-147, 164-228): one HIP kernel applies bias, activation and
+residual to the float32 sums, rounded once.  Training also writes ``z = x @ weight + bias``, in the operands' dtype,
+when there is an activation; its backward is one pass over the gradient and ``z`` (``dz = dy * act'(z)`` and the
+bias gradient) and the two products ``dz @ weight^T`` and ``x^T @ dz``.  The gradients are deterministic.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib as L
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # MTX_ACT_*
+
+
+def _check(x, weight, bias, activation, residual):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(k for k in ACTIVATIONS if k)} or None, got {activation!r}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"linear takes x [..., K] and weight [K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N = weight.shape[1]
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
+        raise ValueError(f"residual must have the output's shape {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
+    for t in (x, weight, bias, residual):
+        if t is None:
+            continue
+        if t.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"linear takes float32 or bfloat16 operands, got {t.dtype}")
+        if t.dtype != x.dtype:
+            raise TypeError(f"linear operands must share one dtype, got {x.dtype} and {t.dtype}")
+
+
+def _sizes(x, weight):
+    K, N = weight.shape
+    M = 1
+    for d in x.shape[:-1]:
+        M *= d
+    return M, K, N
+
+
+def _workspace(M, K, N, dev):
+    return L.workspace(L.query("mtx_linear_workspace_size", M, K, N), dev)
+
+
+def _forward(x, weight, bias, act, residual, keep):
+    dev = L.require_device(x, weight, bias, residual)
+    x, weight = x.contiguous(), weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    M, K, N = _sizes(x, weight)
+    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+    pre = torch.empty((M, N), dtype=x.dtype, device=dev) if keep and act else None
+    ws = _workspace(M, K, N, dev)
+    with L.on_device(dev):
+        L.call("mtx_linear", L.ptr(x), L.ptr(weight), L.ptr(bias), L.ptr(residual), L.dtype_code(x.dtype), M, K, N, act,
+               L.ptr(out), L.ptr(pre), L.ptr(ws), ws.numel(), L.stream(dev))
+    return out, pre
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        out, pre = _forward(x, weight, bias, act, residual, True)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act = act
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, pre = ctx.saved_tensors
+        need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
+        dev = L.require_device(x, weight, dy)
+        x, weight, dy = x.contiguous(), weight.contiguous(), dy.contiguous()
+        M, K, N = _sizes(x, weight)
+        code, act = L.dtype_code(x.dtype), ctx.act
+        ws = _workspace(M, K, N, dev)
+        dx = dw = db = None
+        dz = dy
+        with L.on_device(dev):
+            st = L.stream(dev)
+            if need_b or (act and (need_x or need_w)):
+                dz = torch.empty((M, N), dtype=x.dtype, device=dev) if act else dy
+                db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
+                L.call("mtx_linear_act_bwd", L.ptr(dy), L.ptr(pre), code, M, N, act, L.ptr(dz if act else None), L.ptr(db),
+                       L.ptr(ws), ws.numel(), st)
+            if need_x:
+                dx = torch.empty_like(x)
+                L.call("mtx_linear_dx", L.ptr(dz), L.ptr(weight), code, M, K, N, L.ptr(dx), L.ptr(ws), ws.numel(), st)
+            if need_w:
+                dw = torch.empty_like(weight)
+                L.call("mtx_linear_dw", L.ptr(x), L.ptr(dz), code, M, K, N, L.ptr(dw), L.ptr(ws), ws.numel(), st)
+        return dx, dw, db, None, dy if need_r else None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ weight + bias) + residual`` as one kernel (the products of mintext/modules/linear.py:123-147, 164-228).
+
+    Args:
+        x: [..., K], float32 or bfloat16.
+        weight: [K, N] in x's dtype (the layout of ``grouped_matmul``'s weights, one group).
+        bias: [N] or None.
+        activation: None, "relu", "silu", "gelu" (erf) or "gelu_tanh".
+        residual: [..., N] or None, added after the activation.
+
+    Returns:
+        [..., N] in x's dtype.  Differentiable (once) in all four tensors.
+    """
+    _check(x, weight, bias, activation, residual)
+    act = ACTIVATIONS[activation]
+    if L.plain_forward(x, weight, bias, residual):
+        return _forward(x, weight, bias, act, residual, False)[0]
+    return _Linear.apply(x, weight, bias, act, residual)

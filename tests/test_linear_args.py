@@ -1,0 +1,51 @@
+"""Calls of the dense product that are refused, before anything is launched (host only)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from mintext_amd import _lib as L
+from mintext_amd.kernels import linear
+
+
+def z(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("args, kwargs, error", [
+    ((z(4, 8), z(9, 8)), {}, ValueError),                                    # K differs
+    ((z(4, 8), z(2, 8, 8)), {}, ValueError),                                 # a stack of weights
+    ((z(4, 8), z(8, 16), z(8)), {}, ValueError),                             # bias of another length
+    ((z(4, 8), z(8, 16), z(1, 16)), {}, ValueError),
+    ((z(4, 8), z(8, 16)), dict(residual=z(16)), ValueError),                 # broadcast by the caller, not here
+    ((z(4, 8), z(8, 16)), dict(activation="tanh"), ValueError),
+    ((z(4, 8), z(8, 16, dtype=torch.float32)), {}, TypeError),               # mixed types
+    ((z(4, 8), z(8, 16), z(16, dtype=torch.float32)), {}, TypeError),
+    ((z(4, 8, dtype=torch.float16), z(8, 16, dtype=torch.float16)), {}, TypeError),
+    ((z(4, 8), z(8, 16)), {}, RuntimeError),                                 # no device
+])
+def test_refusals(args, kwargs, error):
+    with pytest.raises(error):
+        linear(*args, **kwargs)
+
+
+def test_entry_points_refuse():
+    lib = L.lib()
+    buf = ctypes.create_string_buffer(1 << 20)
+    d, P, n = ctypes.addressof(buf), None, 1 << 20
+    ok = lambda M, K, N: lib.mtx_linear_workspace_size(M, K, N)
+    assert ok(16, 8, 8) >= 0 and ok(-1, 8, 8) < 0
+    call = lambda *a: lib.mtx_linear(*a)
+    assert call(d, d, P, P, 2, 4, 8, 8, 0, d, P, d, n, P) == L.MTX_ERR_ARG       # dtype
+    assert call(d, d, P, P, 1, 4, 8, 8, 5, d, P, d, n, P) == L.MTX_ERR_ARG       # activation
+    assert call(d, d, P, P, 1, -4, 8, 8, 0, d, P, d, n, P) == L.MTX_ERR_ARG
+    assert call(P, d, P, P, 1, 4, 8, 8, 0, d, P, d, n, P) == L.MTX_ERR_ARG       # no x
+    assert call(d, d, P, P, 1, 4, 8, 8, 0, P, P, d, n, P) == L.MTX_ERR_ARG       # no out
+    assert call(d, d, P, P, 1, 1 << 23, 8, 8, 0, d, P, d, 1 << 40, P) == L.MTX_ERR_UNSUPPORTED
+    assert call(d, d, P, P, 1, 4096, 8, 8, 0, d, P, P, 0, P) == L.MTX_ERR_WORKSPACE
+    assert lib.mtx_linear_dx(d, d, 1, 4096, 8, 8, d, P, 0, P) == L.MTX_ERR_WORKSPACE
+    assert lib.mtx_linear_dw(d, P, 1, 4, 8, 8, d, d, n, P) == L.MTX_ERR_ARG
+    assert lib.mtx_linear_act_bwd(d, P, 1, 4, 8, 2, d, d, d, n, P) == L.MTX_ERR_ARG  # an activation without z
+    assert lib.mtx_linear_act_bwd(d, P, 1, 4, 8, 9, d, d, d, n, P) == L.MTX_ERR_ARG
