@@ -50,6 +50,9 @@
  *   mtx_linear, mtx_linear_dx, mtx_linear_dw, mtx_linear_act_bwd
  *                          <- Linear.__call__ and the products of MLP (mintext/modules/linear.py:
  *                             123-147, 164-228) with bias, activation and residual, and their VJP
+ *   mtx_newton_schulz, mtx_muon_update
+ *                          <- the Muon optimiser over expert stacks (mintext/optim/optimizer.py:
+ *                             92-168)
  *   mtx_transpose_batched  <- _import_expert_weights / _export_expert_weights
  *                             (mintext/checkpoint/conversion.py:80-166), on the device
  */
@@ -434,6 +437,31 @@ int mtx_linear_dw(const void* x, const void* dz, int dtype, int64_t M, int64_t K
                   void* workspace, int64_t workspace_bytes, void* stream);
 int mtx_linear_act_bwd(const void* dy, const void* pre, int dtype, int64_t M, int64_t N, int act, void* dz,
                        void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- orthogonalised updates ---------------------------------------------------------------
+ * Muon over stacked expert weights (mintext/optim/optimizer.py:92-168), each of the E matrices by
+ * itself.  Strides in elements: matrix to matrix (batch) and row to row; columns are consecutive.
+ * mtx_newton_schulz: X = x[e] / (|x[e]|_F + eps) (eps > 0), then `steps` times
+ *   X <- a X + (b A + c A^2) X, A = X X^T on the smaller side; out[e] = X in x's dtype.
+ * mtx_muon_update: m <- beta m + (1 - beta) g; u = nesterov ? (1 - beta) g + beta m : m;
+ *   w <- (1 - lr weight_decay) w - lr factor O(u), O as above; lr from *lr_dev unless that is NULL.
+ *   w (param) and m (float32) are updated in place and must not overlap each other or g.
+ * schedule (host memory): 9 floats a step: a, b, c, the scales (powers of two) under which f16
+ *   holds A, Q = a I + b A + c A^2, Q A, the group's product P of Qs and X after it, and whether
+ *   the step ends a group (1) or the next one goes on from Q A Q (0).  P's scale is Q's at the
+ *   first step of a group.  The scales have to keep each matrix's singular values below 65504.
+ * planes: 1 = matrices in one f16 plane between products, 2 = in two (float32 results).
+ * E <= 65535, M and N <= 2^20, min(M, N) <= 2^15.  Large stacks go through in parts, so that the
+ * workspace stays below 4 GiB or one matrix's need.                                          */
+int64_t mtx_newton_schulz_workspace_size(int64_t E, int64_t M, int64_t N, int planes);
+int mtx_newton_schulz(const void* x, int dtype, int64_t E, int64_t M, int64_t N, int64_t x_batch, int64_t x_row,
+                      const float* schedule, int steps, float eps, int planes, void* out, int64_t out_batch,
+                      int64_t out_row, void* workspace, int64_t workspace_bytes, void* stream);
+int mtx_muon_update(void* param, int param_dtype, int64_t p_batch, int64_t p_row, const void* grad,
+                    int grad_dtype, int64_t g_batch, int64_t g_row, float* momentum, int64_t m_batch,
+                    int64_t m_row, int64_t E, int64_t M, int64_t N, double beta, int nesterov, float lr,
+                    const float* lr_dev, float weight_decay, float factor, const float* schedule, int steps,
+                    float eps, int planes, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- expert weight layouts -------------------------------------------------------------
  * Batched transpose-copy (the per-expert HF <-> fused conversions of

@@ -6,8 +6,8 @@ behind the C-ABI of include/mintext_moe.h.  ``mintext_amd.kernels`` mirrors the 
 ``mintext.kernels`` package; ``mintext_amd.moe`` composes the expert layer.
 """
 from . import _lib
-from .kernels import (grouped_matmul, grouped_matmul_swiglu, grouped_matmul_vjp, linear, route, route_topk,
-                      tgmm, unroute)
+from .kernels import (grouped_matmul, grouped_matmul_swiglu, grouped_matmul_vjp, linear, muon_update,
+                      newton_schulz, route, route_topk, tgmm, unroute)
 
 __all__ = ["route", "unroute", "grouped_matmul", "grouped_matmul_vjp", "tgmm", "route_topk",
-           "grouped_matmul_swiglu", "linear", "_lib"]
+           "grouped_matmul_swiglu", "linear", "newton_schulz", "muon_update", "_lib"]

@@ -33,6 +33,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 # name -> (restype, argtypes); kept in the order of the header
 SIGNATURES = {
@@ -96,6 +97,10 @@ SIGNATURES = {
     "mtx_linear_dx": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "mtx_linear_dw": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "mtx_linear_act_bwd": (_I, [_P, _P, _I, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
+    "mtx_newton_schulz_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
+    "mtx_newton_schulz": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _F, _I, _P, _I64, _I64, _P, _I64, _P]),
+    "mtx_muon_update": (_I, [_P, _I, _I64, _I64, _P, _I, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _F, _P,
+                             _F, _F, _P, _I, _F, _I, _P, _I64, _P]),
     "mtx_transpose_batched": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P]),
     "mtx_stream_copy": (_I, [_P, _P, _I64, _I, _I64, _P]),
 }

@@ -1,0 +1,212 @@
+"""Orthogonalised updates of (stacked) weight matrices: Newton-Schulz products and the Muon step.
+
+The optimiser side of ``tgmm``'s weight gradients (the reference's optimiser runs Muon with dimension numbers for the
+experts' stacks, mintext/optim/optimizer.py:92-168): every matrix of a stack [..., M, N] is orthogonalised by itself,
+all of them in the same launches.
+
+``newton_schulz`` maps the singular values of ``x / (|x|_F + eps)`` by ``steps`` odd quintics a s + b s^3 + c s^5, which
+brings them near 1 and keeps the singular vectors.  ``muon_update`` does an optimiser step in place:
+
+    m <- beta m + (1 - beta) g;   u = (1 - beta) g + beta m (Nesterov) or m
+    w <- (1 - lr weight_decay) w - lr factor newton_schulz(u)
+
+Precision.  Products run on the 16-bit matrix cores with float32 sums: "half" holds the matrices between products in f16
+(11 bits, under power-of-two scales that their bounded singular values allow), "full" in two f16 planes (22 bits, three
+times the products).  The default goes by the type of what is returned or updated: "full" for float32, "half" for
+bfloat16, whose rounding is coarser.  A result of "half" is some tenths of a per cent off for gradients of
+rank 8 and more, before it is rounded.  The Frobenius norm is summed in float64 and momentum is float32.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from .. import _lib as L
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_GROUP = 3  # steps between two Gram products, at most
+
+
+@functools.lru_cache(maxsize=64)
+def _schedule(steps: int, coefficients: tuple):
+    """The 9 floats a step of ``mtx_newton_schulz``: coefficients, scales, and where a group of steps ends.
+
+    The singular values start in [0, 1] (the Frobenius norm bounds them), so those of every matrix on the way have a
+    bound; an entry is at most its matrix's largest singular value.  Each scale is the largest power of two that
+    keeps 1.25 times the bound inside f16.
+    """
+    triples = [coefficients] * steps if not isinstance(coefficients[0], tuple) else list(coefficients)
+    groups = -(-steps // _GROUP)
+    sizes = [steps // groups + (g < steps % groups) for g in range(groups)]
+    last = [sum(sizes[:g + 1]) - 1 for g in range(groups)]
+
+    def scale(bound):
+        if not bound < 2.0 ** 12:
+            raise ValueError("these coefficients let singular values in [0, 1] grow out of range")
+        return 2.0 ** min(20, math.floor(math.log2(60000 / (1.25 * max(bound, 2.0 ** -8)))))
+
+    top, flat, first = 1.0, [], True
+    for i, (a, b, c) in enumerate(triples):
+        if first:
+            start = [top * k / 2048 for k in range(2049)]
+            s, p = start, [1.0] * len(start)
+        q = [a + b * t * t + c * t ** 4 for t in s]
+        p = [u * v for u, v in zip(p, q)]
+        bound_t = max(abs(v) * t * t for v, t in zip(q, s))
+        sq = scale(max(abs(v) for v in q))
+        flat += [a, b, c, scale(max(t * t for t in s)), sq, scale(bound_t),
+                 sq if first else scale(max(abs(v) for v in p)), 0.0, float(i in last)]
+        s = [abs(v) * t for v, t in zip(q, s)]
+        top = max(s)
+        flat[-2] = scale(top)
+        first = i in last
+    return (ctypes.c_float * len(flat))(*flat)
+
+
+def _arguments(steps, coefficients, eps, precision, dtype):
+    if not isinstance(steps, int) or not 1 <= steps <= 64:
+        raise ValueError(f"steps must be an int from 1 to 64, got {steps!r}")
+    if not eps > 0:
+        raise ValueError(f"eps must be positive, got {eps!r}")
+    if precision not in (None, "half", "full"):
+        raise ValueError(f'precision must be "half", "full" or None, got {precision!r}')
+    try:
+        if isinstance(coefficients[0], (tuple, list)):
+            c = tuple(tuple(float(v) for v in t) for t in coefficients)
+            good = len(c) == steps and all(len(t) == 3 for t in c)
+        else:
+            c = tuple(float(v) for v in coefficients)
+            good = len(c) == 3
+    except (TypeError, IndexError):
+        good = False
+    if not good or not all(math.isfinite(v) for t in c for v in (t if isinstance(t, tuple) else (t,))):
+        raise ValueError("coefficients must be three finite numbers, or three for each step")
+    planes = 2 if precision == "full" or (precision is None and dtype == torch.float32) else 1
+    return _schedule(steps, c), planes
+
+
+def _check_stack(t: torch.Tensor, name: str):
+    if t.dim() < 2:
+        raise ValueError(f"{name} must be a matrix or a stack of them, got {tuple(t.shape)}")
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """As [E, M, N] with rows of consecutive elements, copied where it has to be."""
+    M, N = t.shape[-2:]
+    t = t.reshape(math.prod(t.shape[:-2]), M, N)
+    if t.numel() == 0 or (t.stride(2) == 1 or N == 1) and (t.stride(1) >= N or M == 1):
+        return t
+    return t.contiguous()
+
+
+def _strides(t: torch.Tensor) -> tuple[int, int]:
+    """(batch, row) of a [E, M, N] stack; what a size of 1 never uses is set to what dense storage has."""
+    E, M, N = t.shape
+    row = t.stride(1) if M > 1 else N
+    return (t.stride(0) if E > 1 else M * row), row
+
+
+def _writable(t: torch.Tensor, name: str) -> torch.Tensor:
+    """As [E, M, N] without a copy, its elements apart from each other."""
+    M, N = t.shape[-2:]
+    E = math.prod(t.shape[:-2])
+    if t.numel() == 0:
+        return t.reshape(E, M, N)
+    try:
+        v = t.detach().view(E, M, N)
+    except RuntimeError:
+        raise ValueError(f"{name} is updated in place: its leading dimensions must be mergeable into one") from None
+    batch, row = _strides(v)
+    apart = batch >= (M - 1) * row + N or row >= (E - 1) * batch + N and batch >= N
+    if (v.stride(2) != 1 and N > 1) or row < N or (E > 1 and not apart):
+        raise ValueError(f"{name} is updated in place: it needs rows of consecutive elements that do not overlap")
+    return v
+
+
+def newton_schulz(x: torch.Tensor, steps: int = 5, *, coefficients=COEFFICIENTS, eps: float = 1e-7,
+                  precision: str | None = None) -> torch.Tensor:
+    """Orthogonalise each matrix of ``x`` [..., M, N] by ``steps`` Newton-Schulz products.
+
+    X <- x / (|x|_F + eps), then ``steps`` times X <- a X + (b A + c A^2) X with A = X X^T.  A matrix of zeros stays
+    zeros; one that holds a NaN or an infinity becomes NaN, without touching the others.
+
+    Args:
+        x: float32 or bfloat16, any strides (rows that are not consecutive elements are copied first).
+        coefficients: (a, b, c), or such a triple for each step.
+        precision: "half", "full" or None, by x's dtype (see the module).
+
+    Returns:
+        a dense tensor of x's shape and dtype.  Not differentiable.
+    """
+    _check_stack(x, "x")
+    sched, planes = _arguments(steps, coefficients, eps, precision, x.dtype)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("newton_schulz is not differentiable: pass x.detach()")
+    dev = L.require_device(x)
+    v = _readable(x)
+    E, M, N = v.shape
+    out = torch.empty((E, M, N), dtype=x.dtype, device=dev)
+    ws = L.workspace(L.query("mtx_newton_schulz_workspace_size", E, M, N, planes), dev)
+    with L.on_device(dev):
+        L.call("mtx_newton_schulz", L.ptr(v), L.dtype_code(x.dtype), E, M, N, *_strides(v), sched, steps, eps, planes,
+               L.ptr(out), M * N, N, L.ptr(ws), ws.numel(), L.stream(dev))
+    return out.view(x.shape)
+
+
+def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, *, lr, beta: float = 0.95,
+                nesterov: bool = True, weight_decay: float = 0.0, scale: str | float = "spectral", steps: int = 5,
+                coefficients=COEFFICIENTS, eps: float = 1e-7, precision: str | None = None) -> torch.Tensor:
+    """One Muon step of a stack of weights, in place (formulas in the module's docstring).
+
+    Args:
+        param: [..., M, N] weights used as ``x @ param``, float32 or bfloat16; updated in place.  A view with rows of
+            consecutive elements will do, e.g. the gate half ``gate_up[..., :I]`` of a fused stack.
+        grad: its gradient, of the same shape, float32 or bfloat16.
+        momentum: float32 of the same shape, updated in place (zeros before the first step).
+        lr: learning rate, a number or a float32 device tensor of one element (read when the step runs, so that a
+            captured step follows it).
+        scale: factor of the update: "spectral" sqrt(max(1, N / M)), "rms" 0.2 sqrt(max(M, N)), or a number.
+        precision: as in ``newton_schulz``, by param's dtype.
+
+    Returns:
+        param.
+    """
+    for t, name in ((param, "param"), (grad, "grad"), (momentum, "momentum")):
+        _check_stack(t, name)
+        if t.shape != param.shape:
+            raise ValueError(f"{name} must have param's shape {tuple(param.shape)}, got {tuple(t.shape)}")
+    if momentum.dtype != torch.float32:
+        raise TypeError(f"momentum must be float32, got {momentum.dtype}")
+    sched, planes = _arguments(steps, coefficients, eps, precision, param.dtype)
+    M, N = param.shape[-2:]
+    if scale == "spectral":
+        factor = math.sqrt(max(1.0, N / max(M, 1)))
+    elif scale == "rms":
+        factor = 0.2 * math.sqrt(max(M, N))
+    elif isinstance(scale, (int, float)):
+        factor = float(scale)
+    else:
+        raise ValueError(f'scale must be "spectral", "rms" or a number, got {scale!r}')
+    lr_dev = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype != torch.float32 or lr.numel() != 1:
+            raise TypeError("lr must be a number or a float32 tensor of one element")
+        lr, lr_dev = 0.0, lr
+    p, m = _writable(param, "param"), _writable(momentum, "momentum")
+    if param.numel() and len({param.data_ptr(), grad.data_ptr(), momentum.data_ptr()}) < 3:
+        raise ValueError("param, grad and momentum must be three different tensors")
+    dev = L.require_device(param, grad, momentum, lr_dev)
+    g = _readable(grad.detach())
+    E = p.shape[0]
+    ws = L.workspace(L.query("mtx_newton_schulz_workspace_size", E, M, N, planes), dev)
+    with L.on_device(dev):
+        L.call("mtx_muon_update", L.ptr(p), L.dtype_code(p.dtype), *_strides(p), L.ptr(g), L.dtype_code(g.dtype),
+               *_strides(g), L.ptr(m), *_strides(m), E, M, N, beta, int(nesterov), lr, L.ptr(lr_dev), weight_decay, factor,
+               sched, steps, eps, planes, L.ptr(ws), ws.numel(), L.stream(dev))
+    torch.autograd.graph.increment_version([param, momentum])
+    return param
