@@ -4,20 +4,22 @@
 // S x L matrix.  With Q = a I + b A + c A^2 this is X <- Q X, and A itself becomes Q A Q, all of them polynomials of
 // the first A: symmetric, and they commute.  So g steps need one Gram product, S x S symmetric products and one
 // product X <- P X with P = Q_g ... Q_1, in all 3 S^2 L + (4 g - 3) S^3 operations (a symmetric product computes
-// half its tiles), where a step by itself needs 3 S^2 L + S^3: five steps as three and two need 0.48 of
-// the operations at L = 2.67 S (768 x 2048: 30 S^3 instead of 45, and 63 if all tiles were computed), the same
-// number at L = S.  A group holds at most three steps: A's small eigenvalues are squares of X's and grow by a^2 a
-// step, so what the rounding of A adds grows as well and is not taken back before the next Gram product.  In
-// simulation (512 x 1536 and the like, f16 operands) five steps as 3 + 2 end 0.1 to 0.3 % off for spectra from
-// normal entries to rank 8, as 5 single steps 0.1 to 2.7 %, as 2 + 3 up to 1.6 %, as one group of five up to 14 % or
-// beyond f16's range; with bf16 operands single steps end 1 to 80 % off.
+// half its tiles), where a step by itself needs 3 S^2 L + S^3.  At L = 2.67 S (768 x 2048) five steps need
+// 45 S^3 by themselves (63 if all tiles were computed), 35 as 2 + 2 + 1, 30 as 3 + 2; at L = S always 20.
+// A's small eigenvalues are squares of X's and grow by a^2 a step, so what the rounding of A adds grows as well and is
+// not taken back before the next Gram product: a group holds three steps at most.  In simulation with gradients of
+// rank 1 to full rank (f16 operands) five steps end 0.07 to 0.19 % off as 2 + 2 + 1, 0.1 to 0.5 % as 3 + 2, up to 14 %
+// or beyond f16's range as one group.  The caller chooses: 2 where the result itself is asked for, 3 where it is
+// a small change of weights.
 //
 // Numbers: |x|_F bounds every singular value by 1 and the polynomials bound them from there, so every matrix has a
 // power-of-two scale, chosen by the caller from those bounds, that puts it into f16's range: 11 bits where
 // bf16 has 8, at the same matrix-core rate ("half").  f32 results take two f16 planes, hi + lo, and three products for
-// one ("full": 22 bits).  Sums are f32, |x|_F is summed in f64.  The diagonals of Q and P, where their size is, are
-// f32 vectors beside the f16 matrices: rounding them to f16 would cost more than all else (rank 8: 0.85 % instead
-// of 0.28 %).  Momentum is f32.
+// one ("full": 22 bits).  Sums are f32, |x|_F is summed in f64.  Two things cost more than all other roundings and are
+// kept apart.  The diagonals of Q and P, where their size is, are f32 vectors beside the f16 matrices (rank 8: 0.28
+// instead of 0.85 % off).  And X has its lo plane in "half" too: in X <- P X the diagonal's share, in f32 on the way
+// out, takes hi + lo, as in the directions in which X is small P is a multiple of I (rank 32, 2 + 2 + 1: 0.17
+// instead of 0.63 %).  Momentum is f32.
 #include "common.h"
 #include "dense_tile.h"
 #include "f32_tile.h"
@@ -315,7 +317,8 @@ struct ApplyArgs {
   const f16* p;
   const float* pd;   // P's diagonal
   const f16* x;
-  f16* xo;           // OUT_X
+  const f16* xl;     // x's lo plane, or nullptr
+  f16 *xo, *xol;     // OUT_X: both planes
   void* out;         // OUT_STORE: the result; OUT_STEP: the weights
   int64_t out_batch, out_row;
   int dtype, vec;    // of out; whether its rows are 16-byte aligned
@@ -365,12 +368,14 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
       const int64_t at = (int64_t)r * s.Np + c;
       const f16x8 h = *(const f16x8*)(X + at);
       f16x8 l;
-      if (TWO) l = *(const f16x8*)(X + a.x_plane + at);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) l[q] = (f16)0.0f;
+      if (a.xl) l = *(const f16x8*)(a.xl + e * s.xs + at);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const bool in = r < s.M && c + q < s.N;
         const float d = in ? pd[TALL ? c + q : r] : 0.0f;
-        y[q] = in ? s_acc * y[q] + d * s_x * ((float)h[q] + (TWO ? (float)l[q] : 0.0f)) : 0.0f;
+        y[q] = in ? s_acc * y[q] + d * s_x * ((float)h[q] + (float)l[q]) : 0.0f;
       }
       if constexpr (OUT == OUT_X) {
         f16x8 hi, lo;
@@ -380,9 +385,8 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
           hi[q] = (f16)z;
           lo[q] = (f16)(z - (float)hi[q]);
         }
-        f16* o = a.xo + e * s.xs + at;
-        *(f16x8*)o = hi;
-        if (TWO) *(f16x8*)(o + a.x_plane) = lo;
+        *(f16x8*)(a.xo + e * s.xs + at) = hi;
+        *(f16x8*)(a.xol + e * s.xs + at) = lo;
       } else {
         auto put = [&](auto* o) {
           typedef typename std::remove_pointer<decltype(o)>::type D;
@@ -456,7 +460,7 @@ static int64_t parts_of(int64_t E, const Shape& s) {
 // Matrices that go through the chain together.
 constexpr int64_t kChunkBytes = (int64_t)4 << 30;
 static int64_t matrix_bytes(const Shape& s, int planes) {
-  return (2 * s.xs + 5 * s.ms) * 2 * planes + 4 * round_up((int64_t)s.S * 4, 256) + 1024 * 8 + 256;
+  return (4 * s.xs + 5 * s.ms * planes) * 2 + 4 * round_up((int64_t)s.S * 4, 256) + 1024 * 8 + 256;
 }
 static int64_t chunk_of(int64_t E, const Shape& s, int planes) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(E, kChunkBytes / matrix_bytes(s, planes)));
@@ -468,7 +472,7 @@ static int64_t workspace_bytes(int64_t E, const Shape& s, int planes) {
   b += round_up(n * 512 * 8, 256);                        // partial sums
   b += round_up(n * (int64_t)sizeof(Scale), 256);
   b += 3 * round_up(n * s.S * 4, 256);                    // diagonals
-  b += 2 * round_up(n * s.xs * 2 * planes, 256);          // X, twice
+  b += 2 * round_up(n * s.xs * 4, 256);                   // X, twice, two planes each
   b += 5 * round_up(n * s.ms * 2 * planes, 256);          // A, T and three of Q and P
   return b;
 }
@@ -488,18 +492,20 @@ struct Job {
 template <bool TALL, bool TWO>
 static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched, int steps, float eps, char* ws,
                      hipStream_t st) {
-  constexpr int planes = TWO ? 2 : 1;
+  constexpr int planes = TWO ? 2 : 1;  // of the S x S matrices
   auto take = [&](int64_t bytes) { char* p = ws; ws += round_up(bytes, 256); return p; };
   double* part = (double*)take(E * 512 * 8);
   Scale* scales = (Scale*)take(E * (int64_t)sizeof(Scale));
   float* diag[3];
   for (auto& d : diag) d = (float*)take(E * s.S * 4);
   f16* X[2];
-  for (auto& x : X) x = (f16*)take(E * s.xs * 2 * planes);
+  for (auto& x : X) x = (f16*)take(E * s.xs * 4);
   f16 *A = (f16*)take(E * s.ms * 2 * planes), *Tm = (f16*)take(E * s.ms * 2 * planes), *Q[3];
   for (auto& q : Q) q = (f16*)take(E * s.ms * 2 * planes);
   const int64_t x_plane = E * s.xs, m_plane = E * s.ms;
 
+  // in "half" f16 holds a bf16 x as it is
+  const bool first_lo = TWO || j.src.m || j.gdtype == MTX_F32;
   const int parts = (int)parts_of(E, s);
   const int rows = (int)ceil_div(s.M, parts), rows_p = (int)ceil_div(s.Mp, parts);
   const dim3 grid((unsigned)parts, (unsigned)E);
@@ -507,7 +513,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   do {                                                                                                              \
     hipLaunchKernelGGL((norm_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, rows, part);                   \
     hipLaunchKernelGGL((convert_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, s.Mp, s.Np, rows_p, part, parts, \
-                       eps, X[0], TWO ? X[0] + x_plane : nullptr, scales);                                          \
+                       eps, X[0], first_lo ? X[0] + x_plane : nullptr, scales);                                        \
   } while (0)
   if (j.gdtype == MTX_F32) {
     if (j.gvec) MTX_PREP(float, true);
@@ -579,7 +585,9 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
     a.p = Q[p];
     a.pd = diag[p];
     a.x = X[cur];
+    a.xl = first_lo || x_scale != 0.0f ? X[cur] + x_plane : nullptr;
     a.xo = X[cur ^ 1];
+    a.xol = X[cur ^ 1] + x_plane;
     a.out = j.out;
     a.out_batch = j.out_batch;
     a.out_row = j.out_row;

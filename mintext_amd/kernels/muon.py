@@ -27,11 +27,12 @@ import torch
 from .. import _lib as L
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-_GROUP = 3  # steps between two Gram products, at most
+# Steps between two Gram products, at most: fewer products with three, smaller errors with two
+_GROUP_RESULT, _GROUP_STEP = 2, 3
 
 
 @functools.lru_cache(maxsize=64)
-def _schedule(steps: int, coefficients: tuple):
+def _schedule(steps: int, coefficients: tuple, group: int):
     """The 9 floats a step of ``mtx_newton_schulz``: coefficients, scales, and where a group of steps ends.
 
     The singular values start in [0, 1] (the Frobenius norm bounds them), so those of every matrix on the way have a
@@ -39,7 +40,7 @@ def _schedule(steps: int, coefficients: tuple):
     keeps 1.25 times the bound inside f16.
     """
     triples = [coefficients] * steps if not isinstance(coefficients[0], tuple) else list(coefficients)
-    groups = -(-steps // _GROUP)
+    groups = -(-steps // group)
     sizes = [steps // groups + (g < steps % groups) for g in range(groups)]
     last = [sum(sizes[:g + 1]) - 1 for g in range(groups)]
 
@@ -66,7 +67,7 @@ def _schedule(steps: int, coefficients: tuple):
     return (ctypes.c_float * len(flat))(*flat)
 
 
-def _arguments(steps, coefficients, eps, precision, dtype):
+def _arguments(steps, coefficients, eps, precision, dtype, group):
     if not isinstance(steps, int) or not 1 <= steps <= 64:
         raise ValueError(f"steps must be an int from 1 to 64, got {steps!r}")
     if not eps > 0:
@@ -85,7 +86,7 @@ def _arguments(steps, coefficients, eps, precision, dtype):
     if not good or not all(math.isfinite(v) for t in c for v in (t if isinstance(t, tuple) else (t,))):
         raise ValueError("coefficients must be three finite numbers, or three for each step")
     planes = 2 if precision == "full" or (precision is None and dtype == torch.float32) else 1
-    return _schedule(steps, c), planes
+    return _schedule(steps, c, group), planes
 
 
 def _check_stack(t: torch.Tensor, name: str):
@@ -144,7 +145,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, *, coefficients=COEFFICIENTS,
         a dense tensor of x's shape and dtype.  Not differentiable.
     """
     _check_stack(x, "x")
-    sched, planes = _arguments(steps, coefficients, eps, precision, x.dtype)
+    sched, planes = _arguments(steps, coefficients, eps, precision, x.dtype, _GROUP_RESULT)
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("newton_schulz is not differentiable: pass x.detach()")
     dev = L.require_device(x)
@@ -182,7 +183,7 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
             raise ValueError(f"{name} must have param's shape {tuple(param.shape)}, got {tuple(t.shape)}")
     if momentum.dtype != torch.float32:
         raise TypeError(f"momentum must be float32, got {momentum.dtype}")
-    sched, planes = _arguments(steps, coefficients, eps, precision, param.dtype)
+    sched, planes = _arguments(steps, coefficients, eps, precision, param.dtype, _GROUP_STEP)
     M, N = param.shape[-2:]
     if scale == "spectral":
         factor = math.sqrt(max(1.0, N / max(M, 1)))

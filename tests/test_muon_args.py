@@ -59,9 +59,10 @@ def test_muon_update_refuses(args, kwargs, error):
         muon_update(*args, **kwargs)
 
 
+@pytest.mark.parametrize("group", [1, 2, 3])
 @pytest.mark.parametrize("steps", range(1, 10))
-def test_schedule(steps):
-    s = list(_schedule(steps, COEFFICIENTS))
+def test_schedule(steps, group):
+    s = list(_schedule(steps, COEFFICIENTS, group))
     rows = [s[9 * i:9 * i + 9] for i in range(steps)]
     ends = [r[8] for r in rows]
     assert ends[-1] == 1.0
@@ -71,7 +72,7 @@ def test_schedule(steps):
         if e:
             sizes.append(size)
             size = 0
-    assert sum(sizes) == steps and max(sizes) <= 3 and sizes == sorted(sizes, reverse=True)
+    assert sum(sizes) == steps and max(sizes) <= group and sizes == sorted(sizes, reverse=True)
     first = True
     for r in rows:
         assert all(math.log2(v).is_integer() for v in r[3:8])
@@ -96,7 +97,7 @@ def test_entry_points_refuse():
     lib = L.lib()
     buf = ctypes.create_string_buffer(4096)
     d, N_ = ctypes.addressof(buf), None
-    sched = _schedule(5, COEFFICIENTS)
+    sched = _schedule(5, COEFFICIENTS, 3)
     size = lib.mtx_newton_schulz_workspace_size
     assert size(4, 64, 32, 1) > 0 and size(4, 64, 32, 2) > size(4, 64, 32, 1)
     assert size(4, 64, 32, 3) < 0 and size(-1, 64, 32, 1) < 0 and size(1, 1 << 16, 1 << 16, 1) < 0
