@@ -126,13 +126,15 @@ __global__ __launch_bounds__(256) void norm_kernel(Source s, int M, int N, int r
   __syncthreads();
   if (threadIdx.x == 0) part[e * gridDim.x + blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
 }
-// X = x 2^e in f16, hi and lo planes where there are two, zeros past the last row and column, with e such that |x|_F + eps
+// X = x 2^e in f16, hi and lo planes where there are two, and what f32 holds beyond them (a bit at most: the steps carry
+// it up by a^5 where x is singular), zeros past the last row and column, with e such that |x|_F + eps
 // comes to [2^13, 2^14): a bf16 x is held exactly but for elements below 2^-27 of its norm.  Every workgroup adds the
 // parts of its matrix in the same order.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void convert_kernel(Source s, int M, int N, int Mp, int Np, int rows,
                                                       const double* __restrict__ part, int nparts, float eps,
-                                                      f16* __restrict__ X, f16* __restrict__ Xlo, Scale* scales) {
+                                                      f16* __restrict__ X, f16* __restrict__ Xlo,
+                                                      f16* __restrict__ Xrest, Scale* scales) {
   __shared__ double w[4];
   const int64_t e = blockIdx.y;
   double sum = 0.0;
@@ -153,16 +155,18 @@ __global__ __launch_bounds__(256) void convert_kernel(Source s, int M, int N, in
     const int r = r0 + i / nc, c = i % nc * 8;
     float u[8] = {};
     if (r < M && c < N) load_update<T, VEC, false>(s, e, r, c, N, u);
-    f16x8 hi, lo;
+    f16x8 hi, lo, rest;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const float v = ldexpf(u[q], ex);
       hi[q] = (f16)v;
       lo[q] = (f16)(v - (float)hi[q]);
+      rest[q] = (f16)(v - (float)hi[q] - (float)lo[q]);
     }
     const int64_t at = e * Mp * (int64_t)Np + (int64_t)r * Np + c;
     *(f16x8*)(X + at) = hi;
     if (Xlo) *(f16x8*)(Xlo + at) = lo;
+    if (Xrest) *(f16x8*)(Xrest + at) = rest;
   }
 }
 
@@ -317,7 +321,7 @@ struct ApplyArgs {
   const f16* p;
   const float* pd;   // P's diagonal
   const f16* x;
-  const f16* xl;     // x's lo plane, or nullptr
+  const f16 *xl, *xr;  // x's lo plane and the rest of the first x in "full", or nullptr
   f16 *xo, *xol;     // OUT_X: both planes
   void* out;         // OUT_STORE: the result; OUT_STEP: the weights
   int64_t out_batch, out_row;
@@ -371,11 +375,15 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
 #pragma unroll
       for (int q = 0; q < 8; ++q) l[q] = (f16)0.0f;
       if (a.xl) l = *(const f16x8*)(a.xl + e * s.xs + at);
+      f16x8 rest;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) rest[q] = (f16)0.0f;
+      if (TWO && a.xr) rest = *(const f16x8*)(a.xr + e * s.xs + at);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const bool in = r < s.M && c + q < s.N;
         const float d = in ? pd[TALL ? c + q : r] : 0.0f;
-        y[q] = in ? s_acc * y[q] + d * s_x * ((float)h[q] + (float)l[q]) : 0.0f;
+        y[q] = in ? s_acc * y[q] + d * s_x * ((float)h[q] + ((float)l[q] + (float)rest[q])) : 0.0f;
       }
       if constexpr (OUT == OUT_X) {
         f16x8 hi, lo;
@@ -460,7 +468,7 @@ static int64_t parts_of(int64_t E, const Shape& s) {
 // Matrices that go through the chain together.
 constexpr int64_t kChunkBytes = (int64_t)4 << 30;
 static int64_t matrix_bytes(const Shape& s, int planes) {
-  return (4 * s.xs + 5 * s.ms * planes) * 2 + 4 * round_up((int64_t)s.S * 4, 256) + 1024 * 8 + 256;
+  return ((4 + planes - 1) * s.xs + 5 * s.ms * planes) * 2 + 4 * round_up((int64_t)s.S * 4, 256) + 1024 * 8 + 256;
 }
 static int64_t chunk_of(int64_t E, const Shape& s, int planes) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(E, kChunkBytes / matrix_bytes(s, planes)));
@@ -472,7 +480,7 @@ static int64_t workspace_bytes(int64_t E, const Shape& s, int planes) {
   b += round_up(n * 512 * 8, 256);                        // partial sums
   b += round_up(n * (int64_t)sizeof(Scale), 256);
   b += 3 * round_up(n * s.S * 4, 256);                    // diagonals
-  b += 2 * round_up(n * s.xs * 4, 256);                   // X, twice, two planes each
+  b += 2 * round_up(n * s.xs * 4, 256) + (planes - 1) * round_up(n * s.xs * 2, 256);  // X, twice, in planes
   b += 5 * round_up(n * s.ms * 2 * planes, 256);          // A, T and three of Q and P
   return b;
 }
@@ -500,6 +508,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   for (auto& d : diag) d = (float*)take(E * s.S * 4);
   f16* X[2];
   for (auto& x : X) x = (f16*)take(E * s.xs * 4);
+  f16* rest = TWO ? (f16*)take(E * s.xs * 2) : nullptr;
   f16 *A = (f16*)take(E * s.ms * 2 * planes), *Tm = (f16*)take(E * s.ms * 2 * planes), *Q[3];
   for (auto& q : Q) q = (f16*)take(E * s.ms * 2 * planes);
   const int64_t x_plane = E * s.xs, m_plane = E * s.ms;
@@ -513,7 +522,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   do {                                                                                                              \
     hipLaunchKernelGGL((norm_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, rows, part);                   \
     hipLaunchKernelGGL((convert_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, s.Mp, s.Np, rows_p, part, parts, \
-                       eps, X[0], first_lo ? X[0] + x_plane : nullptr, scales);                                        \
+                       eps, X[0], first_lo ? X[0] + x_plane : nullptr, rest, scales);                                      \
   } while (0)
   if (j.gdtype == MTX_F32) {
     if (j.gvec) MTX_PREP(float, true);
@@ -586,6 +595,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
     a.pd = diag[p];
     a.x = X[cur];
     a.xl = first_lo || x_scale != 0.0f ? X[cur] + x_plane : nullptr;
+    a.xr = x_scale == 0.0f ? rest : nullptr;
     a.xo = X[cur ^ 1];
     a.xol = X[cur ^ 1] + x_plane;
     a.out = j.out;
