@@ -52,6 +52,21 @@ struct Operand {
   int left;
 };
 
+// A pointer that is the same in every lane, in scalar registers whatever the compiler can prove.
+__device__ __forceinline__ const char* uniform(const void* p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const char*)((uint64_t)lo | ((uint64_t)hi << 32));
+}
+
+// Eight values to consecutive elements on a 16-byte boundary, rounded to nearest even by the conversion instructions.
+__device__ __forceinline__ void store8(float* p, const float v[8]) { st8(p, 0, v); }
+__device__ __forceinline__ void store8(uint16_t* p, const float v[8]) {
+  typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+  *(bf16x8*)p = bf16x8{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3],
+                       (__bf16)v[4], (__bf16)v[5], (__bf16)v[6], (__bf16)v[7]};
+}
+
 __device__ __forceinline__ int row_off(int r, int c) { return r * 64 + ((c ^ ((r >> 2) & 3)) << 4); }
 template <int COLS>
 __device__ __forceinline__ int col_off(int k, int c) { return k * (COLS * 2) + ((c ^ ((k & 3) << 2)) << 4); }
@@ -109,7 +124,9 @@ struct Tile {
     const uint32_t lds_base = lds_addr(lds);
     const uint32_t wave_u = (uint32_t)__builtin_amdgcn_readfirstlane(wave);
     // The stage that is loaded next; stages past the end re-read the last one into a slot that is no longer read.
-    const char *pa = (const char*)a.p[0], *pb = (const char*)b.p[0];
+    const char* const planes_a[2] = {uniform(a.p[0]), uniform(a.p[TWO ? 1 : 0])};
+    const char* const planes_b[2] = {uniform(b.p[0]), uniform(b.p[TWO ? 1 : 0])};
+    const char *pa = planes_a[0], *pb = planes_b[0];
     int64_t at_a = 0, at_b = 0;  // TWO: byte offset of the reduction element in either plane
     int next = 0, part = 0;
     bool last = nk == 1;
@@ -123,8 +140,8 @@ struct Tile {
           at_a += a_step;
           at_b += b_step;
         }
-        pa = (const char*)a.p[part == 2] + at_a;
-        pb = (const char*)b.p[part == 1] + at_b;
+        pa = (part == 2 ? planes_a[1] : planes_a[0]) + at_a;
+        pb = (part == 1 ? planes_b[1] : planes_b[0]) + at_b;
       } else {
         pa += a_step;
         pb += b_step;
@@ -252,7 +269,8 @@ struct Tile {
     __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
     asm volatile("" ::: "memory");
   }
-  static constexpr int OUT_STEPS = TN * 2;  // of 64 lanes x 8 columns
+  static constexpr int OUT_STEPS = TN * 2;  // of 64 lanes x 8 columns; a lane's columns are the same in each
+  static_assert(64 % (TN * 4) == 0, "whole rows a step");
   static __device__ __forceinline__ int out_row(int it) { return (it * 64 + (threadIdx.x & 63)) / (TN * 4); }
   static __device__ __forceinline__ int out_col(int it) { return (it * 64 + (threadIdx.x & 63)) % (TN * 4) * 8; }
   static __device__ __forceinline__ void get(const char* mine, int it, float v[8]) {

@@ -189,81 +189,138 @@ struct SymArgs {
   const Scale* scales;  // Gram product of the first X: multiplies s_acc; or nullptr
 };
 
-template <class T, bool TWO>
+// Eight columns of up to NP f16 planes for each step of a wave's 32 rows, loaded together: the loads of a block of rows
+// are in flight while the one before is worked on.
+template <class T, int NP>
+struct Block {
+  f16x8 x[NP][T::OUT_STEPS];
+  // `at(it)`: offset of the lane's columns in step `it`, of an element that exists
+  template <class At>
+  __device__ __forceinline__ void load(int p, const f16* m, At at) {
+    if (!m) return;
+#pragma unroll
+    for (int it = 0; it < T::OUT_STEPS; ++it) x[p][it] = *(const f16x8*)(m + at(it));
+  }
+};
+
+// Eight f32 values as f16, and what that leaves of them.
+__device__ __forceinline__ f16x8 round8(const float y[8]) {
+  f16x8 h;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) h[q] = (f16)y[q];
+  return h;
+}
+__device__ __forceinline__ f16x8 rest8(const float y[8], const f16x8& h) {
+  f16x8 l;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) l[q] = (f16)(y[q] - (float)h[q]);
+  return l;
+}
+// y += k x, a single instruction an element
+__device__ __forceinline__ void add8(float y[8], const f16x8& x, float k) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) y[q] = __builtin_fmaf((float)x[q], k, y[q]);
+}
+
+// The scales are multiplied together before the elements are seen, and the diagonal is looked for only where a tile has
+// it: an epilogue of 56 instructions an element cost more than the products of 768 elements (156 us for 128
+// matrices of 768 x 768; 58 us at the matrix cores' peak).
+template <class T, bool ADD, bool TWO>
 __device__ __forceinline__ void sym_out(const SymArgs& a, const Sym& p, int64_t e, int m0, int n0,
                                         const f32x16 (&acc)[T::TM][T::TN], char* lds) {
   constexpr int TN = T::TN, HROW = TN * 64;  // bytes of a staged f16 row
+  constexpr int NP = TWO ? 4 : 2, AHEAD = TWO && TN == 4 ? 1 : 2;  // blocks of addends in registers
   static_assert(T::NW * (T::OUT_BYTES + (TWO ? 2 : 1) * 32 * HROW) <= T::LDS_BYTES, "staging fits the ring");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   char* mine = T::out_lds(lds);
   char* turn = lds + T::NW * T::OUT_BYTES + wave * ((TWO ? 2 : 1) * 32 * HROW);
-  const int wr = m0 + (wave / T::WN) * (T::TM * 32), wc = n0 + (wave % T::WN) * (TN * 32);
+  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c = n0 + (wave % T::WN) * (TN * 32) + T::out_col(0);
   const int S = a.S, Sp = a.Sp;
-  const float s_acc = p.s_acc * (a.scales ? a.scales[e].gram : 1.0f);
+  const float k_acc = p.s_acc * p.s_out * (a.scales ? a.scales[e].gram : 1.0f), k_v = p.s_v * p.s_out;
   f16* out = p.out + e * a.out_batch;
-  const f16 *u = p.cs ? p.u + e * a.in_batch : nullptr, *v = p.s_v != 0.0f ? p.v + e * a.in_batch : nullptr;
-  const float *rs = p.rs ? p.rs + e * S : nullptr, *cs = p.cs ? p.cs + e * S : nullptr;
-  float* diag = p.diag ? p.diag + e * S : nullptr;
-  auto addend = [&](const f16* m, int r, int c, float f[8]) {
-    const f16x8 h = *(const f16x8*)(m + (int64_t)r * Sp + c);
-    f16x8 l;
-    if (TWO) l = *(const f16x8*)(m + a.in_plane + (int64_t)r * Sp + c);
+  const f16 *u = ADD && p.cs ? p.u + e * a.in_batch : nullptr, *v = ADD ? p.v + e * a.in_batch : nullptr;
+  const float* rs = ADD && p.rs ? p.rs + e * Sp : nullptr;
+  float* diag = p.diag ? p.diag + e * Sp : nullptr;
+  float cs[8], k_u[8];
+  if (u) {
+    ld8(p.cs + e * Sp, min(c, Sp - 8), cs);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) f[q] = (float)h[q] + (TWO ? (float)l[q] : 0.0f);
+    for (int q = 0; q < 8; ++q) k_u[q] = cs[q] * (p.s_u * p.s_out);
+  }
+  Block<T, NP> add[AHEAD];
+  auto ahead = [&](int i) {
+    auto at = [&](int it) { return (int64_t)min(wr + i * 32 + T::out_row(it), S - 1) * Sp + min(c, Sp - 8); };
+    Block<T, NP>& b = add[i % AHEAD];
+    b.load(0, v, at);
+    b.load(1, u, at);
+    if constexpr (TWO) {
+      b.load(2, v ? v + a.in_plane : nullptr, at);
+      b.load(3, u ? u + a.in_plane : nullptr, at);
+    }
   };
+  if (ADD) ahead(0);
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
+    if (ADD && AHEAD == 2 && i + 1 < T::TM) ahead(i + 1);
+    if (ADD && AHEAD == 1 && i > 0) ahead(i);
     T::put(acc[i], mine);
-#pragma unroll 2
+    const Block<T, NP>& b = add[i % AHEAD];
+#pragma unroll
     for (int it = 0; it < T::OUT_STEPS; ++it) {
-      const int lr = T::out_row(it), lc = T::out_col(it), r = wr + i * 32 + lr, c = wc + lc;
-      float x[8];
-      T::get(mine, it, x);
-      f16x8 hi, lo;
+      const int lr = T::out_row(it), r = wr + i * 32 + lr;
+      const float rr = ADD && rs ? rs[min(r, S - 1)] : 1.0f;
+      float y[8];
+      T::get(mine, it, y);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) hi[q] = lo[q] = (f16)0.0f;
-      if (r < S && c < Sp) {
-        const float rr = rs ? rs[r] : 1.0f;
-        float f[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] *= s_acc;
-        if (v) {
-          addend(v, r, c, f);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] += p.s_v * rr * f[q];
-        }
+      for (int q = 0; q < 8; ++q) y[q] *= k_acc;
+      if (ADD) {
+        add8(y, b.x[0][it], rr * k_v);
+        if (TWO) add8(y, b.x[TWO ? 2 : 0][it], rr * k_v);
         if (u) {
-          addend(u, r, c, f);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] += p.s_u * (c + q < S ? cs[c + q] : 0.0f) * f[q];
-        }
+          for (int q = 0; q < 8; ++q) y[q] = __builtin_fmaf((float)b.x[1][it][q], k_u[q], y[q]);
+          if (TWO) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (c + q == r) {
-            x[q] += p.d0 + (u && rs ? rr * cs[r] : 0.0f);
-            if (diag) {
-              diag[r] = x[q];
-              x[q] = 0.0f;
-            }
+            for (int q = 0; q < 8; ++q) y[q] = __builtin_fmaf((float)b.x[TWO ? 3 : 1][it][q], k_u[q], y[q]);
           }
-          const float y = c + q < S ? x[q] * p.s_out : 0.0f;
-          hi[q] = (f16)y;
-          lo[q] = (f16)(y - (float)hi[q]);
         }
+      }
+      if (m0 == n0 && ADD) {
+        const int dq = r - c;  // the diagonal's place among the lane's columns
+        if (dq >= 0 && dq < 8) {
+          float d = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            if (q == dq) d = y[q] + (p.d0 + (u && rs ? rr * cs[q] : 0.0f)) * p.s_out;
+          }
+          if (diag && r < Sp) diag[r] = r < S ? d / p.s_out : 0.0f;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) y[q] = q == dq ? (diag ? 0.0f : d) : y[q];
+        }
+      }
+      if (c + 8 > S) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) y[q] = c + q < S ? y[q] : 0.0f;
+      }
+      f16x8 hi = round8(y), lo;
+      if (TWO) lo = rest8(y, hi);
+      if (r < S && c < Sp) {
         *(f16x8*)(out + (int64_t)r * Sp + c) = hi;
         if (TWO) *(f16x8*)(out + a.out_plane + (int64_t)r * Sp + c) = lo;
       }
       if (m0 != n0) {
-        char* at = turn + lr * HROW + (((lc >> 3) ^ ((lr & 3) << 1)) << 4);
-        *(f16x8*)at = hi;
-        if (TWO) *(f16x8*)(at + 32 * HROW) = lo;
+        const uint32_t keep = r < S ? 0xFFFFFFFFu : 0u;
+        char* at = turn + lr * HROW + (((T::out_col(0) >> 3) ^ ((lr & 3) << 1)) << 4);
+        *(u32x4*)at = __builtin_bit_cast(u32x4, hi) & keep;
+        if (TWO) *(u32x4*)(at + 32 * HROW) = __builtin_bit_cast(u32x4, lo) & keep;
       }
     }
     if (m0 == n0) continue;
     // the mirrored tile: 16 lanes read 16 columns of eight rows each, turned; 64 contiguous bytes a row of it
     __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
     asm volatile("" ::: "memory");
-#pragma unroll 2
+    const int wc = n0 + (wave % T::WN) * (TN * 32);
+#pragma unroll
     for (int it = 0; it < TN * 2; ++it) {
       const int rb = (lane >> 4) * 8, cb = it * 16;
       const int row = wc + cb + (lane & 15), col = wr + i * 32 + rb;
@@ -293,15 +350,16 @@ __device__ __forceinline__ void lower(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// COLS: the reduction runs down u's and v's columns (the Gram product of a tall X); otherwise along their rows.
-template <class T, bool COLS, bool TWO>
+// GRAM: X times itself, no addends.  COLS: the reduction runs down u's and v's columns (the Gram product of a tall X);
+// otherwise along their rows.
+template <class T, bool GRAM, bool COLS, bool TWO>
 __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void sym_kernel(SymArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
   const int nt = (a.S + T::BM - 1) / T::BM, per = nt * (nt + 1) / 2;
   const int t = tile_of(blockIdx.x, a.np * a.E * per);
   if (t < 0) return;
   const int64_t e = t / per % a.E;
-  const Sym p = a.p[t / per / a.E];
+  const Sym p = t / per < a.E ? a.p[0] : a.p[1];
   int i, j;
   lower(t % per, i, j);
   const int m0 = i * T::BM, n0 = j * T::BM;
@@ -312,7 +370,7 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void sym_kernel(SymArg
   f32x16 acc[T::TM][T::TN];
   T::product(operand(p.u, m0), operand(p.v, n0), a.K, lds, acc);
   __syncthreads();
-  sym_out<T, TWO>(a, p, e, m0, n0, acc, lds);
+  sym_out<T, !GRAM, TWO>(a, p, e, m0, n0, acc, lds);
 }
 
 // ---- X <- P X (tall: X P) ----------------------------------------------------------------------------------------
@@ -335,7 +393,8 @@ struct ApplyArgs {
   float lr, decay, factor;
   const float* lr_dev;
 };
-template <class T, bool TALL, bool TWO, int OUT>
+// D: the type of what is stored or stepped.
+template <class T, bool TALL, bool TWO, int OUT, typename D>
 __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(ApplyArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
   const Shape s = a.s;
@@ -358,68 +417,87 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
   char* mine = T::out_lds(lds);
   const int wr = m0 + (wave / T::WN) * (T::TM * 32), wc = n0 + (wave % T::WN) * (T::TN * 32);
   const float s_x = a.scales ? a.scales[e].x : a.s_x, s_acc = s_x * a.s_p;
-  const float* pd = a.pd + e * s.S;
+  const float* pd = a.pd + e * s.Sp;
   const float lr = OUT == OUT_STEP ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.0f;
+  const f16 *xl = a.xl ? a.xl + e * s.xs : nullptr, *xr = TWO && a.xr ? a.xr + e * s.xs : nullptr;
+  const int c = wc + T::out_col(0);
+  constexpr int NP = TWO ? 3 : 2, DV = sizeof(D) / 2;  // 16-byte pieces of eight D
+  constexpr int AHEAD = T::TN == 4 && (TWO || (OUT == OUT_STEP && DV == 2)) ? 1 : 2;
+  Block<T, NP> add[AHEAD];
+  u32x4 old[AHEAD][OUT == OUT_STEP ? T::OUT_STEPS : 1][DV];  // the weights before the step
+  D* out = OUT == OUT_X ? nullptr : (D*)a.out + e * a.out_batch;
+  const bool vec = a.vec;
+  auto ahead = [&](int i) {
+    if (OUT == OUT_STEP && vec) {
+#pragma unroll
+      for (int it = 0; it < T::OUT_STEPS; ++it) {
+        const D* w = out + (int64_t)min(wr + i * 32 + T::out_row(it), s.M - 1) * a.out_row + min(c, s.N - 8);
+#pragma unroll
+        for (int d = 0; d < DV; ++d) old[i % AHEAD][it][d] = ((const u32x4*)w)[d];
+      }
+    }
+    auto at = [&](int it) { return (int64_t)min(wr + i * 32 + T::out_row(it), s.Mp - 1) * s.Np + min(c, s.Np - 8); };
+    Block<T, NP>& b = add[i % AHEAD];
+    b.load(0, X, at);
+    b.load(1, xl, at);
+    if constexpr (TWO) b.load(2, xr, at);
+  };
+  float dc[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) dc[q] = 0.0f;
+  if (TALL) ld8(pd, min(c, s.Sp - 8), dc);
+  ahead(0);
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
+    if (AHEAD == 2 && i + 1 < T::TM) ahead(i + 1);
+    if (AHEAD == 1 && i > 0) ahead(i);
     T::put(acc[i], mine);
-#pragma unroll 2
+    const Block<T, NP>& b = add[i % AHEAD];
+#pragma unroll
     for (int it = 0; it < T::OUT_STEPS; ++it) {
-      const int r = wr + i * 32 + T::out_row(it), c = wc + T::out_col(it);
-      if (r >= (OUT == OUT_X ? s.Mp : s.M) || c >= (OUT == OUT_X ? s.Np : s.N)) continue;
+      const int r = wr + i * 32 + T::out_row(it);
       float y[8];
       T::get(mine, it, y);
-      const int64_t at = (int64_t)r * s.Np + c;
-      const f16x8 h = *(const f16x8*)(X + at);
-      f16x8 l;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) l[q] = (f16)0.0f;
-      if (a.xl) l = *(const f16x8*)(a.xl + e * s.xs + at);
-      f16x8 rest;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) rest[q] = (f16)0.0f;
-      if (TWO && a.xr) rest = *(const f16x8*)(a.xr + e * s.xs + at);
+      const float dr = TALL ? 0.0f : pd[min(r, s.Sp - 1)];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const bool in = r < s.M && c + q < s.N;
-        const float d = in ? pd[TALL ? c + q : r] : 0.0f;
-        y[q] = in ? s_acc * y[q] + d * s_x * ((float)h[q] + ((float)l[q] + (float)rest[q])) : 0.0f;
+        const float k = (TALL ? dc[q] : dr) * s_x;
+        y[q] = __builtin_fmaf((float)b.x[0][it][q], k, y[q] * s_acc);
+        if (xl) y[q] = __builtin_fmaf((float)b.x[1][it][q], k, y[q]);
+        if (TWO && xr) y[q] = __builtin_fmaf((float)b.x[TWO ? 2 : 1][it][q], k, y[q]);
       }
+      if (r >= (OUT == OUT_X ? s.Mp : s.M) || c >= (OUT == OUT_X ? s.Np : s.N)) continue;
       if constexpr (OUT == OUT_X) {
-        f16x8 hi, lo;
+        if (r >= s.M || c + 8 > s.N) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float z = y[q] * a.s_out;
-          hi[q] = (f16)z;
-          lo[q] = (f16)(z - (float)hi[q]);
+          for (int q = 0; q < 8; ++q) y[q] = r < s.M && c + q < s.N ? y[q] : 0.0f;
         }
-        *(f16x8*)(a.xo + e * s.xs + at) = hi;
-        *(f16x8*)(a.xol + e * s.xs + at) = lo;
+        const int64_t at = e * s.xs + (int64_t)r * s.Np + c;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) y[q] *= a.s_out;
+        const f16x8 hi = round8(y);
+        *(f16x8*)(a.xo + at) = hi;
+        *(f16x8*)(a.xol + at) = rest8(y, hi);
       } else {
-        auto put = [&](auto* o) {
-          typedef typename std::remove_pointer<decltype(o)>::type D;
-          o += e * a.out_batch + (int64_t)r * a.out_row + c;
+        D* o = out + (int64_t)r * a.out_row + c;
+        if constexpr (OUT == OUT_STEP) {
           float w[8];
-          if (OUT == OUT_STEP) {
-            if (a.vec) {
-              ld8(o, 0, w);
-            } else {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) w[q] = c + q < s.N ? gld<D>(o, q) : 0.0f;
-            }
-#pragma unroll
-            for (int q = 0; q < 8; ++q) y[q] = w[q] * (1.0f - lr * a.decay) - lr * a.factor * y[q];
-          }
-          if (a.vec) {
-            st8(o, 0, y);
+          if (vec) {
+            ld8((const D*)old[i % AHEAD][it], 0, w);
           } else {
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (c + q < s.N) gst<D>(o, q, y[q]);
+            for (int q = 0; q < 8; ++q) w[q] = c + q < s.N ? gld<D>(o, q) : 0.0f;
           }
-        };
-        if (a.dtype == MTX_F32) put((float*)a.out);
-        else put((uint16_t*)a.out);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) y[q] = w[q] * (1.0f - lr * a.decay) - lr * a.factor * y[q];
+        }
+        if (vec) {
+          store8(o, y);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (c + q < s.N) gst<D>(o, q, y[q]);
+        }
       }
     }
   }
@@ -431,32 +509,36 @@ template <bool A, bool B, bool TWO> using Small = Tile<F16, 2, 2, 2, 2, 4, A, B,
 
 constexpr int kBigTiles = 192;
 
-template <bool COLS, bool TWO>
+template <bool GRAM, bool COLS, bool TWO>
 static int launch_sym(const SymArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { const int64_t n = ceil_div(a.S, b); return a.np * a.E * (n * (n + 1) / 2); };
   if (tiles(256) >= kBigTiles && a.S >= 256)
-    hipLaunchKernelGGL((sym_kernel<Big<COLS, COLS, TWO>, COLS, TWO>), dim3((unsigned)tiles_grid(tiles(256))), dim3(256), 0,
+    hipLaunchKernelGGL((sym_kernel<Big<COLS, COLS, TWO>, GRAM, COLS, TWO>), dim3((unsigned)tiles_grid(tiles(256))), dim3(256), 0,
                        st, a);
   else
-    hipLaunchKernelGGL((sym_kernel<Small<COLS, COLS, TWO>, COLS, TWO>), dim3((unsigned)tiles_grid(tiles(128))), dim3(256),
+    hipLaunchKernelGGL((sym_kernel<Small<COLS, COLS, TWO>, GRAM, COLS, TWO>), dim3((unsigned)tiles_grid(tiles(128))), dim3(256),
                        0, st, a);
   return check_launch();
 }
-template <bool TALL, bool TWO, int OUT>
+template <bool TALL, bool TWO, int OUT, typename D>
 static int launch_apply_out(const ApplyArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { return a.E * ceil_div(a.s.Mp, b) * ceil_div(a.s.Np, b); };
   if (tiles(256) >= kBigTiles && a.s.S >= 256)
-    hipLaunchKernelGGL((apply_kernel<Big<false, !TALL, TWO>, TALL, TWO, OUT>), dim3((unsigned)tiles_grid(tiles(256))),
+    hipLaunchKernelGGL((apply_kernel<Big<false, !TALL, TWO>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(256))),
                        dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((apply_kernel<Small<false, !TALL, TWO>, TALL, TWO, OUT>), dim3((unsigned)tiles_grid(tiles(128))),
+    hipLaunchKernelGGL((apply_kernel<Small<false, !TALL, TWO>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(128))),
                        dim3(256), 0, st, a);
   return check_launch();
 }
 template <bool TALL, bool TWO>
 static int launch_apply(int out, const ApplyArgs& a, hipStream_t st) {
-  return out == OUT_X ? launch_apply_out<TALL, TWO, OUT_X>(a, st)
-         : out == OUT_STORE ? launch_apply_out<TALL, TWO, OUT_STORE>(a, st) : launch_apply_out<TALL, TWO, OUT_STEP>(a, st);
+  if (out == OUT_X) return launch_apply_out<TALL, TWO, OUT_X, uint16_t>(a, st);
+  if (a.dtype == MTX_F32)
+    return out == OUT_STORE ? launch_apply_out<TALL, TWO, OUT_STORE, float>(a, st)
+                            : launch_apply_out<TALL, TWO, OUT_STEP, float>(a, st);
+  return out == OUT_STORE ? launch_apply_out<TALL, TWO, OUT_STORE, uint16_t>(a, st)
+                          : launch_apply_out<TALL, TWO, OUT_STEP, uint16_t>(a, st);
 }
 
 // Workgroups of a matrix in the norm and conversion launches.
@@ -468,7 +550,7 @@ static int64_t parts_of(int64_t E, const Shape& s) {
 // Matrices that go through the chain together.
 constexpr int64_t kChunkBytes = (int64_t)4 << 30;
 static int64_t matrix_bytes(const Shape& s, int planes) {
-  return ((4 + planes - 1) * s.xs + 5 * s.ms * planes) * 2 + 4 * round_up((int64_t)s.S * 4, 256) + 1024 * 8 + 256;
+  return ((4 + planes - 1) * s.xs + 5 * s.ms * planes) * 2 + 4 * round_up((int64_t)s.Sp * 4, 256) + 1024 * 8 + 256;
 }
 static int64_t chunk_of(int64_t E, const Shape& s, int planes) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(E, kChunkBytes / matrix_bytes(s, planes)));
@@ -479,7 +561,7 @@ static int64_t workspace_bytes(int64_t E, const Shape& s, int planes) {
   int64_t b = 0;
   b += round_up(n * 512 * 8, 256);                        // partial sums
   b += round_up(n * (int64_t)sizeof(Scale), 256);
-  b += 3 * round_up(n * s.S * 4, 256);                    // diagonals
+  b += 3 * round_up(n * s.Sp * 4, 256);                    // diagonals
   b += 2 * round_up(n * s.xs * 4, 256) + (planes - 1) * round_up(n * s.xs * 2, 256);  // X, twice, in planes
   b += 5 * round_up(n * s.ms * 2 * planes, 256);          // A, T and three of Q and P
   return b;
@@ -505,7 +587,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   double* part = (double*)take(E * 512 * 8);
   Scale* scales = (Scale*)take(E * (int64_t)sizeof(Scale));
   float* diag[3];
-  for (auto& d : diag) d = (float*)take(E * s.S * 4);
+  for (auto& d : diag) d = (float*)take(E * s.Sp * 4);
   f16* X[2];
   for (auto& x : X) x = (f16*)take(E * s.xs * 4);
   f16* rest = TWO ? (f16*)take(E * s.xs * 2) : nullptr;
@@ -558,7 +640,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
       g.scales = x_scale == 0.0f ? scales : nullptr;
       g.p[0] = Sym{X[cur], X[cur], A, nullptr, nullptr, nullptr, x_scale == 0.0f ? 1.0f : 1.0f / (x_scale * x_scale),
                    0.0f, 0.0f, 0.0f, sA};
-      rc = launch_sym<TALL, TWO>(g, st);
+      rc = launch_sym<true, TALL, TWO>(g, st);
       if (rc != MTX_OK) return rc;
     }
     m.K = s.Sp;
@@ -568,7 +650,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
     const int q = p < 0 ? 0 : (p + 1) % 3, np = p < 0 ? q : (p + 2) % 3;
     m.np = 1;
     m.p[0] = Sym{A, A, Q[q], diag[q], nullptr, nullptr, c[2] / (sA * sA), c[1] / sA, 0.0f, c[0], sQ};
-    rc = launch_sym<false, TWO>(m, st);
+    rc = launch_sym<false, false, TWO>(m, st);
     if (rc != MTX_OK) return rc;
     // P <- Q P and T = Q A in one launch, then A <- Q T
     m.np = 0;
@@ -578,7 +660,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
     }
     if (!ends) m.p[m.np++] = Sym{Q[q], A, Tm, nullptr, diag[q], nullptr, 1.0f / (sQ * sA), 1.0f / sA, 0.0f, 0.0f, sT};
     if (m.np > 0) {
-      rc = launch_sym<false, TWO>(m, st);
+      rc = launch_sym<false, false, TWO>(m, st);
       if (rc != MTX_OK) return rc;
     }
     p = np;
@@ -586,7 +668,7 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
       const float sA2 = c[3 + 9];
       m.np = 1;
       m.p[0] = Sym{Q[q], Tm, A, nullptr, diag[q], nullptr, 1.0f / (sQ * sT), 1.0f / sT, 0.0f, 0.0f, sA2};
-      rc = launch_sym<false, TWO>(m, st);
+      rc = launch_sym<false, false, TWO>(m, st);
       if (rc != MTX_OK) return rc;
       continue;
     }
