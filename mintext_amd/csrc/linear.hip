@@ -2,8 +2,10 @@
 //
 // The bias, the activation, the residual and, for training, the copy of z = x w + bias that the gradient needs
 // are applied to the f32 sums on their way out, so that z costs at most one write and the rest no
-// pass of their own.  Kernels: f32 matrix-core tiles (f32_tile.h), any size and alignment.
+// pass of their own.  bf16 with rows of whole 16-byte chunks runs on the 16-bit matrix cores (dense_tile.h), 256 x 256
+// tiles or, where those are few, 128 x 128; everything else on f32 matrix-core tiles (f32_tile.h).
 #include "common.h"
+#include "dense_tile.h"
 #include "f32_tile.h"
 #include <algorithm>
 
@@ -91,6 +93,68 @@ __global__ __launch_bounds__(f32mm::NT) void f32_kernel(Args p) {
     float y = activate(z, p.act);
     if (p.residual) y += gld<T>((const T*)p.residual, r * cols + n);
     gst<T>((T*)p.out, r * cols + n, y);
+  }
+}
+
+// ---- bf16, rows of whole 16-byte chunks: tiles of the 16-bit matrix cores -----------------------------------------
+using dense::Operand;
+template <int MODE, bool TAIL> using Big = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, MODE == DW, MODE != DX, TAIL>;
+template <int MODE, bool TAIL> using Small = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, MODE == DW, MODE != DX, TAIL>;
+
+// z = v + bias, out = act(z) + residual for eight columns
+__device__ __forceinline__ void finish8(const Args& p, int r, int c, float v[8]) {
+  const int64_t at = (int64_t)r * p.cols + c;
+  if (p.bias) {
+    float b[8];
+    ld8((const uint16_t*)p.bias, c, b);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] += b[q];
+  }
+  if (p.pre) dense::store8((uint16_t*)p.pre + at, v);
+  if (p.act != MTX_ACT_NONE) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = activate(v[q], p.act);
+  }
+  if (p.residual) {
+    float b[8];
+    ld8((const uint16_t*)p.residual, at, b);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] += b[q];
+  }
+  dense::store8((uint16_t*)p.out + at, v);
+}
+
+// Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2.
+constexpr int kGroup = 8;
+template <class T, int MODE>
+__global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void tile_kernel(Args p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
+  const int nm = (p.rows + T::BM - 1) / T::BM, nn = (p.cols + T::BN - 1) / T::BN;
+  const int t = dense::tile_of(blockIdx.x, nm * nn);
+  if (t < 0) return;
+  const int g = t / (kGroup * nn), gs = min(kGroup, nm - g * kGroup), in = t - g * kGroup * nn;
+  const int m0 = (g * kGroup + in % gs) * T::BM, n0 = in / gs * T::BN;
+  const uint16_t *a = (const uint16_t*)p.a, *b = (const uint16_t*)p.b;
+  const uint16_t* pa = MODE == DW ? a + m0 : a + (int64_t)m0 * p.red;
+  const uint16_t* pb = MODE == DX ? b + (int64_t)n0 * p.red : b + n0;
+  const Operand oa{{pa, pa}, MODE == DW ? p.rows : p.red, p.rows - m0};
+  const Operand ob{{pb, pb}, MODE == DX ? p.red : p.cols, p.cols - n0};
+  dense::f32x16 acc[T::TM][T::TN];
+  T::product(oa, ob, p.red, lds, acc);
+  __syncthreads();
+  const int wave = threadIdx.x >> 6;
+  char* mine = T::out_lds(lds);
+  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c = n0 + (wave % T::WN) * (T::TN * 32) + T::out_col(0);
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    T::put(acc[i], mine);
+#pragma unroll 2
+    for (int it = 0; it < T::OUT_STEPS; ++it) {
+      const int r = wr + i * 32 + T::out_row(it);
+      float v[8];
+      T::get(mine, it, v);
+      if (r < p.rows && c < p.cols) finish8(p, r, c, v);
+    }
   }
 }
 
@@ -185,9 +249,34 @@ static int check_sizes(int dtype, int64_t M, int64_t K, int64_t N) {
   return MTX_OK;
 }
 
+// The 16-bit tiles take rows of whole 16-byte chunks: of both operands, and of what is read and written beside them.
+static bool takes_tiles(int mode, const Args& p) {
+  const int la = mode == DW ? p.rows : p.red, lb = mode == DX ? p.red : p.cols;
+  return p.red > 0 && la % 8 == 0 && lb % 8 == 0 && p.cols % 8 == 0 && aligned16(p.a) && aligned16(p.b) &&
+         aligned16(p.out) && aligned16(p.bias) && aligned16(p.residual) && aligned16(p.pre);
+}
+
+template <int MODE, bool TAIL>
+static int launch_tiles(const Args& p, hipStream_t st) {
+  auto tiles = [&](int b) { return ceil_div(p.rows, b) * ceil_div(p.cols, b); };
+  if (tiles(256) >= 192)
+    hipLaunchKernelGGL((tile_kernel<Big<MODE, TAIL>, MODE>), dim3((unsigned)dense::tiles_grid(tiles(256))), dim3(256), 0, st,
+                       p);
+  else
+    hipLaunchKernelGGL((tile_kernel<Small<MODE, TAIL>, MODE>), dim3((unsigned)dense::tiles_grid(tiles(128))), dim3(256), 0,
+                       st, p);
+  return check_launch();
+}
+template <int MODE>
+static int launch_tiles(const Args& p, hipStream_t st) {
+  return p.red % dense::BKS ? launch_tiles<MODE, true>(p, st) : launch_tiles<MODE, false>(p, st);
+}
+
 static int launch_product(int mode, const Args& p, int dtype, hipStream_t st) {
   if (p.rows == 0 || p.cols == 0) return MTX_OK;
   if (!p.out || (p.red > 0 && (!p.a || !p.b))) return MTX_ERR_ARG;
+  if (dtype == MTX_BF16 && takes_tiles(mode, p))
+    return mode == FWD ? launch_tiles<FWD>(p, st) : mode == DX ? launch_tiles<DX>(p, st) : launch_tiles<DW>(p, st);
 #define MTX_F32_MODE(T) \
   (mode == FWD ? launch_f32<T, FWD>(p, st) : mode == DX ? launch_f32<T, DX>(p, st) : launch_f32<T, DW>(p, st))
   return dtype == MTX_F32 ? MTX_F32_MODE(float) : MTX_F32_MODE(uint16_t);
