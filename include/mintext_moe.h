@@ -47,7 +47,7 @@
  *   mtx_quant_fp8_weights_t, mtx_gmm_fp8_dlhs, mtx_quant_fp8_grouped_t, mtx_tgmm_fp8
  *                          <- no counterpart; fp8 forms of the dlhs and tgmm backward
  *                             (grouped_matmul.py:151-187, 197-235)
- *   mtx_linear, mtx_linear_dx, mtx_linear_dw, mtx_linear_act_bwd
+ *   mtx_linear, mtx_linear_bwd
  *                          <- Linear.__call__ and the products of MLP (mintext/modules/linear.py:
  *                             123-147, 164-228) with bias, activation and residual, and their VJP
  *   mtx_newton_schulz, mtx_muon_update
@@ -416,12 +416,12 @@ int mtx_gmm_fp8_gathered(const uint8_t* xq, const float* x_scale, int64_t x_rows
  * surrounds them in a layer, and their gradient.  Dense row-major operands of one dtype (F32 or
  * BF16), any sizes up to 65535 * 64 each, any alignment; sums in float32, one rounding at the end.
  * mtx_linear:     z = x[M,K] @ w[K,N] + bias[N];  out[M,N] = act(z) + residual[M,N].  bias, residual
- *                 and pre may be NULL; pre[M,N] receives z (for mtx_linear_act_bwd).
- * mtx_linear_act_bwd: dz = dy * act'(pre) (not written for MTX_ACT_NONE, where pre and dz may be
- *                 NULL: dz is dy) and, unless dbias is NULL, dbias[N] = column sums of dz in float32.
- * mtx_linear_dx:  dx[M,K] = dz[M,N] @ w[K,N]^T.   mtx_linear_dw: dw[K,N] = x[M,K]^T @ dz[M,N].
- * One workspace size serves the four (act_bwd: that of K = 0 or more); none may be shared by two
- * calls that can run at the same time.                                                     */
+ *                 and pre may be NULL; pre[M,N] receives z (for mtx_linear_bwd).
+ * mtx_linear_bwd: dz = dy * act'(pre), written to dz[M,N] (pre and dz may be NULL for MTX_ACT_NONE,
+ *                 where dz is dy); dx[M,K] = dz @ w^T, dw[K,N] = x^T @ dz, dbias[N] = column sums
+ *                 of dz; those of the three that are NULL are left out.
+ * One workspace size serves both; a workspace must not be shared by two calls that can run at the
+ * same time.                                                                               */
 #define MTX_ACT_NONE       0
 #define MTX_ACT_RELU       1
 #define MTX_ACT_SILU       2
@@ -431,12 +431,9 @@ int64_t mtx_linear_workspace_size(int64_t M, int64_t K, int64_t N);
 int mtx_linear(const void* x, const void* w, const void* bias, const void* residual, int dtype, int64_t M,
                int64_t K, int64_t N, int act, void* out, void* pre, void* workspace,
                int64_t workspace_bytes, void* stream);
-int mtx_linear_dx(const void* dz, const void* w, int dtype, int64_t M, int64_t K, int64_t N, void* dx,
-                  void* workspace, int64_t workspace_bytes, void* stream);
-int mtx_linear_dw(const void* x, const void* dz, int dtype, int64_t M, int64_t K, int64_t N, void* dw,
-                  void* workspace, int64_t workspace_bytes, void* stream);
-int mtx_linear_act_bwd(const void* dy, const void* pre, int dtype, int64_t M, int64_t N, int act, void* dz,
-                       void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre, int dtype, int64_t M,
+                   int64_t K, int64_t N, int act, void* dz, void* dx, void* dw, void* dbias,
+                   void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- orthogonalised updates ---------------------------------------------------------------
  * Muon over stacked expert weights (mintext/optim/optimizer.py:92-168), each of the E matrices by

@@ -94,9 +94,7 @@ SIGNATURES = {
     "mtx_quant_fp8_operands": (_I, [_I, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _P, _P, _P, _P, _P]),
     "mtx_linear_workspace_size": (_I64, [_I64, _I64, _I64]),
     "mtx_linear": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
-    "mtx_linear_dx": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _P]),
-    "mtx_linear_dw": (_I, [_P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _P]),
-    "mtx_linear_act_bwd": (_I, [_P, _P, _I, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
+    "mtx_linear_bwd": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P, _I64, _P]),
     "mtx_newton_schulz_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
     "mtx_newton_schulz": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _F, _I, _P, _I64, _I64, _P, _I64, _P]),
     "mtx_muon_update": (_I, [_P, _I, _I64, _I64, _P, _I, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _F, _P,

@@ -23,6 +23,8 @@ struct Args {
   void* pre;             // [rows][cols]: z, or nullptr
   int act;
   int rows, cols, red;   // of the product
+  int pieces;            // the reduction is split over so many workgroups; more than one: f32 sums to `part`
+  float* part;           // [pieces][rows][cols]
 };
 
 // The activations.  -inf gives NaN in all but ReLU (0 x inf), as the formulas do.
@@ -33,6 +35,24 @@ __device__ __forceinline__ float activate(float z, int act) {
     case MTX_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
     case MTX_ACT_GELU_TANH:  // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u))
       return z / (1.0f + expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
+    default: return z;
+  }
+}
+// The same for results in bf16, with the hardware's exp2 and reciprocal: in the 256-row tiles' way out the exact
+// functions took a fifth of the products' time.  erfc(x) = P(1 / (1 + 0.3275911 x)) exp(-x^2) is Abramowitz and Stegun's
+// 7.1.26, |error| <= 1.5e-7.
+__device__ __forceinline__ float activate_fast(float z, int act) {
+  switch (act) {
+    case MTX_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case MTX_ACT_SILU: return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+    case MTX_ACT_GELU: {
+      const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+      const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+      const float c = p * __expf(-x * x);  // erfc(|z| / sqrt 2)
+      return 0.5f * z * (z < 0.0f ? c : 2.0f - c);
+    }
+    case MTX_ACT_GELU_TANH:
+      return z * __builtin_amdgcn_rcpf(1.0f + __expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
     default: return z;
   }
 }
@@ -60,26 +80,29 @@ __global__ __launch_bounds__(f32mm::NT) void f32_kernel(Args p) {
   using namespace f32mm;
   __shared__ __attribute__((aligned(16))) float as[TILE], bs[TILE];
   const int64_t r0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-  const int64_t rows = p.rows, cols = p.cols, red = p.red;
+  const int64_t rows = p.rows, cols = p.cols;
   const T *A = (const T*)p.a, *B = (const T*)p.b;
+  const int stages = (p.red + KS - 1) / KS, piece = blockIdx.z;
+  const int64_t kb = (int64_t)piece * stages / p.pieces * KS;
+  const int64_t red = min((int64_t)(piece + 1) * stages / p.pieces * KS, (int64_t)p.red);  // of this piece: [kb, red)
   auto at_a = [&](int r, int c, int s) -> const T* {
     if (MODE == DW) {
-      const int64_t k = (int64_t)s * KS + r, m = r0 + c;
+      const int64_t k = kb + (int64_t)s * KS + r, m = r0 + c;
       return k < red && m < rows ? A + k * rows + m : nullptr;
     }
-    const int64_t m = r0 + r, k = (int64_t)s * KS + c;
-    return m < rows && k < red ? A + m * red + k : nullptr;
+    const int64_t m = r0 + r, k = kb + (int64_t)s * KS + c;
+    return m < rows && k < red ? A + m * p.red + k : nullptr;
   };
   auto at_b = [&](int r, int c, int s) -> const T* {
     if (MODE == DX) {
-      const int64_t n = n0 + r, k = (int64_t)s * KS + c;
-      return n < cols && k < red ? B + n * red + k : nullptr;
+      const int64_t n = n0 + r, k = kb + (int64_t)s * KS + c;
+      return n < cols && k < red ? B + n * p.red + k : nullptr;
     }
-    const int64_t k = (int64_t)s * KS + r, n = n0 + c;
+    const int64_t k = kb + (int64_t)s * KS + r, n = n0 + c;
     return k < red && n < cols ? B + k * cols + n : nullptr;
   };
   f32x16 acc;
-  mainloop<T, MODE == DW, MODE != DX, VEC>(acc, p.red, as, bs, at_a, at_b, A, B);
+  mainloop<T, MODE == DW, MODE != DX, VEC>(acc, (int)(red - kb), as, bs, at_a, at_b, A, B);
   const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) >> 1, wn = (threadIdx.x >> 6) & 1;
   const int64_t n = n0 + wn * 32 + (lane & 31);
   if (n >= cols) return;
@@ -88,6 +111,10 @@ __global__ __launch_bounds__(f32mm::NT) void f32_kernel(Args p) {
   for (int v = 0; v < 16; ++v) {
     const int64_t r = r0 + wm * 32 + 8 * (v / 4) + 4 * (lane >> 5) + v % 4;
     if (r >= rows) continue;
+    if (p.pieces > 1) {
+      p.part[((int64_t)piece * rows + r) * cols + n] = acc[v];
+      continue;
+    }
     const float z = acc[v] + bias;
     if (p.pre) gst<T>((T*)p.pre, r * cols + n, z);
     float y = activate(z, p.act);
@@ -101,60 +128,239 @@ using dense::Operand;
 template <int MODE, bool TAIL> using Big = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, MODE == DW, MODE != DX, TAIL>;
 template <int MODE, bool TAIL> using Small = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, MODE == DW, MODE != DX, TAIL>;
 
-// z = v + bias, out = act(z) + residual for eight columns
-__device__ __forceinline__ void finish8(const Args& p, int r, int c, float v[8]) {
-  const int64_t at = (int64_t)r * p.cols + c;
+// z = v + bias, out = act(z) + residual for eight columns; `bias` and `residual` are those eight of them
+__device__ __forceinline__ void finish8(const Args& p, int act, int64_t at, float v[8], const float bias[8],
+                                        const uint16_t* residual) {
   if (p.bias) {
-    float b[8];
-    ld8((const uint16_t*)p.bias, c, b);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] += b[q];
+    for (int q = 0; q < 8; ++q) v[q] += bias[q];
   }
   if (p.pre) dense::store8((uint16_t*)p.pre + at, v);
-  if (p.act != MTX_ACT_NONE) {
+  if (act != MTX_ACT_NONE) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = activate(v[q], p.act);
+    for (int q = 0; q < 8; ++q) v[q] = activate_fast(v[q], act);
   }
   if (p.residual) {
     float b[8];
-    ld8((const uint16_t*)p.residual, at, b);
+    ld8(residual, 0, b);
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] += b[q];
   }
   dense::store8((uint16_t*)p.out + at, v);
 }
+__device__ __forceinline__ void finish8(const Args& p, int r, int c, float v[8]) {
+  const int64_t at = (int64_t)r * p.cols + c;
+  float bias[8];
+  if (p.bias) ld8((const uint16_t*)p.bias, c, bias);
+  finish8(p, p.act, at, v, bias, (const uint16_t*)p.residual + at);
+}
 
 // Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2.
 constexpr int kGroup = 8;
-template <class T, int MODE>
+template <class T, int MODE, int ACT>
 __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void tile_kernel(Args p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
   const int nm = (p.rows + T::BM - 1) / T::BM, nn = (p.cols + T::BN - 1) / T::BN;
-  const int t = dense::tile_of(blockIdx.x, nm * nn);
-  if (t < 0) return;
+  const int id = dense::tile_of(blockIdx.x, nm * nn * p.pieces);
+  if (id < 0) return;
+  const int t = id / p.pieces, piece = id % p.pieces, stages = (p.red + dense::BKS - 1) / dense::BKS;
+  const int k0 = (int)((int64_t)piece * stages / p.pieces) * dense::BKS;
+  const int k1 = min((int)((int64_t)(piece + 1) * stages / p.pieces) * dense::BKS, p.red);
   const int g = t / (kGroup * nn), gs = min(kGroup, nm - g * kGroup), in = t - g * kGroup * nn;
   const int m0 = (g * kGroup + in % gs) * T::BM, n0 = in / gs * T::BN;
   const uint16_t *a = (const uint16_t*)p.a, *b = (const uint16_t*)p.b;
-  const uint16_t* pa = MODE == DW ? a + m0 : a + (int64_t)m0 * p.red;
-  const uint16_t* pb = MODE == DX ? b + (int64_t)n0 * p.red : b + n0;
+  const uint16_t* pa = MODE == DW ? a + (int64_t)k0 * p.rows + m0 : a + (int64_t)m0 * p.red + k0;
+  const uint16_t* pb = MODE == DX ? b + (int64_t)n0 * p.red + k0 : b + (int64_t)k0 * p.cols + n0;
   const Operand oa{{pa, pa}, MODE == DW ? p.rows : p.red, p.rows - m0};
   const Operand ob{{pb, pb}, MODE == DX ? p.red : p.cols, p.cols - n0};
   dense::f32x16 acc[T::TM][T::TN];
-  T::product(oa, ob, p.red, lds, acc);
+  T::product(oa, ob, k1 - k0, lds, acc);
   __syncthreads();
   const int wave = threadIdx.x >> 6;
   char* mine = T::out_lds(lds);
   const int wr = m0 + (wave / T::WN) * (T::TM * 32), c = n0 + (wave % T::WN) * (T::TN * 32) + T::out_col(0);
+  if (T::BM == 128 && p.pieces > 1) {
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+      T::put(acc[i], mine);
+#pragma unroll
+      for (int it = 0; it < T::OUT_STEPS; ++it) {
+        const int r = wr + i * 32 + T::out_row(it);
+        float v[8];
+        T::get(mine, it, v);
+        if (r < p.rows && c < p.cols) st8(p.part + ((int64_t)piece * p.rows + r) * p.cols + c, 0, v);
+      }
+    }
+    return;
+  }
+  float bias[8];
+  if (p.bias) ld8((const uint16_t*)p.bias, min(c, p.cols - 8), bias);
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
+    // the residuals of 32 rows are on their way while the rows go through LDS
+    dense::u32x4 res[T::OUT_STEPS];
+    if (p.residual) {
+#pragma unroll
+      for (int it = 0; it < T::OUT_STEPS; ++it) {
+        const int r = min(wr + i * 32 + T::out_row(it), p.rows - 1);
+        res[it] = *(const dense::u32x4*)((const uint16_t*)p.residual + (int64_t)r * p.cols + min(c, p.cols - 8));
+      }
+    }
     T::put(acc[i], mine);
-#pragma unroll 2
+#pragma unroll
     for (int it = 0; it < T::OUT_STEPS; ++it) {
       const int r = wr + i * 32 + T::out_row(it);
       float v[8];
       T::get(mine, it, v);
-      if (r < p.rows && c < p.cols) finish8(p, r, c, v);
+      if (r < p.rows && c < p.cols) finish8(p, ACT, (int64_t)r * p.cols + c, v, bias, (const uint16_t*)&res[it]);
     }
+  }
+}
+
+// ---- few rows (serving): the time is that of reading w once ---------------------------------------------------------
+// A workgroup owns 128 columns and a piece of the reduction; its waves (eight, or four where 64 rows need the registers) take the piece's 32-element chunks in turn,
+// w straight from memory into registers (two chunks of 8 KB a wave in flight), turned into MFMA operands by byte
+// permutes, 16 rows of x a block.  The waves' sums are added in wave order, the pieces' by finish_kernel in piece order.
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+template <int J>
+__device__ __forceinline__ bf16x8 column(const u32x4 (&in)[8]) {
+  constexpr uint32_t sel = (J & 1) ? 0x07060302u : 0x05040100u;
+  u32x4 v;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = __builtin_amdgcn_perm(in[2 * q + 1][J / 2], in[2 * q][J / 2], sel);
+  return __builtin_bit_cast(bf16x8, v);
+}
+constexpr int kThinCols = 128, kThinChunk = 32;
+// TB: blocks of 16 rows; NW: waves; STREAM: loads of w that leave no copy in the memory-side cache
+template <int TB, int NW, bool STREAM>
+__global__ __launch_bounds__(NW * 64) void thin_kernel(Args p) {
+  constexpr int PADN = kThinCols + 4, kThinWaves = NW;
+  __shared__ __attribute__((aligned(16))) float part[kThinWaves][16][PADN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nn = (p.cols + kThinCols - 1) / kThinCols, nt = blockIdx.x % nn, piece = blockIdx.x / nn;
+  const int chunks = (p.red + kThinChunk - 1) / kThinChunk;
+  const int c0 = (int)((int64_t)piece * chunks / p.pieces), c1 = (int)((int64_t)(piece + 1) * chunks / p.pieces);
+  const int l16 = lane & 15, kq = lane >> 4, nb = (p.rows + 15) >> 4;
+  const int col = min(nt * kThinCols + l16 * 8, p.cols - 8);  // past the end: the last columns again, not stored
+  const uint16_t* W = (const uint16_t*)p.b + col;
+  const uint16_t* x[TB];
+#pragma unroll
+  for (int b = 0; b < TB; ++b) x[b] = (const uint16_t*)p.a + (int64_t)min(b * 16 + l16, p.rows - 1) * p.red;
+  struct Chunk {
+    u32x4 w[8];
+    u32x4 x[TB];
+  };
+  auto load = [&](Chunk& c, int ck) {
+    const int k = min(ck * kThinChunk + kq * 8, p.red - 8);  // past the end: re-read, zeroed in both operands
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const u32x4* q = (const u32x4*)(W + (int64_t)(k + i) * p.cols);
+      c.w[i] = STREAM ? __builtin_nontemporal_load(q) : *q;
+    }
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+      if (b < nb) c.x[b] = *(const u32x4*)(x[b] + k);
+  };
+  f32x4 acc[8][TB];
+#pragma unroll
+  for (int f = 0; f < 8; ++f)
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[f][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto use = [&](Chunk& c, int ck) {
+    if (ck * kThinChunk + kThinChunk > p.red) {
+      const uint32_t keep = ck * kThinChunk + kq * 8 < p.red ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c.w[i] &= keep;
+#pragma unroll
+      for (int b = 0; b < TB; ++b) c.x[b] &= keep;
+    }
+    const bf16x8 wf[8] = {column<0>(c.w), column<1>(c.w), column<2>(c.w), column<3>(c.w),
+                          column<4>(c.w), column<5>(c.w), column<6>(c.w), column<7>(c.w)};
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+      if (b >= nb) continue;
+      const bf16x8 xf = __builtin_bit_cast(bf16x8, c.x[b]);
+#pragma unroll
+      for (int f = 0; f < 8; ++f) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[f], xf, acc[f][b], 0, 0, 0);
+    }
+  };
+  {
+    Chunk a, b;
+#pragma unroll
+    for (int i = 0; i < TB; ++i) a.x[i] = b.x[i] = u32x4{0u, 0u, 0u, 0u};
+    int ck = c0 + wave;
+    if (ck < c1) load(a, ck);
+    for (; ck + 2 * kThinWaves < c1; ck += 2 * kThinWaves) {
+      load(b, ck + kThinWaves);
+      use(a, ck);
+      load(a, ck + 2 * kThinWaves);
+      use(b, ck + kThinWaves);
+    }
+    if (ck + kThinWaves < c1) {
+      load(b, ck + kThinWaves);
+      use(a, ck);
+      use(b, ck + kThinWaves);
+    } else if (ck < c1) {
+      use(a, ck);
+    }
+  }
+  // acc[f][b][r] of lane l: row 16 b + l % 16, column 8 (4 (l / 16) + r) + f of the workgroup's
+#pragma unroll
+  for (int b = 0; b < TB; ++b) {
+    if (b >= nb) break;
+    if (b > 0) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float* o = &part[wave][l16][8 * (4 * kq + r)];
+      *(f32x4*)o = f32x4{acc[0][b][r], acc[1][b][r], acc[2][b][r], acc[3][b][r]};
+      *(f32x4*)(o + 4) = f32x4{acc[4][b][r], acc[5][b][r], acc[6][b][r], acc[7][b][r]};
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * kThinCols / 8; i += kThinWaves * 64) {
+      const int row = i / (kThinCols / 8), c = i % (kThinCols / 8) * 8;
+      const int r = b * 16 + row, oc = nt * kThinCols + c;
+      if (r >= p.rows || oc >= p.cols) continue;
+      float v[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x4 s = *(const f32x4*)&part[0][row][c + 4 * h];
+#pragma unroll
+        for (int w = 1; w < kThinWaves; ++w) s += *(const f32x4*)&part[w][row][c + 4 * h];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[4 * h + q] = s[q];
+      }
+      if (p.pieces > 1) st8(p.part + ((int64_t)piece * p.rows + r) * p.cols + oc, 0, v);
+      else finish8(p, r, oc, v);
+    }
+  }
+}
+
+// The pieces' sums in piece order, and the epilogue.  V: columns a thread.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void finish_kernel(Args p) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, n = (int64_t)p.rows * p.cols;
+  if (i >= n) return;
+  float v[V];
+  if constexpr (V == 8) {
+    ld8(p.part, i, v);
+    for (int s = 1; s < p.pieces; ++s) {
+      float w[8];
+      ld8(p.part + s * n, i, w);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += w[q];
+    }
+    finish8(p, (int)(i / p.cols), (int)(i % p.cols), v);
+  } else {
+    float z = p.part[i];
+    for (int s = 1; s < p.pieces; ++s) z += p.part[s * n + i];
+    const int64_t c = i % p.cols;
+    if (p.bias) z += gld<T>((const T*)p.bias, c);
+    if (p.pre) gst<T>((T*)p.pre, i, z);
+    float y = activate(z, p.act);
+    if (p.residual) y += gld<T>((const T*)p.residual, i);
+    gst<T>((T*)p.out, i, y);
   }
 }
 
@@ -206,13 +412,22 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
     part[(int64_t)blockIdx.y * N + col] = t;
   }
 }
+// 32 columns and eight sums of every eighth range each (73 ranges of 7168 columns: 19 us with a thread a column)
 template <typename T>
 __global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ part, int n, int64_t N,
                                                          T* __restrict__ out) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= N) return;
+  __shared__ float s[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + tx;
   float t = 0.0f;
-  for (int i = 0; i < n; ++i) t += part[(int64_t)i * N + c];
+  if (c < N) {
+#pragma unroll 4
+    for (int i = ty; i < n; i += 8) t += part[(int64_t)i * N + c];
+  }
+  s[ty][tx] = t;
+  __syncthreads();
+  if (ty > 0 || c >= N) return;
+  for (int y = 1; y < 8; ++y) t += s[y][tx];
   gst<T>(out, c, t);
 }
 
@@ -222,23 +437,6 @@ static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 static int64_t slope_ranges(int64_t M, int64_t N) {
   const int64_t by_cols = ceil_div(N, 256);
   return std::max<int64_t>(1, std::min<int64_t>(ceil_div(M, 4 * kSlopeRows), 2048 / std::max<int64_t>(1, by_cols)));
-}
-
-template <typename T, int MODE>
-static int launch_f32(const Args& p, hipStream_t st) {
-  const dim3 grid((unsigned)ceil_div(p.cols, 64), (unsigned)ceil_div(p.rows, 64));
-  if (grid.y > 65535) return MTX_ERR_UNSUPPORTED;
-  // the operands' row lengths
-  const int la = MODE == DW ? p.rows : p.red, lb = MODE == DX ? p.red : p.cols;
-  const bool vec = std::is_same<T, float>::value && la % 4 == 0 && lb % 4 == 0 && aligned16(p.a) && aligned16(p.b);
-  if constexpr (std::is_same<T, float>::value) {
-    if (vec) {
-      hipLaunchKernelGGL((f32_kernel<T, MODE, 4>), grid, dim3(f32mm::NT), 0, st, p);
-      return check_launch();
-    }
-  }
-  hipLaunchKernelGGL((f32_kernel<T, MODE, 1>), grid, dim3(f32mm::NT), 0, st, p);
-  return check_launch();
 }
 
 static int check_sizes(int dtype, int64_t M, int64_t K, int64_t N) {
@@ -256,31 +454,111 @@ static bool takes_tiles(int mode, const Args& p) {
          aligned16(p.out) && aligned16(p.bias) && aligned16(p.residual) && aligned16(p.pre);
 }
 
-template <int MODE, bool TAIL>
-static int launch_tiles(const Args& p, hipStream_t st) {
-  auto tiles = [&](int b) { return ceil_div(p.rows, b) * ceil_div(p.cols, b); };
-  if (tiles(256) >= 192)
-    hipLaunchKernelGGL((tile_kernel<Big<MODE, TAIL>, MODE>), dim3((unsigned)dense::tiles_grid(tiles(256))), dim3(256), 0, st,
-                       p);
-  else
-    hipLaunchKernelGGL((tile_kernel<Small<MODE, TAIL>, MODE>), dim3((unsigned)dense::tiles_grid(tiles(128))), dim3(256), 0,
-                       st, p);
+// How a product runs, by its sizes alone, and in how many pieces of its reduction.
+enum { PATH_F32, PATH_BIG, PATH_SMALL, PATH_THIN };
+struct Plan {
+  int path, pieces;
+};
+constexpr int kThinRows = 64;
+static Plan plan(int mode, bool tiles, int64_t rows, int64_t cols, int64_t red) {
+  auto count = [&](int64_t b) { return ceil_div(rows, b) * ceil_div(cols, b); };
+  const int64_t stages = ceil_div(red, 32);
+  // pieces that bring `n` workgroups to `want`, of `least` stages or more
+  auto split = [&](int64_t n, int64_t want, int64_t least) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / n, stages / least), 32));
+  };
+  if (!tiles) return {PATH_F32, split(count(64), 512, 8)};
+  if (mode == FWD && rows <= kThinRows) return {PATH_THIN, split(ceil_div(cols, kThinCols), 256, 16)};
+  if (count(256) >= 192) return {PATH_BIG, 1};
+  return {PATH_SMALL, split(count(128), 512, 16)};
+}
+static int64_t part_bytes(int64_t rows, int64_t cols, int64_t red, int mode) {
+  int64_t b = 0;
+  if (rows > 0 && cols > 0)
+    for (const bool tiles : {false, true}) {
+      const Plan p = plan(mode, tiles, rows, cols, red);
+      if (p.pieces > 1) b = std::max<int64_t>(b, p.pieces * rows * cols * 4);
+    }
+  return b;
+}
+
+template <typename T, int MODE>
+static int launch_f32(const Args& p, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div(p.cols, 64), (unsigned)ceil_div(p.rows, 64), (unsigned)p.pieces);
+  if (grid.y > 65535) return MTX_ERR_UNSUPPORTED;
+  // the operands' row lengths
+  const int la = MODE == DW ? p.rows : p.red, lb = MODE == DX ? p.red : p.cols;
+  const bool vec = std::is_same<T, float>::value && la % 4 == 0 && lb % 4 == 0 && aligned16(p.a) && aligned16(p.b);
+  if constexpr (std::is_same<T, float>::value) {
+    if (vec) {
+      hipLaunchKernelGGL((f32_kernel<T, MODE, 4>), grid, dim3(f32mm::NT), 0, st, p);
+      return check_launch();
+    }
+  }
+  hipLaunchKernelGGL((f32_kernel<T, MODE, 1>), grid, dim3(f32mm::NT), 0, st, p);
+  return check_launch();
+}
+
+template <int MODE, bool TAIL, int ACT>
+static int launch_tiles(const Args& p, bool big, hipStream_t st) {
+  auto grid = [&](int b) {
+    return dim3((unsigned)dense::tiles_grid(ceil_div(p.rows, b) * ceil_div(p.cols, b) * p.pieces));
+  };
+  if (big) hipLaunchKernelGGL((tile_kernel<Big<MODE, TAIL>, MODE, ACT>), grid(256), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((tile_kernel<Small<MODE, TAIL>, MODE, ACT>), grid(128), dim3(256), 0, st, p);
   return check_launch();
 }
 template <int MODE>
-static int launch_tiles(const Args& p, hipStream_t st) {
-  return p.red % dense::BKS ? launch_tiles<MODE, true>(p, st) : launch_tiles<MODE, false>(p, st);
+static int launch_mode(const Args& p, int path, int dtype, hipStream_t st) {
+  if (path == PATH_F32) return dtype == MTX_F32 ? launch_f32<float, MODE>(p, st) : launch_f32<uint16_t, MODE>(p, st);
+  if (path == PATH_THIN) {
+    const dim3 grid((unsigned)(ceil_div(p.cols, kThinCols) * p.pieces));
+    // half the memory-side cache or more: nothing of w is found there again by the time it is next used
+    const bool stream = (int64_t)p.red * p.cols * 2 >= (int64_t)128 << 20;
+#define MTX_THIN(TB, NW)                                                                                      \
+  do {                                                                                                        \
+    if (stream) hipLaunchKernelGGL((thin_kernel<TB, NW, true>), grid, dim3(NW * 64), 0, st, p);               \
+    else hipLaunchKernelGGL((thin_kernel<TB, NW, false>), grid, dim3(NW * 64), 0, st, p);                     \
+  } while (0)
+    if (p.rows <= 16) MTX_THIN(1, 8);
+    else if (p.rows <= 32) MTX_THIN(2, 8);
+    else MTX_THIN(4, 4);
+#undef MTX_THIN
+    return check_launch();
+  }
+  const bool big = path == PATH_BIG;
+#define MTX_TILES(ACT) \
+  return p.red % dense::BKS ? launch_tiles<MODE, true, ACT>(p, big, st) : launch_tiles<MODE, false, ACT>(p, big, st)
+  if constexpr (MODE == FWD) {
+    // the activation is applied where the reduction is whole: by finish_kernel if it is in pieces
+    switch (p.pieces > 1 ? MTX_ACT_NONE : p.act) {
+      case MTX_ACT_RELU: MTX_TILES(MTX_ACT_RELU);
+      case MTX_ACT_SILU: MTX_TILES(MTX_ACT_SILU);
+      case MTX_ACT_GELU: MTX_TILES(MTX_ACT_GELU);
+      case MTX_ACT_GELU_TANH: MTX_TILES(MTX_ACT_GELU_TANH);
+    }
+  }
+  MTX_TILES(MTX_ACT_NONE);
+#undef MTX_TILES
 }
 
-static int launch_product(int mode, const Args& p, int dtype, hipStream_t st) {
+static int launch_product(int mode, Args p, int dtype, void* ws, hipStream_t st) {
   if (p.rows == 0 || p.cols == 0) return MTX_OK;
   if (!p.out || (p.red > 0 && (!p.a || !p.b))) return MTX_ERR_ARG;
-  if (dtype == MTX_BF16 && takes_tiles(mode, p))
-    return mode == FWD ? launch_tiles<FWD>(p, st) : mode == DX ? launch_tiles<DX>(p, st) : launch_tiles<DW>(p, st);
-#define MTX_F32_MODE(T) \
-  (mode == FWD ? launch_f32<T, FWD>(p, st) : mode == DX ? launch_f32<T, DX>(p, st) : launch_f32<T, DW>(p, st))
-  return dtype == MTX_F32 ? MTX_F32_MODE(float) : MTX_F32_MODE(uint16_t);
-#undef MTX_F32_MODE
+  const bool tiles = dtype == MTX_BF16 && takes_tiles(mode, p);
+  const Plan how = plan(mode, tiles, p.rows, p.cols, p.red);
+  p.pieces = how.pieces;
+  p.part = (float*)ws;
+  if (p.pieces > 1 && (!ws || !aligned16(ws))) return MTX_ERR_WORKSPACE;
+  const int rc = mode == FWD ? launch_mode<FWD>(p, how.path, dtype, st)
+                 : mode == DX ? launch_mode<DX>(p, how.path, dtype, st) : launch_mode<DW>(p, how.path, dtype, st);
+  if (rc != MTX_OK || p.pieces == 1) return rc;
+  const int64_t n = (int64_t)p.rows * p.cols;
+  if (tiles) hipLaunchKernelGGL((finish_kernel<uint16_t, 8>), dim3((unsigned)ceil_div(n, 2048)), dim3(256), 0, st, p);
+  else if (dtype == MTX_F32)
+    hipLaunchKernelGGL((finish_kernel<float, 1>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((finish_kernel<uint16_t, 1>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, p);
+  return check_launch();
 }
 
 }  // namespace lin
@@ -290,7 +568,10 @@ using namespace mtx;
 
 extern "C" int64_t mtx_linear_workspace_size(int64_t M, int64_t K, int64_t N) {
   if (M < 0 || K < 0 || N < 0) return -1;
-  return lin::slope_ranges(M, N) * N * 4;
+  int64_t b = lin::slope_ranges(M, N) * N * 4;
+  b = std::max(b, lin::part_bytes(M, N, K, lin::FWD));
+  b = std::max(b, lin::part_bytes(M, K, N, lin::DX));
+  return std::max(b, lin::part_bytes(K, N, M, lin::DW));
 }
 
 extern "C" int mtx_linear(const void* x, const void* w, const void* bias, const void* residual, int dtype, int64_t M,
@@ -300,37 +581,13 @@ extern "C" int mtx_linear(const void* x, const void* w, const void* bias, const 
   if (rc != MTX_OK) return rc;
   if (act < MTX_ACT_NONE || act > MTX_ACT_GELU_TANH) return MTX_ERR_ARG;
   if (workspace_bytes < mtx_linear_workspace_size(M, K, N)) return MTX_ERR_WORKSPACE;
-  const lin::Args p{x, w, out, bias, residual, pre, act, (int)M, (int)N, (int)K};
-  return lin::launch_product(lin::FWD, p, dtype, (hipStream_t)stream);
+  const lin::Args p{x, w, out, bias, residual, pre, act, (int)M, (int)N, (int)K, 1, nullptr};
+  return lin::launch_product(lin::FWD, p, dtype, workspace, (hipStream_t)stream);
 }
 
-extern "C" int mtx_linear_dx(const void* dz, const void* w, int dtype, int64_t M, int64_t K, int64_t N, void* dx,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
-  const int rc = lin::check_sizes(dtype, M, K, N);
-  if (rc != MTX_OK) return rc;
-  if (workspace_bytes < mtx_linear_workspace_size(M, K, N)) return MTX_ERR_WORKSPACE;
-  const lin::Args p{dz, w, dx, nullptr, nullptr, nullptr, MTX_ACT_NONE, (int)M, (int)K, (int)N};
-  return lin::launch_product(lin::DX, p, dtype, (hipStream_t)stream);
-}
-
-extern "C" int mtx_linear_dw(const void* x, const void* dz, int dtype, int64_t M, int64_t K, int64_t N, void* dw,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
-  const int rc = lin::check_sizes(dtype, M, K, N);
-  if (rc != MTX_OK) return rc;
-  if (workspace_bytes < mtx_linear_workspace_size(M, K, N)) return MTX_ERR_WORKSPACE;
-  const lin::Args p{x, dz, dw, nullptr, nullptr, nullptr, MTX_ACT_NONE, (int)K, (int)N, (int)M};
-  return lin::launch_product(lin::DW, p, dtype, (hipStream_t)stream);
-}
-
-extern "C" int mtx_linear_act_bwd(const void* dy, const void* pre, int dtype, int64_t M, int64_t N, int act, void* dz,
-                                  void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
-  const int rc = lin::check_sizes(dtype, M, 0, N);
-  if (rc != MTX_OK) return rc;
-  if (act < MTX_ACT_NONE || act > MTX_ACT_GELU_TANH) return MTX_ERR_ARG;
-  if (workspace_bytes < mtx_linear_workspace_size(M, 0, N) || (dbias && N > 0 && !workspace)) return MTX_ERR_WORKSPACE;
-  if (N == 0 || (act == MTX_ACT_NONE && !dbias)) return MTX_OK;
-  if (M > 0 && (!dy || (act != MTX_ACT_NONE && (!pre || !dz)))) return MTX_ERR_ARG;
-  hipStream_t st = (hipStream_t)stream;
+// dz and the column sums of dz; dz is dy where there is no activation.
+static int launch_slope(const void* dy, const void* pre, int dtype, int64_t M, int64_t N, int act, void* dz, void* dbias,
+                        void* workspace, hipStream_t st) {
   const int64_t ranges = lin::slope_ranges(M, N);
   const int64_t range = round_up(ceil_div(M, ranges), lin::kSlopeRows);
   float* part = dbias ? (float*)workspace : nullptr;
@@ -346,12 +603,39 @@ extern "C" int mtx_linear_act_bwd(const void* dy, const void* pre, int dtype, in
     else MTX_SLOPE(uint16_t, 1);
   }
 #undef MTX_SLOPE
-  const int e = check_launch();
-  if (e != MTX_OK || !dbias) return e;
-  const dim3 grid((unsigned)ceil_div(N, 256));
-  if (dtype == MTX_F32)
-    hipLaunchKernelGGL(lin::column_sum_kernel<float>, grid, dim3(256), 0, st, part, (int)ranges, N, (float*)dbias);
-  else
-    hipLaunchKernelGGL(lin::column_sum_kernel<uint16_t>, grid, dim3(256), 0, st, part, (int)ranges, N, (uint16_t*)dbias);
+  if (dbias) {
+    const dim3 grid((unsigned)ceil_div(N, 32));
+    if (dtype == MTX_F32)
+      hipLaunchKernelGGL(lin::column_sum_kernel<float>, grid, dim3(256), 0, st, part, (int)ranges, N, (float*)dbias);
+    else
+      hipLaunchKernelGGL(lin::column_sum_kernel<uint16_t>, grid, dim3(256), 0, st, part, (int)ranges, N,
+                         (uint16_t*)dbias);
+  }
   return check_launch();
+}
+
+extern "C" int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre, int dtype, int64_t M,
+                              int64_t K, int64_t N, int act, void* dz, void* dx, void* dw, void* dbias, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  int rc = lin::check_sizes(dtype, M, K, N);
+  if (rc != MTX_OK) return rc;
+  if (act < MTX_ACT_NONE || act > MTX_ACT_GELU_TANH) return MTX_ERR_ARG;
+  const bool slope = act != MTX_ACT_NONE && (dx || dw || dbias);
+  if (M > 0 && N > 0 && ((!dy && (dx || dw || dbias)) || (slope && (!pre || !dz)))) return MTX_ERR_ARG;
+  if (M > 0 && N > 0 && K > 0 && ((dx && !w) || (dw && !x))) return MTX_ERR_ARG;
+  if (workspace_bytes < mtx_linear_workspace_size(M, K, N) || (dbias && N > 0 && !workspace)) return MTX_ERR_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  if (N > 0 && (slope || dbias)) {
+    rc = launch_slope(dy, pre, dtype, M, N, act, dz, dbias, workspace, st);
+    if (rc != MTX_OK) return rc;
+  }
+  const void* g = act == MTX_ACT_NONE ? dy : dz;
+  if (dx) {
+    const lin::Args p{g, w, dx, nullptr, nullptr, nullptr, MTX_ACT_NONE, (int)M, (int)K, (int)N, 1, nullptr};
+    rc = lin::launch_product(lin::DX, p, dtype, workspace, st);
+    if (rc != MTX_OK) return rc;
+  }
+  if (!dw) return MTX_OK;
+  const lin::Args p{x, g, dw, nullptr, nullptr, nullptr, MTX_ACT_NONE, (int)K, (int)N, (int)M, 1, nullptr};
+  return lin::launch_product(lin::DW, p, dtype, workspace, st);
 }

@@ -78,23 +78,15 @@ class _Linear(torch.autograd.Function):
         dev = L.require_device(x, weight, dy)
         x, weight, dy = x.contiguous(), weight.contiguous(), dy.contiguous()
         M, K, N = _sizes(x, weight)
-        code, act = L.dtype_code(x.dtype), ctx.act
+        act = ctx.act
+        dz = torch.empty((M, N), dtype=x.dtype, device=dev) if act and (need_x or need_w or need_b) else None
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
         ws = _workspace(M, K, N, dev)
-        dx = dw = db = None
-        dz = dy
         with L.on_device(dev):
-            st = L.stream(dev)
-            if need_b or (act and (need_x or need_w)):
-                dz = torch.empty((M, N), dtype=x.dtype, device=dev) if act else dy
-                db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
-                L.call("mtx_linear_act_bwd", L.ptr(dy), L.ptr(pre), code, M, N, act, L.ptr(dz if act else None), L.ptr(db),
-                       L.ptr(ws), ws.numel(), st)
-            if need_x:
-                dx = torch.empty_like(x)
-                L.call("mtx_linear_dx", L.ptr(dz), L.ptr(weight), code, M, K, N, L.ptr(dx), L.ptr(ws), ws.numel(), st)
-            if need_w:
-                dw = torch.empty_like(weight)
-                L.call("mtx_linear_dw", L.ptr(x), L.ptr(dz), code, M, K, N, L.ptr(dw), L.ptr(ws), ws.numel(), st)
+            L.call("mtx_linear_bwd", L.ptr(dy), L.ptr(x), L.ptr(weight), L.ptr(pre), L.dtype_code(x.dtype), M, K, N, act,
+                   L.ptr(dz), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), ws.numel(), L.stream(dev))
         return dx, dw, db, None, dy if need_r else None
 
 

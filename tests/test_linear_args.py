@@ -45,7 +45,13 @@ def test_entry_points_refuse():
     assert call(d, d, P, P, 1, 4, 8, 8, 0, P, P, d, n, P) == L.MTX_ERR_ARG       # no out
     assert call(d, d, P, P, 1, 1 << 23, 8, 8, 0, d, P, d, 1 << 40, P) == L.MTX_ERR_UNSUPPORTED
     assert call(d, d, P, P, 1, 4096, 8, 8, 0, d, P, P, 0, P) == L.MTX_ERR_WORKSPACE
-    assert lib.mtx_linear_dx(d, d, 1, 4096, 8, 8, d, P, 0, P) == L.MTX_ERR_WORKSPACE
-    assert lib.mtx_linear_dw(d, P, 1, 4, 8, 8, d, d, n, P) == L.MTX_ERR_ARG
-    assert lib.mtx_linear_act_bwd(d, P, 1, 4, 8, 2, d, d, d, n, P) == L.MTX_ERR_ARG  # an activation without z
-    assert lib.mtx_linear_act_bwd(d, P, 1, 4, 8, 9, d, d, d, n, P) == L.MTX_ERR_ARG
+    back = lambda dy, x, w, pre, act, dz, dx, dw, db, ws=d, size=n, M=4: lib.mtx_linear_bwd(
+        dy, x, w, pre, 1, M, 8, 8, act, dz, dx, dw, db, ws, size, P)
+    assert back(d, d, d, P, 0, P, d, P, P, ws=P, size=0, M=4096) == L.MTX_ERR_WORKSPACE
+    assert back(d, d, d, P, 2, d, d, d, d) == L.MTX_ERR_ARG      # an activation without z
+    assert back(d, d, d, d, 2, P, d, d, d) == L.MTX_ERR_ARG      # nowhere to write dz
+    assert back(d, d, d, d, 9, d, d, d, d) == L.MTX_ERR_ARG
+    assert back(P, d, d, P, 0, P, d, P, P) == L.MTX_ERR_ARG      # no gradient
+    assert back(d, P, d, P, 0, P, P, d, P) == L.MTX_ERR_ARG      # dw without x
+    assert back(d, d, P, P, 0, P, d, P, P) == L.MTX_ERR_ARG      # dx without w
+    assert back(d, d, d, P, 0, P, P, P, P) == L.MTX_OK           # nothing asked for
