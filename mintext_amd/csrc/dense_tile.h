@@ -18,6 +18,7 @@
 #pragma once
 #include "common.h"
 #include "lds_dma.h"
+#include <type_traits>
 
 namespace mtx {
 namespace dense {
@@ -67,12 +68,24 @@ __device__ __forceinline__ void store8(uint16_t* p, const float v[8]) {
                        (__bf16)v[4], (__bf16)v[5], (__bf16)v[6], (__bf16)v[7]};
 }
 
+// Diagonal matrices that are multiplied in beside the product: C += D B + A D', D = diag(row), D' = diag(col), for operands
+// whose reduction index is the output's row (D) or column (D') index.  Where a stage's reduction elements are a block's
+// own rows (columns), one more MFMA takes that 32 x 32 block of D in A's place (D' in B's), made in registers: what
+// an f16 matrix lost of its f32 diagonal joins the product with no access to memory.
+// CONST: D = (hi + lo) I instead, for both planes of B.
+struct Diagonal {
+  const float *row, *col;  // of the whole matrices, or nullptr
+  float hi, lo;            // CONST
+  int m0, n0, m, n;        // the tile's first row and column; rows and columns of C that exist
+};
+enum { DIAG_NONE = 0, DIAG_VECTORS = 1, DIAG_CONST = 2 };
+
 __device__ __forceinline__ int row_off(int r, int c) { return r * 64 + ((c ^ ((r >> 2) & 3)) << 4); }
 template <int COLS>
 __device__ __forceinline__ int col_off(int k, int c) { return k * (COLS * 2) + ((c ^ ((k & 3) << 2)) << 4); }
 
 template <class F, int TM_, int TN_, int WM_, int WN_, int NST_, bool A_COLS, bool B_COLS, bool TAIL = false,
-          bool TWO = false>
+          bool TWO = false, int DIAG = DIAG_NONE>
 struct Tile {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NST = NST_, PD = NST - 1;
   static constexpr int NW = WM * WN, NT = NW * 64, BM = 32 * TM * WM, BN = 32 * TN * WN;
@@ -104,7 +117,7 @@ struct Tile {
   // acc = the product over reduction elements [0, K) (K > 0; without TAIL a multiple of 32, with it a multiple of 8
   // where an operand has it contiguous).  Ends with no load in flight, but the waves not in step.
   static __device__ __forceinline__ void product(const Operand& a, const Operand& b, int K, char* lds,
-                                                 f32x16 (&acc)[TM][TN]) {
+                                                 f32x16 (&acc)[TM][TN], const Diagonal* dg = nullptr) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / WN, wn = wave % WN;
     const int nk1 = (K + BKS - 1) / BKS, nk = TWO ? 3 * nk1 : nk1;
@@ -204,6 +217,69 @@ struct Tile {
 #pragma unroll
         for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
 
+    // the lane's elements of the diagonals: row or column lane % 32 of each block
+    float drow[DIAG == DIAG_VECTORS ? TM : 1], dcol[DIAG == DIAG_VECTORS ? TN : 1];
+    const int row0 = DIAG ? __builtin_amdgcn_readfirstlane(dg->m0 + wm * (TM * 32)) : 0;
+    const int col0 = DIAG ? __builtin_amdgcn_readfirstlane(dg->n0 + wn * (TN * 32)) : 0;
+    bool has_row = DIAG == DIAG_CONST, has_col = false;
+    if constexpr (DIAG == DIAG_VECTORS) {
+      has_row = dg->row != nullptr;
+      has_col = dg->col != nullptr;
+      if (has_row) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) drow[i] = row0 + i * 32 + frow < dg->m ? dg->row[row0 + i * 32 + frow] : 0.0f;
+      }
+      if (has_col) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) dcol[j] = col0 + j * 32 + frow < dg->n ? dg->col[col0 + j * 32 + frow] : 0.0f;
+      }
+    }
+    // substep `sub` of the 32 x 32 diagonal block with v in the lane's row
+    auto diagonal = [&](float v, int sub) -> x8 {
+      const typename F::elem e = (typename F::elem)v;
+      const int at = frow - sub * 16 - 8 * fhalf;
+      x8 d;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) d[q] = q == at ? e : (typename F::elem)0.0f;
+      return d;
+    };
+    auto diagonals = [&](int kt, int sub) {
+      const int part = TWO ? kt % 3 : 0, k = (TWO ? kt / 3 : kt) * BKS;
+      if constexpr (DIAG == DIAG_CONST) {
+        if (part == 2 || k < row0 || k >= row0 + TM * 32) return;
+        const x8 hi = diagonal(dg->hi, sub), lo = diagonal(dg->lo, sub);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if (k != row0 + i * 32) continue;
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            acc[i][j] = F::mfma(fb[sub][j], hi, acc[i][j]);
+            if (part == 0) acc[i][j] = F::mfma(fb[sub][j], lo, acc[i][j]);
+          }
+        }
+      } else if constexpr (DIAG == DIAG_VECTORS) {
+        if (part != 0) return;
+        if (has_row && k >= row0 && k < row0 + TM * 32) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            if (k != row0 + i * 32) continue;
+            const x8 d = diagonal(drow[i], sub);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = F::mfma(fb[sub][j], d, acc[i][j]);
+          }
+        }
+        if (has_col && k >= col0 && k < col0 + TN * 32) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            if (k != col0 + j * 32) continue;
+            const x8 d = diagonal(dcol[j], sub);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) acc[i][j] = F::mfma(d, fa[sub][i], acc[i][j]);
+          }
+        }
+      }
+    };
+
     // prologue: stages 0 .. PD-1 in flight, stage 0 landed and visible
 #pragma unroll
     for (int s = 0; s < PD; ++s) {
@@ -218,17 +294,13 @@ struct Tile {
     // A stage is 2 x S slots in a fixed order: one MFMA, one fragment read of the other buffer, and the stage's
     // ring loads spread evenly, so that a SIMD's MFMA pipe is not held up by a burst of loads.
     constexpr int S = TM * TN;
-    for (int kt = 0; kt < nk; ++kt) {
+    auto half = [&](auto which, int kt) {
+      constexpr int sub = decltype(which)::value;
+      if (TAIL && kt == nk - 1 && tail < BKS) mask(sub, sub);
+      if constexpr (DIAG != DIAG_NONE) diagonals(kt, sub);
 #pragma unroll
-      for (int q = 0; q < 2 * S; ++q) {
-        const int sub = q / S, qq = q % S, i = qq / TN, j = qq % TN;
-        if (q == S && kt == 0) {
-          // stage 1 landed and visible before its first fragment reads below
-          __builtin_amdgcn_sched_barrier(0);
-          __builtin_amdgcn_s_waitcnt(MTX_VMCNT(LPS * (PD - 2) + LPS / 2));
-          __builtin_amdgcn_s_barrier();
-        }
-        if (TAIL && qq == 0 && kt == nk - 1 && tail < BKS) mask(sub, sub);
+      for (int qq = 0; qq < S; ++qq) {
+        const int i = qq / TN, j = qq % TN;
         __builtin_amdgcn_sched_barrier(0);
         acc[i][j] = F::mfma(fb[sub][j], fa[sub][i], acc[i][j]);
         // a substep with fewer MFMAs than fragments reads the rest in its last slot
@@ -240,8 +312,18 @@ struct Tile {
         }
 #pragma unroll
         for (int d = 0; d < LPS; ++d)
-          if ((d * 2 * S) / LPS == q) issue(kt + PD, d);
+          if ((d * 2 * S) / LPS == sub * S + qq) issue(kt + PD, d);
       }
+    };
+    for (int kt = 0; kt < nk; ++kt) {
+      half(std::integral_constant<int, 0>(), kt);
+      if (kt == 0) {
+        // stage 1 landed and visible before its first fragment reads below
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(MTX_VMCNT(LPS * (PD - 2) + LPS / 2));
+        __builtin_amdgcn_s_barrier();
+      }
+      half(std::integral_constant<int, 1>(), kt);
       advance();
       __builtin_amdgcn_sched_barrier(0);
       // Stage kt + 2 landed before the barrier makes it visible.  A bare s_barrier: the slot refilled next held
@@ -268,6 +350,13 @@ struct Tile {
             f32x4{acc[j][4 * g], acc[j][4 * g + 1], acc[j][4 * g + 2], acc[j][4 * g + 3]};
     __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
     asm volatile("" ::: "memory");
+  }
+  // The same for results in 16 bits: 32 rows of TN * 64 bytes, 16-byte chunk c of row r at c ^ (r % chunks).
+  static constexpr int OUT16_BYTES = 32 * TN * 64;  // of a wave and plane
+  static __device__ __forceinline__ int out16_off(int r, int c) { return r * (TN * 64) + ((c ^ (r & (TN * 4 - 1))) << 4); }
+  static __device__ __forceinline__ s16x4 out16_tr(const char* mine, int r, int c) {  // four rows from r of column ..
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(mine + out16_off(r, c >> 3) + (c & 7) * 2));
   }
   static constexpr int OUT_STEPS = TN * 2;  // of 64 lanes x 8 columns; a lane's columns are the same in each
   static_assert(64 % (TN * 4) == 0, "whole rows a step");

@@ -16,10 +16,10 @@
 // power-of-two scale, chosen by the caller from those bounds, that puts it into f16's range: 11 bits where
 // bf16 has 8, at the same matrix-core rate ("half").  f32 results take two f16 planes, hi + lo, and three products for
 // one ("full": 22 bits).  Sums are f32, |x|_F is summed in f64.  Two things cost more than all other roundings and are
-// kept apart.  The diagonals of Q and P, where their size is, are f32 vectors beside the f16 matrices (rank 8: 0.28
-// instead of 0.85 % off).  And X has its lo plane in "half" too: in X <- P X the diagonal's share, in f32 on the way
-// out, takes hi + lo, as in the directions in which X is small P is a multiple of I (rank 32, 2 + 2 + 1: 0.17
-// instead of 0.63 %).  Momentum is f32.
+// kept apart.  What f16 loses of the diagonals of Q and P, where their size is, is an f32 vector beside the matrix and
+// joins each product as a diagonal matrix (rank 8: 0.28 instead of 0.85 % off).  And in "half" X has what f16
+// loses of it as 8-bit floats: in X <- P X the diagonal's share, in f32 on the way out, takes it too, as in the
+// directions in which X is small P is a multiple of I (rank 32, 2 + 2 + 1: 0.17 instead of 0.63 %).  Momentum is f32.
 #include "common.h"
 #include "dense_tile.h"
 #include "f32_tile.h"
@@ -126,15 +126,38 @@ __global__ __launch_bounds__(256) void norm_kernel(Source s, int M, int N, int r
   __syncthreads();
   if (threadIdx.x == 0) part[e * gridDim.x + blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
 }
-// X = x 2^e in f16, hi and lo planes where there are two, and what f32 holds beyond them (a bit at most: the steps carry
-// it up by a^5 where x is singular), zeros past the last row and column, with e such that |x|_F + eps
+// Eight e5m2 values (an f16 with two bits of mantissa, so of the same range) and back.
+__device__ __forceinline__ uint64_t pack8(const float v[8]) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int x = __builtin_amdgcn_cvt_pk_bf8_f32(v[4 * h], v[4 * h + 1], 0, false);
+    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(v[4 * h + 2], v[4 * h + 3], x, true);
+  }
+  return (uint64_t)w[0] | ((uint64_t)w[1] << 32);
+}
+__device__ __forceinline__ void unpack8(uint64_t p, float v[8]) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int w = (int)(p >> (32 * h));
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_bf8(w, false), b = __builtin_amdgcn_cvt_pk_f32_bf8(w, true);
+    v[4 * h] = a[0];
+    v[4 * h + 1] = a[1];
+    v[4 * h + 2] = b[0];
+    v[4 * h + 3] = b[1];
+  }
+}
+// X = x 2^e in f16; beside it either what that loses as 8-bit floats or the lo plane and what f32 holds beyond it (a bit
+// at most: the steps carry it up by a^5 where x is singular); zeros past the last row and column, with e such that |x|_F + eps
 // comes to [2^13, 2^14): a bf16 x is held exactly but for elements below 2^-27 of its norm.  Every workgroup adds the
 // parts of its matrix in the same order.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void convert_kernel(Source s, int M, int N, int Mp, int Np, int rows,
                                                       const double* __restrict__ part, int nparts, float eps,
                                                       f16* __restrict__ X, f16* __restrict__ Xlo,
-                                                      f16* __restrict__ Xrest, Scale* scales) {
+                                                      f16* __restrict__ Xrest, uint64_t* __restrict__ Xlo8,
+                                                      Scale* scales) {
   __shared__ double w[4];
   const int64_t e = blockIdx.y;
   double sum = 0.0;
@@ -165,176 +188,110 @@ __global__ __launch_bounds__(256) void convert_kernel(Source s, int M, int N, in
     }
     const int64_t at = e * Mp * (int64_t)Np + (int64_t)r * Np + c;
     *(f16x8*)(X + at) = hi;
-    if (Xlo) *(f16x8*)(Xlo + at) = lo;
-    if (Xrest) *(f16x8*)(Xrest + at) = rest;
+    if (Xlo8) {
+      float l[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) l[q] = (float)lo[q];
+      Xlo8[at / 8] = pack8(l);
+    }
+    if (Xlo) {
+      *(f16x8*)(Xlo + at) = lo;
+      *(f16x8*)(Xrest + at) = rest;
+    }
   }
 }
 
 // ---- symmetric S x S products ----------------------------------------------------------------------------------
-// out = s_acc (U V) + s_v rs V + s_u U cs + d0 I (+ diag(rs cs) where both are given), element (r, c) of V times rs[r]
-// (1 without rs) and of U times cs[c].  With `diag` the diagonal goes there and is zero in the matrix.
-// Everything in f16 carries its scale; the s_ undo them, `s_out` is out's.
+// out = s_acc (U V + diagonal terms) + d0 I.  The diagonal terms are diag(row) V + U diag(col), or w V.  With `full`,
+// the f32 diagonal goes there, in true units, and what the matrix loses of it to `rest`, in the matrix's.
 struct Sym {
   const f16 *u, *v;
   f16* out;
-  float* diag;
-  const float *rs, *cs;
-  float s_acc, s_v, s_u, d0, s_out;
+  float *full, *rest;
+  const float *row, *col;
+  float s_acc, d0, s_out;  // s_acc: everything to out's units; d0 in true units
 };
 struct SymArgs {
   Sym p[2];             // problems of one launch (the same sizes)
   int np, E, S, Sp, K;  // K: reduction
+  float w_hi, w_lo;
   int64_t ld;           // of u and v
   int64_t in_batch, in_plane, out_batch, out_plane;  // elements from matrix to matrix, and from hi to lo plane
   const Scale* scales;  // Gram product of the first X: multiplies s_acc; or nullptr
 };
 
-// Eight columns of up to NP f16 planes for each step of a wave's 32 rows, loaded together: the loads of a block of rows
-// are in flight while the one before is worked on.
-template <class T, int NP>
-struct Block {
-  f16x8 x[NP][T::OUT_STEPS];
-  // `at(it)`: offset of the lane's columns in step `it`, of an element that exists
-  template <class At>
-  __device__ __forceinline__ void load(int p, const f16* m, At at) {
-    if (!m) return;
-#pragma unroll
-    for (int it = 0; it < T::OUT_STEPS; ++it) x[p][it] = *(const f16x8*)(m + at(it));
-  }
-};
-
-// Eight f32 values as f16, and what that leaves of them.
-__device__ __forceinline__ f16x8 round8(const float y[8]) {
-  f16x8 h;
-#pragma unroll
-  for (int q = 0; q < 8; ++q) h[q] = (f16)y[q];
-  return h;
-}
-__device__ __forceinline__ f16x8 rest8(const float y[8], const f16x8& h) {
-  f16x8 l;
-#pragma unroll
-  for (int q = 0; q < 8; ++q) l[q] = (f16)(y[q] - (float)h[q]);
-  return l;
-}
-// y += k x, a single instruction an element
-__device__ __forceinline__ void add8(float y[8], const f16x8& x, float k) {
-#pragma unroll
-  for (int q = 0; q < 8; ++q) y[q] = __builtin_fmaf((float)x[q], k, y[q]);
-}
-
-// The scales are multiplied together before the elements are seen, and the diagonal is looked for only where a tile has
-// it: an epilogue of 56 instructions an element cost more than the products of 768 elements (156 us for 128
-// matrices of 768 x 768; 58 us at the matrix cores' peak).
-template <class T, bool ADD, bool TWO>
+template <class T, bool TWO>
 __device__ __forceinline__ void sym_out(const SymArgs& a, const Sym& p, int64_t e, int m0, int n0,
                                         const f32x16 (&acc)[T::TM][T::TN], char* lds) {
-  constexpr int TN = T::TN, HROW = TN * 64;  // bytes of a staged f16 row
-  constexpr int NP = TWO ? 4 : 2, AHEAD = TWO && TN == 4 ? 1 : 2;  // blocks of addends in registers
-  static_assert(T::NW * (T::OUT_BYTES + (TWO ? 2 : 1) * 32 * HROW) <= T::LDS_BYTES, "staging fits the ring");
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  char* mine = T::out_lds(lds);
-  char* turn = lds + T::NW * T::OUT_BYTES + wave * ((TWO ? 2 : 1) * 32 * HROW);
-  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c = n0 + (wave % T::WN) * (TN * 32) + T::out_col(0);
+  constexpr int TN = T::TN, PL = TWO ? 2 : 1;
+  static_assert(T::NW * PL * T::OUT16_BYTES <= T::LDS_BYTES, "staging fits the ring");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, frow = lane & 31, h = lane >> 5;
+  char* mine = lds + wave * (PL * T::OUT16_BYTES);
+  const int wr = m0 + (wave / T::WN) * (T::TM * 32), wc = n0 + (wave % T::WN) * (TN * 32);
   const int S = a.S, Sp = a.Sp;
-  const float k_acc = p.s_acc * p.s_out * (a.scales ? a.scales[e].gram : 1.0f), k_v = p.s_v * p.s_out;
+  const float k = p.s_acc * (a.scales ? a.scales[e].gram : 1.0f);
   f16* out = p.out + e * a.out_batch;
-  const f16 *u = ADD && p.cs ? p.u + e * a.in_batch : nullptr, *v = ADD ? p.v + e * a.in_batch : nullptr;
-  const float* rs = ADD && p.rs ? p.rs + e * Sp : nullptr;
-  float* diag = p.diag ? p.diag + e * Sp : nullptr;
-  float cs[8], k_u[8];
-  if (u) {
-    ld8(p.cs + e * Sp, min(c, Sp - 8), cs);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) k_u[q] = cs[q] * (p.s_u * p.s_out);
-  }
-  Block<T, NP> add[AHEAD];
-  auto ahead = [&](int i) {
-    auto at = [&](int it) { return (int64_t)min(wr + i * 32 + T::out_row(it), S - 1) * Sp + min(c, Sp - 8); };
-    Block<T, NP>& b = add[i % AHEAD];
-    b.load(0, v, at);
-    b.load(1, u, at);
-    if constexpr (TWO) {
-      b.load(2, v ? v + a.in_plane : nullptr, at);
-      b.load(3, u ? u + a.in_plane : nullptr, at);
-    }
-  };
-  if (ADD) ahead(0);
+  const bool edge = m0 + T::BM > S || n0 + T::BN > S;
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
-    if (ADD && AHEAD == 2 && i + 1 < T::TM) ahead(i + 1);
-    if (ADD && AHEAD == 1 && i > 0) ahead(i);
-    T::put(acc[i], mine);
-    const Block<T, NP>& b = add[i % AHEAD];
+    const int r = wr + i * 32 + frow;
 #pragma unroll
-    for (int it = 0; it < T::OUT_STEPS; ++it) {
-      const int lr = T::out_row(it), r = wr + i * 32 + lr;
-      const float rr = ADD && rs ? rs[min(r, S - 1)] : 1.0f;
-      float y[8];
-      T::get(mine, it, y);
+    for (int j = 0; j < TN; ++j) {
+      float y[16];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) y[q] *= k_acc;
-      if (ADD) {
-        add8(y, b.x[0][it], rr * k_v);
-        if (TWO) add8(y, b.x[TWO ? 2 : 0][it], rr * k_v);
-        if (u) {
+      for (int v = 0; v < 16; ++v) y[v] = acc[i][j][v] * k;  // column wc + 32 j + 8 (v / 4) + 4 h + v % 4
+      if (edge) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) y[q] = __builtin_fmaf((float)b.x[1][it][q], k_u[q], y[q]);
-          if (TWO) {
+        for (int v = 0; v < 16; ++v) y[v] = r < S && wc + j * 32 + 8 * (v / 4) + 4 * h + v % 4 < S ? y[v] : 0.0f;
+      }
+      static_assert(T::TM == TN, "a wave's part that the diagonal crosses has it in its blocks i = j");
+      if (i == j && wr == wc && p.full) {
+        // the lane that has the diagonal's element of its row: 8 (v / 4) + 4 h + v % 4 = r % 32
+        const int at = ((frow >> 2) & 1) == h ? (frow >> 3) * 4 + (frow & 3) : -1;
+        float d = 0.0f;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) y[q] = __builtin_fmaf((float)b.x[TWO ? 3 : 1][it][q], k_u[q], y[q]);
-          }
+        for (int v = 0; v < 16; ++v) {
+          if (v == at) d = y[v] += r < S ? p.d0 * p.s_out : 0.0f;
+        }
+        if (at >= 0 && r < Sp) {
+          const f16 hi = (f16)d, lo = (f16)(d - (float)hi);
+          p.full[e * Sp + r] = d / p.s_out;
+          p.rest[e * Sp + r] = TWO ? d - (float)hi - (float)lo : d - (float)hi;
         }
       }
-      if (m0 == n0 && ADD) {
-        const int dq = r - c;  // the diagonal's place among the lane's columns
-        if (dq >= 0 && dq < 8) {
-          float d = 0.0f;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            if (q == dq) d = y[q] + (p.d0 + (u && rs ? rr * cs[q] : 0.0f)) * p.s_out;
-          }
-          if (diag && r < Sp) diag[r] = r < S ? d / p.s_out : 0.0f;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) y[q] = q == dq ? (diag ? 0.0f : d) : y[q];
-        }
-      }
-      if (c + 8 > S) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) y[q] = c + q < S ? y[q] : 0.0f;
-      }
-      f16x8 hi = round8(y), lo;
-      if (TWO) lo = rest8(y, hi);
-      if (r < S && c < Sp) {
-        *(f16x8*)(out + (int64_t)r * Sp + c) = hi;
-        if (TWO) *(f16x8*)(out + a.out_plane + (int64_t)r * Sp + c) = lo;
-      }
-      if (m0 != n0) {
-        const uint32_t keep = r < S ? 0xFFFFFFFFu : 0u;
-        char* at = turn + lr * HROW + (((T::out_col(0) >> 3) ^ ((lr & 3) << 1)) << 4);
-        *(u32x4*)at = __builtin_bit_cast(u32x4, hi) & keep;
-        if (TWO) *(u32x4*)(at + 32 * HROW) = __builtin_bit_cast(u32x4, lo) & keep;
+      for (int g = 0; g < 4; ++g) {
+        typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+        const f16x4 hi = {(f16)y[4 * g], (f16)y[4 * g + 1], (f16)y[4 * g + 2], (f16)y[4 * g + 3]};
+        char* to = mine + T::out16_off(frow, j * 4 + g) + 8 * h;
+        *(f16x4*)to = hi;
+        if (TWO)
+          *(f16x4*)(to + T::OUT16_BYTES) =
+              f16x4{(f16)(y[4 * g] - (float)hi[0]), (f16)(y[4 * g + 1] - (float)hi[1]),
+                    (f16)(y[4 * g + 2] - (float)hi[2]), (f16)(y[4 * g + 3] - (float)hi[3])};
       }
     }
-    if (m0 == n0) continue;
-    // the mirrored tile: 16 lanes read 16 columns of eight rows each, turned; 64 contiguous bytes a row of it
     __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
     asm volatile("" ::: "memory");
-    const int wc = n0 + (wave % T::WN) * (TN * 32);
 #pragma unroll
-    for (int it = 0; it < TN * 2; ++it) {
-      const int rb = (lane >> 4) * 8, cb = it * 16;
-      const int row = wc + cb + (lane & 15), col = wr + i * 32 + rb;
-      const int n = cb + 4 * (lane & 3), k = rb + ((lane & 15) >> 2);
+    for (int pl = 0; pl < PL; ++pl) {
+      const char* from = mine + pl * T::OUT16_BYTES;
+      f16* o = out + pl * a.out_plane;
 #pragma unroll
-      for (int pl = 0; pl < (TWO ? 2 : 1); ++pl) {
-        const char* base = turn + pl * 32 * HROW;
-        auto tr = [&](int kk) {
-          return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-              base + kk * HROW + (((n >> 3) ^ ((kk & 3) << 1)) << 4) + (n & 7) * 2));
-        };
-        const s16x4 both[2] = {tr(k), tr(k + 4)};
-        if (row < S && col < Sp)
-          *(f16x8*)(out + pl * a.out_plane + (int64_t)row * Sp + col) = __builtin_bit_cast(f16x8, both);
+      for (int it = 0; it < TN * 2; ++it) {  // whole rows
+        const int q = it * 64 + lane, lr = q / (TN * 4), c = wc + q % (TN * 4) * 8, row = wr + i * 32 + lr;
+        const u32x4 x = *(const u32x4*)(from + T::out16_off(lr, q % (TN * 4)));
+        if (row < S && c < Sp) *(u32x4*)(o + (int64_t)row * Sp + c) = x;
+      }
+      if (n0 >= m0) continue;
+      // the mirrored tile: 16 lanes read 16 columns of eight rows each, turned; 64 contiguous bytes a row of it
+#pragma unroll
+      for (int it = 0; it < TN * 2; ++it) {
+        const int rb = (lane >> 4) * 8, cb = it * 16;
+        const int row = wc + cb + (lane & 15), col = wr + i * 32 + rb;
+        const int c = cb + 4 * (lane & 3), kr = rb + ((lane & 15) >> 2);
+        const s16x4 both[2] = {T::out16_tr(from, kr, c), T::out16_tr(from, kr + 4, c)};
+        if (row < S && col < Sp) *(u32x4*)(o + (int64_t)row * Sp + col) = __builtin_bit_cast(u32x4, both);
       }
     }
     __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
@@ -350,9 +307,9 @@ __device__ __forceinline__ void lower(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// GRAM: X times itself, no addends.  COLS: the reduction runs down u's and v's columns (the Gram product of a tall X);
+// COLS: the reduction runs down u's and v's columns (the Gram product of a tall X);
 // otherwise along their rows.
-template <class T, bool GRAM, bool COLS, bool TWO>
+template <class T, bool COLS, bool TWO, int DIAG>
 __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void sym_kernel(SymArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
   const int nt = (a.S + T::BM - 1) / T::BM, per = nt * (nt + 1) / 2;
@@ -368,19 +325,66 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void sym_kernel(SymArg
     return Operand{{at, at + a.in_plane}, a.ld, (COLS ? a.Sp : a.S) - x0};
   };
   f32x16 acc[T::TM][T::TN];
-  T::product(operand(p.u, m0), operand(p.v, n0), a.K, lds, acc);
+  const Diagonal dg{p.row ? p.row + e * a.Sp : nullptr, p.col ? p.col + e * a.Sp : nullptr, a.w_hi, a.w_lo, m0, n0, a.S, a.S};
+  T::product(operand(p.u, m0), operand(p.v, n0), a.K, lds, acc, &dg);
   __syncthreads();
-  sym_out<T, !GRAM, TWO>(a, p, e, m0, n0, acc, lds);
+  sym_out<T, TWO>(a, p, e, m0, n0, acc, lds);
+}
+
+// q += b A + a I where c is 0 or too small beside b for the product to carry b (MTX's schedules seldom are): q holds c A^2, or
+// nothing yet (`fresh`).  A thread takes eight columns.
+__global__ __launch_bounds__(256) void poly_kernel(const f16* A, f16* q, float* full, float* rest, int S, int Sp, int64_t plane,
+                                                   float a, float b, float s_a, float s_q, int fresh, int two) {
+  const int64_t e = blockIdx.y, ms = (int64_t)S * Sp;
+  const int i = blockIdx.x * 256 + threadIdx.x, r = i / (Sp / 8), c = i % (Sp / 8) * 8;
+  if (r >= Sp) return;
+  if (r >= S) {
+    if (c == 0) full[e * Sp + r] = rest[e * Sp + r] = 0.0f;
+    return;
+  }
+  const int64_t at = e * ms + (int64_t)r * Sp + c;
+  const f16x8 h = *(const f16x8*)(A + at), l = two ? *(const f16x8*)(A + plane + at) : f16x8{};
+  const f16x8 qh = fresh ? f16x8{} : *(const f16x8*)(q + at), ql = two && !fresh ? *(const f16x8*)(q + plane + at) : f16x8{};
+  f16x8 hi, lo;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const bool d = c + k == r;
+    float y = (float)qh[k] + (float)ql[k] + (d && !fresh ? rest[e * Sp + r] : 0.0f);
+    y += ((float)h[k] + (float)l[k]) * (b * s_q / s_a) + (d ? a * s_q : 0.0f);
+    hi[k] = (f16)y;
+    lo[k] = (f16)(y - (float)hi[k]);
+    if (d) {
+      full[e * Sp + r] = y / s_q;
+      rest[e * Sp + r] = y - (float)hi[k] - (two ? (float)lo[k] : 0.0f);
+    }
+  }
+  *(f16x8*)(q + at) = hi;
+  if (two) *(f16x8*)(q + plane + at) = lo;
+}
+
+// Eight f32 values as f16, and what that leaves of them.
+__device__ __forceinline__ f16x8 round8(const float y[8]) {
+  f16x8 h;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) h[q] = (f16)y[q];
+  return h;
+}
+__device__ __forceinline__ f16x8 rest8(const float y[8], const f16x8& h) {
+  f16x8 l;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) l[q] = (f16)(y[q] - (float)h[q]);
+  return l;
 }
 
 // ---- X <- P X (tall: X P) ----------------------------------------------------------------------------------------
 enum { OUT_X = 0, OUT_STORE = 1, OUT_STEP = 2 };
 struct ApplyArgs {
   const f16* p;
-  const float* pd;   // P's diagonal
+  const float *pd, *pr;  // P's diagonal, and what the matrix has lost of it
   const f16* x;
-  const f16 *xl, *xr;  // x's lo plane and the rest of the first x in "full", or nullptr
-  f16 *xo, *xol;     // OUT_X: both planes
+  const void* xl;    // what x lacks: "half" 8-bit floats, "full" (the first x) f16; or nullptr
+  f16* xo;           // OUT_X: hi plane, and in "full" behind it lo
+  uint64_t* xol;     // OUT_X in "half": what hi lacks
   void* out;         // OUT_STORE: the result; OUT_STEP: the weights
   int64_t out_batch, out_row;
   int dtype, vec;    // of out; whether its rows are 16-byte aligned
@@ -411,7 +415,9 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
   const Operand oa{{pa, pa + (TALL ? a.x_plane : a.p_plane)}, TALL ? s.Np : s.Sp, TALL ? s.Mp - m0 : max(s.S - m0, 1)};
   const Operand ob{{pb, pb + (TALL ? a.p_plane : a.x_plane)}, TALL ? s.Sp : s.Np, TALL ? max(s.S - n0, 1) : s.Np - n0};
   f32x16 acc[T::TM][T::TN];
-  T::product(oa, ob, s.Sp, lds, acc);
+  const float* pr = a.pr + e * s.Sp;
+  const Diagonal dg{TALL ? nullptr : pr, TALL ? pr : nullptr, 0.0f, 0.0f, m0, n0, TALL ? s.M : s.S, TALL ? s.S : s.N};
+  T::product(oa, ob, s.Sp, lds, acc, &dg);
   __syncthreads();
   const int wave = threadIdx.x >> 6;
   char* mine = T::out_lds(lds);
@@ -419,11 +425,12 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
   const float s_x = a.scales ? a.scales[e].x : a.s_x, s_acc = s_x * a.s_p;
   const float* pd = a.pd + e * s.Sp;
   const float lr = OUT == OUT_STEP ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.0f;
-  const f16 *xl = a.xl ? a.xl + e * s.xs : nullptr, *xr = TWO && a.xr ? a.xr + e * s.xs : nullptr;
+  typedef typename std::conditional<TWO, f16x8, uint64_t>::type Lack;  // eight elements of what x lacks
+  const Lack* xl = a.xl ? (const Lack*)a.xl + e * (s.xs / 8) : nullptr;
   const int c = wc + T::out_col(0);
-  constexpr int NP = TWO ? 3 : 2, DV = sizeof(D) / 2;  // 16-byte pieces of eight D
-  constexpr int AHEAD = T::TN == 4 && (TWO || (OUT == OUT_STEP && DV == 2)) ? 1 : 2;
-  Block<T, NP> add[AHEAD];
+  constexpr int DV = sizeof(D) / 2;  // 16-byte pieces of eight D
+  constexpr int AHEAD = T::TN == 4 && OUT == OUT_STEP && DV == 2 ? 1 : 2;  // blocks of rows in registers
+  Lack lack[AHEAD][T::OUT_STEPS];
   u32x4 old[AHEAD][OUT == OUT_STEP ? T::OUT_STEPS : 1][DV];  // the weights before the step
   D* out = OUT == OUT_X ? nullptr : (D*)a.out + e * a.out_batch;
   const bool vec = a.vec;
@@ -436,11 +443,11 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
         for (int d = 0; d < DV; ++d) old[i % AHEAD][it][d] = ((const u32x4*)w)[d];
       }
     }
-    auto at = [&](int it) { return (int64_t)min(wr + i * 32 + T::out_row(it), s.Mp - 1) * s.Np + min(c, s.Np - 8); };
-    Block<T, NP>& b = add[i % AHEAD];
-    b.load(0, X, at);
-    b.load(1, xl, at);
-    if constexpr (TWO) b.load(2, xr, at);
+    if (xl) {
+#pragma unroll
+      for (int it = 0; it < T::OUT_STEPS; ++it)
+        lack[i % AHEAD][it] = xl[((int64_t)min(wr + i * 32 + T::out_row(it), s.Mp - 1) * s.Np + min(c, s.Np - 8)) / 8];
+    }
   };
   float dc[8];
 #pragma unroll
@@ -452,19 +459,24 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
     if (AHEAD == 2 && i + 1 < T::TM) ahead(i + 1);
     if (AHEAD == 1 && i > 0) ahead(i);
     T::put(acc[i], mine);
-    const Block<T, NP>& b = add[i % AHEAD];
 #pragma unroll
     for (int it = 0; it < T::OUT_STEPS; ++it) {
       const int r = wr + i * 32 + T::out_row(it);
       float y[8];
       T::get(mine, it, y);
-      const float dr = TALL ? 0.0f : pd[min(r, s.Sp - 1)];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float k = (TALL ? dc[q] : dr) * s_x;
-        y[q] = __builtin_fmaf((float)b.x[0][it][q], k, y[q] * s_acc);
-        if (xl) y[q] = __builtin_fmaf((float)b.x[1][it][q], k, y[q]);
-        if (TWO && xr) y[q] = __builtin_fmaf((float)b.x[TWO ? 2 : 1][it][q], k, y[q]);
+      for (int q = 0; q < 8; ++q) y[q] *= s_acc;
+      if (xl) {
+        const float dr = TALL ? 0.0f : pd[min(r, s.Sp - 1)];
+        float l[8];
+        if constexpr (TWO) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) l[q] = (float)lack[i % AHEAD][it][q];
+        } else {
+          unpack8(lack[i % AHEAD][it], l);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) y[q] = __builtin_fmaf(l[q], (TALL ? dc[q] : dr) * s_x, y[q]);
       }
       if (r >= (OUT == OUT_X ? s.Mp : s.M) || c >= (OUT == OUT_X ? s.Np : s.N)) continue;
       if constexpr (OUT == OUT_X) {
@@ -477,7 +489,13 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
         for (int q = 0; q < 8; ++q) y[q] *= a.s_out;
         const f16x8 hi = round8(y);
         *(f16x8*)(a.xo + at) = hi;
-        *(f16x8*)(a.xol + at) = rest8(y, hi);
+        if constexpr (TWO) {
+          *(f16x8*)(a.xo + a.x_plane + at) = rest8(y, hi);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) y[q] -= (float)hi[q];
+          a.xol[at / 8] = pack8(y);
+        }
       } else {
         D* o = out + (int64_t)r * a.out_row + c;
         if constexpr (OUT == OUT_STEP) {
@@ -504,30 +522,30 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
 }
 
 // ---- the chain of launches ---------------------------------------------------------------------------------------
-template <bool A, bool B, bool TWO> using Big = Tile<F16, 4, 4, 2, 2, 4, A, B, false, TWO>;
-template <bool A, bool B, bool TWO> using Small = Tile<F16, 2, 2, 2, 2, 4, A, B, false, TWO>;
+template <bool A, bool B, bool TWO, int DIAG> using Big = Tile<F16, 4, 4, 2, 2, 4, A, B, false, TWO, DIAG>;
+template <bool A, bool B, bool TWO, int DIAG> using Small = Tile<F16, 2, 2, 2, 2, 4, A, B, false, TWO, DIAG>;
 
 constexpr int kBigTiles = 192;
 
-template <bool GRAM, bool COLS, bool TWO>
+template <bool COLS, bool TWO, int DIAG>
 static int launch_sym(const SymArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { const int64_t n = ceil_div(a.S, b); return a.np * a.E * (n * (n + 1) / 2); };
   if (tiles(256) >= kBigTiles && a.S >= 256)
-    hipLaunchKernelGGL((sym_kernel<Big<COLS, COLS, TWO>, GRAM, COLS, TWO>), dim3((unsigned)tiles_grid(tiles(256))), dim3(256), 0,
-                       st, a);
+    hipLaunchKernelGGL((sym_kernel<Big<COLS, COLS, TWO, DIAG>, COLS, TWO, DIAG>), dim3((unsigned)tiles_grid(tiles(256))),
+                       dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((sym_kernel<Small<COLS, COLS, TWO>, GRAM, COLS, TWO>), dim3((unsigned)tiles_grid(tiles(128))), dim3(256),
-                       0, st, a);
+    hipLaunchKernelGGL((sym_kernel<Small<COLS, COLS, TWO, DIAG>, COLS, TWO, DIAG>), dim3((unsigned)tiles_grid(tiles(128))),
+                       dim3(256), 0, st, a);
   return check_launch();
 }
 template <bool TALL, bool TWO, int OUT, typename D>
 static int launch_apply_out(const ApplyArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { return a.E * ceil_div(a.s.Mp, b) * ceil_div(a.s.Np, b); };
   if (tiles(256) >= kBigTiles && a.s.S >= 256)
-    hipLaunchKernelGGL((apply_kernel<Big<false, !TALL, TWO>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(256))),
+    hipLaunchKernelGGL((apply_kernel<Big<false, !TALL, TWO, DIAG_VECTORS>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(256))),
                        dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((apply_kernel<Small<false, !TALL, TWO>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(128))),
+    hipLaunchKernelGGL((apply_kernel<Small<false, !TALL, TWO, DIAG_VECTORS>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(128))),
                        dim3(256), 0, st, a);
   return check_launch();
 }
@@ -549,8 +567,10 @@ static int64_t parts_of(int64_t E, const Shape& s) {
 
 // Matrices that go through the chain together.
 constexpr int64_t kChunkBytes = (int64_t)4 << 30;
+// bytes an element of X takes: the first, with what it lacks, and the second
+static int64_t x_bytes(int planes) { return planes == 2 ? 6 + 4 : 3 + 3; }
 static int64_t matrix_bytes(const Shape& s, int planes) {
-  return ((4 + planes - 1) * s.xs + 5 * s.ms * planes) * 2 + 4 * round_up((int64_t)s.Sp * 4, 256) + 1024 * 8 + 256;
+  return x_bytes(planes) * s.xs + 10 * s.ms * planes + 7 * round_up((int64_t)s.Sp * 4, 256) + 1024 * 8 + 256;
 }
 static int64_t chunk_of(int64_t E, const Shape& s, int planes) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(E, kChunkBytes / matrix_bytes(s, planes)));
@@ -561,8 +581,9 @@ static int64_t workspace_bytes(int64_t E, const Shape& s, int planes) {
   int64_t b = 0;
   b += round_up(n * 512 * 8, 256);                        // partial sums
   b += round_up(n * (int64_t)sizeof(Scale), 256);
-  b += 3 * round_up(n * s.Sp * 4, 256);                    // diagonals
-  b += 2 * round_up(n * s.xs * 4, 256) + (planes - 1) * round_up(n * s.xs * 2, 256);  // X, twice, in planes
+  b += 6 * round_up(n * s.Sp * 4, 256);                    // diagonals, and what the matrices lose of them
+  for (const int64_t x : {2 * planes, planes == 2 ? 2 : 1, 2 * planes, planes == 2 ? 0 : 1})
+    b += round_up(n * s.xs * x, 256);                      // X, twice, and what it lacks
   b += 5 * round_up(n * s.ms * 2 * planes, 256);          // A, T and three of Q and P
   return b;
 }
@@ -586,17 +607,20 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   auto take = [&](int64_t bytes) { char* p = ws; ws += round_up(bytes, 256); return p; };
   double* part = (double*)take(E * 512 * 8);
   Scale* scales = (Scale*)take(E * (int64_t)sizeof(Scale));
-  float* diag[3];
-  for (auto& d : diag) d = (float*)take(E * s.Sp * 4);
+  float *full[3], *rest[3];
+  for (auto& d : full) d = (float*)take(E * s.Sp * 4);
+  for (auto& d : rest) d = (float*)take(E * s.Sp * 4);
   f16* X[2];
-  for (auto& x : X) x = (f16*)take(E * s.xs * 4);
-  f16* rest = TWO ? (f16*)take(E * s.xs * 2) : nullptr;
+  void* lack[2];
+  X[0] = (f16*)take(E * s.xs * 2 * planes);
+  lack[0] = take(E * s.xs * planes);
+  X[1] = (f16*)take(E * s.xs * 2 * planes);
+  lack[1] = TWO ? nullptr : take(E * s.xs);
   f16 *A = (f16*)take(E * s.ms * 2 * planes), *Tm = (f16*)take(E * s.ms * 2 * planes), *Q[3];
   for (auto& q : Q) q = (f16*)take(E * s.ms * 2 * planes);
   const int64_t x_plane = E * s.xs, m_plane = E * s.ms;
 
-  // in "half" f16 holds a bf16 x as it is
-  const bool first_lo = TWO || j.src.m || j.gdtype == MTX_F32;
+  const bool first_lacks = TWO || j.src.m || j.gdtype == MTX_F32;  // in "half" f16 holds a bf16 x as it is
   const int parts = (int)parts_of(E, s);
   const int rows = (int)ceil_div(s.M, parts), rows_p = (int)ceil_div(s.Mp, parts);
   const dim3 grid((unsigned)parts, (unsigned)E);
@@ -604,7 +628,8 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   do {                                                                                                              \
     hipLaunchKernelGGL((norm_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, rows, part);                   \
     hipLaunchKernelGGL((convert_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, s.Mp, s.Np, rows_p, part, parts, \
-                       eps, X[0], first_lo ? X[0] + x_plane : nullptr, rest, scales);                                      \
+                       eps, X[0], TWO ? X[0] + x_plane : nullptr, TWO ? (f16*)lack[0] : nullptr,                    \
+                       !TWO && first_lacks ? (uint64_t*)lack[0] : nullptr, scales);                                 \
   } while (0)
   if (j.gdtype == MTX_F32) {
     if (j.gvec) MTX_PREP(float, true);
@@ -638,9 +663,9 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
       g.in_batch = s.xs;
       g.in_plane = x_plane;
       g.scales = x_scale == 0.0f ? scales : nullptr;
-      g.p[0] = Sym{X[cur], X[cur], A, nullptr, nullptr, nullptr, x_scale == 0.0f ? 1.0f : 1.0f / (x_scale * x_scale),
-                   0.0f, 0.0f, 0.0f, sA};
-      rc = launch_sym<true, TALL, TWO>(g, st);
+      g.p[0] = Sym{X[cur], X[cur], A, nullptr, nullptr, nullptr, nullptr,
+                   sA * (x_scale == 0.0f ? 1.0f : 1.0f / (x_scale * x_scale)), 0.0f, sA};
+      rc = launch_sym<TALL, TWO, DIAG_NONE>(g, st);
       if (rc != MTX_OK) return rc;
     }
     m.K = s.Sp;
@@ -648,38 +673,51 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
     m.in_batch = s.ms;
     m.in_plane = m_plane;
     const int q = p < 0 ? 0 : (p + 1) % 3, np = p < 0 ? q : (p + 2) % 3;
+    // Q = a I + c (A + (b / c) I) A: the product carries b where f16 holds (b / c) sA
+    const float w = c[2] != 0.0f ? c[1] / c[2] * sA : 0.0f;
+    const bool carried = c[2] != 0.0f && fabsf(w) <= 60000.0f;
     m.np = 1;
-    m.p[0] = Sym{A, A, Q[q], diag[q], nullptr, nullptr, c[2] / (sA * sA), c[1] / sA, 0.0f, c[0], sQ};
-    rc = launch_sym<false, false, TWO>(m, st);
-    if (rc != MTX_OK) return rc;
+    if (c[2] != 0.0f) {
+      m.w_hi = carried ? (float)(f16)w : 0.0f;
+      m.w_lo = carried ? w - m.w_hi : 0.0f;
+      m.p[0] = Sym{A, A, Q[q], full[q], rest[q], nullptr, nullptr, c[2] / (sA * sA) * sQ, carried ? c[0] : 0.0f, sQ};
+      rc = launch_sym<false, TWO, DIAG_CONST>(m, st);
+      if (rc != MTX_OK) return rc;
+    }
+    if (!carried) {
+      hipLaunchKernelGGL(poly_kernel, dim3((unsigned)ceil_div((int64_t)s.Sp * (s.Sp / 8), 256), (unsigned)E), dim3(256), 0, st,
+                         A, Q[q], full[q], rest[q], s.S, s.Sp, m_plane, c[0], c[1], sA, sQ, c[2] == 0.0f, TWO);
+      rc = check_launch();
+      if (rc != MTX_OK) return rc;
+    }
     // P <- Q P and T = Q A in one launch, then A <- Q T
     m.np = 0;
     if (p >= 0) {
       const float sPp = c[6 - 9];
-      m.p[m.np++] = Sym{Q[q], Q[p], Q[np], diag[np], diag[q], diag[p], 1.0f / (sQ * sPp), 1.0f / sPp, 1.0f / sQ, 0.0f, sP};
+      m.p[m.np++] = Sym{Q[q], Q[p], Q[np], full[np], rest[np], rest[q], rest[p], sP / (sQ * sPp), 0.0f, sP};
     }
-    if (!ends) m.p[m.np++] = Sym{Q[q], A, Tm, nullptr, diag[q], nullptr, 1.0f / (sQ * sA), 1.0f / sA, 0.0f, 0.0f, sT};
+    if (!ends) m.p[m.np++] = Sym{Q[q], A, Tm, nullptr, nullptr, rest[q], nullptr, sT / (sQ * sA), 0.0f, sT};
     if (m.np > 0) {
-      rc = launch_sym<false, false, TWO>(m, st);
+      rc = launch_sym<false, TWO, DIAG_VECTORS>(m, st);
       if (rc != MTX_OK) return rc;
     }
     p = np;
     if (!ends) {
       const float sA2 = c[3 + 9];
       m.np = 1;
-      m.p[0] = Sym{Q[q], Tm, A, nullptr, diag[q], nullptr, 1.0f / (sQ * sT), 1.0f / sT, 0.0f, 0.0f, sA2};
-      rc = launch_sym<false, false, TWO>(m, st);
+      m.p[0] = Sym{Q[q], Tm, A, nullptr, nullptr, rest[q], nullptr, sA2 / (sQ * sT), 0.0f, sA2};
+      rc = launch_sym<false, TWO, DIAG_VECTORS>(m, st);
       if (rc != MTX_OK) return rc;
       continue;
     }
     ApplyArgs a{};
     a.p = Q[p];
-    a.pd = diag[p];
+    a.pd = full[p];
+    a.pr = rest[p];
     a.x = X[cur];
-    a.xl = first_lo || x_scale != 0.0f ? X[cur] + x_plane : nullptr;
-    a.xr = x_scale == 0.0f ? rest : nullptr;
+    a.xl = x_scale == 0.0f ? (first_lacks ? lack[0] : nullptr) : (TWO ? nullptr : lack[cur]);
     a.xo = X[cur ^ 1];
-    a.xol = X[cur ^ 1] + x_plane;
+    a.xol = TWO ? nullptr : (uint64_t*)lack[cur ^ 1];
     a.out = j.out;
     a.out_batch = j.out_batch;
     a.out_row = j.out_row;

@@ -58,7 +58,10 @@ def _schedule(steps: int, coefficients: tuple, group: int):
         p = [u * v for u, v in zip(p, q)]
         bound_t = max(abs(v) * t * t for v, t in zip(q, s))
         sq = scale(max(abs(v) for v in q))
-        flat += [a, b, c, scale(max(t * t for t in s)), sq, scale(bound_t),
+        sa = scale(max(t * t for t in s))
+        if 0 < abs(b) < 100 * abs(c):  # the product that squares A carries b as (b / c) sa, in f16 as well
+            sa = min(sa, 2.0 ** math.floor(math.log2(60000 * abs(c / b))))
+        flat += [a, b, c, sa, sq, scale(bound_t),
                  sq if first else scale(max(abs(v) for v in p)), 0.0, float(i in last)]
         s = [abs(v) * t for v, t in zip(q, s)]
         top = max(s)
