@@ -93,7 +93,7 @@ struct Tile {
   static constexpr int LDS_BYTES = NST * STAGE;
   static constexpr int A_INSTR = A_BYTES / 1024 / NW, B_INSTR = B_BYTES / 1024 / NW, LPS = A_INSTR + B_INSTR;
   static_assert(A_BYTES % (1024 * NW) == 0 && B_BYTES % (1024 * NW) == 0, "whole load instructions per wave");
-  static_assert(LPS % 2 == 0 && PD >= 2, "the first stage's wait counts half of a stage's loads");
+  static_assert(PD >= 3, "a stage's fragments are read from half a stage ahead");
   static_assert(!(TAIL && TWO), "two planes come padded");
   typedef typename F::x8 x8;
 
@@ -243,51 +243,58 @@ struct Tile {
       for (int q = 0; q < 8; ++q) d[q] = q == at ? e : (typename F::elem)0.0f;
       return d;
     };
-    auto diagonals = [&](int kt, int sub) {
+    // Behind a stage's products and before the barrier that lets its slot go: the fragments are read again, so that the
+    // loop's own registers and order stay as they are (with the terms among the products those took a quarter longer).
+    auto diagonals = [&](int kt) {
       const int part = TWO ? kt % 3 : 0, k = (TWO ? kt / 3 : kt) * BKS;
-      if constexpr (DIAG == DIAG_CONST) {
-        if (part == 2 || k < row0 || k >= row0 + TM * 32) return;
-        const x8 hi = diagonal(dg->hi, sub), lo = diagonal(dg->lo, sub);
+      const char* st = lds + slot(kt) * STAGE;
+      auto frag_a = [&](int i, int sub) {
+        return fragment(st, std::bool_constant<A_COLS>(), std::integral_constant<int, BM>(), wm * (TM * 32) + i * 32, sub);
+      };
+      auto frag_b = [&](int j, int sub) {
+        return fragment(st + A_BYTES, std::bool_constant<B_COLS>(), std::integral_constant<int, BN>(),
+                        wn * (TN * 32) + j * 32, sub);
+      };
+      if (DIAG == DIAG_CONST ? part == 2 : part != 0) return;
+      if (has_row && k >= row0 && k < row0 + TM * 32) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           if (k != row0 + i * 32) continue;
 #pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            acc[i][j] = F::mfma(fb[sub][j], hi, acc[i][j]);
-            if (part == 0) acc[i][j] = F::mfma(fb[sub][j], lo, acc[i][j]);
+          for (int sub = 0; sub < 2; ++sub) {
+            const x8 d = diagonal(DIAG == DIAG_CONST ? dg->hi : drow[DIAG == DIAG_CONST ? 0 : i], sub);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = F::mfma(frag_b(j, sub), d, acc[i][j]);
+            if (DIAG == DIAG_CONST && part == 0) {
+              const x8 lo = diagonal(dg->lo, sub);
+#pragma unroll
+              for (int j = 0; j < TN; ++j) acc[i][j] = F::mfma(frag_b(j, sub), lo, acc[i][j]);
+            }
           }
         }
-      } else if constexpr (DIAG == DIAG_VECTORS) {
-        if (part != 0) return;
-        if (has_row && k >= row0 && k < row0 + TM * 32) {
+      }
+      if (DIAG == DIAG_VECTORS && has_col && k >= col0 && k < col0 + TN * 32) {
 #pragma unroll
-          for (int i = 0; i < TM; ++i) {
-            if (k != row0 + i * 32) continue;
-            const x8 d = diagonal(drow[i], sub);
+        for (int j = 0; j < TN; ++j) {
+          if (k != col0 + j * 32) continue;
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = F::mfma(fb[sub][j], d, acc[i][j]);
-          }
-        }
-        if (has_col && k >= col0 && k < col0 + TN * 32) {
+          for (int sub = 0; sub < 2; ++sub) {
+            const x8 d = diagonal(dcol[DIAG == DIAG_VECTORS ? j : 0], sub);
 #pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            if (k != col0 + j * 32) continue;
-            const x8 d = diagonal(dcol[j], sub);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) acc[i][j] = F::mfma(d, fa[sub][i], acc[i][j]);
+            for (int i = 0; i < TM; ++i) acc[i][j] = F::mfma(d, frag_a(i, sub), acc[i][j]);
           }
         }
       }
     };
 
-    // prologue: stages 0 .. PD-1 in flight, stage 0 landed and visible
+    // prologue: stages 0 .. PD-1 in flight, stages 0 and 1 landed and visible
 #pragma unroll
     for (int s = 0; s < PD; ++s) {
 #pragma unroll
       for (int d = 0; d < LPS; ++d) issue(s, d);
       advance();
     }
-    __builtin_amdgcn_s_waitcnt(MTX_VMCNT(LPS * (PD - 1)));
+    __builtin_amdgcn_s_waitcnt(MTX_VMCNT(LPS * (PD - 2)));
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < TM + TN; ++r) read(0, 0, 0, r);
@@ -297,7 +304,6 @@ struct Tile {
     auto half = [&](auto which, int kt) {
       constexpr int sub = decltype(which)::value;
       if (TAIL && kt == nk - 1 && tail < BKS) mask(sub, sub);
-      if constexpr (DIAG != DIAG_NONE) diagonals(kt, sub);
 #pragma unroll
       for (int qq = 0; qq < S; ++qq) {
         const int i = qq / TN, j = qq % TN;
@@ -317,15 +323,10 @@ struct Tile {
     };
     for (int kt = 0; kt < nk; ++kt) {
       half(std::integral_constant<int, 0>(), kt);
-      if (kt == 0) {
-        // stage 1 landed and visible before its first fragment reads below
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(MTX_VMCNT(LPS * (PD - 2) + LPS / 2));
-        __builtin_amdgcn_s_barrier();
-      }
       half(std::integral_constant<int, 1>(), kt);
       advance();
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (DIAG != DIAG_NONE) diagonals(kt);
       // Stage kt + 2 landed before the barrier makes it visible.  A bare s_barrier: the slot refilled next held
       // stage kt, whose fragments this iteration's MFMAs consumed.
       __builtin_amdgcn_s_waitcnt(MTX_VMCNT(LPS * (PD - 2)));
