@@ -88,6 +88,7 @@ template <class F, int TM_, int TN_, int WM_, int WN_, int NST_, bool A_COLS, bo
           bool TWO = false, int DIAG = DIAG_NONE>
 struct Tile {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NST = NST_, PD = NST - 1;
+  static constexpr bool cols = A_COLS;
   static constexpr int NW = WM * WN, NT = NW * 64, BM = 32 * TM * WM, BN = 32 * TN * WN;
   static constexpr int A_BYTES = BM * BKS * 2, B_BYTES = BN * BKS * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int LDS_BYTES = NST * STAGE;

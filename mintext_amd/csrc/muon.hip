@@ -32,6 +32,7 @@ namespace ns {
 using namespace dense;
 typedef _Float16 f16;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 
 // What a stack's matrices share.  Tall (M > N): X is kept as it is, [M][N], and the Gram side is its columns.
 struct Shape {
@@ -261,7 +262,6 @@ __device__ __forceinline__ void sym_out(const SymArgs& a, const Sym& p, int64_t 
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
         const f16x4 hi = {(f16)y[4 * g], (f16)y[4 * g + 1], (f16)y[4 * g + 2], (f16)y[4 * g + 3]};
         char* to = mine + T::out16_off(frow, j * 4 + g) + 8 * h;
         *(f16x4*)to = hi;
@@ -521,6 +521,145 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
   }
 }
 
+// ---- S <= 128: the Gram product and all S x S products of a group in one workgroup --------------------------------
+// Between launches such products wait for memory and for each other, 8 to 10 us apiece for 2 of work (8 x 128 x 512: 26
+// launches, 185 us).  Here one workgroup takes a matrix from X to P: A and P stay in its registers in f32, the operands
+// of a product in LDS in two f16 planes, in "half" too, as the products cost little.  Two slots of 64 KB: Q, and in
+// turn A, T and P.
+constexpr int kChainS = 128;
+struct ChainArgs {
+  const f16* x;
+  SymArgs m;             // of P: out's layout (p[0].out, full, rest), E, S, Sp; and scales
+  int K;                 // reduction of the Gram product
+  int64_t ld, x_batch, x_plane;
+  float x_undo;          // undoes the scale of x (squared); the first x: from m.scales
+  int steps;
+  float sched[3][9];
+};
+template <class T, bool TWO>
+__global__ __launch_bounds__(256, 1) void chain_kernel(ChainArgs a) {
+  constexpr int SLOT = kChainS * kChainS * 4;  // two planes
+  __shared__ __attribute__((aligned(1024))) char lds[2 * SLOT];
+  static_assert(T::BM == kChainS && T::BN == kChainS && T::LDS_BYTES <= 2 * SLOT, "one tile");
+  const int64_t e = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, frow = lane & 31, h = lane >> 5;
+  const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64, S = a.m.S;
+  constexpr bool COLS = T::cols;
+  f32x16 A[2][2], P[2][2], acc[2][2];
+  {
+    const f16* x = a.x + e * a.x_batch;
+    const Operand o{{x, x + a.x_plane}, a.ld, COLS ? a.m.Sp : S};
+    T::product(o, o, a.K, lds, acc);
+    __syncthreads();
+  }
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) f(i, j, v, wr + i * 32 + frow, wc + j * 32 + 8 * (v / 4) + 4 * h + v % 4);
+  };
+  const float gram = a.m.scales ? a.m.scales[e].gram : a.x_undo;
+  each([&](int i, int j, int v, int r, int c) { A[i][j][v] = r < S && c < S ? acc[i][j][v] * gram : 0.0f; });
+  char* const slot[2] = {lds, lds + SLOT};
+  auto at = [&](int r, int c16) { return r * 256 + ((c16 ^ (r & 15)) << 4); };
+  auto put = [&](char* to, const f32x16 (&m)[2][2], float scale) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f16x4 hi, lo;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float y = m[i][j][4 * g + q] * scale;
+            hi[q] = (f16)y;
+            lo[q] = (f16)(y - (float)hi[q]);
+          }
+          char* p = to + at(wr + i * 32 + frow, (wc + j * 32) / 8 + g) + 8 * h;
+          *(f16x4*)p = hi;
+          *(f16x4*)(p + SLOT / 2) = lo;
+        }
+  };
+  // acc = u v, symmetric, all workgroup; reads end before the next barrier
+  const int steps16 = (S + 15) / 16;
+  auto multiply = [&](const char* u, const char* v) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+    if (wr >= S || wc >= S) return;
+    for (int k = 0; k < steps16; ++k) {
+      f16x8 fu[2][2], fv[2][2];
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          fu[pl][i] = *(const f16x8*)(u + pl * (SLOT / 2) + at(wr + i * 32 + frow, 2 * k + h));
+          fv[pl][i] = *(const f16x8*)(v + pl * (SLOT / 2) + at(wc + i * 32 + frow, 2 * k + h));
+        }
+#pragma unroll
+      for (int t = 0; t < 3; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = F16::mfma(fv[t == 1][j], fu[t == 2][i], acc[i][j]);
+    }
+  };
+  put(slot[0], A, a.sched[0][3]);
+  __syncthreads();
+  for (int n = 0; n < a.steps; ++n) {
+    const float* c = a.sched[n];
+    const float sA = c[3], sQ = c[4], sT = c[5];
+    const bool last = n + 1 == a.steps;
+    multiply(slot[0], slot[0]);  // A A
+    const float k2 = c[2] / (sA * sA);
+    each([&](int i, int j, int v, int r, int cc) {
+      acc[i][j][v] = k2 * acc[i][j][v] + c[1] * A[i][j][v] + (r == cc && r < S ? c[0] : 0.0f);
+    });
+    put(slot[1], acc, sQ);
+    if (n == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) P[i][j] = acc[i][j];
+    }
+    __syncthreads();
+    if (!last) {
+      multiply(slot[1], slot[0]);  // T = Q A
+      const float kt = sT / (sQ * sA);
+      each([&](int i, int j, int v, int, int) { acc[i][j][v] *= kt; });
+      __syncthreads();
+      put(slot[0], acc, 1.0f);
+      __syncthreads();
+      multiply(slot[1], slot[0]);  // the next A = Q T
+      const float ka = 1.0f / (sQ * sT);
+      each([&](int i, int j, int v, int, int) { A[i][j][v] = acc[i][j][v] * ka; });
+      __syncthreads();
+    }
+    if (n > 0) {
+      const float sP = a.sched[n - 1][6];
+      put(slot[0], P, sP);
+      __syncthreads();
+      multiply(slot[1], slot[0]);  // P = Q P
+      const float kp = 1.0f / (sQ * sP);
+      each([&](int i, int j, int v, int, int) { P[i][j][v] = acc[i][j][v] * kp; });
+      __syncthreads();
+    }
+    if (!last) {
+      put(slot[0], A, a.sched[n + 1][3]);
+      __syncthreads();
+    }
+  }
+  SymArgs m = a.m;
+  m.scales = nullptr;
+  sym_out<T, TWO>(m, m.p[0], e, 0, 0, P, lds);
+}
+
 // ---- the chain of launches ---------------------------------------------------------------------------------------
 template <bool A, bool B, bool TWO, int DIAG> using Big = Tile<F16, 4, 4, 2, 2, 4, A, B, false, TWO, DIAG>;
 template <bool A, bool B, bool TWO, int DIAG> using Small = Tile<F16, 2, 2, 2, 2, 4, A, B, false, TWO, DIAG>;
@@ -536,6 +675,11 @@ static int launch_sym(const SymArgs& a, hipStream_t st) {
   else
     hipLaunchKernelGGL((sym_kernel<Small<COLS, COLS, TWO, DIAG>, COLS, TWO, DIAG>), dim3((unsigned)tiles_grid(tiles(128))),
                        dim3(256), 0, st, a);
+  return check_launch();
+}
+template <bool TALL, bool TWO>
+static int launch_chain(const ChainArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((chain_kernel<Small<TALL, TALL, TWO, DIAG_NONE>, TWO>), dim3((unsigned)a.m.E), dim3(256), 0, st, a);
   return check_launch();
 }
 template <bool TALL, bool TWO, int OUT, typename D>
@@ -650,11 +794,73 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   m.out_plane = m_plane;
   int cur = 0;          // X of the group
   float x_scale = 0.0f;  // of X; 0: the first, by matrix
-  int p = -1;           // Q[p], diag[p] hold P
+  int p = -1;           // Q[p], full[p], rest[p] hold P
+  // X <- P X behind step i, which ends its group; P in Q[p]
+  auto launch_group_apply = [&](int i, int p) {
+    const float sP = sched[9 * i + 6], sX = sched[9 * i + 7];
+    ApplyArgs a{};
+    a.p = Q[p];
+    a.pd = full[p];
+    a.pr = rest[p];
+    a.x = X[cur];
+    a.xl = x_scale == 0.0f ? (first_lacks ? lack[0] : nullptr) : (TWO ? nullptr : lack[cur]);
+    a.xo = X[cur ^ 1];
+    a.xol = TWO ? nullptr : (uint64_t*)lack[cur ^ 1];
+    a.out = j.out;
+    a.out_batch = j.out_batch;
+    a.out_row = j.out_row;
+    a.dtype = j.dtype;
+    a.vec = j.vec;
+    a.s = s;
+    a.E = (int)E;
+    a.p_plane = m_plane;
+    a.x_plane = x_plane;
+    a.s_p = 1.0f / sP;
+    a.scales = x_scale == 0.0f ? scales : nullptr;
+    a.s_x = x_scale == 0.0f ? 0.0f : 1.0f / x_scale;
+    a.s_out = sX;
+    a.lr = j.lr;
+    a.decay = j.decay;
+    a.factor = j.factor;
+    a.lr_dev = j.lr_dev;
+    const int rc = launch_apply<TALL, TWO>(i + 1 == steps ? j.step : OUT_X, a, st);
+    x_scale = sX;
+    cur ^= 1;
+    return rc;
+  };
   for (int i = 0; i < steps; ++i) {
     const float* c = sched + 9 * i;
-    const float sA = c[3], sQ = c[4], sT = c[5], sP = c[6], sX = c[7];
+    const float sA = c[3], sQ = c[4], sT = c[5], sP = c[6];
     const bool ends = c[8] != 0.0f || i + 1 == steps;
+    if (s.S <= kChainS && p < 0) {
+      // the whole group at once, as far as it is three steps long at most
+      int n = 1;
+      while (sched[9 * (i + n - 1) + 8] == 0.0f && i + n < steps && n < 4) ++n;
+      if (n <= 3) {
+        ChainArgs a{};
+        a.x = X[cur];
+        a.m = m;
+        a.m.p[0] = Sym{nullptr, nullptr, Q[0], full[0], rest[0], nullptr, nullptr, sched[9 * (i + n - 1) + 6], 0.0f,
+                       sched[9 * (i + n - 1) + 6]};
+        a.m.scales = x_scale == 0.0f ? scales : nullptr;
+        a.K = TALL ? s.Mp : s.Np;
+        a.ld = s.Np;
+        a.x_batch = s.xs;
+        a.x_plane = x_plane;
+        a.x_undo = x_scale == 0.0f ? 0.0f : 1.0f / (x_scale * x_scale);
+        a.steps = n;
+        for (int k = 0; k < n; ++k)
+          for (int q = 0; q < 9; ++q) a.sched[k][q] = sched[9 * (i + k) + q];
+        rc = launch_chain<TALL, TWO>(a, st);
+        if (rc != MTX_OK) return rc;
+        i += n - 1;
+        p = 0;
+        rc = launch_group_apply(i, 0);
+        if (rc != MTX_OK) return rc;
+        p = -1;
+        continue;
+      }
+    }
     if (p < 0) {
       SymArgs g = m;
       g.np = 1;
@@ -710,35 +916,8 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
       if (rc != MTX_OK) return rc;
       continue;
     }
-    ApplyArgs a{};
-    a.p = Q[p];
-    a.pd = full[p];
-    a.pr = rest[p];
-    a.x = X[cur];
-    a.xl = x_scale == 0.0f ? (first_lacks ? lack[0] : nullptr) : (TWO ? nullptr : lack[cur]);
-    a.xo = X[cur ^ 1];
-    a.xol = TWO ? nullptr : (uint64_t*)lack[cur ^ 1];
-    a.out = j.out;
-    a.out_batch = j.out_batch;
-    a.out_row = j.out_row;
-    a.dtype = j.dtype;
-    a.vec = j.vec;
-    a.s = s;
-    a.E = (int)E;
-    a.p_plane = m_plane;
-    a.x_plane = x_plane;
-    a.s_p = 1.0f / sP;
-    a.scales = x_scale == 0.0f ? scales : nullptr;
-    a.s_x = x_scale == 0.0f ? 0.0f : 1.0f / x_scale;
-    a.s_out = sX;
-    a.lr = j.lr;
-    a.decay = j.decay;
-    a.factor = j.factor;
-    a.lr_dev = j.lr_dev;
-    rc = launch_apply<TALL, TWO>(i + 1 == steps ? j.step : OUT_X, a, st);
+    rc = launch_group_apply(i, p);
     if (rc != MTX_OK) return rc;
-    x_scale = sX;
-    cur ^= 1;
     p = -1;
   }
   return MTX_OK;

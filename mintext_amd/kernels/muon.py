@@ -27,8 +27,9 @@ import torch
 from .. import _lib as L
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-# Steps between two Gram products, at most: fewer products with three, smaller errors with two
-_GROUP_RESULT, _GROUP_STEP = 2, 3
+# Steps between two Gram products, at most: fewer products with three, smaller errors with two, except for matrices whose
+# products between the two are held in 22 bits in any case
+_GROUP_RESULT, _GROUP_STEP, _SMALL = 2, 3, 128
 
 
 @functools.lru_cache(maxsize=64)
@@ -70,7 +71,7 @@ def _schedule(steps: int, coefficients: tuple, group: int):
     return (ctypes.c_float * len(flat))(*flat)
 
 
-def _arguments(steps, coefficients, eps, precision, dtype, group):
+def _arguments(steps, coefficients, eps, precision, t, group):
     if not isinstance(steps, int) or not 1 <= steps <= 64:
         raise ValueError(f"steps must be an int from 1 to 64, got {steps!r}")
     if not eps > 0:
@@ -88,7 +89,9 @@ def _arguments(steps, coefficients, eps, precision, dtype, group):
         good = False
     if not good or not all(math.isfinite(v) for t in c for v in (t if isinstance(t, tuple) else (t,))):
         raise ValueError("coefficients must be three finite numbers, or three for each step")
-    planes = 2 if precision == "full" or (precision is None and dtype == torch.float32) else 1
+    planes = 2 if precision == "full" or (precision is None and t.dtype == torch.float32) else 1
+    if min(t.shape[-2:]) <= _SMALL:
+        group = _GROUP_STEP
     return _schedule(steps, c, group), planes
 
 
@@ -148,7 +151,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, *, coefficients=COEFFICIENTS,
         a dense tensor of x's shape and dtype.  Not differentiable.
     """
     _check_stack(x, "x")
-    sched, planes = _arguments(steps, coefficients, eps, precision, x.dtype, _GROUP_RESULT)
+    sched, planes = _arguments(steps, coefficients, eps, precision, x, _GROUP_RESULT)
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("newton_schulz is not differentiable: pass x.detach()")
     dev = L.require_device(x)
@@ -186,7 +189,7 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
             raise ValueError(f"{name} must have param's shape {tuple(param.shape)}, got {tuple(t.shape)}")
     if momentum.dtype != torch.float32:
         raise TypeError(f"momentum must be float32, got {momentum.dtype}")
-    sched, planes = _arguments(steps, coefficients, eps, precision, param.dtype, _GROUP_STEP)
+    sched, planes = _arguments(steps, coefficients, eps, precision, param, _GROUP_STEP)
     M, N = param.shape[-2:]
     if scale == "spectral":
         factor = math.sqrt(max(1.0, N / max(M, 1)))

@@ -81,7 +81,7 @@ def groups_of(steps, most):
 
 def tolerance(x, want, full, eps=1e-7, steps=5, coef=COEF, most=2):
     """(2-norm, largest) error allowed before the output is rounded, of one matrix."""
-    groups = groups_of(steps, most)
+    groups = groups_of(steps, 3 if min(x.shape) <= 128 else most)
     same, count = chain64(x, groups, eps, coef)
     assert (same - want).norm() <= 1e-9 * want.norm()  # the groups change nothing in exact arithmetic
     signs = torch.Generator(device=x.device).manual_seed(1)
