@@ -593,21 +593,31 @@ __global__ __launch_bounds__(256, 1) void chain_kernel(ChainArgs a) {
 #pragma unroll
         for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
     if (wr >= S || wc >= S) return;
-    for (int k = 0; k < steps16; ++k) {
-      f16x8 fu[2][2], fv[2][2];
+    // the next 16 elements' operands are read while these are multiplied
+    f16x8 fu[2][2][2], fv[2][2][2];
+    auto read = [&](int b, int k) {
 #pragma unroll
       for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          fu[pl][i] = *(const f16x8*)(u + pl * (SLOT / 2) + at(wr + i * 32 + frow, 2 * k + h));
-          fv[pl][i] = *(const f16x8*)(v + pl * (SLOT / 2) + at(wc + i * 32 + frow, 2 * k + h));
+          fu[b][pl][i] = *(const f16x8*)(u + pl * (SLOT / 2) + at(wr + i * 32 + frow, 2 * k + h));
+          fv[b][pl][i] = *(const f16x8*)(v + pl * (SLOT / 2) + at(wc + i * 32 + frow, 2 * k + h));
         }
+    };
+    auto use = [&](int b) {
 #pragma unroll
       for (int t = 0; t < 3; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) acc[i][j] = F16::mfma(fv[t == 1][j], fu[t == 2][i], acc[i][j]);
+          for (int j = 0; j < 2; ++j) acc[i][j] = F16::mfma(fv[b][t == 1][j], fu[b][t == 2][i], acc[i][j]);
+    };
+    read(0, 0);
+    for (int k = 0; k < steps16; k += 2) {
+      read(1, min(k + 1, 7));
+      use(0);
+      read(0, min(k + 2, 7));
+      if (k + 1 < steps16) use(1);
     }
   };
   put(slot[0], A, a.sched[0][3]);
