@@ -420,8 +420,8 @@ int mtx_gmm_fp8_gathered(const uint8_t* xq, const float* x_scale, int64_t x_rows
  * mtx_linear_bwd: dz = dy * act'(pre), written to dz[M,N] (pre and dz may be NULL for MTX_ACT_NONE,
  *                 where dz is dy); dx[M,K] = dz @ w^T, dw[K,N] = x^T @ dz, dbias[N] = column sums
  *                 of dz; those of the three that are NULL are left out.
- * One workspace size serves both; a workspace must not be shared by two calls that can run at the
- * same time.                                                                               */
+ * One workspace size (16-byte aligned) serves both; a workspace must not be shared by two calls that
+ * can run at the same time.                                                                */
 #define MTX_ACT_NONE       0
 #define MTX_ACT_RELU       1
 #define MTX_ACT_SILU       2
@@ -449,7 +449,7 @@ int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre
  *   first step of a group.  The scales have to keep each matrix's singular values below 65504.
  * planes: 1 = matrices in one f16 plane between products, 2 = in two (float32 results).
  * E <= 65535, M and N <= 2^20, min(M, N) <= 2^15.  Large stacks go through in parts, so that the
- * workspace stays below 4 GiB or one matrix's need.                                          */
+ * workspace (256-byte aligned) stays below 4 GiB or one matrix's need.                        */
 int64_t mtx_newton_schulz_workspace_size(int64_t E, int64_t M, int64_t N, int planes);
 int mtx_newton_schulz(const void* x, int dtype, int64_t E, int64_t M, int64_t N, int64_t x_batch, int64_t x_row,
                       const float* schedule, int steps, float eps, int planes, void* out, int64_t out_batch,

@@ -2,8 +2,9 @@
 //
 // The bias, the activation, the residual and, for training, the copy of z = x w + bias that the gradient needs
 // are applied to the f32 sums on their way out, so that z costs at most one write and the rest no
-// pass of their own.  bf16 with rows of whole 16-byte chunks runs on the 16-bit matrix cores (dense_tile.h), 256 x 256
-// tiles or, where those are few, 128 x 128; everything else on f32 matrix-core tiles (f32_tile.h).
+// pass of their own.  bf16 with rows of whole 16-byte chunks runs on the 16-bit matrix cores (dense_tile.h), in tiles of
+// 256 x 256 or, where those are few, 256 x 128 or 128 x 128, and up to 64 rows on a kernel that streams w;
+// everything else on f32 matrix-core tiles (f32_tile.h).
 #include "common.h"
 #include "dense_tile.h"
 #include "f32_tile.h"
@@ -126,6 +127,7 @@ __global__ __launch_bounds__(f32mm::NT) void f32_kernel(Args p) {
 // ---- bf16, rows of whole 16-byte chunks: tiles of the 16-bit matrix cores -----------------------------------------
 using dense::Operand;
 template <int MODE, bool TAIL> using Big = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, MODE == DW, MODE != DX, TAIL>;
+template <int MODE, bool TAIL> using Mid = dense::Tile<dense::Bf16, 4, 2, 2, 2, 4, MODE == DW, MODE != DX, TAIL>;
 template <int MODE, bool TAIL> using Small = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, MODE == DW, MODE != DX, TAIL>;
 
 // z = v + bias, out = act(z) + residual for eight columns; `bias` and `residual` are those eight of them
@@ -455,13 +457,13 @@ static bool takes_tiles(int mode, const Args& p) {
 }
 
 // How a product runs, by its sizes alone, and in how many pieces of its reduction.
-enum { PATH_F32, PATH_BIG, PATH_SMALL, PATH_THIN };
+enum { PATH_F32, PATH_BIG, PATH_MID, PATH_SMALL, PATH_THIN };
 struct Plan {
   int path, pieces;
 };
 constexpr int kThinRows = 64;
 static Plan plan(int mode, bool tiles, int64_t rows, int64_t cols, int64_t red) {
-  auto count = [&](int64_t b) { return ceil_div(rows, b) * ceil_div(cols, b); };
+  auto count = [&](int64_t b, int64_t n = 0) { return ceil_div(rows, b) * ceil_div(cols, n ? n : b); };
   const int64_t stages = ceil_div(red, 32);
   // pieces that bring `n` workgroups to `want`, of `least` stages or more
   auto split = [&](int64_t n, int64_t want, int64_t least) {
@@ -469,7 +471,10 @@ static Plan plan(int mode, bool tiles, int64_t rows, int64_t cols, int64_t red) 
   };
   if (!tiles) return {PATH_F32, split(count(64), 512, 8)};
   if (mode == FWD && rows <= kThinRows) return {PATH_THIN, split(ceil_div(cols, kThinCols), 256, 16)};
+  // three quarters of the CUs with a tile each: below that the smaller tiles are ahead (4093 x 7168 by 7168 x 2048, 128 tiles
+  // of 256 x 256: 156 us in tiles of 128 x 128, 128 in tiles of 256 x 128)
   if (count(256) >= 192) return {PATH_BIG, 1};
+  if (count(256, 128) >= 192) return {PATH_MID, 1};
   return {PATH_SMALL, split(count(128), 512, 16)};
 }
 static int64_t part_bytes(int64_t rows, int64_t cols, int64_t red, int mode) {
@@ -500,12 +505,14 @@ static int launch_f32(const Args& p, hipStream_t st) {
 }
 
 template <int MODE, bool TAIL, int ACT>
-static int launch_tiles(const Args& p, bool big, hipStream_t st) {
-  auto grid = [&](int b) {
-    return dim3((unsigned)dense::tiles_grid(ceil_div(p.rows, b) * ceil_div(p.cols, b) * p.pieces));
+static int launch_tiles(const Args& p, int path, hipStream_t st) {
+  auto grid = [&](int bm, int bn) {
+    return dim3((unsigned)dense::tiles_grid(ceil_div(p.rows, bm) * ceil_div(p.cols, bn) * p.pieces));
   };
-  if (big) hipLaunchKernelGGL((tile_kernel<Big<MODE, TAIL>, MODE, ACT>), grid(256), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((tile_kernel<Small<MODE, TAIL>, MODE, ACT>), grid(128), dim3(256), 0, st, p);
+  if (path == PATH_BIG) hipLaunchKernelGGL((tile_kernel<Big<MODE, TAIL>, MODE, ACT>), grid(256, 256), dim3(256), 0, st, p);
+  else if (path == PATH_MID)
+    hipLaunchKernelGGL((tile_kernel<Mid<MODE, TAIL>, MODE, ACT>), grid(256, 128), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((tile_kernel<Small<MODE, TAIL>, MODE, ACT>), grid(128, 128), dim3(256), 0, st, p);
   return check_launch();
 }
 template <int MODE>
@@ -526,9 +533,8 @@ static int launch_mode(const Args& p, int path, int dtype, hipStream_t st) {
 #undef MTX_THIN
     return check_launch();
   }
-  const bool big = path == PATH_BIG;
 #define MTX_TILES(ACT) \
-  return p.red % dense::BKS ? launch_tiles<MODE, true, ACT>(p, big, st) : launch_tiles<MODE, false, ACT>(p, big, st)
+  return p.red % dense::BKS ? launch_tiles<MODE, true, ACT>(p, path, st) : launch_tiles<MODE, false, ACT>(p, path, st)
   if constexpr (MODE == FWD) {
     // the activation is applied where the reduction is whole: by finish_kernel if it is in pieces
     switch (p.pieces > 1 ? MTX_ACT_NONE : p.act) {

@@ -307,8 +307,7 @@ __device__ __forceinline__ void lower(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// COLS: the reduction runs down u's and v's columns (the Gram product of a tall X);
-// otherwise along their rows.
+// COLS: the reduction runs down u's and v's columns (the Gram product of a tall X); otherwise along their rows.
 template <class T, bool COLS, bool TWO, int DIAG>
 __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void sym_kernel(SymArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
@@ -331,8 +330,8 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void sym_kernel(SymArg
   sym_out<T, TWO>(a, p, e, m0, n0, acc, lds);
 }
 
-// q += b A + a I where c is 0 or too small beside b for the product to carry b (MTX's schedules seldom are): q holds c A^2, or
-// nothing yet (`fresh`).  A thread takes eight columns.
+// q += b A + a I where c is 0 or too small beside b for the product that squares A to carry b: q holds c A^2, or nothing yet
+// (`fresh`).  A thread takes eight columns; a pass over A and Q.
 __global__ __launch_bounds__(256) void poly_kernel(const f16* A, f16* q, float* full, float* rest, int S, int Sp, int64_t plane,
                                                    float a, float b, float s_a, float s_q, int fresh, int two) {
   const int64_t e = blockIdx.y, ms = (int64_t)S * Sp;
@@ -937,7 +936,7 @@ static int run(Job j, int64_t E, int64_t M, int64_t N, const float* sched, int s
                int64_t ws_bytes, hipStream_t st) {
   if (E == 0 || M == 0 || N == 0) return MTX_OK;
   const Shape s = shape_of(M, N);
-  if (!ws || ws_bytes < workspace_bytes(E, s, planes)) return MTX_ERR_WORKSPACE;
+  if (!ws || (uintptr_t)ws % 256 || ws_bytes < workspace_bytes(E, s, planes)) return MTX_ERR_WORKSPACE;
   const int64_t chunk = chunk_of(E, s, planes);
   const int gsize = dtype_size(j.gdtype), osize = dtype_size(j.dtype);
   for (int64_t e = 0; e < E; e += chunk) {

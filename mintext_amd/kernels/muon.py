@@ -215,5 +215,5 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
         L.call("mtx_muon_update", L.ptr(p), L.dtype_code(p.dtype), *_strides(p), L.ptr(g), L.dtype_code(g.dtype),
                *_strides(g), L.ptr(m), *_strides(m), E, M, N, beta, int(nesterov), lr, L.ptr(lr_dev), weight_decay, factor,
                sched, steps, eps, planes, L.ptr(ws), ws.numel(), L.stream(dev))
-    torch.autograd.graph.increment_version([param, momentum])
+    torch.autograd.graph.increment_version([t for t in (param, momentum) if not t.is_inference()])
     return param

@@ -123,7 +123,8 @@ def test_few_rows(dev, size):
 
 
 @pytest.mark.parametrize("size", [(1531, 1536, 704), (2048, 2048, 768), (1025, 4096, 1288), (4099, 512, 2056),
-                                  (8192, 128, 256), (130, 7168, 2048)])
+                                  (8192, 128, 256), (130, 7168, 2048), (4099, 520, 2056), (4099, 72, 4104),
+                                  (300, 4104, 4104)])
 def test_large(dev, size):
     n = size[0] % 5
     check(dev, *size, torch.bfloat16, ACTS[n], True, n % 2 == 0, True)
