@@ -194,11 +194,12 @@ def stream(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
+_here = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """Context in which ``device`` is the current one, which is where a kernel is launched."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def plain_forward(*tensors) -> bool:

@@ -8,6 +8,8 @@ bias gradient) and the two products ``dz @ weight^T`` and ``x^T @ dz``.  The gra
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -17,77 +19,67 @@ ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # MTX_
 
 
 def _check(x, weight, bias, activation, residual):
-    if activation not in ACTIVATIONS:
+    """(M, K, N, activation code); a serving call spends as long on the host as on the GPU, hence no loops."""
+    act = ACTIVATIONS.get(activation, -1)
+    if act < 0:
         raise ValueError(f"activation must be one of {sorted(k for k in ACTIVATIONS if k)} or None, got {activation!r}")
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[0]:
-        raise ValueError(f"linear takes x [..., K] and weight [K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    N = weight.shape[1]
-    if bias is not None and tuple(bias.shape) != (N,):
+    xs, ws = x.shape, weight.shape
+    if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[0]:
+        raise ValueError(f"linear takes x [..., K] and weight [K, N], got {tuple(xs)} and {tuple(ws)}")
+    K, N = ws
+    if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
-        raise ValueError(f"residual must have the output's shape {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
-    for t in (x, weight, bias, residual):
-        if t is None:
-            continue
-        if t.dtype not in (torch.float32, torch.bfloat16):
-            raise TypeError(f"linear takes float32 or bfloat16 operands, got {t.dtype}")
-        if t.dtype != x.dtype:
-            raise TypeError(f"linear operands must share one dtype, got {x.dtype} and {t.dtype}")
+    if residual is not None and residual.shape != (*xs[:-1], N):
+        raise ValueError(f"residual must have the output's shape {(*xs[:-1], N)}, got {tuple(residual.shape)}")
+    dt = x.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float32:
+        raise TypeError(f"linear takes float32 or bfloat16 operands, got {dt}")
+    if (weight.dtype is not dt or (bias is not None and bias.dtype is not dt)
+            or (residual is not None and residual.dtype is not dt)):
+        raise TypeError(f"linear operands must share one dtype, {dt} as x")
+    return (x.numel() // K if K else math.prod(xs[:-1])), K, N, act
 
 
-def _sizes(x, weight):
-    K, N = weight.shape
-    M = 1
-    for d in x.shape[:-1]:
-        M *= d
-    return M, K, N
-
-
-def _workspace(M, K, N, dev):
-    return L.workspace(L.query("mtx_linear_workspace_size", M, K, N), dev)
-
-
-def _forward(x, weight, bias, act, residual, keep):
+def _forward(x, weight, bias, residual, sizes, keep):
     dev = L.require_device(x, weight, bias, residual)
+    M, K, N, act = sizes
     x, weight = x.contiguous(), weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
-    M, K, N = _sizes(x, weight)
     out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
     pre = torch.empty((M, N), dtype=x.dtype, device=dev) if keep and act else None
-    ws = _workspace(M, K, N, dev)
+    ws = L.workspace(L.query("mtx_linear_workspace_size", M, K, N), dev)
     with L.on_device(dev):
-        L.call("mtx_linear", L.ptr(x), L.ptr(weight), L.ptr(bias), L.ptr(residual), L.dtype_code(x.dtype), M, K, N, act,
-               L.ptr(out), L.ptr(pre), L.ptr(ws), ws.numel(), L.stream(dev))
+        L.call("mtx_linear", x.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(residual), L.dtype_code(x.dtype), M, K, N,
+               act, out.data_ptr(), L.ptr(pre), ws.data_ptr(), ws.numel(), L.stream(dev))
     return out, pre
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, act, residual):
-        out, pre = _forward(x, weight, bias, act, residual, True)
+    def forward(ctx, x, weight, bias, residual, sizes):
+        out, pre = _forward(x, weight, bias, residual, sizes, True)
         ctx.save_for_backward(x, weight, pre)
-        ctx.act = act
+        ctx.sizes = sizes
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, pre = ctx.saved_tensors
-        need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         dev = L.require_device(x, weight, dy)
         x, weight, dy = x.contiguous(), weight.contiguous(), dy.contiguous()
-        M, K, N = _sizes(x, weight)
-        act = ctx.act
+        M, K, N, act = ctx.sizes
         dz = torch.empty((M, N), dtype=x.dtype, device=dev) if act and (need_x or need_w or need_b) else None
         dx = torch.empty_like(x) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
-        ws = _workspace(M, K, N, dev)
+        ws = L.workspace(L.query("mtx_linear_workspace_size", M, K, N), dev)
         with L.on_device(dev):
             L.call("mtx_linear_bwd", L.ptr(dy), L.ptr(x), L.ptr(weight), L.ptr(pre), L.dtype_code(x.dtype), M, K, N, act,
                    L.ptr(dz), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), ws.numel(), L.stream(dev))
-        return dx, dw, db, None, dy if need_r else None
+        return dx, dw, db, dy if need_r else None, None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
@@ -104,8 +96,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     Returns:
         [..., N] in x's dtype.  Differentiable (once) in all four tensors.
     """
-    _check(x, weight, bias, activation, residual)
-    act = ACTIVATIONS[activation]
+    sizes = _check(x, weight, bias, activation, residual)
     if L.plain_forward(x, weight, bias, residual):
-        return _forward(x, weight, bias, act, residual, False)[0]
-    return _Linear.apply(x, weight, bias, act, residual)
+        return _forward(x, weight, bias, residual, sizes, False)[0]
+    return _Linear.apply(x, weight, bias, residual, sizes)
