@@ -76,6 +76,8 @@ __device__ __forceinline__ float activation_slope(float z, int act) {
 }
 
 // ---- any size and alignment: 64 x 64 tiles, products and sums in f32 --------------------------------------
+// Small products are bound by the length of one tile's chain of stages, hence the split (plan()); large ones by the f32
+// matrix cores: 1000 x 2000 x 1000 takes 51 us, 79 TFLOP/s of 154.
 template <typename T, int MODE, int VEC>
 __global__ __launch_bounds__(f32mm::NT) void f32_kernel(Args p) {
   using namespace f32mm;
@@ -157,7 +159,11 @@ __device__ __forceinline__ void finish8(const Args& p, int r, int c, float v[8])
   finish8(p, p.act, at, v, bias, (const uint16_t*)p.residual + at);
 }
 
-// Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2.
+// Bound by the matrix cores in large products: 8192 x 4096 x 14336 in 780 to 800 us, 1.2 PFLOP/s, which is what a plain
+// library product of the size reaches (813 us); 4093 x 2048 x 7168 in 111, its gradients in 134 and 119.  Of few
+// tiles it is the length of a tile's reduction that counts, which plan() splits.
+// Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2
+// (8192 x 4096 x 14336: 805 us without groups, 778 in groups of 4, 783 of 8, 790 of 16).
 constexpr int kGroup = 8;
 template <class T, int MODE, int ACT>
 __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void tile_kernel(Args p) {
@@ -223,6 +229,8 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void tile_
 // A workgroup owns 128 columns and a piece of the reduction; its waves (eight, or four where 64 rows need the registers) take the piece's 32-element chunks in turn,
 // w straight from memory into registers (two chunks of 8 KB a wave in flight), turned into MFMA operands by byte
 // permutes, 16 rows of x a block.  The waves' sums are added in wave order, the pieces' by finish_kernel in piece order.
+// 1 x 4096 x 14336 with w from memory: 24 us in all, 4.9 TB/s (20 in this kernel, 4 in finish_kernel's launch); 61 x 2048
+// x 7168 16 us, 12 of them here.
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -339,7 +347,8 @@ __global__ __launch_bounds__(NW * 64) void thin_kernel(Args p) {
   }
 }
 
-// The pieces' sums in piece order, and the epilogue.  V: columns a thread.
+// The pieces' sums in piece order, and the epilogue.  V: columns a thread.  4 to 6 us: a launch and a
+// chain of loads.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void finish_kernel(Args p) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, n = (int64_t)p.rows * p.cols;
@@ -368,7 +377,8 @@ __global__ __launch_bounds__(256) void finish_kernel(Args p) {
 
 // ---- dz = dy act'(z) and the column sums of dz ---------------------------------------------------------------
 // A workgroup takes 32 lanes x V columns of a range of rows, eight rows at a time, and leaves f32 sums of its range; a
-// second launch adds the ranges in order, so the sums do not depend on timing.  One pass over dy and z.
+// second launch adds the ranges in order, so the sums do not depend on timing.  One pass over dy and z: 4093 x 7168 in
+// bf16, 176 MB, in 36 us with the second launch, 4.9 TB/s (41 with half as many ranges); 8192 x 14336 150 us, 4.7 TB/s.
 constexpr int kSlopeRows = 8;
 template <typename T, int V>
 __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const T* __restrict__ pre, int64_t M,
@@ -435,10 +445,11 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict
 
 static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
-// Row ranges of slope_kernel: some thousand workgroups, ranges of whole row groups.
+// Row ranges of slope_kernel: up to 4096 workgroups (twice as many, of half the rows at least: 39 instead of 36 us), ranges of
+// whole row groups.
 static int64_t slope_ranges(int64_t M, int64_t N) {
   const int64_t by_cols = ceil_div(N, 256);
-  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(M, 4 * kSlopeRows), 2048 / std::max<int64_t>(1, by_cols)));
+  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(M, 4 * kSlopeRows), 4096 / std::max<int64_t>(1, by_cols)));
 }
 
 static int check_sizes(int dtype, int64_t M, int64_t K, int64_t N) {
@@ -461,6 +472,8 @@ enum { PATH_F32, PATH_BIG, PATH_MID, PATH_SMALL, PATH_THIN };
 struct Plan {
   int path, pieces;
 };
+// rows the thin kernel holds in registers, where it is ahead of tiles of 128 rows: 17 x 4096 x 14336 26.0 us against 27.4,
+// 64 rows 31.4 against 34.0; 24 x 2048 x 7168 12.2 against 13.9, 64 rows 14.9 against 15.4
 constexpr int kThinRows = 64;
 static Plan plan(int mode, bool tiles, int64_t rows, int64_t cols, int64_t red) {
   auto count = [&](int64_t b, int64_t n = 0) { return ceil_div(rows, b) * ceil_div(cols, n ? n : b); };
@@ -469,12 +482,18 @@ static Plan plan(int mode, bool tiles, int64_t rows, int64_t cols, int64_t red) 
   auto split = [&](int64_t n, int64_t want, int64_t least) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / n, stages / least), 32));
   };
-  if (!tiles) return {PATH_F32, split(count(64), 512, 8)};
+  // 517 x 258 x 706: 14.4 us in pieces of 4 stages or more, 18.0 of 8, 15.5 of 2; 1000 x 2000 x 1000 50.9, 52.9, 49.1
+  if (!tiles) return {PATH_F32, split(count(64), 512, 4)};
+  // one workgroup a CU: 1 x 4096 x 14336 takes 24.9 us in 2 pieces of 112 workgroups, 30.1 in one, 29.7 in 400 workgroups;
+  // 1 x 14336 x 4096 26.9 in 8 pieces, 30.0 in half as many, 30.5 in twice as many
   if (mode == FWD && rows <= kThinRows) return {PATH_THIN, split(ceil_div(cols, kThinCols), 256, 16)};
-  // three quarters of the CUs with a tile each: below that the smaller tiles are ahead (4093 x 7168 by 7168 x 2048, 128 tiles
-  // of 256 x 256: 156 us in tiles of 128 x 128, 128 in tiles of 256 x 128)
-  if (count(256) >= 192) return {PATH_BIG, 1};
+  // One round of a tile of 256 x 256 a CU takes 1, of 256 x 128 0.8, of 128 x 128 two a CU 1.05, and a second round is
+  // paid whole: the middle ones where they fill one round (300 x 4096 x 16384, 256 of them: 62 us against 80 in 128 large
+  // and 77 in 384 small ones), the large ones behind that (5000 x 4096 x 2048, 160 of them: 83 us against 115 in 320 middle
+  // and 109 in 640 small ones), the small ones below (200 x 4096 x 16384, 256 of them: 56 us against 71 and 81).
+  if (count(256, 128) > 256) return {PATH_BIG, 1};
   if (count(256, 128) >= 192) return {PATH_MID, 1};
+  // pieces of 16 stages or more (1531 x 1536 x 704: 17 us, 31 in one piece, 20 where pieces may have 8 stages)
   return {PATH_SMALL, split(count(128), 512, 16)};
 }
 static int64_t part_bytes(int64_t rows, int64_t cols, int64_t red, int mode) {
@@ -520,7 +539,8 @@ static int launch_mode(const Args& p, int path, int dtype, hipStream_t st) {
   if (path == PATH_F32) return dtype == MTX_F32 ? launch_f32<float, MODE>(p, st) : launch_f32<uint16_t, MODE>(p, st);
   if (path == PATH_THIN) {
     const dim3 grid((unsigned)(ceil_div(p.cols, kThinCols) * p.pieces));
-    // half the memory-side cache or more: nothing of w is found there again by the time it is next used
+    // half the memory-side cache or more: nothing of w is found there again by the time it is next used (8 x 8192 x 28672:
+    // 73 us against 81; w of 29 MB used again and again: 8.5 us streamed, 6.6 kept)
     const bool stream = (int64_t)p.red * p.cols * 2 >= (int64_t)128 << 20;
 #define MTX_THIN(TB, NW)                                                                                      \
   do {                                                                                                        \

@@ -130,6 +130,13 @@ def test_large(dev, size):
     check(dev, *size, torch.bfloat16, ACTS[n], True, n % 2 == 0, True)
 
 
+@pytest.mark.parametrize("size", [(3330, 136, 2056), (3330, 128, 2056), (3330, 2056, 136), (3330, 2056, 128),
+                                  (150, 3336, 2056), (96, 3336, 2056), (4099, 2056, 72), (5000, 264, 2056)])
+def test_each_product_in_each_tile(dev, size):
+    """The forward product and both gradients in middle and in large tiles that hang over, with whole and cut stages."""
+    check(dev, *size, torch.bfloat16, "silu", True, False, True)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_empty(dev, dtype):
     from mintext_amd.kernels import linear
