@@ -673,12 +673,20 @@ __global__ __launch_bounds__(256, 1) void chain_kernel(ChainArgs a) {
 template <bool A, bool B, bool TWO, int DIAG> using Big = Tile<F16, 4, 4, 2, 2, 4, A, B, false, TWO, DIAG>;
 template <bool A, bool B, bool TWO, int DIAG> using Small = Tile<F16, 2, 2, 2, 2, 4, A, B, false, TWO, DIAG>;
 
-constexpr int kBigTiles = 192;
+// Whether a launch takes its `big` tiles of 256 x 256, one a CU, rather than `small` ones of 128 x 128, two a CU.  A round of
+// small ones takes 0.7 of one of big ones, and a last round that is not full costs about half of what it lacks, but
+// one is always paid whole.  Symmetric products, big against small: 16 x 1408 (336, 1056 tiles) 97, 80 us; 24 x 1024
+// (240, 864) 46, 54; 10 x 1024 (100, 360) 35, 25; 128 x 768 (768, 2688) 122, 142.  X <- P X: 12 x 2048 x 1408 (576, 2112)
+// 152, 167; 1 x 2048 x 7168 (224, 896) 70, 82.
+static bool takes_big(int64_t S, int64_t big, int64_t small) {
+  const double rounds = big / 256.0, cost = std::max(1.0, 0.5 * (rounds + std::ceil(rounds)));
+  return S >= 256 && cost <= 0.7 * std::max(1.0, small / 512.0);
+}
 
 template <bool COLS, bool TWO, int DIAG>
 static int launch_sym(const SymArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { const int64_t n = ceil_div(a.S, b); return a.np * a.E * (n * (n + 1) / 2); };
-  if (tiles(256) >= kBigTiles && a.S >= 256)
+  if (takes_big(a.S, tiles(256), tiles(128)))
     hipLaunchKernelGGL((sym_kernel<Big<COLS, COLS, TWO, DIAG>, COLS, TWO, DIAG>), dim3((unsigned)tiles_grid(tiles(256))),
                        dim3(256), 0, st, a);
   else
@@ -694,7 +702,7 @@ static int launch_chain(const ChainArgs& a, hipStream_t st) {
 template <bool TALL, bool TWO, int OUT, typename D>
 static int launch_apply_out(const ApplyArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { return a.E * ceil_div(a.s.Mp, b) * ceil_div(a.s.Np, b); };
-  if (tiles(256) >= kBigTiles && a.s.S >= 256)
+  if (takes_big(a.s.S, tiles(256), tiles(128)))
     hipLaunchKernelGGL((apply_kernel<Big<false, !TALL, TWO, DIAG_VECTORS>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(256))),
                        dim3(256), 0, st, a);
   else

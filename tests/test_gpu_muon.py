@@ -138,6 +138,18 @@ def test_many_and_large(dev, size, precision):
     assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("precision", ["half", "full"])
+@pytest.mark.parametrize("size", [(80, 500, 548, 600), (80, 552, 504, 100)])
+def test_large_tiles_hang_over(dev, size, precision):
+    """Stacks with enough large tiles for the symmetric products too, whose last tile is not full."""
+    from mintext_amd.kernels import newton_schulz
+
+    x = gradient(dev, *size, torch.bfloat16)
+    got = newton_schulz(x.float(), precision=precision)
+    held(got, x, precision == "full", V, which=[0, 1, 40, 79])
+    assert torch.isfinite(got).all()
+
+
 def test_in_parts(dev):
     """A stack whose workspace would pass 4 GiB goes through in parts."""
     from mintext_amd import _lib as L
