@@ -5,12 +5,12 @@
 // the first A: symmetric, and they commute.  So g steps need one Gram product, S x S symmetric products and one
 // product X <- P X with P = Q_g ... Q_1, in all 3 S^2 L + (4 g - 3) S^3 operations (a symmetric product computes
 // half its tiles), where a step by itself needs 3 S^2 L + S^3.  At L = 2.67 S (768 x 2048) five steps need
-// 45 S^3 by themselves (63 if all tiles were computed), 35 as 2 + 2 + 1, 30 as 3 + 2; at L = S always 20.
+// 45 S^3 by themselves (63 if all tiles were computed), 35 as 2 + 2 + 1, 30 as 3 + 2; at L = S always 20, fastest by themselves.
 // A's small eigenvalues are squares of X's and grow by a^2 a step, so what the rounding of A adds grows as well and is
 // not taken back before the next Gram product: a group holds three steps at most.  In simulation with gradients of
 // rank 1 to full rank (f16 operands) five steps end 0.07 to 0.19 % off as 2 + 2 + 1, 0.1 to 0.5 % as 3 + 2, up to 14 %
 // or beyond f16's range as one group.  The caller chooses: 2 where the result itself is asked for, 3 where it is
-// a small change of weights.
+// a small change of weights, 1 for matrices that are nearly square.
 //
 // Numbers: |x|_F bounds every singular value by 1 and the polynomials bound them from there, so every matrix has a
 // power-of-two scale, chosen by the caller from those bounds, that puts it into f16's range: 11 bits where
@@ -108,7 +108,8 @@ __device__ __forceinline__ void load_update(const Source& s, int64_t e, int64_t 
     }
   }
 }
-// The workgroups of matrix e leave f64 sums of their rows' squares in part[e][blockIdx.x].
+// The workgroups of matrix e leave f64 sums of their rows' squares in part[e][blockIdx.x].  A pass over x bound by memory:
+// 128 x 768 x 2048 in bf16 90 us, 4.5 TB/s.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void norm_kernel(Source s, int M, int N, int rows, double* __restrict__ part) {
   __shared__ double w[4];
@@ -152,7 +153,7 @@ __device__ __forceinline__ void unpack8(uint64_t p, float v[8]) {
 // X = x 2^e in f16; beside it either what that loses as 8-bit floats or the lo plane and what f32 holds beyond it (a bit
 // at most: the steps carry it up by a^5 where x is singular); zeros past the last row and column, with e such that |x|_F + eps
 // comes to [2^13, 2^14): a bf16 x is held exactly but for elements below 2^-27 of its norm.  Every workgroup adds the
-// parts of its matrix in the same order.
+// parts of its matrix in the same order.  Bound by memory: 128 x 768 x 2048 in bf16 148 us, 5.4 TB/s.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void convert_kernel(Source s, int M, int N, int Mp, int Np, int rows,
                                                       const double* __restrict__ part, int nparts, float eps,
@@ -307,6 +308,9 @@ __device__ __forceinline__ void lower(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
+// One workgroup a tile of the lower triangle, which it also stores mirrored: 128 Gram products of 768 x 2048 take 214 us,
+// 0.96 PFLOP/s of the tiles computed, and 128 products of 768^3 about 120 us, 0.64: with 24 ring stages a tile the way out
+// (f16 through LDS, once in rows and once turned) is 50 us of it, and the tiles of a CU do not overlap it with products.
 // COLS: the reduction runs down u's and v's columns (the Gram product of a tall X); otherwise along their rows.
 template <class T, bool COLS, bool TWO, int DIAG>
 __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void sym_kernel(SymArgs a) {
@@ -396,6 +400,10 @@ struct ApplyArgs {
   float lr, decay, factor;
   const float* lr_dev;
 };
+// One workgroup a tile of X, the diagonal's share, the scale and the optimiser's step on its way out.  Long reductions
+// are bound by the matrix cores (2048 x 7168: 1.04 PFLOP/s), 128 x 768 x 2048 by both: 450 to 570 us, 330 of them products,
+// the rest 1.2 GB of X and what it lacks, read and written while the CU's matrix cores wait.  What the way out reads is loaded
+// a block of 32 rows ahead; with the old weights and X's lost part as the accumulators' start the kernel took 1.4 times as long.
 // D: the type of what is stored or stepped.
 template <class T, bool TALL, bool TWO, int OUT, typename D>
 __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(ApplyArgs a) {
@@ -521,8 +529,9 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
 }
 
 // ---- S <= 128: the Gram product and all S x S products of a group in one workgroup --------------------------------
-// Between launches such products wait for memory and for each other, 8 to 10 us apiece for 2 of work (8 x 128 x 512: 26
-// launches, 185 us).  Here one workgroup takes a matrix from X to P: A and P stay in its registers in f32, the operands
+// Between launches such products wait for memory and for each other, 8 to 10 us apiece for 2 of work (8 x 128 x 512 in f32: 26
+// launches and 185 us that way, 6 launches and 113 us this way, 43 of them a group of three steps here, a chain of eight
+// products that each wait for the one before).  Here one workgroup takes a matrix from X to P: A and P stay in its registers in f32, the operands
 // of a product in LDS in two f16 planes, in "half" too, as the products cost little.  Two slots of 64 KB: Q, and in
 // turn A, T and P.
 constexpr int kChainS = 128;
@@ -720,13 +729,14 @@ static int launch_apply(int out, const ApplyArgs& a, hipStream_t st) {
                           : launch_apply_out<TALL, TWO, OUT_STEP, uint16_t>(a, st);
 }
 
-// Workgroups of a matrix in the norm and conversion launches.
+// Workgroups of a matrix in the norm and conversion launches: 2048 in all (half or twice as many: the same within 2 %).
 static int64_t parts_of(int64_t E, const Shape& s) {
   const int64_t by_size = std::max<int64_t>(1, s.xs / 8192);
   return std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(by_size, s.Mp), std::min<int64_t>(512, ceil_div(2048, E))));
 }
 
-// Matrices that go through the chain together.
+// The workspace that matrices of one chain share: 64 x 2048 x 7168 takes 26.3 ms with 16 GiB, 26.7 with 4, 30.6 with 1 and 35.8
+// with a quarter, as fewer tiles fill a launch's last round.
 constexpr int64_t kChunkBytes = (int64_t)4 << 30;
 // bytes an element of X takes: the first, with what it lacks, and the second
 static int64_t x_bytes(int planes) { return planes == 2 ? 6 + 4 : 3 + 3; }

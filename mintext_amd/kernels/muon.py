@@ -27,9 +27,12 @@ import torch
 from .. import _lib as L
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-# Steps between two Gram products, at most: fewer products with three, smaller errors with two, except for matrices whose
-# products between the two are held in 22 bits in any case
-_GROUP_RESULT, _GROUP_STEP, _SMALL = 2, 3, 128
+# Steps between two Gram products, at most: fewer products with three, smaller errors with fewer (128 x 768 x 2048, five steps:
+# 3.30 ms in threes, 3.65 in twos, 4.39 by themselves).  Matrices of _SMALL or less on a side take threes in any case: their
+# products in between are held in 22 bits (64 x 128 x 1408 in float32 212 us, 265 in twos).  Those near square gain nothing
+# from groups, whose symmetric products cost what the others save: one of 2048 x 2048 takes 366 us in single steps, 405 in
+# twos, 419 in threes; 8 of 1024 x 1280 445, 446, 440; 128 of 768 x 1152 3.02 ms, 2.85, 2.71.
+_GROUP_RESULT, _GROUP_STEP, _SMALL, _SQUARE = 2, 3, 128, 1.25
 
 
 @functools.lru_cache(maxsize=64)
@@ -92,6 +95,8 @@ def _arguments(steps, coefficients, eps, precision, t, group):
     planes = 2 if precision == "full" or (precision is None and t.dtype == torch.float32) else 1
     if min(t.shape[-2:]) <= _SMALL:
         group = _GROUP_STEP
+    elif max(t.shape[-2:]) <= _SQUARE * min(t.shape[-2:]):
+        group = 1
     return _schedule(steps, c, group), planes
 
 

@@ -81,7 +81,8 @@ def groups_of(steps, most):
 
 def tolerance(x, want, full, eps=1e-7, steps=5, coef=COEF, most=2):
     """(2-norm, largest) error allowed before the output is rounded, of one matrix."""
-    groups = groups_of(steps, 3 if min(x.shape) <= 128 else most)
+    S, L = min(x.shape), max(x.shape)
+    groups = groups_of(steps, 3 if S <= 128 else 1 if L <= 1.25 * S else most)
     same, count = chain64(x, groups, eps, coef)
     assert (same - want).norm() <= 1e-9 * want.norm()  # the groups change nothing in exact arithmetic
     signs = torch.Generator(device=x.device).manual_seed(1)
@@ -139,7 +140,7 @@ def test_many_and_large(dev, size, precision):
 
 
 @pytest.mark.parametrize("precision", ["half", "full"])
-@pytest.mark.parametrize("size", [(80, 500, 548, 600), (80, 552, 504, 100)])
+@pytest.mark.parametrize("size", [(80, 500, 548, 600), (80, 552, 504, 100), (80, 500, 704, 600), (80, 704, 504, 100)])
 def test_large_tiles_hang_over(dev, size, precision):
     """Stacks with enough large tiles for the symmetric products too, whose last tile is not full."""
     from mintext_amd.kernels import newton_schulz
