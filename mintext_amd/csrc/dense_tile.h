@@ -6,7 +6,7 @@
 // registers).  Either operand may have its reduction contiguous in memory ("rows": A [m][k], B [n][k]) or
 // strided ("cols": A [k][m], B [k][n]); the latter is turned by ds_read_b64_tr_b16.  LDS layouts of a stage:
 //   rows: 64 bytes a row, 16-byte chunk c of row r at chunk c ^ ((r >> 2) & 3)
-//   cols: one line a reduction element, chunk c of element k at chunk c ^ 4 (k & 3)
+//   cols: one line a reduction element, chunk c of element k at chunk c ^ 4 (k & 3) (64 columns: c ^ 2 (k & 2))
 // with which neither the loads' writes nor the fragment reads conflict.
 //
 // A 256 x 256 tile keeps 256 accumulators a lane and one workgroup a CU; what bounds it is the matrix cores at the clock that the
@@ -85,8 +85,11 @@ struct Diagonal {
 enum { DIAG_NONE = 0, DIAG_VECTORS = 1, DIAG_CONST = 2 };
 
 __device__ __forceinline__ int row_off(int r, int c) { return r * 64 + ((c ^ ((r >> 2) & 3)) << 4); }
+// what chunks of line k of a cols operand are turned by: lines of 64 columns take turns with the next but one
 template <int COLS>
-__device__ __forceinline__ int col_off(int k, int c) { return k * (COLS * 2) + ((c ^ ((k & 3) << 2)) << 4); }
+__device__ __forceinline__ int col_turn(int k) { return COLS == 64 ? (k & 2) << 1 : (k & 3) << 2; }
+template <int COLS>
+__device__ __forceinline__ int col_off(int k, int c) { return k * (COLS * 2) + ((c ^ col_turn<COLS>(k)) << 4); }
 
 template <class F, int TM_, int TN_, int WM_, int WN_, int NST_, bool A_COLS, bool B_COLS, bool TAIL = false,
           bool TWO = false, int DIAG = DIAG_NONE>
@@ -111,7 +114,7 @@ struct Tile {
     const int seg = wave * INSTR + i;
     if constexpr (COLS) {
       constexpr int CH = W / 8, PER = 64 / CH;  // chunks per line, lines per instruction
-      const int k = seg * PER + lane / CH, c = (lane % CH) ^ ((k & 3) << 2);
+      const int k = seg * PER + lane / CH, c = (lane % CH) ^ col_turn<W>(k);
       return (uint32_t)min(k, kleft - 1) * (uint32_t)(o.ld * 2) + (uint32_t)min(c * 8, o.left - 8) * 2u;
     } else {
       const int r = seg * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 2) & 3);

@@ -681,6 +681,7 @@ __global__ __launch_bounds__(256, 1) void chain_kernel(ChainArgs a) {
 // ---- the chain of launches ---------------------------------------------------------------------------------------
 template <bool A, bool B, bool TWO, int DIAG> using Big = Tile<F16, 4, 4, 2, 2, 4, A, B, false, TWO, DIAG>;
 template <bool A, bool B, bool TWO, int DIAG> using Small = Tile<F16, 2, 2, 2, 2, 4, A, B, false, TWO, DIAG>;
+template <bool A, bool B, bool TWO, int DIAG> using Least = Tile<F16, 1, 1, 2, 2, 8, A, B, false, TWO, DIAG>;
 
 // Whether a launch takes its `big` tiles of 256 x 256, one a CU, rather than `small` ones of 128 x 128, two a CU.  A round of
 // small ones takes 0.7 of one of big ones, and a last round that is not full costs about half of what it lacks, but
@@ -692,10 +693,18 @@ static bool takes_big(int64_t S, int64_t big, int64_t small) {
   return S >= 256 && cost <= 0.7 * std::max(1.0, small / 512.0);
 }
 
+// Where all tiles of 64 x 64 find a place at once, two a CU, it is one tile's chain of stages and its way out that count, and the
+// smallest is the quickest: 1 x 1024 (136 of them, 36 of 128 x 128) 9 us against 13 and its Gram product with 4096 20
+// against 35, 8 x 256 in f32 8 against 13; with more than that 1 x 2048 (528, 136) 28 against 22.
+constexpr int64_t kLeastTiles = 512;
+
 template <bool COLS, bool TWO, int DIAG>
 static int launch_sym(const SymArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { const int64_t n = ceil_div(a.S, b); return a.np * a.E * (n * (n + 1) / 2); };
-  if (takes_big(a.S, tiles(256), tiles(128)))
+  if (tiles(64) <= kLeastTiles)
+    hipLaunchKernelGGL((sym_kernel<Least<COLS, COLS, TWO, DIAG>, COLS, TWO, DIAG>), dim3((unsigned)tiles_grid(tiles(64))),
+                       dim3(256), 0, st, a);
+  else if (takes_big(a.S, tiles(256), tiles(128)))
     hipLaunchKernelGGL((sym_kernel<Big<COLS, COLS, TWO, DIAG>, COLS, TWO, DIAG>), dim3((unsigned)tiles_grid(tiles(256))),
                        dim3(256), 0, st, a);
   else
