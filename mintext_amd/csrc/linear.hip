@@ -226,8 +226,8 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void tile_
 }
 
 // ---- few rows (serving): the time is that of reading w once ---------------------------------------------------------
-// A workgroup owns 128 columns and a piece of the reduction; its waves (eight, or four where 64 rows need the registers) take the piece's 32-element chunks in turn,
-// w straight from memory into registers (two chunks of 8 KB a wave in flight), turned into MFMA operands by byte
+// A workgroup owns 128 columns and a piece of the reduction; its waves (eight, or four where 64 rows need the registers)
+// take the piece's 32-element chunks in turn, w straight from memory into registers (two chunks of 8 KB a wave in flight), turned into MFMA operands by byte
 // permutes, 16 rows of x a block.  The waves' sums are added in wave order, the pieces' by finish_kernel in piece order.
 // 1 x 4096 x 14336 with w from memory: 24 us in all, 4.9 TB/s (20 in this kernel, 4 in finish_kernel's launch); 61 x 7168
 // x 2048 16 us, 12 of them here.
