@@ -530,7 +530,7 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
 
 // ---- S <= 128: the Gram product and all S x S products of a group in one workgroup --------------------------------
 // Between launches such products wait for memory and for each other, 8 to 10 us apiece for 2 of work (8 x 128 x 512 in f32:
-// 26 launches and 185 us that way, 6 launches and 113 us this way, 43 of them a group of three steps here, a chain of
+// 26 launches and 185 us that way, 6 launches and 107 us this way, 43 of them a group of three steps here, a chain of
 // eight products that each wait for the one before).  Here one workgroup takes a matrix from X to P: A and P stay in its
 // registers in f32, the operands of a product in LDS in two f16 planes, in "half" too, as the products cost little.
 // Two slots of 64 KB: Q, and in turn A, T and P.
@@ -695,7 +695,8 @@ static bool takes_big(int64_t S, int64_t big, int64_t small) {
 
 // Where all tiles of 64 x 64 find a place at once, two a CU, it is one tile's chain of stages and its way out that count, and the
 // smallest is the quickest: 1 x 1024 (136 of them, 36 of 128 x 128) 9 us against 13 and its Gram product with 4096 20
-// against 35, 8 x 256 in f32 8 against 13; with more than that 1 x 2048 (528, 136) 28 against 22.
+// against 35, 8 x 256 in f32 8 against 13; with more than that 1 x 2048 (528, 136) 28 against 22.  X <- P X likewise: 8 x 128 x
+// 512 in f32, five steps with two of them, 107 us against 113.
 constexpr int64_t kLeastTiles = 512;
 
 template <bool COLS, bool TWO, int DIAG>
@@ -720,7 +721,10 @@ static int launch_chain(const ChainArgs& a, hipStream_t st) {
 template <bool TALL, bool TWO, int OUT, typename D>
 static int launch_apply_out(const ApplyArgs& a, hipStream_t st) {
   auto tiles = [&](int b) { return a.E * ceil_div(a.s.Mp, b) * ceil_div(a.s.Np, b); };
-  if (takes_big(a.s.S, tiles(256), tiles(128)))
+  if (tiles(64) <= kLeastTiles)
+    hipLaunchKernelGGL((apply_kernel<Least<false, !TALL, TWO, DIAG_VECTORS>, TALL, TWO, OUT, D>),
+                       dim3((unsigned)tiles_grid(tiles(64))), dim3(256), 0, st, a);
+  else if (takes_big(a.s.S, tiles(256), tiles(128)))
     hipLaunchKernelGGL((apply_kernel<Big<false, !TALL, TWO, DIAG_VECTORS>, TALL, TWO, OUT, D>), dim3((unsigned)tiles_grid(tiles(256))),
                        dim3(256), 0, st, a);
   else

@@ -269,6 +269,27 @@ def test_muon_update(dev, size, types):
             assert off.norm() <= norm and (off.abs() <= tol).all(), (e, float(off.norm()), float(norm))
 
 
+@pytest.mark.parametrize("pt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [(30, 200, 300), (30, 304, 200), (80, 500, 704), (80, 703, 504)])
+def test_muon_update_of_many(dev, size, pt):
+    """Stacks whose step runs on the middle (30) and on the large tiles (80); rows of whole 16-byte pieces, and not."""
+    from mintext_amd.kernels import muon_update
+
+    E, M, N = size
+    g = torch.Generator().manual_seed(sum(size))
+    p = (torch.randn(*size, generator=g) * 0.02).to(pt).to(dev)
+    m = torch.randn(*size, generator=g).to(dev)
+    grad = gradient(dev, E, M, N, 150, pt)
+    which = [0, 1, E // 2, E - 1]
+    refs = [step64(p[e], grad[e], m[e], 0.02, 0.9, True, 0.1, 0.3, pt == torch.float32) for e in which]
+    muon_update(p, grad, m, lr=0.02, beta=0.9, weight_decay=0.1, scale=0.3)
+    for e, (w, m1, tol_m, (norm, tol)) in zip(which, refs):
+        assert ((m[e].double() - m1).abs() <= tol_m).all()
+        off = p[e].double() - w
+        assert off.norm() <= norm and (off.abs() <= tol).all(), (e, float(off.norm()), float(norm))
+    assert torch.isfinite(p).all()
+
+
 def test_muon_update_views(dev):
     """The halves of a fused stack step by themselves; the rest of it is not written."""
     from mintext_amd.kernels import muon_update
