@@ -529,11 +529,12 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
 }
 
 // ---- S <= 128: the Gram product and all S x S products of a group in one workgroup --------------------------------
-// Between launches such products wait for memory and for each other, 8 to 10 us apiece for 2 of work (8 x 128 x 512 in f32:
-// 26 launches and 185 us that way, 6 launches and 107 us this way, 43 of them a group of three steps here, a chain of
-// eight products that each wait for the one before).  Here one workgroup takes a matrix from X to P: A and P stay in its
-// registers in f32, the operands of a product in LDS in two f16 planes, in "half" too, as the products cost little.
-// Two slots of 64 KB: Q, and in turn A, T and P.
+// Between launches such products wait for memory and for each other, 5 to 9 us apiece for 2 of work.  Here one workgroup
+// takes a matrix from X to P, a chain of up to eight products that each wait for the one before: A and P stay in its
+// registers in f32, the operands of a product in LDS in two f16 planes, in "half" too, as the products cost little.  Two
+// slots of 64 KB: Q, and in turn A, T and P.  8 x 128 x 512 in f32: 6 launches and 107 us, 43 a group of three steps here,
+// where products by themselves take 26 launches and 124; 64 x 128 x 1408 210 against 237, 1 x 64 x 256 80 against 88.
+// "half" is level (84 and 82, 135 and 134, 69 and 68) with f32 accuracy in between and a quarter of the launches.
 constexpr int kChainS = 128;
 struct ChainArgs {
   const f16* x;
