@@ -19,7 +19,7 @@ ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # MTX_
 
 
 def _check(x, weight, bias, activation, residual):
-    """(M, K, N, activation code); a serving call spends as long on the host as on the GPU, hence no loops."""
+    """The activation's code; a serving call spends as long on the host as on the GPU, hence no loops."""
     act = ACTIVATIONS.get(activation, -1)
     if act < 0:
         raise ValueError(f"activation must be one of {sorted(k for k in ACTIVATIONS if k)} or None, got {activation!r}")
@@ -37,12 +37,17 @@ def _check(x, weight, bias, activation, residual):
     if (weight.dtype is not dt or (bias is not None and bias.dtype is not dt)
             or (residual is not None and residual.dtype is not dt)):
         raise TypeError(f"linear operands must share one dtype, {dt} as x")
-    return (x.numel() // K if K else math.prod(xs[:-1])), K, N, act
+    return act
 
 
-def _forward(x, weight, bias, residual, sizes, keep):
+def _sizes(x, weight):
+    K, N = weight.shape
+    return (x.numel() // K if K else math.prod(x.shape[:-1])), K, N
+
+
+def _forward(x, weight, bias, residual, act, keep):
     dev = L.require_device(x, weight, bias, residual)
-    M, K, N, act = sizes
+    M, K, N = _sizes(x, weight)
     x, weight = x.contiguous(), weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
@@ -56,11 +61,12 @@ def _forward(x, weight, bias, residual, sizes, keep):
 
 
 class _Linear(torch.autograd.Function):
+    # The sizes are taken in here: a jit trace calls this again for other tensors, with its first call's other arguments.
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, sizes):
-        out, pre = _forward(x, weight, bias, residual, sizes, True)
+    def forward(ctx, x, weight, bias, residual, act):
+        out, pre = _forward(x, weight, bias, residual, act, True)
         ctx.save_for_backward(x, weight, pre)
-        ctx.sizes = sizes
+        ctx.act = act
         return out
 
     @staticmethod
@@ -70,7 +76,7 @@ class _Linear(torch.autograd.Function):
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         dev = L.require_device(x, weight, dy)
         x, weight, dy = x.contiguous(), weight.contiguous(), dy.contiguous()
-        M, K, N, act = ctx.sizes
+        (M, K, N), act = _sizes(x, weight), ctx.act
         dz = torch.empty((M, N), dtype=x.dtype, device=dev) if act and (need_x or need_w or need_b) else None
         dx = torch.empty_like(x) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
@@ -96,7 +102,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     Returns:
         [..., N] in x's dtype.  Differentiable (once) in all four tensors.
     """
-    sizes = _check(x, weight, bias, activation, residual)
+    act = _check(x, weight, bias, activation, residual)
     if L.plain_forward(x, weight, bias, residual):
-        return _forward(x, weight, bias, residual, sizes, False)[0]
-    return _Linear.apply(x, weight, bias, residual, sizes)
+        return _forward(x, weight, bias, residual, act, False)[0]
+    return _Linear.apply(x, weight, bias, residual, act)
