@@ -213,6 +213,16 @@ def plain_forward(*tensors) -> bool:
     return getattr(torch.autograd.forward_ad, "_current_level", 0) < 0 and _functorch_level() is None
 
 
+def refuse_watched(name: str, *tensors) -> None:
+    """Raise for an op without an autograd Function where something would have to see it: a jit trace, which
+    records none of the kernels it launches, or a forward-mode tangent, which its result would not have."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{name} cannot be recorded by a jit trace")
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative: pass tensors without a tangent (x.detach())")
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
 

@@ -153,8 +153,10 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, *, coefficients=COEFFICIENTS,
         precision: "half", "full" or None, by x's dtype (see the module).
 
     Returns:
-        a dense tensor of x's shape and dtype.  Not differentiable.
+        a dense tensor of x's shape and dtype.  Not differentiable: an x that requires a gradient or has a
+        forward-mode tangent is refused, and so is a jit trace.
     """
+    L.refuse_watched("newton_schulz", x)
     _check_stack(x, "x")
     sched, planes = _arguments(steps, coefficients, eps, precision, x, _GROUP_RESULT)
     if x.requires_grad and torch.is_grad_enabled():
@@ -186,8 +188,9 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
         precision: as in ``newton_schulz``, by param's dtype.
 
     Returns:
-        param.
+        param.  A tensor with a forward-mode tangent is refused, and so is a jit trace.
     """
+    L.refuse_watched("muon_update", param, grad, momentum, lr if isinstance(lr, torch.Tensor) else None)
     for t, name in ((param, "param"), (grad, "grad"), (momentum, "momentum")):
         _check_stack(t, name)
         if t.shape != param.shape:
