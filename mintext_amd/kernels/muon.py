@@ -140,6 +140,35 @@ def _writable(t: torch.Tensor, name: str) -> torch.Tensor:
     return v
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [E, M, N] stacks, of which one is as ``_writable`` returns it, share memory.  Stacks that lie between
+    each other's rows with the same strides (halves of a fused buffer) do not; with others they count as sharing it."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    E, M, N = a.shape
+    da, db = ([s * t.element_size() for s in _strides(t)] for t in (a, b))
+    na, nb = N * a.element_size(), N * b.element_size()
+    apart = b.data_ptr() - a.data_ptr()
+    extent = lambda d, n: (E - 1) * d[0] + (M - 1) * d[1] + n
+    if apart >= extent(da, na) or -apart >= extent(db, nb):
+        return False
+    steps = [(d, n) for d, e, n in zip(da, db, (E, M)) if n > 1]
+    if any(d != e for d, e, n in zip(da, db, (E, M)) if n > 1):
+        return True
+    # Is there a whole combination of the strides that brings a row of b to a row of a?  The smaller stride's reach lies
+    # within the larger one, so that each has two candidates.
+    steps.sort(reverse=True)
+    reach = max(na, nb)
+    for d, n in reversed(steps):
+        if reach > d:
+            return True
+        reach += (n - 1) * d
+    rests = [apart]
+    for d, n in steps:
+        rests = [r - k * d for r in rests for k in (r // d, r // d + 1) if abs(k) < n]
+    return any(-nb < r < na for r in rests)
+
+
 def newton_schulz(x: torch.Tensor, steps: int = 5, *, coefficients=COEFFICIENTS, eps: float = 1e-7,
                   precision: str | None = None) -> torch.Tensor:
     """Orthogonalise each matrix of ``x`` [..., M, N] by ``steps`` Newton-Schulz products.
@@ -181,7 +210,8 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
         param: [..., M, N] weights used as ``x @ param``, float32 or bfloat16; updated in place.  A view with rows of
             consecutive elements will do, e.g. the gate half ``gate_up[..., :I]`` of a fused stack.
         grad: its gradient, of the same shape, float32 or bfloat16.
-        momentum: float32 of the same shape, updated in place (zeros before the first step).
+        momentum: float32 of the same shape, updated in place (zeros before the first step).  The three must not share
+            memory.
         lr: learning rate, a number or a float32 device tensor of one element (read when the step runs, so that a
             captured step follows it).
         scale: factor of the update: "spectral" sqrt(max(1, N / M)), "rms" 0.2 sqrt(max(M, N)), or a number.
@@ -215,8 +245,10 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
     p, m = _writable(param, "param"), _writable(momentum, "momentum")
     if param.numel() and len({param.data_ptr(), grad.data_ptr(), momentum.data_ptr()}) < 3:
         raise ValueError("param, grad and momentum must be three different tensors")
-    dev = L.require_device(param, grad, momentum, lr_dev)
     g = _readable(grad.detach())
+    if _overlap(p, m) or _overlap(p, g) or _overlap(m, g):
+        raise ValueError("param, grad and momentum must not share memory")
+    dev = L.require_device(param, grad, momentum, lr_dev)
     E = p.shape[0]
     ws = L.workspace(L.query("mtx_newton_schulz_workspace_size", E, M, N, planes), dev)
     with L.on_device(dev):
