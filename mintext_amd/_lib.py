@@ -218,6 +218,8 @@ def refuse_watched(name: str, *tensors) -> None:
     records none of the kernels it launches, or a forward-mode tangent, which its result would not have."""
     if torch.jit.is_tracing():
         raise RuntimeError(f"{name} cannot be recorded by a jit trace")
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) < 0:
+        return
     for t in tensors:
         if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError(f"{name} has no forward-mode derivative: pass tensors without a tangent (x.detach())")

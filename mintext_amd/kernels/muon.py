@@ -151,18 +151,24 @@ def _writable(t: torch.Tensor, name: str) -> torch.Tensor:
     return v
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses from the first byte of a [E, M, N] stack to behind its last."""
+    E, M, N = t.shape
+    batch, row = _strides(t)
+    start = t.data_ptr()
+    return start, start + ((E - 1) * batch + (M - 1) * row + N) * t.element_size() if t.numel() else start
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two [E, M, N] stacks, of which one is as ``_writable`` returns it, share memory.  Stacks that lie between
     each other's rows with the same strides (halves of a fused buffer) do not; with others they count as sharing it."""
-    if a.numel() == 0 or b.numel() == 0:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0 or a0 == a1 or b0 == b1:
         return False
     E, M, N = a.shape
     da, db = ([s * t.element_size() for s in _strides(t)] for t in (a, b))
     na, nb = N * a.element_size(), N * b.element_size()
-    apart = b.data_ptr() - a.data_ptr()
-    extent = lambda d, n: (E - 1) * d[0] + (M - 1) * d[1] + n
-    if apart >= extent(da, na) or -apart >= extent(db, nb):
-        return False
+    apart = b0 - a0
     steps = [(d, n) for d, e, n in zip(da, db, (E, M)) if n > 1]
     if any(d != e for d, e, n in zip(da, db, (E, M)) if n > 1):
         return True
@@ -257,7 +263,8 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
     if param.numel() and len({param.data_ptr(), grad.data_ptr(), momentum.data_ptr()}) < 3:
         raise ValueError("param, grad and momentum must be three different tensors")
     g = _readable(grad.detach())
-    if _overlap(p, m) or _overlap(p, g) or _overlap(m, g):
+    spans = sorted(map(_span, (p, m, g)))
+    if (spans[0][1] > spans[1][0] or spans[1][1] > spans[2][0]) and (_overlap(p, m) or _overlap(p, g) or _overlap(m, g)):
         raise ValueError("param, grad and momentum must not share memory")
     dev = L.require_device(param, grad, momentum, lr_dev)
     E = p.shape[0]
