@@ -447,9 +447,12 @@ int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre
  *   holds A, Q = a I + b A + c A^2, Q A, the group's product P of Qs and X after it, and whether
  *   the step ends a group (1) or the next one goes on from Q A Q (0).  P's scale is Q's at the
  *   first step of a group.  The scales have to keep each matrix's singular values below 65504.
- * planes: 1 = matrices in one f16 plane between products, 2 = in two (float32 results).
+ * planes: 1 = matrices in one f16 plane between products, 2 = in two, MTX_NS_F64 = in float64, with
+ *   products and sums in float64 and a, b, c and what float32 has lost of each of them as the
+ *   schedule's first six floats a step (the other three are not read).
  * E <= 65535, M and N <= 2^20, min(M, N) <= 2^15.  Large stacks go through in parts, so that the
  * workspace (256-byte aligned) stays below 4 GiB or one matrix's need.                        */
+#define MTX_NS_F64 64
 int64_t mtx_newton_schulz_workspace_size(int64_t E, int64_t M, int64_t N, int planes);
 int mtx_newton_schulz(const void* x, int dtype, int64_t E, int64_t M, int64_t N, int64_t x_batch, int64_t x_row,
                       const float* schedule, int steps, float eps, int planes, void* out, int64_t out_batch,

@@ -28,6 +28,7 @@ MTX_ERR_HIP = -4
 MTX_F32, MTX_BF16, MTX_FP8E4M3 = 0, 1, 2
 MTX_SCORING_SOFTMAX, MTX_SCORING_SIGMOID_GROUP = 0, 1
 MTX_GMM_OP_FWD, MTX_GMM_OP_SWIGLU, MTX_GMM_OP_DLHS = 0, 1, 2
+MTX_NS_F64 = 64
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64

@@ -15,14 +15,16 @@
 // Numbers: |x|_F bounds every singular value by 1 and the polynomials bound them from there, so every matrix has a
 // power-of-two scale, chosen by the caller from those bounds, that puts it into f16's range: 11 bits where
 // bf16 has 8, at the same matrix-core rate ("half").  f32 results take two f16 planes, hi + lo, and three products for
-// one ("full": 22 bits).  Sums are f32, |x|_F is summed in f64.  Two things cost more than all other roundings and are
-// kept apart.  What f16 loses of the diagonals of Q and P, where their size is, is an f32 vector beside the matrix and
-// joins each product as a diagonal matrix (rank 8: 0.28 instead of 0.85 % off).  And in "half" X has what f16
-// loses of it as 8-bit floats: in X <- P X the diagonal's share, in f32 on the way out, takes it too, as in the
-// directions in which X is small P is a multiple of I (rank 32, 2 + 2 + 1: 0.17 instead of 0.63 %).  Momentum is f32.
+// one ("full": 22 bits).  Sums are f32, |x|_F is summed in f64.  ("double", f64 throughout, has kernels of its own.)  Two
+// things cost more than all other roundings and are kept apart.  What f16 loses of the diagonals of Q and P, where their
+// size is, is an f32 vector beside the matrix and joins each product as a diagonal matrix (rank 8: 0.28 instead of
+// 0.85 % off).  And in "half" X has what f16 loses of it as 8-bit floats: in X <- P X the diagonal's share, in f32 on the
+// way out, takes it too, as in the directions in which X is small P is a multiple of I (rank 32, 2 + 2 + 1: 0.17 instead
+// of 0.63 %).  Momentum is f32.
 #include "common.h"
 #include "dense_tile.h"
 #include "f32_tile.h"
+#include "f64_tile.h"
 #include <algorithm>
 #include <cmath>
 
@@ -150,6 +152,17 @@ __device__ __forceinline__ void unpack8(uint64_t p, float v[8]) {
     v[4 * h + 3] = b[1];
   }
 }
+// |x|_F: the workgroup adds the parts of matrix e, in the same order in each.
+__device__ __forceinline__ double norm_of(const double* __restrict__ part, int64_t e, int nparts) {
+  __shared__ double w[4];
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < nparts; i += 256) sum += part[e * nparts + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  return sqrt((w[0] + w[1]) + (w[2] + w[3]));
+}
 // X = x 2^e in f16; beside it either what that loses as 8-bit floats or the lo plane and what f32 holds beyond it (a bit
 // at most: the steps carry it up by a^5 where x is singular); zeros past the last row and column, with e such that |x|_F + eps
 // comes to [2^13, 2^14): a bf16 x is held exactly but for elements below 2^-27 of its norm.  Every workgroup adds the
@@ -160,15 +173,8 @@ __global__ __launch_bounds__(256) void convert_kernel(Source s, int M, int N, in
                                                       f16* __restrict__ X, f16* __restrict__ Xlo,
                                                       f16* __restrict__ Xrest, uint64_t* __restrict__ Xlo8,
                                                       Scale* scales) {
-  __shared__ double w[4];
   const int64_t e = blockIdx.y;
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < nparts; i += 256) sum += part[e * nparts + i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  const double norm = sqrt((w[0] + w[1]) + (w[2] + w[3])) + (double)eps;
+  const double norm = norm_of(part, e, nparts) + (double)eps;
   const bool fine = norm <= 1e300;  // NaN, infinity: the result is NaN
   const int ex = fine ? 13 - ilogb(norm) : 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -743,6 +749,10 @@ static int launch_apply(int out, const ApplyArgs& a, hipStream_t st) {
                           : launch_apply_out<TALL, TWO, OUT_STEP, uint16_t>(a, st);
 }
 
+// f64: tiles of 64 x 64 from three a CU on, of 32 x 32 below, which fill the chip more evenly (4 x 768 x 768, 576 of the large
+// ones in X <- Q X: 975 us against 1050; with 256 as the bound 4 x 768 x 768 took 1340 where 512 took 1130).
+constexpr int64_t kTiles64 = 768;
+
 // Workgroups of a matrix in the norm and conversion launches: 2048 in all (half or twice as many: the same within 2 %).
 static int64_t parts_of(int64_t E, const Shape& s) {
   const int64_t by_size = std::max<int64_t>(1, s.xs / 8192);
@@ -755,6 +765,7 @@ constexpr int64_t kChunkBytes = (int64_t)4 << 30;
 // bytes an element of X takes: the first, with what it lacks, and the second
 static int64_t x_bytes(int planes) { return planes == 2 ? 6 + 4 : 3 + 3; }
 static int64_t matrix_bytes(const Shape& s, int planes) {
+  if (planes == MTX_NS_F64) return 16 * ((int64_t)s.M * s.N + (int64_t)s.S * s.S) + 512 * 8;
   return x_bytes(planes) * s.xs + 10 * s.ms * planes + 7 * round_up((int64_t)s.Sp * 4, 256) + 1024 * 8 + 256;
 }
 static int64_t chunk_of(int64_t E, const Shape& s, int planes) {
@@ -765,12 +776,113 @@ static int64_t workspace_bytes(int64_t E, const Shape& s, int planes) {
   const int64_t n = chunk_of(E, s, planes);
   int64_t b = 0;
   b += round_up(n * 512 * 8, 256);                        // partial sums
+  if (planes == MTX_NS_F64)                                // X, twice, A and Q
+    return b + 2 * round_up(n * s.M * (int64_t)s.N * 8, 256) + 2 * round_up(n * s.S * (int64_t)s.S * 8, 256);
   b += round_up(n * (int64_t)sizeof(Scale), 256);
   b += 6 * round_up(n * s.Sp * 4, 256);                    // diagonals, and what the matrices lose of them
   for (const int64_t x : {2 * planes, planes == 2 ? 2 : 1, 2 * planes, planes == 2 ? 0 : 1})
     b += round_up(n * s.xs * x, 256);                      // X, twice, and what it lacks
   b += 5 * round_up(n * s.ms * 2 * planes, 256);          // A, T and three of Q and P
   return b;
+}
+
+// ---- float64 ------------------------------------------------------------------------------------------------------
+// Two f16 planes hold 22 bits and f32 sums add 2^-24 of their terms, which the steps carry up by a^5 where x is singular:
+// float32 results in "full" end as far off as f32 products do, 2e-6 at full rank, 3e-5 at rank 32 of 768, 1e-4 at rank 1.
+// Here everything is f64, step by step: a Gram product, Q = a I + b A + c A^2, X <- Q X (tall: X Q).  Small stacks are bound by
+// their 17 launches of 6 to 13 us (8 x 128 x 512: 145 us; "full" 108), large ones by the f64 matrix cores (12 x 768 x 640:
+// 1.7 ms, "full" 0.47).
+struct Step64 {
+  const double *u, *v;  // X or A; X in the last product of a step: u (tall) or v
+  double* out;
+  double a, b, c;
+  Shape s;
+  int E, K;             // K: reduction
+  int64_t ld;           // sym: of u and v, where their rows are reduced
+};
+struct Out64 {  // the last step's: the result or the weights
+  void* out;
+  int64_t batch, row;
+  int dtype, step;
+  float lr, decay, factor;
+  const float* lr_dev;
+};
+// X = x / (|x|_F + eps), dense [M][N].
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void convert64_kernel(Source s, int M, int N, int rows, const double* __restrict__ part,
+                                                        int nparts, float eps, double* __restrict__ X) {
+  const int64_t e = blockIdx.y;
+  const double norm = norm_of(part, e, nparts) + (double)eps;
+  const bool fine = norm <= 1e300;
+  const int nc = (N + 7) / 8, r0 = blockIdx.x * rows, n = max(0, min(rows, M - r0)) * nc;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int r = r0 + i / nc, c = i % nc * 8;
+    float u[8];
+    load_update<T, VEC, false>(s, e, r, c, N, u);
+    double* to = X + (e * M + r) * N + c;
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (c + q < N) to[q] = fine ? (double)u[q] / norm : __builtin_nan("");
+  }
+}
+// out = c U V^T + b U + a I, S x S and symmetric: a tile of the lower triangle, stored mirrored too.  COLS: c U^T V.
+template <int BT, int KS, bool COLS>
+__global__ __launch_bounds__(f64mm::NT) void sym64_kernel(Step64 p) {
+  typedef f64mm::Tile<BT, KS> T;
+  __shared__ __attribute__((aligned(16))) double lds[T::LDS];
+  const int S = p.s.S, nt = (S + BT - 1) / BT, per = nt * (nt + 1) / 2;
+  const int t = dense::tile_of(blockIdx.x, p.E * per);
+  if (t < 0) return;
+  const int64_t e = t / per, ld = COLS ? S : p.ld, size = COLS ? (int64_t)S * p.K : S * p.ld;
+  int i, j;
+  lower(t % per, i, j);
+  const int m0 = i * BT, n0 = j * BT;
+  const double *u = p.u + e * size, *v = p.v + e * size;
+  f64mm::f64x4 acc[T::TB][T::TB];
+  T::template product<!COLS, !COLS>({COLS ? u + m0 : u + m0 * ld, ld, S - m0}, {COLS ? v + n0 : v + n0 * ld, ld, S - n0},
+                                    p.K, lds, acc);
+  double* out = p.out + e * S * (int64_t)S;
+  T::each(acc, [&](int r, int c, double y) {
+    const int64_t row = m0 + r, col = n0 + c;
+    if (row >= S || col >= S) return;
+    y *= p.c;
+    if (p.b != 0.0) y += p.b * u[row * ld + col];
+    if (row == col) y += p.a;
+    out[row * S + col] = y;
+    if (n0 < m0) out[col * S + row] = y;
+  });
+}
+// A tile of X <- Q X (tall: X Q); LAST: to the result or the weights.
+template <int BT, int KS, bool TALL, bool LAST>
+__global__ __launch_bounds__(f64mm::NT) void apply64_kernel(Step64 p, Out64 o) {
+  typedef f64mm::Tile<BT, KS> T;
+  __shared__ __attribute__((aligned(16))) double lds[T::LDS];
+  const int S = p.s.S, M = p.s.M, N = p.s.N, nm = (M + BT - 1) / BT, nn = (N + BT - 1) / BT, per = nm * nn;
+  const int t = dense::tile_of(blockIdx.x, p.E * per);
+  if (t < 0) return;
+  const int64_t e = t / per, xs = (int64_t)M * N, ms = (int64_t)S * S;
+  const int m0 = (TALL ? t % per / nn : t % per % nm) * BT, n0 = (TALL ? t % per % nn : t % per / nm) * BT;
+  const double *Q = (TALL ? p.v : p.u) + e * ms, *X = (TALL ? p.u : p.v) + e * xs;
+  f64mm::f64x4 acc[T::TB][T::TB];
+  if constexpr (TALL) T::template product<true, true>({X + (int64_t)m0 * N, N, M - m0}, {Q + (int64_t)n0 * S, S, S - n0}, S, lds, acc);
+  else T::template product<true, false>({Q + (int64_t)m0 * S, S, S - m0}, {X + n0, N, N - n0}, S, lds, acc);
+  const double lr = LAST && o.step == OUT_STEP ? (double)(o.lr_dev ? *o.lr_dev : o.lr) : 0.0;
+  T::each(acc, [&](int r, int c, double y) {
+    const int64_t row = m0 + r, col = n0 + c;
+    if (row >= M || col >= N) return;
+    if constexpr (!LAST) {
+      p.out[e * xs + row * N + col] = y;
+    } else {
+      const int64_t at = e * o.batch + row * o.row + col;
+      if (o.dtype == MTX_F32) {
+        float* w = (float*)o.out + at;
+        *w = (float)(o.step == OUT_STEP ? *w * (1.0 - lr * o.decay) - lr * o.factor * y : y);
+      } else {
+        uint16_t* w = (uint16_t*)o.out + at;
+        gst<uint16_t>(w, 0, (float)(o.step == OUT_STEP ? bf16_to_f32(*w) * (1.0 - lr * o.decay) - lr * o.factor * y : y));
+      }
+    }
+  });
 }
 
 struct Job {
@@ -964,6 +1076,65 @@ static int run_chunk(const Job& j, int64_t E, const Shape& s, const float* sched
   return MTX_OK;
 }
 
+template <bool COLS>
+static int launch_sym64(const Step64& p, hipStream_t st) {
+  auto tiles = [&](int b) { const int64_t n = ceil_div(p.s.S, b); return p.E * (n * (n + 1) / 2); };
+  if (tiles(64) < kTiles64)
+    hipLaunchKernelGGL((sym64_kernel<32, 32, COLS>), dim3((unsigned)tiles_grid(tiles(32))), dim3(f64mm::NT), 0, st, p);
+  else
+    hipLaunchKernelGGL((sym64_kernel<64, 16, COLS>), dim3((unsigned)tiles_grid(tiles(64))), dim3(f64mm::NT), 0, st, p);
+  return check_launch();
+}
+template <bool TALL, bool LAST>
+static int launch_apply64(const Step64& p, const Out64& o, hipStream_t st) {
+  auto tiles = [&](int b) { return p.E * ceil_div(p.s.M, b) * ceil_div(p.s.N, b); };
+  if (tiles(64) < kTiles64)
+    hipLaunchKernelGGL((apply64_kernel<32, 32, TALL, LAST>), dim3((unsigned)tiles_grid(tiles(32))), dim3(f64mm::NT), 0, st, p, o);
+  else
+    hipLaunchKernelGGL((apply64_kernel<64, 16, TALL, LAST>), dim3((unsigned)tiles_grid(tiles(64))), dim3(f64mm::NT), 0, st, p, o);
+  return check_launch();
+}
+// sched: 9 floats a step: a, b, c, and what f32 has lost of each of them.
+template <bool TALL>
+static int run_chunk64(const Job& j, int64_t E, const Shape& s, const float* sched, int steps, float eps, char* ws,
+                       hipStream_t st) {
+  auto take = [&](int64_t bytes) { char* p = ws; ws += round_up(bytes, 256); return p; };
+  const int64_t xs = (int64_t)s.M * s.N, ms = (int64_t)s.S * s.S;
+  double* part = (double*)take(E * 512 * 8);
+  double* X[2];
+  for (auto& x : X) x = (double*)take(E * xs * 8);
+  double *A = (double*)take(E * ms * 8), *Q = (double*)take(E * ms * 8);
+  const int parts = (int)parts_of(E, s), rows = (int)ceil_div(s.M, parts);
+  const dim3 grid((unsigned)parts, (unsigned)E);
+#define MTX_PREP(T, V)                                                                                               \
+  do {                                                                                                               \
+    hipLaunchKernelGGL((norm_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, rows, part);                    \
+    hipLaunchKernelGGL((convert64_kernel<T, V>), grid, dim3(256), 0, st, j.src, s.M, s.N, rows, part, parts, eps, X[0]); \
+  } while (0)
+  if (j.gdtype == MTX_F32) {
+    if (j.gvec) MTX_PREP(float, true);
+    else MTX_PREP(float, false);
+  } else {
+    if (j.gvec) MTX_PREP(uint16_t, true);
+    else MTX_PREP(uint16_t, false);
+  }
+#undef MTX_PREP
+  int rc = check_launch();
+  const Out64 o{j.out, j.out_batch, j.out_row, j.dtype, j.step, j.lr, j.decay, j.factor, j.lr_dev};
+  for (int i = 0; i < steps && rc == MTX_OK; ++i) {
+    const float* c = sched + 9 * i;
+    double *x = X[i & 1], *next = X[(i + 1) & 1];
+    rc = launch_sym64<TALL>(Step64{x, x, A, 0.0, 0.0, 1.0, s, (int)E, s.L, s.L}, st);
+    if (rc != MTX_OK) return rc;
+    const double c2 = (double)c[2] + c[5];
+    rc = launch_sym64<false>(Step64{A, A, Q, (double)c[0] + c[3], (double)c[1] + c[4], c2, s, (int)E, c2 != 0.0 ? s.S : 0, s.S}, st);
+    if (rc != MTX_OK) return rc;
+    const Step64 a{TALL ? x : Q, TALL ? Q : x, next, 0.0, 0.0, 0.0, s, (int)E, s.S, 0};
+    rc = i + 1 == steps ? launch_apply64<TALL, true>(a, o, st) : launch_apply64<TALL, false>(a, o, st);
+  }
+  return rc;
+}
+
 static int run(Job j, int64_t E, int64_t M, int64_t N, const float* sched, int steps, float eps, int planes, void* ws,
                int64_t ws_bytes, hipStream_t st) {
   if (E == 0 || M == 0 || N == 0) return MTX_OK;
@@ -977,7 +1148,9 @@ static int run(Job j, int64_t E, int64_t M, int64_t N, const float* sched, int s
     if (j.src.m) c.src.m = j.src.m + e * j.src.m_batch;
     c.out = (char*)j.out + e * j.out_batch * osize;
     const int64_t n = std::min(chunk, E - e);
-    const int rc = s.tall ? (planes == 2 ? run_chunk<true, true>(c, n, s, sched, steps, eps, (char*)ws, st)
+    const int rc = planes == MTX_NS_F64 ? (s.tall ? run_chunk64<true>(c, n, s, sched, steps, eps, (char*)ws, st)
+                                                  : run_chunk64<false>(c, n, s, sched, steps, eps, (char*)ws, st))
+                   : s.tall ? (planes == 2 ? run_chunk<true, true>(c, n, s, sched, steps, eps, (char*)ws, st)
                                          : run_chunk<true, false>(c, n, s, sched, steps, eps, (char*)ws, st))
                           : (planes == 2 ? run_chunk<false, true>(c, n, s, sched, steps, eps, (char*)ws, st)
                                          : run_chunk<false, false>(c, n, s, sched, steps, eps, (char*)ws, st));
@@ -990,10 +1163,12 @@ static bool sizes_ok(int64_t E, int64_t M, int64_t N) {
   return E >= 0 && M >= 0 && N >= 0 && E <= 65535 && M <= (1 << 20) && N <= (1 << 20) &&
          std::min(M, N) <= (1 << 15);
 }
-static bool sched_ok(const float* sched, int steps) {
+static bool planes_ok(int planes) { return planes == 1 || planes == 2 || planes == MTX_NS_F64; }
+static bool sched_ok(const float* sched, int steps, int planes) {
   if (!sched || steps < 1 || steps > 64) return false;
   for (int i = 0; i < 9 * steps; ++i)
     if (!std::isfinite(sched[i])) return false;
+  if (planes == MTX_NS_F64) return true;
   for (int i = 0; i < steps; ++i)
     for (int q = 3; q < 8; ++q)
       if (!(sched[9 * i + q] > 0.0f)) return false;
@@ -1011,7 +1186,7 @@ static bool rows_aligned(const void* p, int dtype, int64_t batch, int64_t row, i
 using namespace mtx;
 
 extern "C" int64_t mtx_newton_schulz_workspace_size(int64_t E, int64_t M, int64_t N, int planes) {
-  if (!ns::sizes_ok(E, M, N) || (planes != 1 && planes != 2)) return -1;
+  if (!ns::sizes_ok(E, M, N) || !ns::planes_ok(planes)) return -1;
   if (E == 0 || M == 0 || N == 0) return 0;
   return ns::workspace_bytes(E, ns::shape_of(M, N), planes);
 }
@@ -1019,8 +1194,8 @@ extern "C" int64_t mtx_newton_schulz_workspace_size(int64_t E, int64_t M, int64_
 extern "C" int mtx_newton_schulz(const void* x, int dtype, int64_t E, int64_t M, int64_t N, int64_t x_batch, int64_t x_row,
                                  const float* schedule, int steps, float eps, int planes, void* out, int64_t out_batch,
                                  int64_t out_row, void* workspace, int64_t workspace_bytes, void* stream) {
-  if ((dtype != MTX_F32 && dtype != MTX_BF16) || (planes != 1 && planes != 2) || !(eps > 0.0f)) return MTX_ERR_ARG;
-  if (E < 0 || M < 0 || N < 0 || !ns::sched_ok(schedule, steps)) return MTX_ERR_ARG;
+  if ((dtype != MTX_F32 && dtype != MTX_BF16) || !ns::planes_ok(planes) || !(eps > 0.0f)) return MTX_ERR_ARG;
+  if (E < 0 || M < 0 || N < 0 || !ns::sched_ok(schedule, steps, planes)) return MTX_ERR_ARG;
   if (!ns::sizes_ok(E, M, N)) return MTX_ERR_UNSUPPORTED;
   if (x_row < N || out_row < N || x_batch < 0 || out_batch < 0) return MTX_ERR_ARG;
   if (E * M * N > 0 && (!x || !out)) return MTX_ERR_ARG;
@@ -1043,7 +1218,7 @@ extern "C" int mtx_muon_update(void* param, int param_dtype, int64_t p_batch, in
                                float eps, int planes, void* workspace, int64_t workspace_bytes, void* stream) {
   if ((param_dtype != MTX_F32 && param_dtype != MTX_BF16) || (grad_dtype != MTX_F32 && grad_dtype != MTX_BF16))
     return MTX_ERR_ARG;
-  if ((planes != 1 && planes != 2) || !(eps > 0.0f) || E < 0 || M < 0 || N < 0 || !ns::sched_ok(schedule, steps))
+  if (!ns::planes_ok(planes) || !(eps > 0.0f) || E < 0 || M < 0 || N < 0 || !ns::sched_ok(schedule, steps, planes))
     return MTX_ERR_ARG;
   if (!ns::sizes_ok(E, M, N)) return MTX_ERR_UNSUPPORTED;
   if (p_row < N || g_row < N || m_row < N || p_batch < 0 || g_batch < 0 || m_batch < 0) return MTX_ERR_ARG;

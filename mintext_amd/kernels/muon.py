@@ -10,14 +10,19 @@ brings them near 1 and keeps the singular vectors.  ``muon_update`` does an opti
     m <- beta m + (1 - beta) g;   u = (1 - beta) g + beta m (Nesterov) or m
     w <- (1 - lr weight_decay) w - lr factor newton_schulz(u)
 
-Precision.  Products run on the 16-bit matrix cores with float32 sums: "half" holds the matrices between products in f16
-(11 bits, under power-of-two scales that their bounded singular values allow), "full" in two f16 planes (22 bits, three
-times the products).  The default goes by the type of what is returned or updated: "full" for float32, "half" for
-bfloat16, whose rounding is coarser.  Before it is rounded to its type, a result of five steps with the default
-coefficients is off by 0.05 to 0.5 % in "half" (2-norm; up to 1 % for float32 gradients of rank 1 to 4) and by 6e-6 at most
-in "full", where the float32 sums of the products count for more than the planes.  Rounding errors in directions in
-which x is nearly singular grow as those directions do, by |a| a step: more or steeper steps end further off.
-The Frobenius norm is summed in float64 and momentum is float32.
+Precision.  "half" and "full" run on the 16-bit matrix cores with float32 sums: "half" holds the matrices between products
+in f16 (11 bits, under power-of-two scales that their bounded singular values allow), "full" in two f16 planes (22 bits,
+three times the products).  "double" is float64 throughout, on the float64 matrix cores.  Rounding errors in directions
+in which x is nearly singular grow as those do, by |a| a step, so that what a result is off by depends on x's rank.  Five
+steps with the default coefficients are off, before the result is rounded to its type, by (2-norm)
+
+    "half"    0.04 to 0.5 %, up to 1.4 % for ranks of 4 and less
+    "full"    2e-6 at full rank to 4e-5 at rank 8, up to 1.3e-4 below: what products in float32 throughout come to
+    "double"  1e-12
+
+More or steeper steps end further off.  ``newton_schulz`` takes "double" for float32 and "half" for bfloat16, whose own
+rounding is as coarse; ``muon_update``, where the result is a small change of the weights, "full" for float32 weights and
+"half" for bfloat16.  The Frobenius norm is summed in float64 and momentum is float32.
 """
 from __future__ import annotations
 
@@ -40,6 +45,7 @@ _GROUP_RESULT, _GROUP_STEP, _SMALL, _SQUARE = 2, 3, 128, 1.25
 # where that product would pass what as many steps with the coefficients above reach: steeper ones (8.3, 4.1, 3.9, ..)
 # in threes end 8 % off at rank 8 of 256 x 1024 in "half", 0.4 % this way, as by themselves (simulated roundings).
 _GROWTH = 3.45
+_PLANES = {"half": 1, "full": 2, "double": L.MTX_NS_F64}
 
 
 @functools.lru_cache(maxsize=64)
@@ -85,13 +91,24 @@ def _schedule(steps: int, coefficients: tuple, group: int):
     return (ctypes.c_float * len(flat))(*flat)
 
 
-def _arguments(steps, coefficients, eps, precision, t, group):
+@functools.lru_cache(maxsize=64)
+def _schedule64(steps: int, coefficients: tuple):
+    """The same for float64, whose range needs no scales: in their place what float32 loses of the coefficients."""
+    _schedule(steps, coefficients, 1)  # refuses coefficients that diverge
+    triples = [coefficients] * steps if not isinstance(coefficients[0], tuple) else coefficients
+    single = lambda v: ctypes.c_float(v).value
+    flat = [v for c in triples for v in (*map(single, c), *(v - single(v) for v in c), 0.0, 0.0, 0.0)]
+    return (ctypes.c_float * len(flat))(*flat)
+
+
+def _arguments(steps, coefficients, eps, precision, t, group, single):
+    """(schedule, planes); ``single``: the precision of what is float32."""
     if not isinstance(steps, int) or not 1 <= steps <= 64:
         raise ValueError(f"steps must be an int from 1 to 64, got {steps!r}")
     if not eps > 0:
         raise ValueError(f"eps must be positive, got {eps!r}")
-    if precision not in (None, "half", "full"):
-        raise ValueError(f'precision must be "half", "full" or None, got {precision!r}')
+    if precision not in (None, *_PLANES):
+        raise ValueError(f'precision must be "half", "full", "double" or None, got {precision!r}')
     try:
         if isinstance(coefficients[0], (tuple, list)):
             c = tuple(tuple(float(v) for v in t) for t in coefficients)
@@ -103,7 +120,9 @@ def _arguments(steps, coefficients, eps, precision, t, group):
         good = False
     if not good or not all(math.isfinite(v) for t in c for v in (t if isinstance(t, tuple) else (t,))):
         raise ValueError("coefficients must be three finite numbers, or three for each step")
-    planes = 2 if precision == "full" or (precision is None and t.dtype == torch.float32) else 1
+    planes = _PLANES[precision or (single if t.dtype == torch.float32 else "half")]
+    if planes == L.MTX_NS_F64:
+        return _schedule64(steps, c), planes
     if min(t.shape[-2:]) <= _SMALL:
         group = _GROUP_STEP
     elif max(t.shape[-2:]) <= _SQUARE * min(t.shape[-2:]):
@@ -196,7 +215,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, *, coefficients=COEFFICIENTS,
     Args:
         x: float32 or bfloat16, any strides (rows that are not consecutive elements are copied first).
         coefficients: (a, b, c), or such a triple for each step.
-        precision: "half", "full" or None, by x's dtype (see the module).
+        precision: "half", "full", "double" or None, by x's dtype (see the module).
 
     Returns:
         a dense tensor of x's shape and dtype.  Not differentiable: an x that requires a gradient or has a
@@ -204,7 +223,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, *, coefficients=COEFFICIENTS,
     """
     L.refuse_watched("newton_schulz", x)
     _check_stack(x, "x")
-    sched, planes = _arguments(steps, coefficients, eps, precision, x, _GROUP_RESULT)
+    sched, planes = _arguments(steps, coefficients, eps, precision, x, _GROUP_RESULT, "double")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("newton_schulz is not differentiable: pass x.detach()")
     dev = L.require_device(x)
@@ -244,7 +263,7 @@ def muon_update(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
             raise ValueError(f"{name} must have param's shape {tuple(param.shape)}, got {tuple(t.shape)}")
     if momentum.dtype != torch.float32:
         raise TypeError(f"momentum must be float32, got {momentum.dtype}")
-    sched, planes = _arguments(steps, coefficients, eps, precision, param, _GROUP_STEP)
+    sched, planes = _arguments(steps, coefficients, eps, precision, param, _GROUP_STEP, "full")
     M, N = param.shape[-2:]
     if scale == "spectral":
         factor = math.sqrt(max(1.0, N / max(M, 1)))
