@@ -9,8 +9,8 @@
 // A's small eigenvalues are squares of X's and grow by a^2 a step, so what the rounding of A adds grows as well and is
 // not taken back before the next Gram product: a group holds three steps at most.  In simulation with gradients of
 // rank 1 to full rank (f16 operands) five steps end 0.07 to 0.19 % off as 2 + 2 + 1, 0.1 to 0.5 % as 3 + 2, up to 14 %
-// or beyond f16's range as one group.  The caller chooses: 2 where the result itself is asked for, 3 where it is
-// a small change of weights, 1 for matrices that are nearly square.
+// or beyond f16's range as one group.  The caller chooses: 1 where the result itself is asked for
+// ("full": 2), 3 where it is a small change of weights, 1 for matrices that are nearly square.
 //
 // Numbers: |x|_F bounds every singular value by 1 and the polynomials bound them from there, so every matrix has a
 // power-of-two scale, chosen by the caller from those bounds, that puts it into f16's range: 11 bits where

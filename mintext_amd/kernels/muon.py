@@ -16,9 +16,10 @@ three times the products).  "double" is float64 throughout, on the float64 matri
 in which x is nearly singular grow as those do, by |a| a step, so that what a result is off by depends on x's rank.  Five
 steps with the default coefficients are off, before the result is rounded to its type, by (2-norm)
 
-    "half"    0.04 to 0.5 %, up to 1.4 % for ranks of 4 and less
+    "half"    0.04 to 0.17 % for bfloat16 in newton_schulz; 0.04 to 0.5 % in muon_update, which takes steps in groups,
+              and for float32 x; up to 1.4 % in those for ranks of 4 and less
     "full"    2e-6 at full rank to 4e-5 at rank 8, up to 1.3e-4 below: what products in float32 throughout come to
-    "double"  1e-12
+    "double"  1e-11
 
 More or steeper steps end further off.  ``newton_schulz`` takes "double" for float32 and "half" for bfloat16, whose own
 rounding is as coarse; ``muon_update``, where the result is a small change of the weights, "full" for float32 weights and
@@ -35,12 +36,14 @@ import torch
 from .. import _lib as L
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-# Steps between two Gram products, at most: fewer products with three, smaller errors with fewer (128 x 768 x 2048, five steps:
-# 3.30 ms in threes, 3.65 in twos, 4.39 by themselves).  Matrices of _SMALL or less on a side take threes in any case: their
-# products in between are held in 22 bits (64 x 128 x 1408 in float32 212 us, 265 in twos).  Those near square gain nothing
-# from groups, whose symmetric products cost what the others save: one of 2048 x 2048 takes 366 us in single steps, 405 in
-# twos, 419 in threes; 8 of 1024 x 1280 445, 446, 440; 128 of 768 x 1152 3.02 ms, 2.85, 2.71.
-_GROUP_RESULT, _GROUP_STEP, _SMALL, _SQUARE = 2, 3, 128, 1.25
+# Steps between two Gram products, at most, by planes: fewer products with more, smaller errors with fewer (128 x 768 x 2048 in
+# bfloat16, five steps: 4.07 ms by themselves, 3.46 in twos, 3.30 in threes).  A result in "half" takes single steps, which
+# leave it little more than its rounding to bfloat16 off, 1.75e-3 for 1.66e-3 (twos 2.0 to 2.7e-3); in "full" float32 sums
+# count for more than the groups, and a small change of weights stands threes.  Matrices of _SMALL or less on a side take
+# threes in any case: their products in between are held in 22 bits (64 x 128 x 1408 in float32 212 us, 265 in twos).  Those
+# near square gain nothing from groups, whose symmetric products cost what the others save: one of 2048 x 2048 takes
+# 366 us in single steps, 405 in twos, 419 in threes; 8 of 1024 x 1280 445, 446, 440; 128 of 768 x 1152 3.02 ms, 2.85, 2.71.
+_GROUP_RESULT, _GROUP_STEP, _SMALL, _SQUARE = {1: 1, 2: 2}, {1: 3, 2: 3}, 128, 1.25
 # What a Gram product's rounding becomes grows with the square of the group's product of polynomials, so a group ends early
 # where that product would pass what as many steps with the coefficients above reach: steeper ones (8.3, 4.1, 3.9, ..)
 # in threes end 8 % off at rank 8 of 256 x 1024 in "half", 0.4 % this way, as by themselves (simulated roundings).
@@ -101,8 +104,8 @@ def _schedule64(steps: int, coefficients: tuple):
     return (ctypes.c_float * len(flat))(*flat)
 
 
-def _arguments(steps, coefficients, eps, precision, t, group, single):
-    """(schedule, planes); ``single``: the precision of what is float32."""
+def _arguments(steps, coefficients, eps, precision, t, groups, single):
+    """(schedule, planes); ``groups``: the longest, by planes; ``single``: the precision of what is float32."""
     if not isinstance(steps, int) or not 1 <= steps <= 64:
         raise ValueError(f"steps must be an int from 1 to 64, got {steps!r}")
     if not eps > 0:
@@ -123,8 +126,9 @@ def _arguments(steps, coefficients, eps, precision, t, group, single):
     planes = _PLANES[precision or (single if t.dtype == torch.float32 else "half")]
     if planes == L.MTX_NS_F64:
         return _schedule64(steps, c), planes
+    group = groups[planes]
     if min(t.shape[-2:]) <= _SMALL:
-        group = _GROUP_STEP
+        group = 3
     elif max(t.shape[-2:]) <= _SQUARE * min(t.shape[-2:]):
         group = 1
     return _schedule(steps, c, group), planes

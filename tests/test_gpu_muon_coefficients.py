@@ -52,27 +52,30 @@ def test_newton_schulz(dev, coefficients, steps, size, copies, precision):
         held(got[:1], x[None].to(dev), True, 2.0 ** -24, steps=steps, coef=c)
     else:
         want = O.newton_schulz(x, triples(c, steps))
-        assert off(got[0].double().cpu(), want) <= 1.5 * oracle_error(x, want, c, steps, 2) + 2.0 ** -24
+        assert off(got[0].double().cpu(), want) <= 1.5 * oracle_error(x, want, c, steps, 1) + 2.0 ** -24
 
 
-@pytest.mark.parametrize("coefficients", [CUBIC, FAINT, MIXED, STEEP], ids=["cubic", "faint", "mixed", "steep"])
+@pytest.mark.parametrize("steps", [2, 3, 4, 5, 7])
+@pytest.mark.parametrize("coefficients", [CUBIC, FAINT, EVEN, MIXED, STEEP], ids=["cubic", "faint", "even", "mixed", "steep"])
 @pytest.mark.parametrize("size", [*SIZES, (256, 1024, 8)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_muon_update(dev, coefficients, size, dtype):
+def test_muon_update(dev, coefficients, size, dtype, steps):
     """Groups of up to three."""
     from mintext_amd.kernels import muon_update
 
-    c = coefficients[:5] if isinstance(coefficients[0], tuple) else coefficients
+    steps = min(steps, 5) if coefficients is STEEP else steps
+    c = coefficients[:steps] if isinstance(coefficients[0], tuple) else coefficients
     x = gradient(*size)
     g = torch.Generator().manual_seed(3)
     p = (torch.randn(x.shape, generator=g) * 0.02).to(dtype)
     got = p.to(dev)
-    muon_update(got, x.to(dev), torch.zeros(x.shape, device=dev), lr=0.5, beta=0.0, scale=1.0, coefficients=c, precision="half")
-    o = O.newton_schulz(x, triples(c, 5))
+    muon_update(got, x.to(dev), torch.zeros(x.shape, device=dev), lr=0.5, beta=0.0, scale=1.0, steps=steps, coefficients=c,
+                precision="half")
+    o = O.newton_schulz(x, triples(c, steps))
     want = p.double() - 0.5 * o
     rounding = (torch.finfo(dtype).eps / 2 + 2.0 ** -22) * want.norm()  # of the weights, at most half a step each
-    assert (got.double().cpu() - want).norm() <= 0.5 * 1.5 * oracle_error(x, o, c, 5, 3) * o.norm() + rounding
-    if coefficients is STEEP and size == (256, 1024, 8):
+    assert (got.double().cpu() - want).norm() <= 0.5 * 1.5 * oracle_error(x, o, c, steps, 3) * o.norm() + rounding
+    if coefficients is STEEP and steps == 5 and size == (256, 1024, 8):
         # in groups as long as the default ones the error was 8 % of the orthogonalised gradient; the weights' rounding,
         # 2^-8 |w| = 0.04 at most in bfloat16, is more than 1 % of it (0.014) and less than 8 % (0.11)
         assert (got.double().cpu() - want).norm() <= 0.5 * 0.01 * o.norm() + rounding

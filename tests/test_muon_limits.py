@@ -20,11 +20,10 @@ LIMITS = {
     ("newton_schulz", 128, 512, 1): (1.25e-2, ("diagonal", "remainder")),
     ("newton_schulz", 128, 512, 2): (6.8e-3, ("diagonal", "remainder")),
     ("newton_schulz", 100, 256, 32): (4.3e-3, ("remainder",)),
-    ("newton_schulz", 200, 300, 32): (3.9e-3, ("diagonal", "remainder")),
-    ("newton_schulz", 256, 1024, 2): (7.4e-3, ("remainder",)),
-    ("newton_schulz", 256, 1024, 8): (3.1e-3, ("diagonal", "remainder")),
-    ("newton_schulz", 333, 1001, 32): (3.6e-3, ("diagonal", "remainder")),
-    ("newton_schulz", 704, 504, 8): (3.6e-3, ("diagonal", "remainder")),
+    ("newton_schulz", 200, 300, 32): (2.2e-3, ("remainder",)),
+    ("newton_schulz", 256, 1024, 8): (2.8e-3, ("remainder",)),
+    ("newton_schulz", 333, 1001, 600): (1.02e-3, ("remainder",)),
+    ("newton_schulz", 704, 504, 100): (1.5e-3, ("remainder",)),
     ("newton_schulz", 300, 264, 32): (2.1e-3, ("remainder",)),
     ("muon_update", 128, 512, 2): (6.8e-3, ("diagonal", "remainder")),
     ("muon_update", 256, 1024, 2): (1e-2, ("diagonal", "remainder")),
@@ -41,7 +40,7 @@ def off(got, want):
 def group_of(op, M, N):
     if min(M, N) <= 128:
         return 3
-    return 1 if max(M, N) <= 1.25 * min(M, N) else 2 if op == "newton_schulz" else 3
+    return 1 if op == "newton_schulz" or max(M, N) <= 1.25 * min(M, N) else 3
 
 
 @pytest.mark.parametrize("case", LIMITS, ids=lambda c: "-".join(map(str, c)))
@@ -75,3 +74,17 @@ def test_the_operator_keeps_them(dev, case, copies):
     got = orthogonalised(op, x.to(dev).expand(copies, M, N).contiguous()).double().cpu()
     assert torch.equal(got, got[:1].expand_as(got))
     assert off(got[0], want) <= LIMITS[case][0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(152, 472, 941), (1216, 384, 3143), (168, 1584, 335), (256, 1024, 100), (300, 700, 32)])
+def test_bfloat16_results_are_little_more_than_rounded(dev, size):
+    """The rounding of a bfloat16 result and 1.5 times the oracle's error with single steps, which are independent; in
+    groups of two the second alone was as large as the first."""
+    from mintext_amd.kernels import newton_schulz
+
+    x = gradient(*size).bfloat16()
+    want = O.newton_schulz(x, [COEFFICIENTS] * 5)
+    own = off(O.chain(x, rows(5, COEFFICIENTS, 1), 1), want)
+    rounding = off(want.bfloat16().double(), want)
+    assert off(newton_schulz(x.to(dev)).double().cpu(), want) <= ((1.5 * own) ** 2 + rounding ** 2) ** 0.5
