@@ -414,12 +414,13 @@ int mtx_gmm_fp8_gathered(const uint8_t* xq, const float* x_scale, int64_t x_rows
 /* ---- dense product with epilogue ---------------------------------------------------------
  * The dense Linear and MLP products of mintext/modules/linear.py:123-147, 164-228 with what
  * surrounds them in a layer, and their gradient.  Dense row-major operands of one dtype (F32 or
- * BF16), any sizes up to 65535 * 64 each, any alignment; sums in float32, one rounding at the end.
+ * BF16), any sizes up to 65535 * 64 each, any alignment; sums in float32, one rounding at the end
+ * (of pre, dz and each result).
  * mtx_linear:     z = x[M,K] @ w[K,N] + bias[N];  out[M,N] = act(z) + residual[M,N].  bias, residual
  *                 and pre may be NULL; pre[M,N] receives z (for mtx_linear_bwd).
  * mtx_linear_bwd: dz = dy * act'(pre), written to dz[M,N] (pre and dz may be NULL for MTX_ACT_NONE,
- *                 where dz is dy); dx[M,K] = dz @ w^T, dw[K,N] = x^T @ dz, dbias[N] = column sums
- *                 of dz; those of the three that are NULL are left out.
+ *                 where dz is dy); dx[M,K] = dz @ w^T, dw[K,N] = x^T @ dz of the rounded dz, dbias[N] =
+ *                 column sums of dz before it is rounded; those of the three that are NULL are left out.
  * One workspace size (16-byte aligned) serves both; a workspace must not be shared by two calls that
  * can run at the same time.                                                                */
 #define MTX_ACT_NONE       0

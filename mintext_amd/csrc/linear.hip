@@ -4,7 +4,8 @@
 // are applied to the f32 sums on their way out, so that z costs at most one write and the rest no
 // pass of their own.  bf16 with rows of whole 16-byte chunks runs on the 16-bit matrix cores (dense_tile.h), in tiles of
 // 256 x 256 or, where those are few, 256 x 128 or 128 x 128, and up to 64 rows on a kernel that streams w;
-// everything else on f32 matrix-core tiles (f32_tile.h).
+// everything else on f32 matrix-core tiles (f32_tile.h), which for bf16 at other widths is 7 to 16 times slower (4096 x
+// 2048 x 50257 12.5 ms, 50264 columns 0.78; 1 x 2048 x 50257 295 us, 46; 4093 x 2047 x 7167 1805 us, 2048 x 7168 112).
 #include "common.h"
 #include "dense_tile.h"
 #include "f32_tile.h"
@@ -77,7 +78,7 @@ __device__ __forceinline__ float activation_slope(float z, int act) {
 
 // ---- any size and alignment: 64 x 64 tiles, products and sums in f32 --------------------------------------
 // Small products are bound by the length of one tile's chain of stages, hence the split (plan()); large ones by the f32
-// matrix cores: 1000 x 2000 x 1000 takes 51 us, 79 TFLOP/s of 154.
+// matrix cores: 1000 x 2000 x 1000 takes 51 us, 79 TFLOP/s of 154, 8192 x 4096 x 14336 8.3 ms, 116.
 template <typename T, int MODE, int VEC>
 __global__ __launch_bounds__(f32mm::NT) void f32_kernel(Args p) {
   using namespace f32mm;
@@ -377,7 +378,9 @@ __global__ __launch_bounds__(256) void finish_kernel(Args p) {
 
 // ---- dz = dy act'(z) and the column sums of dz ---------------------------------------------------------------
 // A workgroup takes 32 lanes x V columns of a range of rows, eight rows at a time, and leaves f32 sums of its range; a
-// second launch adds the ranges in order, so the sums do not depend on timing.  One pass over dy and z: 4093 x 7168 in
+// second launch adds the ranges in order, so the sums do not depend on timing.  dz is rounded to the operands' type, in
+// which the matrix cores take it (dx and dw end 2.4e-3 off in bf16, the rounding of the result alone is 1.7e-3; a second plane
+// for what it loses would double both products), and z was, as it was saved; the column sums take dz before.  One pass over dy and z: 4093 x 7168 in
 // bf16, 176 MB, in 36 us with the second launch, 4.9 TB/s (41 with half as many ranges); 8192 x 14336 150 us, 4.7 TB/s.
 constexpr int kSlopeRows = 8;
 template <typename T, int V>

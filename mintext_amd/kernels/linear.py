@@ -4,7 +4,14 @@ The dense counterpart of ``grouped_matmul``, for the projections and MLPs around
 ``Linear`` and ``MLP``, mintext/modules/linear.py:123-147, 164-228): one HIP kernel applies bias, activation and
 residual to the float32 sums, rounded once.  Training also writes ``z = x @ weight + bias``, in the operands' dtype,
 when there is an activation; its backward is one pass over the gradient and ``z`` (``dz = dy * act'(z)`` and the
-bias gradient) and the two products ``dz @ weight^T`` and ``x^T @ dz``.  The gradients are deterministic.
+bias gradient) and the two products ``dz @ weight^T`` and ``x^T @ dz``.  ``dz`` is rounded to the operands' dtype for the
+products (the bias gradient sums it before), so that bfloat16 gradients behind an activation end 2.4e-3 off (2-norm)
+where the rounding of the result alone is 1.7e-3.  The gradients are deterministic.
+
+bfloat16 runs on the 16-bit matrix cores where K and N are multiples of 8 and the tensors lie on 16-byte boundaries;
+otherwise its products run in float32, at less than a tenth of the rate where they are large (4096 x 2048 x 50257 takes
+12.5 ms, with 50264 columns 0.78): such widths are worth padding.  float32 runs at up to 116 TFLOP/s, level with a
+library's products and separate passes.
 """
 from __future__ import annotations
 
