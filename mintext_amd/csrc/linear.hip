@@ -161,7 +161,8 @@ __device__ __forceinline__ void finish8(const Args& p, int r, int c, float v[8])
 }
 
 // Bound by the matrix cores in large products: 8192 x 4096 x 14336 in 780 to 800 us, 1.2 PFLOP/s, which is what a plain
-// library product of the size reaches (813 us); 4093 x 2048 x 7168 in 111, its gradients in 134 and 119.  Of few
+// library product of the size reaches (813 us); 4093 x 2048 x 7168 in 111 (137 with z and a residual), its gradients in 129
+// to 134 and 115 to 119.  Of few
 // tiles it is the length of a tile's reduction that counts, which plan() splits.
 // Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2
 // (8192 x 4096 x 14336: 805 us without groups, 778 in groups of 4, 783 of 8, 790 of 16).

@@ -314,8 +314,8 @@ __device__ __forceinline__ void lower(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// One workgroup a tile of the lower triangle, which it also stores mirrored: 128 Gram products of 768 x 2048 take 214 us,
-// 0.96 PFLOP/s of the tiles computed, and 128 products of 768^3 about 120 us, 0.64: with 24 ring stages a tile the way out
+// One workgroup a tile of the lower triangle, which it also stores mirrored: 128 Gram products of 768 x 2048 take 204 to 214 us,
+// 0.96 PFLOP/s of the tiles computed, and 128 products of 768^3 113 to 130 us, 0.64: with 24 ring stages a tile the way out
 // (f16 through LDS, once in rows and once turned) is 50 us of it, and the tiles of a CU do not overlap it with products.
 // COLS: the reduction runs down u's and v's columns (the Gram product of a tall X); otherwise along their rows.
 template <class T, bool COLS, bool TWO, int DIAG>
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(T::NT, T::BM == 256 ? 1 : 2) void apply_kernel(Appl
 // Between launches such products wait for memory and for each other, 5 to 9 us apiece for 2 of work.  Here one workgroup
 // takes a matrix from X to P, a chain of up to eight products that each wait for the one before: A and P stay in its
 // registers in f32, the operands of a product in LDS in two f16 planes, in "half" too, as the products cost little.  Two
-// slots of 64 KB: Q, and in turn A, T and P.  8 x 128 x 512 in f32: 6 launches and 107 us, 43 a group of three steps here,
+// slots of 64 KB: Q, and in turn A, T and P.  8 x 128 x 512 in "full": 6 launches and 107 us, 43 a group of three steps here,
 // where products by themselves take 26 launches and 124; 64 x 128 x 1408 210 against 237, 1 x 64 x 256 80 against 88.
 // "half" is level (84 and 82, 135 and 134, 69 and 68) with f32 accuracy in between and a quarter of the launches.
 constexpr int kChainS = 128;
@@ -702,8 +702,8 @@ static bool takes_big(int64_t S, int64_t big, int64_t small) {
 
 // Where all tiles of 64 x 64 find a place at once, two a CU, it is one tile's chain of stages and its way out that count, and the
 // smallest is the quickest: 1 x 1024 (136 of them, 36 of 128 x 128) 9 us against 13 and its Gram product with 4096 20
-// against 35, 8 x 256 in f32 8 against 13; with more than that 1 x 2048 (528, 136) 28 against 22.  X <- P X likewise: 8 x 128 x
-// 512 in f32, five steps with two of them, 107 us against 113.
+// against 35, 8 x 256 in two planes 8 against 13; with more than that 1 x 2048 (528, 136) 28 against 22.  X <- P X likewise: 8 x 128 x
+// 512 in two planes, five steps with two of them, 107 us against 113.
 constexpr int64_t kLeastTiles = 512;
 
 template <bool COLS, bool TWO, int DIAG>

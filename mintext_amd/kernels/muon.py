@@ -40,7 +40,7 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 # bfloat16, five steps: 4.07 ms by themselves, 3.46 in twos, 3.30 in threes).  A result in "half" takes single steps, which
 # leave it little more than its rounding to bfloat16 off, 1.75e-3 for 1.66e-3 (twos 2.0 to 2.7e-3); in "full" float32 sums
 # count for more than the groups, and a small change of weights stands threes.  Matrices of _SMALL or less on a side take
-# threes in any case: their products in between are held in 22 bits (64 x 128 x 1408 in float32 212 us, 265 in twos).  Those
+# threes in any case: their products in between are held in 22 bits (64 x 128 x 1408 in "full" 212 us, 265 in twos).  Those
 # near square gain nothing from groups, whose symmetric products cost what the others save: one of 2048 x 2048 takes
 # 366 us in single steps, 405 in twos, 419 in threes; 8 of 1024 x 1280 445, 446, 440; 128 of 768 x 1152 3.02 ms, 2.85, 2.71.
 _GROUP_RESULT, _GROUP_STEP, _SMALL, _SQUARE = {1: 1, 2: 2}, {1: 3, 2: 3}, 128, 1.25
