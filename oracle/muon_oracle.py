@@ -6,8 +6,8 @@ side (the products of the reference's optimiser, mintext/optim/optimizer.py:92-1
 
 ``chain`` computes the same in groups of steps, each one Gram product, symmetric S x S products and one product with X, and
 rounds every matrix as it is held between products: in one f16 plane (``planes`` 1) or in two, the diagonals of Q and P and
-what X loses in f16 apart.  Products are in 64 bits: what float32 sums add is a hundredth of one plane's roundings.  ``lose`` leaves out what is kept apart, which says how much of the error it takes away:
-"diagonal" (what f16 loses of the diagonals of Q and P), "remainder" (what it loses of X).
+what X loses in f16 apart.  Products are in 64 bits: what float32 sums add is a hundredth of one plane's roundings.
+``lose`` leaves out what is kept apart, which says how much of the error it takes away: "diagonal" (what f16 loses of the diagonals of Q and P), "remainder" (what it loses of X).
 """
 from __future__ import annotations
 
