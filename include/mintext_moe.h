@@ -50,6 +50,7 @@
  *   mtx_linear, mtx_linear_bwd
  *                          <- Linear.__call__ and the products of MLP (mintext/modules/linear.py:
  *                             123-147, 164-228) with bias, activation and residual, and their VJP
+ *   mtx_norm, mtx_norm_bwd <- RMSNorm (mintext/modules/norm.py:10), layer norm, and their VJP
  *   mtx_newton_schulz, mtx_muon_update
  *                          <- the Muon optimiser over expert stacks (mintext/optim/optimizer.py:
  *                             92-168)
@@ -435,6 +436,24 @@ int mtx_linear(const void* x, const void* w, const void* bias, const void* resid
 int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre, int dtype, int64_t M,
                    int64_t K, int64_t N, int act, void* dz, void* dx, void* dw, void* dbias,
                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- norms ---------------------------------------------------------------------------------
+ * RMSNorm (mintext/modules/norm.py:10) and layer norm of T rows of D values, dense, of one dtype (F32 or
+ * BF16); weight[D] and bias[D] in that or in F32.  1 <= D <= 16384, any alignment; sums in float32.
+ * mtx_norm:     h = x + residual, rounded to dtype (residual and h may both be NULL: h is x);
+ *               rms == 0: y = (h - mean) rstd weight + bias (bias may be NULL), rms != 0: y = h rstd weight.
+ *               mean[T] and rstd[T] may be NULL (mean always with rms).
+ * mtx_norm_bwd: of h, mean and rstd as written there; dh (the gradient of h by itself) may be NULL.
+ *               dx[T,D] is the gradient of x and of residual; dweight[D] and dbias[D] are in weight's
+ *               dtype; those that are NULL are left out (dbias only with dweight).  16-byte aligned workspace,
+ *               not shared by two calls that can run at the same time.                            */
+int mtx_norm(const void* x, const void* residual, const void* weight, const void* bias, int dtype,
+             int weight_dtype, int rms, int64_t T, int64_t D, float eps, void* y, void* h, float* mean,
+             float* rstd, void* stream);
+int64_t mtx_norm_bwd_workspace_size(int64_t T, int64_t D);
+int mtx_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, const float* mean,
+                 const float* rstd, int dtype, int weight_dtype, int rms, int64_t T, int64_t D, void* dx,
+                 void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- orthogonalised updates ---------------------------------------------------------------
  * Muon over stacked expert weights (mintext/optim/optimizer.py:92-168), each of the E matrices by

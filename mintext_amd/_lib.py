@@ -96,6 +96,9 @@ SIGNATURES = {
     "mtx_linear_workspace_size": (_I64, [_I64, _I64, _I64]),
     "mtx_linear": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
     "mtx_linear_bwd": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P, _I64, _P]),
+    "mtx_norm": (_I, [_P, _P, _P, _P, _I, _I, _I, _I64, _I64, _F, _P, _P, _P, _P, _P]),
+    "mtx_norm_bwd_workspace_size": (_I64, [_I64, _I64]),
+    "mtx_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
     "mtx_newton_schulz_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
     "mtx_newton_schulz": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _F, _I, _P, _I64, _I64, _P, _I64, _P]),
     "mtx_muon_update": (_I, [_P, _I, _I64, _I64, _P, _I, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _F, _P,

@@ -1,0 +1,122 @@
+"""Layer norm and RMS norm of rows, with the residual's addition in front, differentiable.
+
+``rms_norm`` is the reference's ``RMSNorm`` (mintext/modules/norm.py:10), the norm in front of every block and of the
+head; ``layer_norm`` is its form with mean and bias.  With ``residual`` one pass computes the new residual stream
+``h = x + residual`` and its norm.  One HIP kernel reads each tensor once; the backward is one pass over ``h`` and the
+gradients and a sum of its workgroups' shares of the weight's and bias's gradients, in a fixed order.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib as L
+
+MAX_WIDTH = 16384
+
+
+def _check(name, x, weight, bias, residual, eps):
+    xs = x.shape
+    if len(xs) < 1 or weight.shape != (xs[-1],):
+        raise ValueError(f"{name} takes x [..., D] and weight [D], got {tuple(xs)} and {tuple(weight.shape)}")
+    if not 0 < xs[-1] <= MAX_WIDTH:
+        raise ValueError(f"{name} takes widths of 1 to {MAX_WIDTH}, got {xs[-1]}")
+    if bias is not None and bias.shape != weight.shape:
+        raise ValueError(f"bias must be [{xs[-1]}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != xs:
+        raise ValueError(f"residual must have x's shape {tuple(xs)}, got {tuple(residual.shape)}")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    dt = x.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float32:
+        raise TypeError(f"{name} takes float32 or bfloat16 tensors, got {dt}")
+    if residual is not None and residual.dtype is not dt:
+        raise TypeError(f"residual must have x's dtype {dt}, got {residual.dtype}")
+    wt = weight.dtype
+    if (wt is not dt and wt is not torch.float32) or (bias is not None and bias.dtype is not wt):
+        raise TypeError(f"weight and bias must share one dtype, {dt} as x or float32")
+
+
+def _forward(x, residual, weight, bias, rms, eps, keep):
+    dev = L.require_device(x, residual, weight, bias)
+    D = x.shape[-1]
+    T = x.numel() // D
+    x, weight = x.contiguous(), weight.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty_like(x)
+    h = None if residual is None else torch.empty_like(x)
+    stats = torch.empty((1 if rms else 2, T), dtype=torch.float32, device=dev) if keep else None
+    rstd = stats[0] if keep else None
+    mean = stats[1] if keep and not rms else None
+    with L.on_device(dev):
+        L.call("mtx_norm", x.data_ptr(), L.ptr(residual), weight.data_ptr(), L.ptr(bias), L.dtype_code(x.dtype),
+               L.dtype_code(weight.dtype), int(rms), T, D, eps, y.data_ptr(), L.ptr(h), L.ptr(mean), L.ptr(rstd), L.stream(dev))
+    return y, (x if h is None else h), stats
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, rms, eps):
+        y, h, stats = _forward(x, residual, weight, bias, rms, eps, True)
+        ctx.save_for_backward(h, weight, stats)
+        ctx.rms, ctx.has_bias, ctx.has_residual = rms, bias is not None, residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, h) if residual is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, stats = ctx.saved_tensors
+        need_x, need_r, need_w, need_b, _, _ = ctx.needs_input_grad
+        if dy is None:  # the sum alone is used
+            return (dh if need_x else None, dh if need_r else None, None, None, None, None)
+        dev = L.require_device(dy, dh, h, weight)
+        dy, weight = dy.contiguous(), weight.contiguous()
+        dh = None if dh is None else dh.contiguous()
+        D = h.shape[-1]
+        T = h.numel() // D
+        dx = torch.empty_like(h) if need_x or need_r else None
+        dw = torch.empty_like(weight) if need_w or need_b else None
+        db = torch.empty_like(weight) if need_b else None
+        ws = L.workspace(L.query("mtx_norm_bwd_workspace_size", T, D) if need_w or need_b else 0, dev)
+        mean = None if ctx.rms else stats[1]
+        with L.on_device(dev):
+            L.call("mtx_norm_bwd", dy.data_ptr(), L.ptr(dh), h.data_ptr(), weight.data_ptr(), L.ptr(mean), stats.data_ptr(),
+                   L.dtype_code(h.dtype), L.dtype_code(weight.dtype), int(ctx.rms), T, D, L.ptr(dx), L.ptr(dw), L.ptr(db),
+                   ws.data_ptr(), ws.numel(), L.stream(dev))
+        return dx if need_x else None, dx if need_r else None, dw if need_w else None, db, None, None
+
+
+def _norm(name, x, weight, bias, rms, eps, residual):
+    eps = float(eps)
+    _check(name, x, weight, bias, residual, eps)
+    if L.plain_forward(x, weight, bias, residual):
+        y, h, _ = _forward(x, residual, weight, bias, rms, eps, False)
+        return y if residual is None else (y, h)
+    return _Norm.apply(x, residual, weight, bias, rms, eps)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, eps: float = 1e-5,
+               residual: torch.Tensor | None = None):
+    """``(h - mean(h)) / sqrt(var(h) + eps) * weight + bias`` over the last dimension, ``h = x + residual``.
+
+    Args:
+        x: [..., D], float32 or bfloat16, D up to 16384.
+        weight: [D], in x's dtype or float32.
+        bias: [D] in the weight's dtype, or None.
+        residual: x's shape and dtype, or None.
+
+    Returns:
+        y in x's shape and dtype; with ``residual`` (y, h), where ``h`` is the sum rounded to x's dtype, of which the
+        norm is taken.  Statistics are in float32.  Differentiable (once) in all four tensors.
+    """
+    return _norm("layer_norm", x, weight, bias, False, eps, residual)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residual: torch.Tensor | None = None):
+    """``h / sqrt(mean(h^2) + eps) * weight`` over the last dimension (mintext/modules/norm.py:10), ``h = x + residual``.
+
+    Arguments, results and gradients as ``layer_norm``'s, without a bias.
+    """
+    return _norm("rms_norm", x, weight, None, True, eps, residual)
