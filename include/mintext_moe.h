@@ -50,6 +50,10 @@
  *   mtx_linear, mtx_linear_bwd
  *                          <- Linear.__call__ and the products of MLP (mintext/modules/linear.py:
  *                             123-147, 164-228) with bias, activation and residual, and their VJP
+ *   mtx_linear_cross_entropy, mtx_linear_cross_entropy_bwd
+ *                          <- the vocabulary-tiled loss with its z-loss (mintext/trainer.py:197-241) and its VJP
+ *   mtx_linear_distillation, mtx_linear_distillation_bwd
+ *                          <- no counterpart; the same against a teacher's top logits
  *   mtx_norm, mtx_norm_bwd <- RMSNorm (mintext/modules/norm.py:10), layer norm, and their VJP
  *   mtx_newton_schulz, mtx_muon_update
  *                          <- the Muon optimiser over expert stacks (mintext/optim/optimizer.py:
@@ -436,6 +440,46 @@ int mtx_linear(const void* x, const void* w, const void* bias, const void* resid
 int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre, int dtype, int64_t M,
                    int64_t K, int64_t N, int act, void* dz, void* dx, void* dw, void* dbias,
                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- losses of a vocabulary-sized head -----------------------------------------------------
+ * z = x[T,D] W, whose logits [T,V] are made in tiles and not stored.  x dense, W dense in one of two orders; both of
+ * one dtype (F32 or BF16) and 16-byte aligned; T, D and V up to 65535 * 64 (D, V at least 1).  Sums in float32.
+ * mtx_linear_cross_entropy: loss[t] = lse[t] - z[t, targets[t]] + z_loss lse[t]^2, lse[t] = log sum exp z[t].
+ *   Tokens whose target is ignore_index have loss 0 and no gradient; those of another target outside [0, V) have
+ *   NaN.  targets: int32, or int64 if targets_64.
+ * mtx_linear_distillation: p = softmax(teacher_logits[t] / temperature) over the entries of a row (K of
+ *   them, K <= 1024) whose index is not negative and whose logit is not -inf; lse[t] = log sum exp(z[t] / temperature);
+ *   loss[t] = temperature^2 sum_k p_k (log p_k - z[t, i_k] / temperature + lse[t]).  A row without such an entry has loss
+ *   0 and no gradient, one with an index of V or more, or a NaN, has NaN; an index that is there twice is two entries.
+ *   entries (mtx_distillation_entries_size bytes, 16-byte aligned) is filled for the backward call.
+ * Both write loss, lse and state[T] (1, 0 for rows left out, NaN) and use chosen[T] (distillation: [T,K]) as scratch.  total
+ *   and count (both or none) receive the sum of the losses and, with `mean`, what it was divided by: the rows that
+ *   are not left out, 1 at least.
+ * The _bwd calls: g is the gradient of total (count as written) or, with count NULL, of loss[T]; dx[T,D] and dw (W's
+ *   order) in dtype, either may be NULL.  dz is rounded to dtype for the products; its columns go through in pieces of 1 GiB
+ *   at most, over which dx is summed in float32.  No two calls that can run at the same time may share a workspace. */
+#define MTX_HEAD_DV 0  /* W[D,V] */
+#define MTX_HEAD_VD 1  /* W[V,D] */
+int64_t mtx_head_loss_workspace_size(int dtype, int64_t T, int64_t D, int64_t V, int order, int backward);
+int64_t mtx_distillation_entries_size(int64_t T, int64_t V, int64_t K);
+int mtx_linear_cross_entropy(const void* x, const void* w, const void* targets, int targets_64, int dtype,
+                             int64_t T, int64_t D, int64_t V, int order, int64_t ignore_index, float z_loss,
+                             int mean, float* loss, float* lse, float* state, float* total, float* count,
+                             float* chosen, void* workspace, int64_t workspace_bytes, void* stream);
+int mtx_linear_cross_entropy_bwd(const float* g, const float* count, const void* x, const void* w,
+                                 const void* targets, int targets_64, const float* lse, const float* state,
+                                 int dtype, int64_t T, int64_t D, int64_t V, int order, float z_loss, void* dx,
+                                 void* dw, void* workspace, int64_t workspace_bytes, void* stream);
+int mtx_linear_distillation(const void* x, const void* w, const void* teacher_idx, int idx_64,
+                            const void* teacher_logits, int logits_dtype, int dtype, int64_t T, int64_t D,
+                            int64_t V, int64_t K, int order, float temperature, int mean, float* loss, float* lse,
+                            float* state, float* total, float* count, float* chosen, void* entries,
+                            int64_t entries_bytes, void* workspace, int64_t workspace_bytes, void* stream);
+int mtx_linear_distillation_bwd(const float* g, const float* count, const void* x, const void* w,
+                                const void* entries, int64_t entries_bytes, const float* lse, const float* state,
+                                int dtype, int64_t T, int64_t D, int64_t V, int64_t K, int order,
+                                float temperature, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
+                                void* stream);
 
 /* ---- norms ---------------------------------------------------------------------------------
  * RMSNorm (mintext/modules/norm.py:10) and layer norm of T rows of D values, dense, of one dtype (F32 or

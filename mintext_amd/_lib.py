@@ -29,6 +29,7 @@ MTX_F32, MTX_BF16, MTX_FP8E4M3 = 0, 1, 2
 MTX_SCORING_SOFTMAX, MTX_SCORING_SIGMOID_GROUP = 0, 1
 MTX_GMM_OP_FWD, MTX_GMM_OP_SWIGLU, MTX_GMM_OP_DLHS = 0, 1, 2
 MTX_NS_F64 = 64
+MTX_HEAD_DV, MTX_HEAD_VD = 0, 1
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -96,6 +97,16 @@ SIGNATURES = {
     "mtx_linear_workspace_size": (_I64, [_I64, _I64, _I64]),
     "mtx_linear": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
     "mtx_linear_bwd": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P, _I64, _P]),
+    "mtx_head_loss_workspace_size": (_I64, [_I, _I64, _I64, _I64, _I, _I]),
+    "mtx_distillation_entries_size": (_I64, [_I64, _I64, _I64]),
+    "mtx_linear_cross_entropy": (_I, [_P, _P, _P, _I, _I, _I64, _I64, _I64, _I, _I64, _F, _I, _P, _P, _P, _P, _P, _P,
+                                      _P, _I64, _P]),
+    "mtx_linear_cross_entropy_bwd": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _I, _F, _P, _P, _P, _I64,
+                                          _P]),
+    "mtx_linear_distillation": (_I, [_P, _P, _P, _I, _P, _I, _I, _I64, _I64, _I64, _I64, _I, _F, _I, _P, _P, _P, _P, _P,
+                                     _P, _P, _I64, _P, _I64, _P]),
+    "mtx_linear_distillation_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _I64, _I, _F, _P, _P,
+                                         _P, _I64, _P]),
     "mtx_norm": (_I, [_P, _P, _P, _P, _I, _I, _I, _I64, _I64, _F, _P, _P, _P, _P, _P]),
     "mtx_norm_bwd_workspace_size": (_I64, [_I64, _I64]),
     "mtx_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I64, _I64, _P, _P, _P, _P, _I64, _P]),

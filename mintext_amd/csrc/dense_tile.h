@@ -51,10 +51,13 @@ constexpr int BKS = 32;  // reduction elements per ring stage
 
 // One operand of a tile: `p[0]` at the tile's first row (or column) of reduction element 0, uniform; `p[1]` the lo
 // plane of it; `ld` its row stride in elements; `left` the rows (rows) or columns (cols) from there that exist.
+// `missing` (cols, TAIL, below 8): lines at the reduction's end that this operand does not have, for which it re-reads its
+// last one; the other operand holds zeros there.
 struct Operand {
   const void* p[2];
   int64_t ld;
   int left;
+  int missing = 0;
 };
 
 // A pointer that is the same in every lane, in scalar registers whatever the compiler can prove.
@@ -95,7 +98,7 @@ template <class F, int TM_, int TN_, int WM_, int WN_, int NST_, bool A_COLS, bo
           bool TWO = false, int DIAG = DIAG_NONE>
 struct Tile {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NST = NST_, PD = NST - 1;
-  static constexpr bool cols = A_COLS;
+  static constexpr bool cols = A_COLS, b_cols = B_COLS;
   static constexpr int NW = WM * WN, NT = NW * 64, BM = 32 * TM * WM, BN = 32 * TN * WN;
   static constexpr int A_BYTES = BM * BKS * 2, B_BYTES = BN * BKS * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int LDS_BYTES = NST * STAGE;
@@ -129,17 +132,17 @@ struct Tile {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / WN, wn = wave % WN;
     const int nk1 = (K + BKS - 1) / BKS, nk = TWO ? 3 * nk1 : nk1;
-    const int tail = K - (nk1 - 1) * BKS;
+    const int tail = K - (nk1 - 1) * BKS, a_tail = tail - (A_COLS ? a.missing : 0), b_tail = tail - (B_COLS ? b.missing : 0);
     uint32_t aoff[A_INSTR], boff[B_INSTR], atail[TAIL ? A_INSTR : 1], btail[TAIL ? B_INSTR : 1];
 #pragma unroll
     for (int i = 0; i < A_INSTR; ++i) {
-      aoff[i] = source<A_COLS, A_INSTR, BM>(a, i, wave, lane, TAIL && nk1 == 1 ? tail : BKS);
-      if constexpr (TAIL) atail[i] = source<A_COLS, A_INSTR, BM>(a, i, wave, lane, tail);
+      aoff[i] = source<A_COLS, A_INSTR, BM>(a, i, wave, lane, TAIL && nk1 == 1 ? a_tail : BKS);
+      if constexpr (TAIL) atail[i] = source<A_COLS, A_INSTR, BM>(a, i, wave, lane, a_tail);
     }
 #pragma unroll
     for (int i = 0; i < B_INSTR; ++i) {
-      boff[i] = source<B_COLS, B_INSTR, BN>(b, i, wave, lane, TAIL && nk1 == 1 ? tail : BKS);
-      if constexpr (TAIL) btail[i] = source<B_COLS, B_INSTR, BN>(b, i, wave, lane, tail);
+      boff[i] = source<B_COLS, B_INSTR, BN>(b, i, wave, lane, TAIL && nk1 == 1 ? b_tail : BKS);
+      if constexpr (TAIL) btail[i] = source<B_COLS, B_INSTR, BN>(b, i, wave, lane, b_tail);
     }
     const int64_t a_step = A_COLS ? a.ld * (BKS * 2) : BKS * 2, b_step = B_COLS ? b.ld * (BKS * 2) : BKS * 2;
     const uint32_t lds_base = lds_addr(lds);

@@ -1,0 +1,167 @@
+// The products of the head's losses in f32 on the f32 matrix cores (f32_tile.h): 64 x 64 tiles of any size and alignment.
+#include "f32_tile.h"
+#include "head_loss.h"
+#include <type_traits>
+
+namespace mtx {
+namespace head {
+
+using f32mm::KS;
+using f32mm::NT;
+constexpr int kRow = 68;  // floats of a row of the tile in LDS
+
+// the tile to LDS, row by row; thread t then holds columns 16 (t % 4) .. of row t / 4
+__device__ __forceinline__ void to_rows(const f32mm::f32x16& acc, float* lds, float v[16]) {
+  const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) >> 1, wn = (threadIdx.x >> 6) & 1;
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    lds[(wm * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4) * kRow + wn * 32 + (lane & 31)] = acc[e];
+  __syncthreads();
+  const float* row = lds + (threadIdx.x >> 2) * kRow + (threadIdx.x & 3) * 16;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = row[e];
+}
+
+template <bool VD, bool DZ, int VEC>
+__global__ __launch_bounds__(NT) void logits_f32_kernel(Logits p) {
+  __shared__ __attribute__((aligned(16))) float lds[2 * f32mm::TILE];
+  static_assert(64 * kRow <= 2 * f32mm::TILE, "the tile fits its operands' place");
+  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
+  const float *X = (const float*)p.x, *W = (const float*)p.w;
+  auto at_x = [&](int r, int c, int s) -> const float* {
+    const int m = m0 + r, k = s * KS + c;
+    return m < p.T && k < p.red ? X + (int64_t)m * p.ldx + k : nullptr;
+  };
+  auto at_w = [&](int r, int c, int s) -> const float* {
+    const int n = VD ? n0 + r : n0 + c, k = VD ? s * KS + c : s * KS + r;
+    return n < p.cols && k < p.red ? W + (VD ? (int64_t)n * p.ldw + k : (int64_t)k * p.ldw + n) : nullptr;
+  };
+  f32mm::f32x16 acc;
+  f32mm::mainloop<float, false, !VD, VEC>(acc, p.red, lds, lds + f32mm::TILE, at_x, at_w, X, W);
+  float v[16];
+  to_rows(acc, lds, v);
+  const int row = m0 + (threadIdx.x >> 2), quarter = threadIdx.x & 3, c0 = n0 + quarter * 16, left = p.cols - c0;
+  const bool live = row < p.T;
+  const int r = live ? row : p.T - 1;
+  float* mine = lds + (threadIdx.x >> 2) * kRow;
+  if constexpr (!DZ) {
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, e < left ? v[e] : -INFINITY);
+    m = fmaxf(m, lane_xchg<0>(m));
+    m = fmaxf(m, lane_xchg<1>(m));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float d = m == -INFINITY ? v[e] : v[e] - m;
+      s += e < left ? exp2f(d * p.scale) : 0.0f;
+    }
+    s += lane_xchg<0>(s);
+    s += lane_xchg<1>(s);
+    if (live && quarter == 0) p.part[(int64_t)((p.v0 + n0) / 64) * p.T + row] = make_float2(m, s);
+    if (!live) return;
+    if (p.e.targets) {
+      const int64_t c = target(p.e, r) - p.v0 - n0;
+      if (quarter == 0 && c >= 0 && c < 64 && c < p.cols - n0) p.chosen[row] = mine[c];
+    } else {
+      const uint16_t* b = p.e.bounds + r * p.e.ldb + (p.v0 + n0) / kBlock;
+      for (int e = b[0] + quarter; e < b[1]; e += 4) {
+        const int c = p.e.idx[(int64_t)r * p.e.K + e] - p.v0 - n0;
+        if ((unsigned)c < 64u) p.chosen[(int64_t)r * p.e.K + e] = mine[c];
+      }
+    }
+  } else {
+    if (!live) return;
+    const float a = p.a[r], b = p.b[r], l2 = p.l2[r];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = a == 0.0f || e >= left ? 0.0f : a * exp2f(__builtin_fmaf(v[e], p.scale, -l2));
+    // the entries among the thread's own columns, in order
+    if (p.e.targets) {
+      const int64_t c = target(p.e, r) - p.v0 - c0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (c == e && e < left) v[e] -= b;
+    } else {
+      const uint16_t* at = p.e.bounds + r * p.e.ldb + (p.v0 + n0) / kBlock;
+      for (int i = at[0]; i < at[1]; ++i) {
+        const int c = p.e.idx[(int64_t)r * p.e.K + i] - p.v0 - c0;
+        const float d = b * p.e.share[(int64_t)r * p.e.K + i];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (c == e) v[e] -= d;
+      }
+    }
+    float* dz = (float*)p.dz + (int64_t)row * p.ldz + c0;
+    st8(dz, 0, v);
+    st8(dz, 8, v + 8);
+  }
+}
+
+template <bool A_COLS, bool B_COLS, int VEC>
+__global__ __launch_bounds__(NT) void product_f32_kernel(Product p) {
+  __shared__ __attribute__((aligned(16))) float as[f32mm::TILE], bs[f32mm::TILE];
+  const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+  const float *A = (const float*)p.a, *B = (const float*)p.b;
+  const int stages = (p.red + KS - 1) / KS, piece = blockIdx.z;
+  const int64_t kb = (int64_t)piece * stages / p.pieces * KS, ke = min((int64_t)(piece + 1) * stages / p.pieces * KS, (int64_t)p.red);
+  auto at_a = [&](int r, int c, int s) -> const float* {
+    const int64_t m = m0 + (A_COLS ? c : r), k = kb + s * KS + (A_COLS ? r : c);
+    return m < p.rows && k < ke ? A + (A_COLS ? k * p.lda + m : m * p.lda + k) : nullptr;
+  };
+  auto at_b = [&](int r, int c, int s) -> const float* {
+    const int64_t n = n0 + (B_COLS ? c : r), k = kb + s * KS + (B_COLS ? r : c);
+    return n < p.cols && k < ke ? B + (B_COLS ? k * p.ldb + n : n * p.ldb + k) : nullptr;
+  };
+  f32mm::f32x16 acc;
+  f32mm::mainloop<float, A_COLS, B_COLS, VEC>(acc, (int)(ke - kb), as, bs, at_a, at_b, A, B);
+  const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) >> 1, wn = (threadIdx.x >> 6) & 1;
+  const int64_t n = n0 + wn * 32 + (lane & 31);
+  if (n >= p.cols) return;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int64_t r = m0 + wm * 32 + 8 * (v / 4) + 4 * (lane >> 5) + v % 4;
+    if (r >= p.rows) continue;
+    float y = acc[v];
+    if (p.acc) {
+      float* s = p.acc + ((int64_t)piece * p.rows + r) * p.ldacc + n;
+      if (p.add) y += *s;
+      if (!p.last) {
+        *s = y;
+        continue;
+      }
+    }
+    ((float*)p.out)[r * p.ldo + n] = y;
+  }
+}
+
+static bool quads(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 4 == 0; }
+
+template <bool VD, bool DZ>
+static int go_logits(const Logits& p, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div(p.cols, 64), (unsigned)ceil_div(p.T, 64));
+  // a whole row of four is inside or outside: of the reduction in x (and W [V][D]), of the columns in W [D][V]
+  const bool vec = quads(p.x, p.ldx) && quads(p.w, p.ldw) && p.red % 4 == 0 && (VD || p.cols % 4 == 0);
+  if (vec) hipLaunchKernelGGL((logits_f32_kernel<VD, DZ, 4>), grid, dim3(NT), 0, st, p);
+  else hipLaunchKernelGGL((logits_f32_kernel<VD, DZ, 1>), grid, dim3(NT), 0, st, p);
+  return check_launch();
+}
+int launch_logits_f32(const Logits& p, bool dz, int order, hipStream_t st) {
+  if (order == ORDER_VD) return dz ? go_logits<true, true>(p, st) : go_logits<true, false>(p, st);
+  return dz ? go_logits<false, true>(p, st) : go_logits<false, false>(p, st);
+}
+
+template <bool A_COLS, bool B_COLS>
+static int go_product(const Product& p, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div(p.cols, 64), (unsigned)ceil_div(p.rows, 64), (unsigned)p.pieces);
+  const bool vec = quads(p.a, p.lda) && quads(p.b, p.ldb) && (A_COLS ? p.rows % 4 == 0 : p.red % 4 == 0) &&
+                   (B_COLS ? p.cols % 4 == 0 : p.red % 4 == 0);
+  if (vec) hipLaunchKernelGGL((product_f32_kernel<A_COLS, B_COLS, 4>), grid, dim3(NT), 0, st, p);
+  else hipLaunchKernelGGL((product_f32_kernel<A_COLS, B_COLS, 1>), grid, dim3(NT), 0, st, p);
+  return check_launch();
+}
+int launch_product_f32(const Product& p, bool a_cols, bool b_cols, hipStream_t st) {
+  if (a_cols) return go_product<true, true>(p, st);
+  return b_cols ? go_product<false, true>(p, st) : go_product<false, false>(p, st);
+}
+
+}  // namespace head
+}  // namespace mtx

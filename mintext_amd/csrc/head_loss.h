@@ -1,0 +1,79 @@
+// What the kernels of the head's losses share: a row's target entries, and the arguments of the products.
+//
+// Of T tokens x [T][D] and the head's weight W the logits z = x W [T][V] are made tile by tile and never stored:
+//   forward   a tile leaves, for each row and block of columns, the maximum m and sum exp((z - m) / tau), and the logits of the
+//             row's entries; merge_kernel joins the blocks.
+//   backward  the vocabulary goes through in pieces: z of a piece again, dz = a softmax(z / tau) - b share (one entry for
+//             cross entropy, a teacher's top ones for distillation) rounded to the operands' type into a workspace, from which
+//             dx += dz W^T (in f32) and dW of the piece = x^T dz.
+// So a step computes 8 T D V operations where 6 would do with the logits kept (a fifth of what they took is saved by
+// neither writing nor reading them), and holds at most kPiece bytes of dz.
+#pragma once
+#include "common.h"
+
+namespace mtx {
+namespace head {
+
+enum { ORDER_DV = 0, ORDER_VD = 1 };  // of the weight in memory
+constexpr int kBlock = 128;           // columns an entry of Entries::bounds stands for
+
+// The classes of a row that its loss names.  Cross entropy: targets[row], int32 or int64.  Distillation: idx and share of
+// row * K .., ascending, and bounds[row * ldb + b], the first of them at column 128 b or behind.
+struct Entries {
+  const void* targets;
+  int wide;  // targets are int64
+  const int32_t* idx;
+  const float* share;
+  const uint16_t* bounds;
+  int64_t ldb;
+  int K;
+};
+__device__ __forceinline__ int64_t target(const Entries& e, int64_t row) {
+  return e.wide ? ((const int64_t*)e.targets)[row] : ((const int32_t*)e.targets)[row];
+}
+
+struct Logits {
+  const void *x, *w;  // w: at column v0
+  int64_t ldx, ldw;
+  int T, red, missing;  // missing: reduction elements that x has (as zeros) and w has not
+  int v0, cols;         // columns of this piece
+  int w_left;           // columns of w that can be read
+  Entries e;
+  float scale;          // log2(e) / tau
+  // forward
+  float2* part;         // [block][T]: maximum of z, sum of exp2((z - maximum) scale)
+  float* chosen;        // [T][K]: z of the entries
+  // backward
+  const float *a, *b, *l2;  // [T]: factors of the softmax and of the shares; log2 of sum exp(z / tau)
+  void* dz;             // [T][ldz], zeros behind the piece's columns
+  int64_t ldz;
+};
+
+// C = A B of a gradient, rows x cols, in `pieces` of the reduction
+struct Product {
+  const void *a, *b;
+  int64_t lda, ldb;
+  int rows, cols, red, missing;  // missing: of B at the reduction's end
+  int a_left, b_left;            // rows or columns of the operands that can be read
+  void* out;
+  int64_t ldo;
+  int pieces;
+  float* acc;                    // [pieces][rows][ldacc] f32, or nullptr: straight to out
+  int64_t ldacc;
+  int add;                       // acc holds sums of earlier calls
+  int last;                      // pieces == 1: the result goes to out
+};
+
+int launch_logits(const Logits& p, bool dz, int order, int path, hipStream_t st);  // bf16
+int launch_product(const Product& p, bool a_cols, bool b_cols, bool small, hipStream_t st);
+int launch_logits_f32(const Logits& p, bool dz, int order, hipStream_t st);
+int launch_product_f32(const Product& p, bool a_cols, bool b_cols, hipStream_t st);
+
+// tiles of the logits: 256 x 256, 128 x 128, 64 x 128 (few rows); f32 64 x 64
+enum { PATH_BIG, PATH_SMALL, PATH_THIN, PATH_F32 };
+inline int tile_rows(int path) { return path == PATH_BIG ? 256 : path == PATH_SMALL ? 128 : 64; }
+inline int tile_cols(int path) { return path == PATH_BIG ? 256 : path == PATH_F32 ? 64 : 128; }
+inline int block_cols(int path) { return path == PATH_BIG ? 128 : 64; }  // of a partial maximum and sum
+
+}  // namespace head
+}  // namespace mtx

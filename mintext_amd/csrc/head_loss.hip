@@ -1,0 +1,604 @@
+// The losses of a vocabulary-sized head without its logits in memory: softmax cross entropy and distillation from a
+// teacher's top logits, with their gradients.  What the products' kernels do is in head_loss.h; here are the kernels beside
+// them and the order in which they run.
+//
+//   cross entropy   L_t = lse_t - z[t, y_t] + c lse_t^2,  dz = g_t ((1 + 2 c lse_t) softmax(z_t) - onehot(y_t))
+//   distillation    p = softmax(teacher / tau) over the row's entries, q = softmax(z / tau),
+//                   L_t = tau^2 sum_k p_k (log p_k - log q[i_k]),  dz = g_t tau (q - sum_k p_k onehot(i_k))
+//
+// A row's state is 1, 0 (left out: the ignored class, no entry; its loss is 0 and its gradient too) or NaN (a class
+// that is none), which its loss and its gradient become.
+#include "head_loss.h"
+#include <algorithm>
+
+namespace mtx {
+namespace head {
+
+constexpr int kMaxEntries = 1024;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// ---- a teacher's entries: shares, in the order of their classes ------------------------------------------------
+// A wave takes a row.  The place of an entry is the number of those before it (K^2 comparisons in LDS: 0.1 ms for 8192
+// rows of 1024 by the rate of the LDS, nothing beside the products).
+struct Prep {
+  const void *idx, *logits;
+  int wide, f32;  // int64 indices; f32 logits (else bf16)
+  int64_t T, V;
+  int K;
+  float inv_tau;
+  int32_t* sorted;
+  float* share;
+  uint16_t* bounds;
+  int64_t ldb;
+  float2* row;  // state, sum p log p
+};
+__device__ __forceinline__ float wave_sum(float v) {
+  v += lane_xchg<0>(v);
+  v += lane_xchg<1>(v);
+  v += lane_xchg<2>(v);
+  v += lane_xchg<3>(v);
+  v += lane_xchg<4>(v);
+  return v + lane_xchg<5>(v);
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, lane_xchg<0>(v));
+  v = fmaxf(v, lane_xchg<1>(v));
+  v = fmaxf(v, lane_xchg<2>(v));
+  v = fmaxf(v, lane_xchg<3>(v));
+  v = fmaxf(v, lane_xchg<4>(v));
+  return fmaxf(v, lane_xchg<5>(v));
+}
+__global__ __launch_bounds__(64) void entries_kernel(Prep p) {
+  __shared__ int32_t at[kMaxEntries], sorted[kMaxEntries];
+  __shared__ float val[kMaxEntries];
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x, base = row * p.K;
+  float m = -INFINITY;
+  bool bad = false;
+  for (int k = lane; k < p.K; k += 64) {
+    const int64_t i = p.wide ? ((const int64_t*)p.idx)[base + k] : ((const int32_t*)p.idx)[base + k];
+    const float t = (p.f32 ? ((const float*)p.logits)[base + k] : bf16_to_f32(((const uint16_t*)p.logits)[base + k])) * p.inv_tau;
+    const bool live = i >= 0 && !(t == -INFINITY);  // NaN counts, and makes the row's shares NaN
+    bad |= i >= p.V || (live && t != t);
+    at[k] = live && i < p.V ? (int32_t)i : INT32_MAX;
+    val[k] = t;
+    if (live) m = fmaxf(m, t);
+  }
+  m = wave_max(m);
+  const bool invalid = __ballot(bad) != 0;
+  __syncthreads();
+  float sum = 0.0f, count = 0.0f;
+  for (int k = lane; k < p.K; k += 64) {
+    const float e = at[k] == INT32_MAX ? 0.0f : expf(val[k] - m);
+    sum += e;
+    count += at[k] == INT32_MAX ? 0.0f : 1.0f;
+  }
+  sum = wave_sum(sum);
+  count = wave_sum(count);
+  const float log_sum = logf(sum);
+  float entropy = 0.0f;
+  for (int k = lane; k < p.K; k += 64) {
+    const int32_t i = at[k];
+    const float d = val[k] - m, share = i == INT32_MAX ? 0.0f : expf(d) / sum;
+    if (share > 0.0f || share != share) entropy += share * (d - log_sum);
+    int place = 0;
+    for (int j = 0; j < p.K; ++j) place += at[j] < i || (at[j] == i && j < k);
+    sorted[place] = i;
+    p.sorted[base + place] = i;
+    p.share[base + place] = share;
+  }
+  entropy = wave_sum(entropy);
+  if (lane == 0) p.row[row] = make_float2(invalid ? NAN : count > 0.0f ? 1.0f : 0.0f, entropy);
+  __syncthreads();
+  const int n = (int)count;
+  for (int64_t b = lane; b < p.ldb; b += 64) {
+    const int64_t first = b * kBlock;
+    int lo = 0, hi = n;  // the first entry at `first` or behind
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sorted[mid] < first) lo = mid + 1;
+      else hi = mid;
+    }
+    p.bounds[row * p.ldb + b] = (uint16_t)lo;
+  }
+}
+
+// ---- the blocks' maxima and sums, and the row's loss -------------------------------------------------------
+// R rows a workgroup, 256 / R threads a row; the joins are in a fixed order.
+struct Merge {
+  const float2* part;
+  int64_t blocks, T, V;
+  Entries e;
+  const float2* row;  // distillation: state, sum p log p
+  const float* chosen;
+  int64_t ignore;
+  float scale, inv_tau, unit, z_loss;  // unit: tau^2
+  float *loss, *lse, *state;           // loss: [T]
+};
+template <int R>
+__global__ __launch_bounds__(256) void merge_kernel(Merge p) {
+  constexpr int G = 256 / R;
+  __shared__ float ms[G][R], ss[G][R];
+  const int tx = threadIdx.x % R, g = threadIdx.x / R;
+  const int64_t row = (int64_t)blockIdx.x * R + tx;
+  const bool live = row < p.T;
+  float m = -INFINITY, s = 0.0f;
+  auto join = [&](float om, float os) {  // -inf with -inf: sums of 0
+    const float n = fmaxf(m, om);
+    s = s * exp2f(m == n ? 0.0f : (m - n) * p.scale) + os * exp2f(om == n ? 0.0f : (om - n) * p.scale);
+    m = n;
+  };
+  if (live) {
+    int64_t b = g;
+    for (; b + 3 * G < p.blocks; b += 4 * G) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = p.part[(b + u * G) * p.T + row];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) join(v[u].x, v[u].y);
+    }
+    for (; b < p.blocks; b += G) {
+      const float2 v = p.part[b * p.T + row];
+      join(v.x, v.y);
+    }
+  }
+  ms[g][tx] = m;
+  ss[g][tx] = s;
+  __syncthreads();
+  m = ms[0][tx];
+  s = ss[0][tx];
+  for (int i = 1; i < G; ++i) join(ms[i][tx], ss[i][tx]);
+  // sum of share (m - z) / tau, whose terms are small where the share is not
+  float below = 0.0f;
+  if (live && !p.e.targets) {
+    const int64_t at = row * p.e.K;
+    const int n = p.e.bounds[row * p.e.ldb + p.e.ldb - 1];
+    for (int k = g; k < n; k += G) {
+      const float w = p.e.share[at + k];
+      if (w != 0.0f) below += w * ((m - p.chosen[at + k]) * p.inv_tau);
+    }
+  }
+  __syncthreads();
+  ms[g][tx] = below;
+  __syncthreads();
+  if (g > 0 || !live) return;
+  for (int i = 1; i < G; ++i) below += ms[i][tx];
+  float state, konst = 0.0f;
+  if (p.e.targets) {
+    const int64_t y = target(p.e, row);
+    state = y == p.ignore ? 0.0f : y < 0 || y >= p.V ? NAN : 1.0f;
+    if (state == 1.0f) below = m - p.chosen[row];
+  } else {
+    state = p.row[row].x;
+    konst = p.row[row].y;
+  }
+  const float log_sum = logf(s), lse = m * p.inv_tau + log_sum;
+  float loss = p.unit * (konst + below + log_sum);
+  if (p.z_loss != 0.0f) loss += p.z_loss * lse * lse;
+  p.loss[row] = state == 0.0f ? 0.0f : state * loss;
+  p.lse[row] = lse;
+  p.state[row] = state;
+}
+
+// The sum of the rows' losses and what it is divided by, in 64 bits and one workgroup's order.
+__global__ __launch_bounds__(1024) void total_kernel(const float* loss, const float* state, int64_t T, int mean, float* out,
+                                                     float* count) {
+  __shared__ double s[16][2];
+  double sum = 0.0, n = 0.0;
+  for (int64_t t = threadIdx.x; t < T; t += 1024) {
+    sum += loss[t];
+    n += state[t] == 0.0f ? 0.0 : 1.0;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    sum += __shfl_xor(sum, d);
+    n += __shfl_xor(n, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    s[threadIdx.x >> 6][0] = sum;
+    s[threadIdx.x >> 6][1] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+  for (int w = 1; w < 16; ++w) {
+    sum += s[w][0];
+    n += s[w][1];
+  }
+  n = mean ? fmax(n, 1.0) : 1.0;
+  *out = (float)(sum / n);
+  *count = (float)n;
+}
+
+// ---- backward: a row's factors ----------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void factors_kernel(const float* g, const float* count, const float* lse, const float* state,
+                                                      int64_t T, float unit, float z_loss, float* a, float* b, float* l2) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= T) return;
+  const float st = state[t], l = lse[t];
+  const float w = st == 0.0f ? 0.0f : st * unit * (count ? g[0] / *count : g[t]);
+  b[t] = w;
+  a[t] = w == 0.0f ? 0.0f : w * (1.0f + 2.0f * z_loss * l);
+  l2[t] = l * kLog2e;
+}
+
+// rows x cols of a bf16 matrix into one with rows of `ld` (a multiple of 8), zeros behind the columns
+__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ in, int64_t ldi, int64_t rows, int64_t cols,
+                                                  uint16_t* __restrict__ out, int64_t ld) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (i >= rows * ld) return;
+  const int64_t r = i / ld, c = i % ld;
+  uint16_t v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = c + q < cols ? in[r * ldi + c + q] : (uint16_t)0;
+  v4u32 o;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) o[q] = (uint32_t)v[2 * q] | ((uint32_t)v[2 * q + 1] << 16);
+  *(v4u32*)(out + i) = o;
+}
+
+// out = the pieces' sums, in order.  V columns a thread.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc, int pieces, int64_t rows, int64_t cols,
+                                                   int64_t ldacc, T* __restrict__ out, int64_t ldo) {
+  const int64_t per = (cols + V - 1) / V, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const int64_t r = i / per, c = i % per * V, at = r * ldacc + c, n = rows * ldacc;
+  if constexpr (V == 8) {
+    float v[8];
+    ld8(acc, at, v);
+    for (int s = 1; s < pieces; ++s) {
+      float o[8];
+      ld8(acc + s * n, at, o);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += o[q];
+    }
+    st8(out, r * ldo + c, v);
+  } else {
+    float v = acc[at];
+    for (int s = 1; s < pieces; ++s) v += acc[s * n + at];
+    if constexpr (sizeof(T) == 4) out[r * ldo + c] = v;
+    else out[r * ldo + c] = f32_to_bf16(v);
+  }
+}
+
+// ---- how a call runs, by its sizes alone --------------------------------------------------------------------------
+constexpr int64_t kPiece = (int64_t)1 << 30;  // bytes of dz held at a time, at most
+constexpr int64_t kCopy = (int64_t)256 << 20;  // bytes of a padded copy of the weight's columns held at a time, at most
+constexpr int kMostPieces = 16;
+
+struct Split {
+  bool small;  // bf16: tiles of 128 x 128, else of 256 x 256
+  int pieces;
+};
+// A product's tiles and pieces by an estimate of its time in us: rounds of the chip by what a stage of 32 takes, and what the
+// pieces' sums take to write, read and join.
+static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
+  const int64_t stages = ceil_div(red, 32);
+  Split best{false, 1};
+  double least = 1e30;
+  for (int kind = 0; kind < (f32 ? 1 : 2); ++kind) {
+    const int64_t side = f32 ? 64 : kind ? 128 : 256, slots = f32 ? 512 : kind ? 512 : 256;
+    const int64_t tiles = ceil_div(rows, side) * ceil_div(cols, side);
+    const double stage = f32 ? 0.9 : kind ? 0.6 : 0.85;
+    for (int s = 1; s <= kMostPieces && (s == 1 || stages / s >= 8); ++s) {
+      const double t = ceil_div(tiles * s, slots) * (ceil_div(stages, s) * stage + 6.0) +
+                       (s > 1 ? s * rows * cols * 8 / 4e6 + 6.0 : 0.0);
+      if (t < least) {
+        least = t;
+        best = {kind == 1, s};
+      }
+    }
+  }
+  return best;
+}
+
+struct Plan {
+  bool f32;
+  int64_t T, D, V, D8;       // D8: x's row length in use
+  int order;
+  bool copy_x, copy_w;
+  int64_t piece;             // columns of a piece, a multiple of 256
+  int path;
+  Split dx, dw;
+  int64_t ld_dx, ld_dw, rows_dw;
+  // bytes from the workspace's start
+  int64_t x, w, part, factors, dz, acc_dx, acc_dw, total;
+};
+static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool backward) {
+  Plan p{};
+  p.f32 = dtype == MTX_F32;
+  p.T = T, p.D = D, p.V = V, p.order = order;
+  const int64_t size = p.f32 ? 4 : 2, all = round_up(V, 256);
+  p.copy_x = !p.f32 && D % 8 != 0;
+  p.copy_w = !p.f32 && (order == ORDER_DV ? V : D) % 8 != 0;
+  p.D8 = p.copy_x ? round_up(D, 8) : D;
+  int64_t most = all;
+  if (p.copy_w) most = std::min(most, std::max<int64_t>(kCopy / (p.D8 * 2) / 256 * 256, 256));
+  if (backward) most = std::min(most, std::max<int64_t>(kPiece / (T * size) / 256 * 256, 256));
+  p.piece = round_up(ceil_div(V, ceil_div(all, most)), 256);
+  const int64_t big = ceil_div(T, 256) * ceil_div(p.piece, 256);
+  p.path = p.f32 ? PATH_F32 : T <= 64 ? PATH_THIN : big >= 192 ? PATH_BIG : PATH_SMALL;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round_up(bytes, 256);
+    return here;
+  };
+  p.x = take(p.copy_x ? T * p.D8 * 2 : 0);
+  p.w = take(p.copy_w ? p.piece * p.D8 * 2 : 0);
+  if (!backward) {
+    p.part = take(round_up(V, tile_cols(p.path)) / block_cols(p.path) * T * 8);
+  } else {
+    p.factors = take(3 * T * 4);
+    p.dz = take(T * p.piece * size);
+    p.dx = split(p.f32, T, D, std::min(p.piece, V));
+    p.ld_dx = round_up(D, 8);
+    p.acc_dx = take(p.dx.pieces > 1 || p.piece < V ? p.dx.pieces * T * p.ld_dx * 4 : 0);
+    const int64_t n = std::min(p.piece, V);
+    p.rows_dw = order == ORDER_DV ? D : n;
+    p.ld_dw = round_up(order == ORDER_DV ? n : D, 8);
+    p.dw = split(p.f32, p.rows_dw, order == ORDER_DV ? n : D, T);
+    p.acc_dw = take(p.dw.pieces > 1 ? p.dw.pieces * p.rows_dw * p.ld_dw * 4 : 0);
+  }
+  p.total = std::max<int64_t>(at, 256);
+  return p;
+}
+
+static int check_sizes(int dtype, int64_t T, int64_t D, int64_t V, int order) {
+  if (dtype != MTX_F32 && dtype != MTX_BF16) return MTX_ERR_ARG;
+  if (order != ORDER_DV && order != ORDER_VD) return MTX_ERR_ARG;
+  if (T < 0 || D <= 0 || V <= 0) return MTX_ERR_ARG;
+  const int64_t most = 65535 * 64;  // rows of tiles in a grid; 32-bit offsets inside a tile
+  if (T > most || D > most || V > most) return MTX_ERR_UNSUPPORTED;
+  return MTX_OK;
+}
+static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+static int pad(const void* in, int64_t ldi, int64_t rows, int64_t cols, char* out, int64_t ld, hipStream_t st) {
+  hipLaunchKernelGGL(pad_kernel, dim3((unsigned)ceil_div(rows * ld, 2048)), dim3(256), 0, st, (const uint16_t*)in, ldi, rows, cols,
+                     (uint16_t*)out, ld);
+  return check_launch();
+}
+// The operands of the logits of columns v0 ..: x and w where they are, or copies with rows of whole 16-byte chunks
+static int operands(const Plan& p, const void* x, const void* w, int64_t v0, char* ws, Logits& a, hipStream_t st) {
+  const int64_t size = p.f32 ? 4 : 2, n = std::min(p.piece, p.V - v0);
+  int rc = MTX_OK;
+  a.x = p.copy_x ? ws + p.x : x;
+  if (p.copy_x && v0 == 0) rc = pad(x, p.D, p.T, p.D, ws + p.x, p.D8, st);
+  a.ldx = p.D8;
+  a.w = (const char*)w + (p.order == ORDER_DV ? v0 : v0 * p.D) * size;
+  a.ldw = p.order == ORDER_DV ? p.V : p.D;
+  a.w_left = (int)n;
+  if (p.copy_w && rc == MTX_OK) {
+    const bool dv = p.order == ORDER_DV;
+    rc = pad(a.w, a.ldw, dv ? p.D : n, dv ? n : p.D, ws + p.w, dv ? p.piece : p.D8, st);
+    a.w = ws + p.w;
+    a.ldw = dv ? p.piece : p.D8;
+    if (dv) a.w_left = (int)p.piece;
+  }
+  a.T = (int)p.T;
+  a.red = (int)p.D8;
+  a.missing = p.order == ORDER_DV ? (int)(p.D8 - p.D) : 0;
+  a.v0 = (int)v0;
+  a.cols = (int)n;
+  return rc;
+}
+static int logits(const Plan& p, const Logits& a, bool dz, hipStream_t st) {
+  return p.f32 ? launch_logits_f32(a, dz, p.order, st) : launch_logits(a, dz, p.order, p.path, st);
+}
+static int product(const Plan& p, const Product& a, bool a_cols, bool b_cols, const Split& s, hipStream_t st) {
+  return p.f32 ? launch_product_f32(a, a_cols, b_cols, st) : launch_product(a, a_cols, b_cols, s.small, st);
+}
+static int join(bool f32, const float* acc, int pieces, int64_t rows, int64_t cols, int64_t ldacc, void* out, int64_t ldo,
+                hipStream_t st) {
+  const bool vec = cols % 8 == 0 && ldo % 8 == 0 && aligned16(out);
+  const dim3 grid((unsigned)ceil_div(rows * (vec ? cols / 8 : cols), 256));
+#define MTX_JOIN(T, V) hipLaunchKernelGGL((join_kernel<T, V>), grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (T*)out, ldo)
+  if (f32) {
+    if (vec) MTX_JOIN(float, 8);
+    else MTX_JOIN(float, 1);
+  } else {
+    if (vec) MTX_JOIN(uint16_t, 8);
+    else MTX_JOIN(uint16_t, 1);
+  }
+#undef MTX_JOIN
+  return check_launch();
+}
+
+// Both losses: the logits' blocks of every piece, their join, and the sum over the rows if `total` is asked for.
+static int forward(const Plan& p, const void* x, const void* w, Merge m, float* chosen, float* total, float* count, int mean,
+                   char* ws, hipStream_t st) {
+  Logits a{};
+  a.e = m.e;
+  a.scale = m.scale;
+  a.part = (float2*)(ws + p.part);
+  a.chosen = chosen;
+  for (int64_t v0 = 0; v0 < p.V; v0 += p.piece) {
+    int rc = operands(p, x, w, v0, ws, a, st);
+    if (rc == MTX_OK) rc = logits(p, a, false, st);
+    if (rc != MTX_OK) return rc;
+  }
+  m.part = a.part;
+  m.blocks = ceil_div(p.V, tile_cols(p.path)) * (tile_cols(p.path) / block_cols(p.path));
+  m.T = p.T;
+  m.V = p.V;
+  m.chosen = chosen;
+  if (p.T > 2048) hipLaunchKernelGGL(merge_kernel<32>, dim3((unsigned)ceil_div(p.T, 32)), dim3(256), 0, st, m);
+  else hipLaunchKernelGGL(merge_kernel<4>, dim3((unsigned)ceil_div(p.T, 4)), dim3(256), 0, st, m);
+  if (total) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, m.loss, m.state, p.T, mean, total, count);
+  return check_launch();
+}
+
+static int backward(const Plan& p, const float* g, const float* count, const void* x, const void* w, const float* lse,
+                    const float* state, const Entries& e, float scale, float unit, float z_loss, void* dx, void* dw, char* ws,
+                    hipStream_t st) {
+  const int64_t size = p.f32 ? 4 : 2;
+  const bool dv = p.order == ORDER_DV;
+  float* f = (float*)(ws + p.factors);
+  hipLaunchKernelGGL(factors_kernel, dim3((unsigned)ceil_div(p.T, 256)), dim3(256), 0, st, g, count, lse, state, p.T, unit, z_loss,
+                     f, f + p.T, f + 2 * p.T);
+  int rc = check_launch();
+  Logits a{};
+  a.e = e;
+  a.scale = scale;
+  a.a = f, a.b = f + p.T, a.l2 = f + 2 * p.T;
+  a.dz = ws + p.dz;
+  a.ldz = p.piece;
+  for (int64_t v0 = 0; v0 < p.V && rc == MTX_OK; v0 += p.piece) {
+    rc = operands(p, x, w, v0, ws, a, st);
+    if (rc == MTX_OK) rc = logits(p, a, true, st);
+    if (rc != MTX_OK) return rc;
+    if (dx) {
+      const int red = p.f32 ? a.cols : (int)round_up(a.cols, 8);  // dz holds zeros behind its columns
+      const bool only = p.piece >= p.V, final = v0 + p.piece >= p.V;
+      // the last piece of the vocabulary may be shorter than what the split was made for
+      const int pieces = (int)std::min<int64_t>(p.dx.pieces, ceil_div(red, 32));
+      Product q{a.dz, a.w, a.ldz, a.ldw, (int)p.T, (int)p.D, red, 0, (int)p.T, (int)(dv ? p.D : p.D8), dx, p.D, pieces, nullptr,
+                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final};
+      if (!dv) q.missing = red - a.cols;
+      if (!(only && p.dx.pieces == 1)) q.acc = (float*)(ws + p.acc_dx);
+      rc = product(p, q, false, !dv, p.dx, st);
+      if (rc == MTX_OK && final && p.dx.pieces > 1) rc = join(p.f32, q.acc, p.dx.pieces, p.T, p.D, p.ld_dx, dx, p.D, st);
+      if (rc != MTX_OK) return rc;
+    }
+    if (dw) {
+      char* out = (char*)dw + (dv ? v0 : v0 * p.D) * size;
+      const int64_t ldo = dv ? p.V : p.D;
+      Product q{};
+      if (dv) q = Product{a.x, a.dz, a.ldx, a.ldz, (int)p.D, a.cols, (int)p.T, 0, (int)p.D8, (int)p.piece, out, ldo, p.dw.pieces};
+      else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, (int)p.T, 0, (int)p.piece, (int)p.D8, out, ldo, p.dw.pieces};
+      q.ldacc = p.ld_dw;
+      q.last = p.dw.pieces == 1;
+      if (p.dw.pieces > 1) q.acc = (float*)(ws + p.acc_dw);
+      rc = product(p, q, true, true, p.dw, st);
+      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, q.rows, q.cols, p.ld_dw, out, ldo, st);
+    }
+  }
+  return rc;
+}
+
+// the teacher's entries as saved from the forward to the backward pass: classes, shares, bounds, rows
+struct Saved {
+  int64_t share, bounds, row, ldb, total;
+};
+static Saved saved(int64_t T, int64_t V, int64_t K) {
+  Saved s;
+  s.ldb = ceil_div(V, kBlock) + 2;  // the blocks' starts and the last one's end, twice: a tile may begin behind the vocabulary
+  s.share = round_up(T * K * 4, 256);
+  s.bounds = s.share + round_up(T * K * 4, 256);
+  s.row = s.bounds + round_up(T * s.ldb * 2, 256);
+  s.total = s.row + round_up(T * 8, 256);
+  return s;
+}
+static Entries entries(char* buf, const Saved& s, int64_t K) {
+  return Entries{nullptr, 0, (const int32_t*)buf, (const float*)(buf + s.share), (const uint16_t*)(buf + s.bounds), s.ldb, (int)K};
+}
+
+}  // namespace head
+}  // namespace mtx
+
+using namespace mtx;
+
+extern "C" int64_t mtx_head_loss_workspace_size(int dtype, int64_t T, int64_t D, int64_t V, int order, int backward) {
+  if (head::check_sizes(dtype, T, D, V, order) != MTX_OK) return -1;
+  return T == 0 ? 256 : head::plan(dtype, T, D, V, order, backward != 0).total;
+}
+extern "C" int64_t mtx_distillation_entries_size(int64_t T, int64_t V, int64_t K) {
+  if (T < 0 || V <= 0 || K <= 0 || K > head::kMaxEntries) return -1;
+  return std::max<int64_t>(head::saved(T, V, K).total, 256);
+}
+
+extern "C" int mtx_linear_cross_entropy(const void* x, const void* w, const void* targets, int targets_64, int dtype, int64_t T,
+                                        int64_t D, int64_t V, int order, int64_t ignore_index, float z_loss, int mean,
+                                        float* loss, float* lse, float* state, float* total, float* count, float* chosen,
+                                        void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace head;
+  const int rc = check_sizes(dtype, T, D, V, order);
+  if (rc != MTX_OK) return rc;
+  if (!(z_loss >= 0.0f && z_loss < INFINITY) || (!total != !count)) return MTX_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  if (T == 0) {
+    if (total) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, state, (int64_t)0, mean, total, count);
+    return check_launch();
+  }
+  if (!x || !w || !targets || !loss || !lse || !state || !chosen || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  const Plan p = plan(dtype, T, D, V, order, false);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
+  Merge m{};
+  m.e = Entries{targets, targets_64, nullptr, nullptr, nullptr, 0, 1};
+  m.ignore = ignore_index;
+  m.scale = kLog2e, m.inv_tau = 1.0f, m.unit = 1.0f, m.z_loss = z_loss;
+  m.loss = loss, m.lse = lse, m.state = state;
+  return forward(p, x, w, m, chosen, total, count, mean, (char*)workspace, st);
+}
+
+extern "C" int mtx_linear_cross_entropy_bwd(const float* g, const float* count, const void* x, const void* w, const void* targets,
+                                            int targets_64, const float* lse, const float* state, int dtype, int64_t T, int64_t D,
+                                            int64_t V, int order, float z_loss, void* dx, void* dw, void* workspace,
+                                            int64_t workspace_bytes, void* stream) {
+  using namespace head;
+  const int rc = check_sizes(dtype, T, D, V, order);
+  if (rc != MTX_OK) return rc;
+  if (T == 0 || (!dx && !dw)) return MTX_OK;
+  if (!g || !x || !w || !targets || !lse || !state || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  const Plan p = plan(dtype, T, D, V, order, true);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
+  const Entries e{targets, targets_64, nullptr, nullptr, nullptr, 0, 1};
+  return backward(p, g, count, x, w, lse, state, e, kLog2e, 1.0f, z_loss, dx, dw, (char*)workspace, (hipStream_t)stream);
+}
+
+extern "C" int mtx_linear_distillation(const void* x, const void* w, const void* teacher_idx, int idx_64,
+                                       const void* teacher_logits, int logits_dtype, int dtype, int64_t T, int64_t D, int64_t V,
+                                       int64_t K, int order, float temperature, int mean, float* loss, float* lse, float* state,
+                                       float* total, float* count, float* chosen, void* entries_buffer, int64_t entries_bytes,
+                                       void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace head;
+  const int rc = check_sizes(dtype, T, D, V, order);
+  if (rc != MTX_OK) return rc;
+  if (K <= 0 || (logits_dtype != MTX_F32 && logits_dtype != MTX_BF16)) return MTX_ERR_ARG;
+  if (K > kMaxEntries) return MTX_ERR_UNSUPPORTED;
+  const float inv = 1.0f / temperature;
+  if (!(temperature > 0.0f && temperature < INFINITY && inv < INFINITY) || (!total != !count)) return MTX_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  if (T == 0) {
+    if (total) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, state, (int64_t)0, mean, total, count);
+    return check_launch();
+  }
+  if (!x || !w || !teacher_idx || !teacher_logits || !loss || !lse || !state || !chosen || !entries_buffer || !aligned16(x) ||
+      !aligned16(w))
+    return MTX_ERR_ARG;
+  const Plan p = plan(dtype, T, D, V, order, false);
+  const Saved s = saved(T, V, K);
+  if (!aligned16(entries_buffer) || entries_bytes < s.total) return MTX_ERR_WORKSPACE;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
+  char* buf = (char*)entries_buffer;
+  const Prep prep{teacher_idx, teacher_logits, idx_64, logits_dtype == MTX_F32, T, V, (int)K, inv, (int32_t*)buf,
+                  (float*)(buf + s.share), (uint16_t*)(buf + s.bounds), s.ldb, (float2*)(buf + s.row)};
+  hipLaunchKernelGGL(entries_kernel, dim3((unsigned)T), dim3(64), 0, st, prep);
+  Merge m{};
+  m.e = entries(buf, s, K);
+  m.row = prep.row;
+  m.scale = kLog2e * inv, m.inv_tau = inv, m.unit = temperature * temperature;
+  m.loss = loss, m.lse = lse, m.state = state;
+  return forward(p, x, w, m, chosen, total, count, mean, (char*)workspace, st);
+}
+
+extern "C" int mtx_linear_distillation_bwd(const float* g, const float* count, const void* x, const void* w,
+                                           const void* entries_buffer, int64_t entries_bytes, const float* lse,
+                                           const float* state, int dtype, int64_t T, int64_t D, int64_t V, int64_t K, int order,
+                                           float temperature, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
+                                           void* stream) {
+  using namespace head;
+  const int rc = check_sizes(dtype, T, D, V, order);
+  if (rc != MTX_OK) return rc;
+  if (K <= 0 || !(temperature > 0.0f && temperature < INFINITY)) return MTX_ERR_ARG;
+  if (K > kMaxEntries) return MTX_ERR_UNSUPPORTED;
+  if (T == 0 || (!dx && !dw)) return MTX_OK;
+  if (!g || !x || !w || !entries_buffer || !lse || !state || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  const Plan p = plan(dtype, T, D, V, order, true);
+  const Saved s = saved(T, V, K);
+  if (!aligned16(entries_buffer) || entries_bytes < s.total) return MTX_ERR_WORKSPACE;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
+  return backward(p, g, count, x, w, lse, state, entries((char*)const_cast<void*>(entries_buffer), s, K), kLog2e / temperature,
+                  temperature, 0.0f, dx, dw, (char*)workspace, (hipStream_t)stream);
+}

@@ -1,0 +1,243 @@
+// The products of the head's losses in bf16 on the 16-bit matrix cores (dense_tile.h), and what their tiles do
+// with the logits on the way out.
+#include "dense_tile.h"
+#include "head_loss.h"
+
+namespace mtx {
+namespace head {
+
+using dense::Operand;
+template <bool VD, bool TAIL> using Big = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, false, !VD, TAIL>;
+template <bool VD, bool TAIL> using Small = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, false, !VD, TAIL>;
+template <bool VD, bool TAIL> using Thin = dense::Tile<dense::Bf16, 1, 2, 2, 2, 6, false, !VD, TAIL>;
+
+// Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2.
+constexpr int kGroup = 8;
+template <class T>
+__device__ __forceinline__ void tile_at(int t, int nm, int nn, int& m0, int& n0) {
+  const int g = t / (kGroup * nn), gs = min(kGroup, nm - g * kGroup), in = t - g * kGroup * nn;
+  m0 = (g * kGroup + in % gs) * T::BM;
+  n0 = in / gs * T::BN;
+}
+// where the way out of a wave (Tile::put) keeps column c of row r
+template <class T>
+__device__ __forceinline__ float* in_lds(char* mine, int r, int c) {
+  return (float*)(mine + r * (T::TN * 128) + (((c >> 2) ^ (r & (T::TN * 8 - 1))) << 4) + (c & 3) * 4);
+}
+
+// A lane holds, of 32 rows at a time, one row's 16 TN values in columns 32 j + 8 g + 4 (lane / 32) + q: the row's maximum and
+// sum are taken in the lane and joined with that of lane ^ 32.  Entries are looked up in LDS, where the 32 rows are put
+// for that only if one of them has an entry among the wave's columns.
+template <class T, bool DZ>
+__global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logits_kernel(Logits p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
+  static_assert(T::NW * T::OUT_BYTES <= T::LDS_BYTES, "the way out fits the ring");
+  constexpr int BC = T::TN * 32;  // the wave's columns
+  const int nm = (p.T + T::BM - 1) / T::BM, nn = (p.cols + T::BN - 1) / T::BN;
+  const int t = dense::tile_of(blockIdx.x, nm * nn);
+  if (t < 0) return;
+  int m0, n0;
+  tile_at<T>(t, nm, nn, m0, n0);
+  const uint16_t *x = (const uint16_t*)p.x + (int64_t)m0 * p.ldx, *w = (const uint16_t*)p.w;
+  w += T::b_cols ? (int64_t)n0 : (int64_t)n0 * p.ldw;
+  const Operand ox{{x, x}, p.ldx, p.T - m0}, ow{{w, w}, p.ldw, p.w_left - n0, p.missing};
+  dense::f32x16 acc[T::TM][T::TN];
+  T::product(ox, ow, p.red, lds, acc);
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  char* mine = T::out_lds(lds);
+  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c0 = n0 + (wave % T::WN) * BC;
+  const int left = p.cols - c0;  // columns that exist from the wave's first
+  const bool cut = left < BC;
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    const int row = wr + i * 32 + (lane & 31);
+    const bool live = row < p.T;
+    const int r = live ? row : p.T - 1;
+    // the row's entries among the wave's columns: [lo, hi) of its list, or column `at`
+    int lo = 0, hi = 0, at = 0;
+    if (p.e.targets) {
+      const int64_t c = target(p.e, r) - p.v0 - c0;
+      if (live && c >= 0 && c < BC && c < left) {
+        at = (int)c;
+        hi = 1;
+      }
+    } else if (live) {
+      const uint16_t* b = p.e.bounds + r * p.e.ldb + (p.v0 + c0) / kBlock;
+      lo = b[0];
+      hi = b[1];
+    }
+    const bool any = __ballot(lo < hi) != 0;
+    if constexpr (!DZ) {
+      if (cut) {
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (32 * j + 8 * (v >> 2) + 4 * half + (v & 3) >= left) acc[i][j][v] = -INFINITY;
+      }
+      float m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[i][j][v]);
+      m = fmaxf(m, lane_xchg<5>(m));
+      const float off = m == -INFINITY ? 0.0f : -m * p.scale;  // nothing but -inf: sums of 0
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], p.scale, off));
+      float sum = (s[0] + s[1]) + (s[2] + s[3]);
+      sum += lane_xchg<5>(sum);
+      if (live && half == 0) p.part[(int64_t)((p.v0 + c0) / BC) * p.T + row] = make_float2(m, sum);
+      if (any) {
+        T::put(acc[i], mine);
+        if (p.e.targets) {
+          if (hi && half == 0) p.chosen[row] = *in_lds<T>(mine, lane & 31, at);
+        } else {
+          for (int e = lo + half; e < hi; e += 2) {
+            const int c = p.e.idx[(int64_t)r * p.e.K + e] - p.v0 - c0;
+            if ((unsigned)c < (unsigned)BC) p.chosen[(int64_t)r * p.e.K + e] = *in_lds<T>(mine, lane & 31, c);
+          }
+        }
+        asm volatile("" ::: "memory");
+      }
+    } else {
+      const float a = p.a[r], b = p.b[r], off = -p.l2[r];
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          float d = a * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], p.scale, off));
+          if (a == 0.0f) d = 0.0f;  // a row that is left out, whatever its logits are
+          if (cut && 32 * j + 8 * (v >> 2) + 4 * half + (v & 3) >= left) d = 0.0f;
+          acc[i][j][v] = d;
+        }
+      T::put(acc[i], mine);
+      if (any) {
+        if (half == 0) {  // one lane a row, in order: an index that is there twice counts twice
+          if (p.e.targets) {
+            if (hi) *in_lds<T>(mine, lane & 31, at) -= b;
+          } else {
+            for (int e = lo; e < hi; ++e) {
+              const int c = p.e.idx[(int64_t)r * p.e.K + e] - p.v0 - c0;
+              if ((unsigned)c < (unsigned)BC) *in_lds<T>(mine, lane & 31, c) -= b * p.e.share[(int64_t)r * p.e.K + e];
+            }
+          }
+        }
+        __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
+        asm volatile("" ::: "memory");
+      }
+      uint16_t* dz = (uint16_t*)p.dz;
+#pragma unroll
+      for (int it = 0; it < T::OUT_STEPS; ++it) {
+        const int o = wr + i * 32 + T::out_row(it);
+        float v[8];
+        T::get(mine, it, v);
+        if (o < p.T) dense::store8(dz + (int64_t)o * p.ldz + c0 + T::out_col(it), v);
+      }
+    }
+  }
+}
+
+// ---- the gradients' products ------------------------------------------------------------------------------------------
+template <bool A_COLS, bool B_COLS, bool TAIL> using GradBig = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, A_COLS, B_COLS, TAIL>;
+template <bool A_COLS, bool B_COLS, bool TAIL> using GradSmall = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, A_COLS, B_COLS, TAIL>;
+
+template <class T>
+__global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void product_kernel(Product p) {
+  __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
+  const int nm = (p.rows + T::BM - 1) / T::BM, nn = (p.cols + T::BN - 1) / T::BN;
+  const int id = dense::tile_of(blockIdx.x, nm * nn * p.pieces);
+  if (id < 0) return;
+  const int t = id / p.pieces, piece = id % p.pieces, stages = (p.red + dense::BKS - 1) / dense::BKS;
+  const int k0 = (int)((int64_t)piece * stages / p.pieces) * dense::BKS;
+  const int k1 = min((int)((int64_t)(piece + 1) * stages / p.pieces) * dense::BKS, p.red);
+  int m0, n0;
+  tile_at<T>(t, nm, nn, m0, n0);
+  const uint16_t *a = (const uint16_t*)p.a, *b = (const uint16_t*)p.b;
+  a += T::cols ? (int64_t)k0 * p.lda + m0 : (int64_t)m0 * p.lda + k0;
+  b += T::b_cols ? (int64_t)k0 * p.ldb + n0 : (int64_t)n0 * p.ldb + k0;
+  const Operand oa{{a, a}, p.lda, p.a_left - m0}, ob{{b, b}, p.ldb, p.b_left - n0, k1 == p.red ? p.missing : 0};
+  dense::f32x16 acc[T::TM][T::TN];
+  T::product(oa, ob, k1 - k0, lds, acc);
+  __syncthreads();
+  const int wave = threadIdx.x >> 6;
+  char* mine = T::out_lds(lds);
+  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c = n0 + (wave % T::WN) * (T::TN * 32) + T::out_col(0);
+  float* sums = p.acc ? p.acc + (int64_t)piece * p.rows * p.ldacc : nullptr;
+  const bool whole = p.ldo % 8 == 0 && p.cols % 8 == 0 && (uintptr_t)p.out % 16 == 0;
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    T::put(acc[i], mine);
+#pragma unroll
+    for (int it = 0; it < T::OUT_STEPS; ++it) {
+      const int r = wr + i * 32 + T::out_row(it);
+      if (r >= p.rows || c >= p.cols) continue;
+      float v[8];
+      T::get(mine, it, v);
+      if (sums) {
+        float* s = sums + (int64_t)r * p.ldacc + c;
+        if (p.add) {
+          float o[8];
+          ld8(s, 0, o);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] += o[q];
+        }
+        if (!p.last) {
+          st8(s, 0, v);
+          continue;
+        }
+      }
+      uint16_t* o = (uint16_t*)p.out + (int64_t)r * p.ldo + c;
+      if (whole) {
+        dense::store8(o, v);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (c + q < p.cols) o[q] = f32_to_bf16(v[q]);
+      }
+    }
+  }
+}
+
+template <class T>
+static int go_logits(const Logits& p, bool dz, hipStream_t st) {
+  const dim3 grid((unsigned)dense::tiles_grid(ceil_div(p.T, T::BM) * ceil_div(p.cols, T::BN)));
+  if (dz) hipLaunchKernelGGL((logits_kernel<T, true>), grid, dim3(T::NT), 0, st, p);
+  else hipLaunchKernelGGL((logits_kernel<T, false>), grid, dim3(T::NT), 0, st, p);
+  return check_launch();
+}
+template <bool VD, bool TAIL>
+static int go_path(const Logits& p, bool dz, int path, hipStream_t st) {
+  if (path == PATH_BIG) return go_logits<Big<VD, TAIL>>(p, dz, st);
+  if (path == PATH_SMALL) return go_logits<Small<VD, TAIL>>(p, dz, st);
+  return go_logits<Thin<VD, TAIL>>(p, dz, st);
+}
+int launch_logits(const Logits& p, bool dz, int order, int path, hipStream_t st) {
+  const bool tail = p.red % dense::BKS != 0 || p.missing > 0;
+  if (order == ORDER_VD) return tail ? go_path<true, true>(p, dz, path, st) : go_path<true, false>(p, dz, path, st);
+  return tail ? go_path<false, true>(p, dz, path, st) : go_path<false, false>(p, dz, path, st);
+}
+
+template <class T>
+static int go_product(const Product& p, hipStream_t st) {
+  const dim3 grid((unsigned)dense::tiles_grid(ceil_div(p.rows, T::BM) * ceil_div(p.cols, T::BN) * p.pieces));
+  hipLaunchKernelGGL(product_kernel<T>, grid, dim3(T::NT), 0, st, p);
+  return check_launch();
+}
+template <bool A_COLS, bool B_COLS, bool TAIL>
+static int go_size(const Product& p, bool small, hipStream_t st) {
+  return small ? go_product<GradSmall<A_COLS, B_COLS, TAIL>>(p, st) : go_product<GradBig<A_COLS, B_COLS, TAIL>>(p, st);
+}
+// A dz [T][piece] or x^T, B W^T in either order or dz: (rows, rows), (rows, cols) and (cols, cols)
+int launch_product(const Product& p, bool a_cols, bool b_cols, bool small, hipStream_t st) {
+  const bool tail = p.red % dense::BKS != 0 || p.missing > 0;
+  if (a_cols) return tail ? go_size<true, true, true>(p, small, st) : go_size<true, true, false>(p, small, st);
+  if (b_cols) return tail ? go_size<false, true, true>(p, small, st) : go_size<false, true, false>(p, small, st);
+  return tail ? go_size<false, false, true>(p, small, st) : go_size<false, false, false>(p, small, st);
+}
+
+}  // namespace head
+}  // namespace mtx
