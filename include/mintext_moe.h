@@ -452,7 +452,7 @@ int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre
  *   loss[t] = temperature^2 sum_k p_k (log p_k - z[t, i_k] / temperature + lse[t]).  A row without such an entry has loss
  *   0 and no gradient, one with an index of V or more, or a NaN, has NaN; an index that is there twice is two entries.
  *   entries (mtx_distillation_entries_size bytes, 16-byte aligned) is filled for the backward call.
- * Both write loss, lse and state[T] (1, 0 for rows left out, NaN) and use chosen[T] (distillation: [T,K]) as scratch.  total
+ * Both write loss, lse, state[T] (1, 0 for rows left out, NaN) and chosen[T] (distillation: [T,K]), the named logits.  total
  *   and count (both or none) receive the sum of the losses and, with `mean`, what it was divided by: the rows that
  *   are not left out, 1 at least.
  * The _bwd calls: g is the gradient of total (count as written) or, with count NULL, of loss[T]; dx[T,D] and dw (W's
@@ -468,7 +468,7 @@ int mtx_linear_cross_entropy(const void* x, const void* w, const void* targets, 
                              float* chosen, void* workspace, int64_t workspace_bytes, void* stream);
 int mtx_linear_cross_entropy_bwd(const float* g, const float* count, const void* x, const void* w,
                                  const void* targets, int targets_64, const float* lse, const float* state,
-                                 int dtype, int64_t T, int64_t D, int64_t V, int order, float z_loss, void* dx,
+                                 const float* chosen, int dtype, int64_t T, int64_t D, int64_t V, int order, float z_loss, void* dx,
                                  void* dw, void* workspace, int64_t workspace_bytes, void* stream);
 int mtx_linear_distillation(const void* x, const void* w, const void* teacher_idx, int idx_64,
                             const void* teacher_logits, int logits_dtype, int dtype, int64_t T, int64_t D,
@@ -477,7 +477,7 @@ int mtx_linear_distillation(const void* x, const void* w, const void* teacher_id
                             int64_t entries_bytes, void* workspace, int64_t workspace_bytes, void* stream);
 int mtx_linear_distillation_bwd(const float* g, const float* count, const void* x, const void* w,
                                 const void* entries, int64_t entries_bytes, const float* lse, const float* state,
-                                int dtype, int64_t T, int64_t D, int64_t V, int64_t K, int order,
+                                const float* chosen, int dtype, int64_t T, int64_t D, int64_t V, int64_t K, int order,
                                 float temperature, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
                                 void* stream);
 

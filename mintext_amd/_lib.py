@@ -101,11 +101,11 @@ SIGNATURES = {
     "mtx_distillation_entries_size": (_I64, [_I64, _I64, _I64]),
     "mtx_linear_cross_entropy": (_I, [_P, _P, _P, _I, _I, _I64, _I64, _I64, _I, _I64, _F, _I, _P, _P, _P, _P, _P, _P,
                                       _P, _I64, _P]),
-    "mtx_linear_cross_entropy_bwd": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _I, _F, _P, _P, _P, _I64,
+    "mtx_linear_cross_entropy_bwd": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I64, _I64, _I64, _I, _F, _P, _P, _P, _I64,
                                           _P]),
     "mtx_linear_distillation": (_I, [_P, _P, _P, _I, _P, _I, _I, _I64, _I64, _I64, _I64, _I, _F, _I, _P, _P, _P, _P, _P,
                                      _P, _P, _I64, _P, _I64, _P]),
-    "mtx_linear_distillation_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _I64, _I, _F, _P, _P,
+    "mtx_linear_distillation_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I, _F, _P, _P,
                                          _P, _I64, _P]),
     "mtx_norm": (_I, [_P, _P, _P, _P, _I, _I, _I, _I64, _I64, _F, _P, _P, _P, _P, _P]),
     "mtx_norm_bwd_workspace_size": (_I64, [_I64, _I64]),

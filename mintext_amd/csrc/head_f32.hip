@@ -71,25 +71,9 @@ __global__ __launch_bounds__(NT) void logits_f32_kernel(Logits p) {
     }
   } else {
     if (!live) return;
-    const float a = p.a[r], b = p.b[r], l2 = p.l2[r];
+    const float a = p.a[r], l2 = p.l2[r];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = a == 0.0f || e >= left ? 0.0f : a * exp2f(__builtin_fmaf(v[e], p.scale, -l2));
-    // the entries among the thread's own columns, in order
-    if (p.e.targets) {
-      const int64_t c = target(p.e, r) - p.v0 - c0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (c == e && e < left) v[e] -= b;
-    } else {
-      const uint16_t* at = p.e.bounds + r * p.e.ldb + (p.v0 + n0) / kBlock;
-      for (int i = at[0]; i < at[1]; ++i) {
-        const int c = p.e.idx[(int64_t)r * p.e.K + i] - p.v0 - c0;
-        const float d = b * p.e.share[(int64_t)r * p.e.K + i];
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (c == e) v[e] -= d;
-      }
-    }
     float* dz = (float*)p.dz + (int64_t)row * p.ldz + c0;
     st8(dz, 0, v);
     st8(dz, 8, v + 8);
@@ -129,7 +113,7 @@ __global__ __launch_bounds__(NT) void product_f32_kernel(Product p) {
         continue;
       }
     }
-    ((float*)p.out)[r * p.ldo + n] = y;
+    ((float*)p.out)[r * p.ldo + n] = p.alpha ? y * *p.alpha : y;
   }
 }
 
@@ -152,8 +136,10 @@ int launch_logits_f32(const Logits& p, bool dz, int order, hipStream_t st) {
 template <bool A_COLS, bool B_COLS>
 static int go_product(const Product& p, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div(p.cols, 64), (unsigned)ceil_div(p.rows, 64), (unsigned)p.pieces);
-  const bool vec = quads(p.a, p.lda) && quads(p.b, p.ldb) && (A_COLS ? p.rows % 4 == 0 : p.red % 4 == 0) &&
-                   (B_COLS ? p.cols % 4 == 0 : p.red % 4 == 0);
+  // a quad that begins inside may end behind the rows, columns or reduction elements where there is something to read: dz has
+  // zeros there, and what other operands give is multiplied by them or not stored
+  const bool vec = quads(p.a, p.lda) && quads(p.b, p.ldb) && (A_COLS ? p.a_left >= round_up(p.rows, 4) : p.lda >= round_up(p.red, 4)) &&
+                   (B_COLS ? p.b_left >= round_up(p.cols, 4) : p.red % 4 == 0);
   if (vec) hipLaunchKernelGGL((product_f32_kernel<A_COLS, B_COLS, 4>), grid, dim3(NT), 0, st, p);
   else hipLaunchKernelGGL((product_f32_kernel<A_COLS, B_COLS, 1>), grid, dim3(NT), 0, st, p);
   return check_launch();

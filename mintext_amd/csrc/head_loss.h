@@ -5,7 +5,9 @@
 //             row's entries; merge_kernel joins the blocks.
 //   backward  the vocabulary goes through in pieces: z of a piece again, dz = a softmax(z / tau) - b share (one entry for
 //             cross entropy, a teacher's top ones for distillation) rounded to the operands' type into a workspace, from which
-//             dx += dz W^T (in f32) and dW of the piece = x^T dz.
+//             dx += dz W^T (in f32) and dW of the piece = x^T dz.  A factor that all rows share (1 / count, the gradient of
+//             the one loss) is left to the products' results: -1 + q is rounded and not a multiple of it that is the same,
+//             and off by the same half step, in every row (4096 x 4096 x 32000: 2.8e-3 off with it in dz).
 // So a step computes 8 T D V operations where 6 would do with the logits kept (a fifth of what they took is saved by
 // neither writing nor reading them), and holds at most kPiece bytes of dz.
 #pragma once
@@ -44,7 +46,7 @@ struct Logits {
   float2* part;         // [block][T]: maximum of z, sum of exp2((z - maximum) scale)
   float* chosen;        // [T][K]: z of the entries
   // backward
-  const float *a, *b, *l2;  // [T]: factors of the softmax and of the shares; log2 of sum exp(z / tau)
+  const float *a, *l2;  // [T]: factor of the softmax; log2 of sum exp(z / tau)
   void* dz;             // [T][ldz], zeros behind the piece's columns
   int64_t ldz;
 };
@@ -62,6 +64,7 @@ struct Product {
   int64_t ldacc;
   int add;                       // acc holds sums of earlier calls
   int last;                      // pieces == 1: the result goes to out
+  const float* alpha;            // factor of the result, or nullptr
 };
 
 int launch_logits(const Logits& p, bool dz, int order, int path, hipStream_t st);  // bf16

@@ -8,6 +8,7 @@
 //
 // A row's state is 1, 0 (left out: the ignored class, no entry; its loss is 0 and its gradient too) or NaN (a class
 // that is none), which its loss and its gradient become.
+#include "f32_tile.h"
 #include "head_loss.h"
 #include <algorithm>
 
@@ -210,15 +211,54 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* loss, const fl
 }
 
 // ---- backward: a row's factors ----------------------------------------------------------------------------------
+// b of the shares and a of the softmax; `count`: the factor that all rows share goes to *alpha, else it is in them
 __global__ __launch_bounds__(256) void factors_kernel(const float* g, const float* count, const float* lse, const float* state,
-                                                      int64_t T, float unit, float z_loss, float* a, float* b, float* l2) {
+                                                      int64_t T, float unit, float z_loss, float* a, float* b, float* l2,
+                                                      float* alpha) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t == 0) *alpha = count ? unit * (g[0] / *count) : 1.0f;
   if (t >= T) return;
   const float st = state[t], l = lse[t];
-  const float w = st == 0.0f ? 0.0f : st * unit * (count ? g[0] / *count : g[t]);
+  const float w = st == 0.0f ? 0.0f : count ? st : st * unit * g[t];
   b[t] = w;
   a[t] = w == 0.0f ? 0.0f : w * (1.0f + 2.0f * z_loss * l);
   l2[t] = l * kLog2e;
+}
+
+// dz of the entries among columns v0 .. v0 + cols, from their logits: a softmax - b (the shares of one class), in the place
+// of what the tile left there.  A thread an entry; the first of several of one class takes them all.
+struct Named {
+  Entries e;
+  const float *chosen, *a, *b, *l2;
+  float scale;
+  int64_t T;
+  int v0, cols;
+  void* dz;
+  int64_t ldz;
+  int f32;
+};
+__global__ __launch_bounds__(256) void named_kernel(Named p) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= p.T * p.e.K) return;
+  const int64_t t = at / p.e.K;
+  const float a = p.a[t], b = p.b[t];
+  if (b == 0.0f) return;
+  int64_t c;
+  float share = 1.0f;
+  if (p.e.targets) {
+    c = target(p.e, t);
+  } else {
+    c = p.e.idx[at];
+    if (at > t * p.e.K && p.e.idx[at - 1] == c) return;
+    share = p.e.share[at];
+  }
+  c -= p.v0;
+  if (c < 0 || c >= p.cols) return;
+  if (!p.e.targets)
+    for (int64_t k = at + 1; k < (t + 1) * p.e.K && p.e.idx[k] == c + p.v0; ++k) share += p.e.share[k];
+  const float v = a * exp2f(__builtin_fmaf(p.chosen[at], p.scale, -p.l2[t])) - b * share;
+  if (p.f32) ((float*)p.dz)[t * p.ldz + c] = v;
+  else ((uint16_t*)p.dz)[t * p.ldz + c] = f32_to_bf16(v);
 }
 
 // rows x cols of a bf16 matrix into one with rows of `ld` (a multiple of 8), zeros behind the columns
@@ -239,7 +279,9 @@ __global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ i
 // out = the pieces' sums, in order.  V columns a thread.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc, int pieces, int64_t rows, int64_t cols,
-                                                   int64_t ldacc, T* __restrict__ out, int64_t ldo) {
+                                                   int64_t ldacc, T* __restrict__ out, int64_t ldo,
+                                                   const float* __restrict__ alpha) {
+  const float f = *alpha;
   const int64_t per = (cols + V - 1) / V, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * per) return;
   const int64_t r = i / per, c = i % per * V, at = r * ldacc + c, n = rows * ldacc;
@@ -252,12 +294,13 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] += o[q];
     }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] *= f;
     st8(out, r * ldo + c, v);
   } else {
     float v = acc[at];
     for (int s = 1; s < pieces; ++s) v += acc[s * n + at];
-    if constexpr (sizeof(T) == 4) out[r * ldo + c] = v;
-    else out[r * ldo + c] = f32_to_bf16(v);
+    gst<T>(out, r * ldo + c, v * f);
   }
 }
 
@@ -329,7 +372,7 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
   if (!backward) {
     p.part = take(round_up(V, tile_cols(p.path)) / block_cols(p.path) * T * 8);
   } else {
-    p.factors = take(3 * T * 4);
+    p.factors = take((3 * T + 1) * 4);
     p.dz = take(T * p.piece * size);
     p.dx = split(p.f32, T, D, std::min(p.piece, V));
     p.ld_dx = round_up(D, 8);
@@ -390,10 +433,10 @@ static int product(const Plan& p, const Product& a, bool a_cols, bool b_cols, co
   return p.f32 ? launch_product_f32(a, a_cols, b_cols, st) : launch_product(a, a_cols, b_cols, s.small, st);
 }
 static int join(bool f32, const float* acc, int pieces, int64_t rows, int64_t cols, int64_t ldacc, void* out, int64_t ldo,
-                hipStream_t st) {
+                const float* alpha, hipStream_t st) {
   const bool vec = cols % 8 == 0 && ldo % 8 == 0 && aligned16(out);
   const dim3 grid((unsigned)ceil_div(rows * (vec ? cols / 8 : cols), 256));
-#define MTX_JOIN(T, V) hipLaunchKernelGGL((join_kernel<T, V>), grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (T*)out, ldo)
+#define MTX_JOIN(T, V) hipLaunchKernelGGL((join_kernel<T, V>), grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (T*)out, ldo, alpha)
   if (f32) {
     if (vec) MTX_JOIN(float, 8);
     else MTX_JOIN(float, 1);
@@ -430,35 +473,38 @@ static int forward(const Plan& p, const void* x, const void* w, Merge m, float* 
 }
 
 static int backward(const Plan& p, const float* g, const float* count, const void* x, const void* w, const float* lse,
-                    const float* state, const Entries& e, float scale, float unit, float z_loss, void* dx, void* dw, char* ws,
+                    const float* state, const float* chosen, const Entries& e, float scale, float unit, float z_loss, void* dx, void* dw, char* ws,
                     hipStream_t st) {
   const int64_t size = p.f32 ? 4 : 2;
   const bool dv = p.order == ORDER_DV;
   float* f = (float*)(ws + p.factors);
   hipLaunchKernelGGL(factors_kernel, dim3((unsigned)ceil_div(p.T, 256)), dim3(256), 0, st, g, count, lse, state, p.T, unit, z_loss,
-                     f, f + p.T, f + 2 * p.T);
+                     f, f + p.T, f + 2 * p.T, f + 3 * p.T);
   int rc = check_launch();
   Logits a{};
   a.e = e;
   a.scale = scale;
-  a.a = f, a.b = f + p.T, a.l2 = f + 2 * p.T;
+  a.a = f, a.l2 = f + 2 * p.T;
+  const float* alpha = f + 3 * p.T;
   a.dz = ws + p.dz;
   a.ldz = p.piece;
   for (int64_t v0 = 0; v0 < p.V && rc == MTX_OK; v0 += p.piece) {
     rc = operands(p, x, w, v0, ws, a, st);
     if (rc == MTX_OK) rc = logits(p, a, true, st);
     if (rc != MTX_OK) return rc;
+    const Named named{e, chosen, f, f + p.T, f + 2 * p.T, scale, p.T, a.v0, a.cols, a.dz, a.ldz, p.f32};
+    hipLaunchKernelGGL(named_kernel, dim3((unsigned)ceil_div(p.T * e.K, 256)), dim3(256), 0, st, named);
     if (dx) {
       const int red = p.f32 ? a.cols : (int)round_up(a.cols, 8);  // dz holds zeros behind its columns
       const bool only = p.piece >= p.V, final = v0 + p.piece >= p.V;
       // the last piece of the vocabulary may be shorter than what the split was made for
       const int pieces = (int)std::min<int64_t>(p.dx.pieces, ceil_div(red, 32));
       Product q{a.dz, a.w, a.ldz, a.ldw, (int)p.T, (int)p.D, red, 0, (int)p.T, (int)(dv ? p.D : p.D8), dx, p.D, pieces, nullptr,
-                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final};
+                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final, alpha};
       if (!dv) q.missing = red - a.cols;
       if (!(only && p.dx.pieces == 1)) q.acc = (float*)(ws + p.acc_dx);
       rc = product(p, q, false, !dv, p.dx, st);
-      if (rc == MTX_OK && final && p.dx.pieces > 1) rc = join(p.f32, q.acc, p.dx.pieces, p.T, p.D, p.ld_dx, dx, p.D, st);
+      if (rc == MTX_OK && final && p.dx.pieces > 1) rc = join(p.f32, q.acc, p.dx.pieces, p.T, p.D, p.ld_dx, dx, p.D, alpha, st);
       if (rc != MTX_OK) return rc;
     }
     if (dw) {
@@ -469,9 +515,10 @@ static int backward(const Plan& p, const float* g, const float* count, const voi
       else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, (int)p.T, 0, (int)p.piece, (int)p.D8, out, ldo, p.dw.pieces};
       q.ldacc = p.ld_dw;
       q.last = p.dw.pieces == 1;
+      q.alpha = alpha;
       if (p.dw.pieces > 1) q.acc = (float*)(ws + p.acc_dw);
       rc = product(p, q, true, true, p.dw, st);
-      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, q.rows, q.cols, p.ld_dw, out, ldo, st);
+      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, q.rows, q.cols, p.ld_dw, out, ldo, alpha, st);
     }
   }
   return rc;
@@ -533,18 +580,18 @@ extern "C" int mtx_linear_cross_entropy(const void* x, const void* w, const void
 }
 
 extern "C" int mtx_linear_cross_entropy_bwd(const float* g, const float* count, const void* x, const void* w, const void* targets,
-                                            int targets_64, const float* lse, const float* state, int dtype, int64_t T, int64_t D,
+                                            int targets_64, const float* lse, const float* state, const float* chosen, int dtype, int64_t T, int64_t D,
                                             int64_t V, int order, float z_loss, void* dx, void* dw, void* workspace,
                                             int64_t workspace_bytes, void* stream) {
   using namespace head;
   const int rc = check_sizes(dtype, T, D, V, order);
   if (rc != MTX_OK) return rc;
   if (T == 0 || (!dx && !dw)) return MTX_OK;
-  if (!g || !x || !w || !targets || !lse || !state || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  if (!g || !x || !w || !targets || !lse || !state || !chosen || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, true);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
   const Entries e{targets, targets_64, nullptr, nullptr, nullptr, 0, 1};
-  return backward(p, g, count, x, w, lse, state, e, kLog2e, 1.0f, z_loss, dx, dw, (char*)workspace, (hipStream_t)stream);
+  return backward(p, g, count, x, w, lse, state, chosen, e, kLog2e, 1.0f, z_loss, dx, dw, (char*)workspace, (hipStream_t)stream);
 }
 
 extern "C" int mtx_linear_distillation(const void* x, const void* w, const void* teacher_idx, int idx_64,
@@ -585,8 +632,8 @@ extern "C" int mtx_linear_distillation(const void* x, const void* w, const void*
 
 extern "C" int mtx_linear_distillation_bwd(const float* g, const float* count, const void* x, const void* w,
                                            const void* entries_buffer, int64_t entries_bytes, const float* lse,
-                                           const float* state, int dtype, int64_t T, int64_t D, int64_t V, int64_t K, int order,
-                                           float temperature, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
+                                           const float* state, const float* chosen, int dtype, int64_t T, int64_t D, int64_t V,
+                                           int64_t K, int order, float temperature, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
                                            void* stream) {
   using namespace head;
   const int rc = check_sizes(dtype, T, D, V, order);
@@ -594,11 +641,11 @@ extern "C" int mtx_linear_distillation_bwd(const float* g, const float* count, c
   if (K <= 0 || !(temperature > 0.0f && temperature < INFINITY)) return MTX_ERR_ARG;
   if (K > kMaxEntries) return MTX_ERR_UNSUPPORTED;
   if (T == 0 || (!dx && !dw)) return MTX_OK;
-  if (!g || !x || !w || !entries_buffer || !lse || !state || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  if (!g || !x || !w || !entries_buffer || !lse || !state || !chosen || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, true);
   const Saved s = saved(T, V, K);
   if (!aligned16(entries_buffer) || entries_bytes < s.total) return MTX_ERR_WORKSPACE;
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
-  return backward(p, g, count, x, w, lse, state, entries((char*)const_cast<void*>(entries_buffer), s, K), kLog2e / temperature,
+  return backward(p, g, count, x, w, lse, state, chosen, entries((char*)const_cast<void*>(entries_buffer), s, K), kLog2e / temperature,
                   temperature, 0.0f, dx, dw, (char*)workspace, (hipStream_t)stream);
 }

@@ -25,14 +25,128 @@ __device__ __forceinline__ float* in_lds(char* mine, int r, int c) {
   return (float*)(mine + r * (T::TN * 128) + (((c >> 2) ^ (r & (T::TN * 8 - 1))) << 4) + (c & 3) * 4);
 }
 
-// A lane holds, of 32 rows at a time, one row's 16 TN values in columns 32 j + 8 g + 4 (lane / 32) + q: the row's maximum and
-// sum are taken in the lane and joined with that of lane ^ 32.  Entries are looked up in LDS, where the 32 rows are put
-// for that only if one of them has an entry among the wave's columns.
+// A lane holds, of 32 rows at a time, one row's 16 TN values in columns 32 j + 8 g + 4 (lane / 32) + q (accumulator j, element
+// 4 g + q): the row's maximum and sum are taken in the lane and joined with that of lane ^ 32.  Entries are looked up in LDS,
+// where the 32 rows are put for that only if one of them has an entry among the wave's columns.
+template <class T>
+__device__ __forceinline__ void forward_out(const Logits& p, dense::f32x16 (&acc)[T::TM][T::TN], char* mine, int wr, int c0) {
+  constexpr int BC = T::TN * 32;  // the wave's columns
+  const int lane = threadIdx.x & 63, half = lane >> 5, left = p.cols - c0;
+  // the rows' entries among the wave's columns: [lo, hi) of their lists, or column lo
+  int lo[T::TM], hi[T::TM];
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    const int row = wr + i * 32 + (lane & 31);
+    lo[i] = hi[i] = 0;
+    if (row >= p.T) continue;
+    if (p.e.targets) {
+      const int64_t c = target(p.e, row) - p.v0 - c0;
+      if (c >= 0 && c < BC && c < left) {
+        lo[i] = (int)c;
+        hi[i] = BC;
+      }
+    } else {
+      const uint16_t* b = p.e.bounds + row * p.e.ldb + (p.v0 + c0) / kBlock;
+      lo[i] = b[0];
+      hi[i] = b[1];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    const int row = wr + i * 32 + (lane & 31);
+    if (left < BC) {
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (32 * j + 8 * (v >> 2) + 4 * half + (v & 3) >= left) acc[i][j][v] = -INFINITY;
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[i][j][v]);
+    m = fmaxf(m, lane_xchg<5>(m));
+    const float off = m == -INFINITY ? 0.0f : -m * p.scale;  // nothing but -inf: a sum of 0
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[v & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], p.scale, off));
+    float sum = (s[0] + s[1]) + (s[2] + s[3]);
+    sum += lane_xchg<5>(sum);
+    if (row < p.T && half == 0) p.part[(int64_t)((p.v0 + c0) / BC) * p.T + row] = make_float2(m, sum);
+    if (__ballot(lo[i] < hi[i]) == 0) continue;
+    T::put(acc[i], mine);
+    if (p.e.targets) {
+      if (hi[i] && half == 0) p.chosen[row] = *in_lds<T>(mine, lane & 31, lo[i]);
+    } else {
+      for (int e = lo[i] + half; e < hi[i]; e += 2) {
+        const int c = p.e.idx[(int64_t)row * p.e.K + e] - p.v0 - c0;
+        if ((unsigned)c < (unsigned)BC) p.chosen[(int64_t)row * p.e.K + e] = *in_lds<T>(mine, lane & 31, c);
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+}
+
+// dz = a softmax, rounded, 32 rows at a time into LDS (16-byte chunk c of a row at chunk c ^ (row % chunks)) and out in whole
+// lines.  What a row's entries take from it is entries_kernel's, which knows their logits.
+template <class T>
+__device__ __forceinline__ void gradient_out(const Logits& p, dense::f32x16 (&acc)[T::TM][T::TN], char* mine, int wr, int c0) {
+  constexpr int BC = T::TN * 32, CH = T::TN * 4, BYTES = 32 * T::TN * 64;  // chunks of a row; bytes of 32 rows
+  typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+  const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31, left = p.cols - c0;
+  float a[T::TM], off[T::TM];
+  bool care = left < BC;
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    const int row = min(wr + i * 32 + r, p.T - 1);
+    a[i] = p.a[row];
+    off[i] = -p.l2[row];
+  }
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) care |= a[i] == 0.0f;
+  care = __ballot(care) != 0;
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float d[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          d[q] = a[i] * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][4 * g + q], p.scale, off[i]));
+        if (care) {  // zeros behind the columns, and in rows that are left out, whatever their logits are
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (a[i] == 0.0f || 32 * j + 8 * g + 4 * half + q >= left) d[q] = 0.0f;
+        }
+        *(bf16x4*)(mine + i * BYTES + r * (CH * 16) + (((j * 4 + g) ^ (r & (CH - 1))) << 4) + half * 8) =
+            bf16x4{(__bf16)d[0], (__bf16)d[1], (__bf16)d[2], (__bf16)d[3]};
+      }
+  }
+  __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
+  asm volatile("" ::: "memory");
+  uint16_t* dz = (uint16_t*)p.dz + c0;
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+    for (int it = 0; it < T::TN * 2; ++it) {
+      const int at = it * 64 + lane, o = at / CH, c = at % CH, row = wr + i * 32 + o;
+      const v4u32 v = *(const v4u32*)(mine + i * BYTES + o * (CH * 16) + ((c ^ (o & (CH - 1))) << 4));
+      if (row < p.T) *(v4u32*)(dz + (int64_t)row * p.ldz + c * 8) = v;
+    }
+}
+
 template <class T, bool DZ>
 __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logits_kernel(Logits p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
-  static_assert(T::NW * T::OUT_BYTES <= T::LDS_BYTES, "the way out fits the ring");
-  constexpr int BC = T::TN * 32;  // the wave's columns
+  constexpr int OUT = DZ ? T::TM * 32 * T::TN * 64 : T::OUT_BYTES;  // of a wave
+  static_assert(T::NW * OUT <= T::LDS_BYTES, "the way out fits the ring");
   const int nm = (p.T + T::BM - 1) / T::BM, nn = (p.cols + T::BN - 1) / T::BN;
   const int t = dense::tile_of(blockIdx.x, nm * nn);
   if (t < 0) return;
@@ -44,101 +158,10 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logit
   dense::f32x16 acc[T::TM][T::TN];
   T::product(ox, ow, p.red, lds, acc);
   __syncthreads();
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
-  char* mine = T::out_lds(lds);
-  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c0 = n0 + (wave % T::WN) * BC;
-  const int left = p.cols - c0;  // columns that exist from the wave's first
-  const bool cut = left < BC;
-#pragma unroll
-  for (int i = 0; i < T::TM; ++i) {
-    const int row = wr + i * 32 + (lane & 31);
-    const bool live = row < p.T;
-    const int r = live ? row : p.T - 1;
-    // the row's entries among the wave's columns: [lo, hi) of its list, or column `at`
-    int lo = 0, hi = 0, at = 0;
-    if (p.e.targets) {
-      const int64_t c = target(p.e, r) - p.v0 - c0;
-      if (live && c >= 0 && c < BC && c < left) {
-        at = (int)c;
-        hi = 1;
-      }
-    } else if (live) {
-      const uint16_t* b = p.e.bounds + r * p.e.ldb + (p.v0 + c0) / kBlock;
-      lo = b[0];
-      hi = b[1];
-    }
-    const bool any = __ballot(lo < hi) != 0;
-    if constexpr (!DZ) {
-      if (cut) {
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (32 * j + 8 * (v >> 2) + 4 * half + (v & 3) >= left) acc[i][j][v] = -INFINITY;
-      }
-      float m = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[i][j][v]);
-      m = fmaxf(m, lane_xchg<5>(m));
-      const float off = m == -INFINITY ? 0.0f : -m * p.scale;  // nothing but -inf: sums of 0
-      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) s[v & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], p.scale, off));
-      float sum = (s[0] + s[1]) + (s[2] + s[3]);
-      sum += lane_xchg<5>(sum);
-      if (live && half == 0) p.part[(int64_t)((p.v0 + c0) / BC) * p.T + row] = make_float2(m, sum);
-      if (any) {
-        T::put(acc[i], mine);
-        if (p.e.targets) {
-          if (hi && half == 0) p.chosen[row] = *in_lds<T>(mine, lane & 31, at);
-        } else {
-          for (int e = lo + half; e < hi; e += 2) {
-            const int c = p.e.idx[(int64_t)r * p.e.K + e] - p.v0 - c0;
-            if ((unsigned)c < (unsigned)BC) p.chosen[(int64_t)r * p.e.K + e] = *in_lds<T>(mine, lane & 31, c);
-          }
-        }
-        asm volatile("" ::: "memory");
-      }
-    } else {
-      const float a = p.a[r], b = p.b[r], off = -p.l2[r];
-#pragma unroll
-      for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          float d = a * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], p.scale, off));
-          if (a == 0.0f) d = 0.0f;  // a row that is left out, whatever its logits are
-          if (cut && 32 * j + 8 * (v >> 2) + 4 * half + (v & 3) >= left) d = 0.0f;
-          acc[i][j][v] = d;
-        }
-      T::put(acc[i], mine);
-      if (any) {
-        if (half == 0) {  // one lane a row, in order: an index that is there twice counts twice
-          if (p.e.targets) {
-            if (hi) *in_lds<T>(mine, lane & 31, at) -= b;
-          } else {
-            for (int e = lo; e < hi; ++e) {
-              const int c = p.e.idx[(int64_t)r * p.e.K + e] - p.v0 - c0;
-              if ((unsigned)c < (unsigned)BC) *in_lds<T>(mine, lane & 31, c) -= b * p.e.share[(int64_t)r * p.e.K + e];
-            }
-          }
-        }
-        __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
-        asm volatile("" ::: "memory");
-      }
-      uint16_t* dz = (uint16_t*)p.dz;
-#pragma unroll
-      for (int it = 0; it < T::OUT_STEPS; ++it) {
-        const int o = wr + i * 32 + T::out_row(it);
-        float v[8];
-        T::get(mine, it, v);
-        if (o < p.T) dense::store8(dz + (int64_t)o * p.ldz + c0 + T::out_col(it), v);
-      }
-    }
-  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c0 = n0 + (wave % T::WN) * (T::TN * 32);
+  if constexpr (DZ) gradient_out<T>(p, acc, lds + wave * OUT, wr, c0);
+  else forward_out<T>(p, acc, lds + wave * OUT, wr, c0);
 }
 
 // ---- the gradients' products ------------------------------------------------------------------------------------------
@@ -167,6 +190,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   char* mine = T::out_lds(lds);
   const int wr = m0 + (wave / T::WN) * (T::TM * 32), c = n0 + (wave % T::WN) * (T::TN * 32) + T::out_col(0);
   float* sums = p.acc ? p.acc + (int64_t)piece * p.rows * p.ldacc : nullptr;
+  const float alpha = p.alpha && (!sums || p.last) ? *p.alpha : 1.0f;
   const bool whole = p.ldo % 8 == 0 && p.cols % 8 == 0 && (uintptr_t)p.out % 16 == 0;
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
@@ -190,6 +214,8 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
           continue;
         }
       }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] *= alpha;
       uint16_t* o = (uint16_t*)p.out + (int64_t)r * p.ldo + c;
       if (whole) {
         dense::store8(o, v);

@@ -101,9 +101,9 @@ class _Loss:
                        L.dtype_code(teacher.dtype), dt, T, D, V, K, order, self.temperature, mean, loss.data_ptr(),
                        lse.data_ptr(), state.data_ptr(), *ends, chosen.data_ptr(), kept.data_ptr(), kept.numel(), ws.data_ptr(),
                        ws.numel(), L.stream(dev))
-        return (loss if total is None else total), (x, weight, kept, rows, count)
+        return (loss if total is None else total), (x, weight, kept, rows, chosen, count)
 
-    def backward(self, g, x, weight, kept, rows, count, K, need_x, need_w):
+    def backward(self, g, x, weight, kept, rows, chosen, count, K, need_x, need_w):
         dev = L.require_device(g, x, weight)
         D, V = weight.shape
         T = x.numel() // D
@@ -117,11 +117,12 @@ class _Loss:
         with L.on_device(dev):
             if K is None:
                 L.call("mtx_linear_cross_entropy_bwd", g.data_ptr(), L.ptr(count), x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
-                       _index64("classes", kept), lse.data_ptr(), state.data_ptr(), dt, T, D, V, order, self.z_loss, L.ptr(dx),
+                       _index64("classes", kept), lse.data_ptr(), state.data_ptr(), chosen.data_ptr(), dt, T, D, V, order, self.z_loss, L.ptr(dx),
                        L.ptr(dw), ws.data_ptr(), ws.numel(), L.stream(dev))
             else:
                 L.call("mtx_linear_distillation_bwd", g.data_ptr(), L.ptr(count), x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
-                       kept.numel(), lse.data_ptr(), state.data_ptr(), dt, T, D, V, K, order, self.temperature, L.ptr(dx),
+                       kept.numel(), lse.data_ptr(), state.data_ptr(), chosen.data_ptr(), dt, T, D, V, K, order, self.temperature,
+                       L.ptr(dx),
                        L.ptr(dw), ws.data_ptr(), ws.numel(), L.stream(dev))
         return dx, dw
 
@@ -129,8 +130,8 @@ class _Loss:
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, classes, teacher, how):
-        out, (xd, wd, kept, rows, count) = how.forward(x, weight, classes, teacher)
-        ctx.save_for_backward(xd, wd, kept, rows, count)
+        out, saved = how.forward(x, weight, classes, teacher)
+        ctx.save_for_backward(*saved)
         ctx.how, ctx.K = how, None if teacher is None else classes.shape[-1]
         return out
 

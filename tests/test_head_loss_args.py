@@ -95,11 +95,11 @@ def test_entry_points_refuse():
         assert ce(**{missing: P}) == L.MTX_ERR_ARG, missing
     assert ce(x=d + 2) == ce(w=d + 8) == L.MTX_ERR_ARG                           # off a 16-byte boundary
     assert ce(ws=P) == ce(n=16) == ce(ws=d + 4) == L.MTX_ERR_WORKSPACE
-    ceb = lambda g=d, x=d, w=d, y=d, lse=d, st=d, dt=1, T=4, V=16, dx=d, dw=d, ws=d, n=big: lib.mtx_linear_cross_entropy_bwd(
-        g, P, x, w, y, 1, lse, st, dt, T, 8, V, 0, 0.0, dx, dw, ws, n, P)
+    ceb = lambda g=d, x=d, w=d, y=d, lse=d, st=d, ch=d, dt=1, T=4, V=16, dx=d, dw=d, ws=d, n=big: lib.mtx_linear_cross_entropy_bwd(
+        g, P, x, w, y, 1, lse, st, ch, dt, T, 8, V, 0, 0.0, dx, dw, ws, n, P)
     assert ceb(dt=2) == L.MTX_ERR_ARG and ceb(V=1 << 23) == L.MTX_ERR_UNSUPPORTED
     assert ceb(dx=P, dw=P) == ceb(T=0) == L.MTX_OK                               # nothing to do
-    for missing in ("g", "x", "w", "y", "lse", "st"):
+    for missing in ("g", "x", "w", "y", "lse", "st", "ch"):
         assert ceb(**{missing: P}) == L.MTX_ERR_ARG, missing
     assert ceb(ws=P) == ceb(n=16) == L.MTX_ERR_WORKSPACE
     kd = lambda x=d, w=d, i=d, t=d, tt=0, dt=1, T=4, K=3, tau=1.0, loss=d, lse=d, st=d, ch=d, e=d, en=big, ws=d, n=big: \
@@ -109,10 +109,10 @@ def test_entry_points_refuse():
     for missing in ("x", "w", "i", "t", "loss", "lse", "st", "ch", "e"):
         assert kd(**{missing: P}) == L.MTX_ERR_ARG, missing
     assert kd(en=16) == kd(e=d + 4) == kd(ws=P) == kd(n=16) == L.MTX_ERR_WORKSPACE
-    kdb = lambda g=d, x=d, w=d, e=d, en=big, lse=d, st=d, T=4, K=3, tau=1.0, dx=d, dw=d, ws=d, n=big: \
-        lib.mtx_linear_distillation_bwd(g, P, x, w, e, en, lse, st, 1, T, 8, 16, K, 0, tau, dx, dw, ws, n, P)
+    kdb = lambda g=d, x=d, w=d, e=d, en=big, lse=d, st=d, ch=d, T=4, K=3, tau=1.0, dx=d, dw=d, ws=d, n=big: \
+        lib.mtx_linear_distillation_bwd(g, P, x, w, e, en, lse, st, ch, 1, T, 8, 16, K, 0, tau, dx, dw, ws, n, P)
     assert kdb(K=0) == kdb(tau=-1.0) == L.MTX_ERR_ARG and kdb(K=1025) == L.MTX_ERR_UNSUPPORTED
     assert kdb(T=0) == kdb(dx=P, dw=P) == L.MTX_OK
-    for missing in ("g", "x", "w", "e", "lse", "st"):
+    for missing in ("g", "x", "w", "e", "lse", "st", "ch"):
         assert kdb(**{missing: P}) == L.MTX_ERR_ARG, missing
     assert kdb(en=16) == kdb(ws=P) == kdb(n=16) == L.MTX_ERR_WORKSPACE
