@@ -456,7 +456,7 @@ int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre
  *   and count (both or none) receive the sum of the losses and, with `mean`, what it was divided by: the rows that
  *   are not left out, 1 at least.
  * The _bwd calls: g is the gradient of total (count as written) or, with count NULL, of loss[T]; dx[T,D] and dw (W's
- *   order) in dtype, either may be NULL.  dz is rounded to dtype for the products; its columns go through in pieces of 1 GiB
+ *   order) in dtype and 16-byte aligned, either may be NULL.  dz is rounded to dtype for the products; its columns go through in pieces of 1 GiB
  *   at most, over which dx is summed in float32.  No two calls that can run at the same time may share a workspace. */
 #define MTX_HEAD_DV 0  /* W[D,V] */
 #define MTX_HEAD_VD 1  /* W[V,D] */

@@ -198,6 +198,7 @@ def require_device(*tensors) -> torch.device:
 
 # Internals of torch that answer without building an object; where one is missing, the public way is taken.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # of a process that has device tensors
 _tracing_state = getattr(torch._C, "_get_tracing_state", None)
 _functorch_level = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", None)
 
@@ -214,7 +215,7 @@ _here = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """Context in which ``device`` is the current one, which is where a kernel is launched."""
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _here if _current_device() == device.index else torch.cuda.device(device)
 
 
 def plain_forward(*tensors) -> bool:

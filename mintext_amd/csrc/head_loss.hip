@@ -105,7 +105,6 @@ __global__ __launch_bounds__(64) void entries_kernel(Prep p) {
 }
 
 // ---- the blocks' maxima and sums, and the row's loss -------------------------------------------------------
-// R rows a workgroup, 256 / R threads a row; the joins are in a fixed order.
 struct Merge {
   const float2* part;
   int64_t blocks, T, V;
@@ -116,69 +115,99 @@ struct Merge {
   float scale, inv_tau, unit, z_loss;  // unit: tau^2
   float *loss, *lse, *state;           // loss: [T]
 };
-template <int R>
-__global__ __launch_bounds__(256) void merge_kernel(Merge p) {
-  constexpr int G = 256 / R;
-  __shared__ float ms[G][R], ss[G][R];
-  const int tx = threadIdx.x % R, g = threadIdx.x / R;
-  const int64_t row = (int64_t)blockIdx.x * R + tx;
-  const bool live = row < p.T;
-  float m = -INFINITY, s = 0.0f;
-  auto join = [&](float om, float os) {  // -inf with -inf: sums of 0
+struct Sum {  // of exp2((z - m) scale)
+  float m, s;
+  __device__ __forceinline__ void join(float om, float os, float scale) {  // -inf with -inf: a sum of 0
     const float n = fmaxf(m, om);
-    s = s * exp2f(m == n ? 0.0f : (m - n) * p.scale) + os * exp2f(om == n ? 0.0f : (om - n) * p.scale);
+    s = s * exp2f(m == n ? 0.0f : (m - n) * scale) + os * exp2f(om == n ? 0.0f : (om - n) * scale);
     m = n;
-  };
-  if (live) {
-    int64_t b = g;
-    for (; b + 3 * G < p.blocks; b += 4 * G) {
-      float2 v[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = p.part[(b + u * G) * p.T + row];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) join(v[u].x, v[u].y);
-    }
-    for (; b < p.blocks; b += G) {
-      const float2 v = p.part[b * p.T + row];
-      join(v.x, v.y);
-    }
   }
-  ms[g][tx] = m;
-  ss[g][tx] = s;
-  __syncthreads();
-  m = ms[0][tx];
-  s = ss[0][tx];
-  for (int i = 1; i < G; ++i) join(ms[i][tx], ss[i][tx]);
-  // sum of share (m - z) / tau, whose terms are small where the share is not
+};
+// blocks first, first + step, .. of a row
+__device__ __forceinline__ Sum sum_blocks(const Merge& p, int64_t row, int64_t first, int64_t step) {
+  Sum a{-INFINITY, 0.0f};
+  int64_t b = first;
+  for (; b + 3 * step < p.blocks; b += 4 * step) {
+    float2 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = p.part[(b + u * step) * p.T + row];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) a.join(v[u].x, v[u].y, p.scale);
+  }
+  for (; b < p.blocks; b += step) {
+    const float2 v = p.part[b * p.T + row];
+    a.join(v.x, v.y, p.scale);
+  }
+  return a;
+}
+// share of entries first, first + step, .. in sum p (m - z) / tau, whose terms are small where the share is not
+__device__ __forceinline__ float below_max(const Merge& p, int64_t row, float m, int first, int step) {
   float below = 0.0f;
-  if (live && !p.e.targets) {
-    const int64_t at = row * p.e.K;
-    const int n = p.e.bounds[row * p.e.ldb + p.e.ldb - 1];
-    for (int k = g; k < n; k += G) {
-      const float w = p.e.share[at + k];
-      if (w != 0.0f) below += w * ((m - p.chosen[at + k]) * p.inv_tau);
-    }
+  if (p.e.targets) return below;
+  const int64_t at = row * p.e.K;
+  const int n = p.e.bounds[row * p.e.ldb + p.e.ldb - 1];
+  for (int k = first; k < n; k += step) {
+    const float w = p.e.share[at + k];
+    if (w != 0.0f) below += w * ((m - p.chosen[at + k]) * p.inv_tau);
   }
-  __syncthreads();
-  ms[g][tx] = below;
-  __syncthreads();
-  if (g > 0 || !live) return;
-  for (int i = 1; i < G; ++i) below += ms[i][tx];
+  return below;
+}
+__device__ __forceinline__ void finish_row(const Merge& p, int64_t row, const Sum& a, float below) {
   float state, konst = 0.0f;
   if (p.e.targets) {
     const int64_t y = target(p.e, row);
     state = y == p.ignore ? 0.0f : y < 0 || y >= p.V ? NAN : 1.0f;
-    if (state == 1.0f) below = m - p.chosen[row];
+    if (state == 1.0f) below = a.m - p.chosen[row];
   } else {
     state = p.row[row].x;
     konst = p.row[row].y;
   }
-  const float log_sum = logf(s), lse = m * p.inv_tau + log_sum;
+  const float log_sum = logf(a.s), lse = a.m * p.inv_tau + log_sum;
   float loss = p.unit * (konst + below + log_sum);
   if (p.z_loss != 0.0f) loss += p.z_loss * lse * lse;
   p.loss[row] = state == 0.0f ? 0.0f : state * loss;
   p.lse[row] = lse;
   p.state[row] = state;
+}
+// 32 rows a workgroup, eight threads a row, joined in order: neighbours read neighbouring rows' blocks.  4096 rows of 250
+// blocks 9 us, 4093 of 1024 28 us.
+__global__ __launch_bounds__(256) void merge_kernel(Merge p) {
+  __shared__ float ms[8][32], ss[8][32];
+  const int tx = threadIdx.x % 32, g = threadIdx.x / 32;
+  const int64_t row = (int64_t)blockIdx.x * 32 + tx;
+  const bool live = row < p.T;
+  Sum a{-INFINITY, 0.0f};
+  if (live) a = sum_blocks(p, row, g, 8);
+  ms[g][tx] = a.m;
+  ss[g][tx] = a.s;
+  __syncthreads();
+  a = Sum{ms[0][tx], ss[0][tx]};
+  for (int i = 1; i < 8; ++i) a.join(ms[i][tx], ss[i][tx], p.scale);
+  float below = live ? below_max(p, row, a.m, g, 8) : 0.0f;
+  __syncthreads();
+  ms[g][tx] = below;
+  __syncthreads();
+  if (g > 0 || !live) return;
+  for (int i = 1; i < 8; ++i) below += ms[i][tx];
+  finish_row(p, row, a, below);
+}
+// A wave a row, for fewer rows than would fill the chip the other way.
+template <int S>
+__device__ __forceinline__ void wave_join(Sum& a, float scale) {
+  if constexpr (S < 6) {
+    const float m = lane_xchg<S>(a.m), s = lane_xchg<S>(a.s);
+    a.join(m, s, scale);
+    wave_join<S + 1>(a, scale);
+  }
+}
+__global__ __launch_bounds__(256) void merge_wave_kernel(Merge p) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= p.T) return;
+  const int lane = threadIdx.x & 63;
+  Sum a = sum_blocks(p, row, lane, 64);
+  wave_join<0>(a, p.scale);
+  const float below = wave_sum(below_max(p, row, a.m, lane, 64));
+  if (lane == 0) finish_row(p, row, a, below);
 }
 
 // The sum of the rows' losses and what it is divided by, in 64 bits and one workgroup's order.
@@ -261,19 +290,67 @@ __global__ __launch_bounds__(256) void named_kernel(Named p) {
   else ((uint16_t*)p.dz)[t * p.ldz + c] = f32_to_bf16(v);
 }
 
-// rows x cols of a bf16 matrix into one with rows of `ld` (a multiple of 8), zeros behind the columns
+// rows x cols of a bf16 matrix into one with rows of `ld` (a multiple of 8), zeros behind the columns.  `in` lies on a 4-byte
+// boundary and has rows of any length: eight elements come as the words that hold them, shifted by one where the first is odd.
 __global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ in, int64_t ldi, int64_t rows, int64_t cols,
                                                   uint16_t* __restrict__ out, int64_t ld) {
+  struct __attribute__((aligned(4))) Words {
+    uint32_t v[4];
+  };
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (i >= rows * ld) return;
-  const int64_t r = i / ld, c = i % ld;
-  uint16_t v[8];
+  const int64_t r = i / ld, c = i - r * ld, e = r * ldi + c, end = (rows - 1) * ldi + cols;
+  v4u32 o = {0u, 0u, 0u, 0u};
+  if (c < cols) {
+    if (e + 9 < end) {  // all the words lie inside
+      const uint32_t* p = (const uint32_t*)in + (e >> 1);
+      const Words w = *(const Words*)p;
+      const uint32_t next = p[4], odd = (e & 1) * 16;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] = c + q < cols ? in[r * ldi + c + q] : (uint16_t)0;
-  v4u32 o;
+      for (int q = 0; q < 4; ++q) o[q] = __builtin_amdgcn_alignbit(q < 3 ? w.v[q < 3 ? q + 1 : 3] : next, w.v[q], odd);
+    } else {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) o[q] = (uint32_t)v[2 * q] | ((uint32_t)v[2 * q + 1] << 16);
+      for (int q = 0; q < 8; ++q)
+        if (e + q < end) o[q / 2] |= (uint32_t)in[e + q] << (16 * (q & 1));
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // what lies behind the row's end
+      const int64_t left = cols - c - 2 * q;
+      if (left < 2) o[q] &= left < 1 ? 0u : 0xFFFFu;
+    }
+  }
   *(v4u32*)(out + i) = o;
+}
+
+// The way back: rows of `ld` elements to rows of any length.  A thread writes what lies between two 16-byte boundaries of `out`
+// (at a row's ends the part of it that is the row's), from the words that hold it.  The gradient of a weight of 704 x 50257
+// written by the tiles themselves, element by element: 199 us instead of 115 and 25.
+__global__ __launch_bounds__(256) void unpad_kernel(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols,
+                                                    uint16_t* __restrict__ out, int64_t ldo) {
+  struct __attribute__((aligned(4))) Words {
+    uint32_t v[4];
+  };
+  const int64_t per = cols / 8 + 2, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const int64_t r = i / per;
+  uint16_t* row = out + r * ldo;
+  const int head = (int)((16 - (uintptr_t)row % 16) % 16 / 2);  // columns before the first boundary
+  const int64_t c = head + (i - r * per - 1) * 8;
+  if (c >= cols || c + 8 <= 0) return;
+  const uint16_t* from = in + r * ld;
+  if (c >= 0 && c + 8 <= cols) {
+    const uint32_t* p = (const uint32_t*)from + (c >> 1);
+    const Words w = *(const Words*)p;
+    const uint32_t odd = (c & 1) * 16, next = odd ? p[4] : 0u;  // odd: column c + 8 or zeros behind the last one
+    v4u32 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = __builtin_amdgcn_alignbit(q < 3 ? w.v[q < 3 ? q + 1 : 3] : next, w.v[q], odd);
+    *(v4u32*)(row + c) = o;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (c + q >= 0 && c + q < cols) row[c + q] = from[c + q];
+  }
 }
 
 // out = the pieces' sums, in order.  V columns a thread.
@@ -324,7 +401,8 @@ static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
     const int64_t tiles = ceil_div(rows, side) * ceil_div(cols, side);
     const double stage = f32 ? 0.9 : kind ? 0.6 : 0.85;
     for (int s = 1; s <= kMostPieces && (s == 1 || stages / s >= 8); ++s) {
-      const double t = ceil_div(tiles * s, slots) * (ceil_div(stages, s) * stage + 6.0) +
+      const double out = f32 ? 4.0 : kind ? 5.0 : 12.0;
+      const double t = ceil_div(tiles * s, slots) * (ceil_div(stages, s) * stage + out) +
                        (s > 1 ? s * rows * cols * 8 / 4e6 + 6.0 : 0.0);
       if (t < least) {
         least = t;
@@ -337,7 +415,7 @@ static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
 
 struct Plan {
   bool f32;
-  int64_t T, D, V, D8;       // D8: x's row length in use
+  int64_t T, D, V, ldx, red;  // ldx: x's row length in use; red: reduction elements of the logits
   int order;
   bool copy_x, copy_w;
   int64_t piece;             // columns of a piece, a multiple of 256
@@ -354,9 +432,12 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
   const int64_t size = p.f32 ? 4 : 2, all = round_up(V, 256);
   p.copy_x = !p.f32 && D % 8 != 0;
   p.copy_w = !p.f32 && (order == ORDER_DV ? V : D) % 8 != 0;
-  p.D8 = p.copy_x ? round_up(D, 8) : D;
+  // Copies have rows of whole 128-byte lines: 1531 x 1001 x 50257, whose rows of 1008 began inside lines, took 241 to 249 us for
+  // the logits.  x's zeros end whole stages where the weight is copied too.
+  p.ldx = p.copy_x ? round_up(D, 64) : D;
+  p.red = !p.copy_x ? D : round_up(D, order == ORDER_VD ? 32 : 8);
   int64_t most = all;
-  if (p.copy_w) most = std::min(most, std::max<int64_t>(kCopy / (p.D8 * 2) / 256 * 256, 256));
+  if (p.copy_w) most = std::min(most, std::max<int64_t>(kCopy / (p.ldx * 2) / 256 * 256, 256));
   if (backward) most = std::min(most, std::max<int64_t>(kPiece / (T * size) / 256 * 256, 256));
   p.piece = round_up(ceil_div(V, ceil_div(all, most)), 256);
   const int64_t big = ceil_div(T, 256) * ceil_div(p.piece, 256);
@@ -367,8 +448,8 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
     at += round_up(bytes, 256);
     return here;
   };
-  p.x = take(p.copy_x ? T * p.D8 * 2 : 0);
-  p.w = take(p.copy_w ? p.piece * p.D8 * 2 : 0);
+  p.x = take(p.copy_x ? T * p.ldx * 2 : 0);
+  p.w = take(p.copy_w ? p.piece * (order == ORDER_DV ? D : p.ldx) * 2 : 0);
   if (!backward) {
     p.part = take(round_up(V, tile_cols(p.path)) / block_cols(p.path) * T * 8);
   } else {
@@ -407,21 +488,21 @@ static int operands(const Plan& p, const void* x, const void* w, int64_t v0, cha
   const int64_t size = p.f32 ? 4 : 2, n = std::min(p.piece, p.V - v0);
   int rc = MTX_OK;
   a.x = p.copy_x ? ws + p.x : x;
-  if (p.copy_x && v0 == 0) rc = pad(x, p.D, p.T, p.D, ws + p.x, p.D8, st);
-  a.ldx = p.D8;
+  if (p.copy_x && v0 == 0) rc = pad(x, p.D, p.T, p.D, ws + p.x, p.ldx, st);
+  a.ldx = p.ldx;
   a.w = (const char*)w + (p.order == ORDER_DV ? v0 : v0 * p.D) * size;
   a.ldw = p.order == ORDER_DV ? p.V : p.D;
   a.w_left = (int)n;
   if (p.copy_w && rc == MTX_OK) {
     const bool dv = p.order == ORDER_DV;
-    rc = pad(a.w, a.ldw, dv ? p.D : n, dv ? n : p.D, ws + p.w, dv ? p.piece : p.D8, st);
+    rc = pad(a.w, a.ldw, dv ? p.D : n, dv ? n : p.D, ws + p.w, dv ? p.piece : p.ldx, st);
     a.w = ws + p.w;
-    a.ldw = dv ? p.piece : p.D8;
+    a.ldw = dv ? p.piece : p.ldx;
     if (dv) a.w_left = (int)p.piece;
   }
   a.T = (int)p.T;
-  a.red = (int)p.D8;
-  a.missing = p.order == ORDER_DV ? (int)(p.D8 - p.D) : 0;
+  a.red = (int)p.red;
+  a.missing = p.order == ORDER_DV ? (int)(p.red - p.D) : 0;
   a.v0 = (int)v0;
   a.cols = (int)n;
   return rc;
@@ -466,8 +547,8 @@ static int forward(const Plan& p, const void* x, const void* w, Merge m, float* 
   m.T = p.T;
   m.V = p.V;
   m.chosen = chosen;
-  if (p.T > 2048) hipLaunchKernelGGL(merge_kernel<32>, dim3((unsigned)ceil_div(p.T, 32)), dim3(256), 0, st, m);
-  else hipLaunchKernelGGL(merge_kernel<4>, dim3((unsigned)ceil_div(p.T, 4)), dim3(256), 0, st, m);
+  if (p.T > 2048) hipLaunchKernelGGL(merge_kernel, dim3((unsigned)ceil_div(p.T, 32)), dim3(256), 0, st, m);
+  else hipLaunchKernelGGL(merge_wave_kernel, dim3((unsigned)ceil_div(p.T, 4)), dim3(256), 0, st, m);
   if (total) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, m.loss, m.state, p.T, mean, total, count);
   return check_launch();
 }
@@ -499,7 +580,7 @@ static int backward(const Plan& p, const float* g, const float* count, const voi
       const bool only = p.piece >= p.V, final = v0 + p.piece >= p.V;
       // the last piece of the vocabulary may be shorter than what the split was made for
       const int pieces = (int)std::min<int64_t>(p.dx.pieces, ceil_div(red, 32));
-      Product q{a.dz, a.w, a.ldz, a.ldw, (int)p.T, (int)p.D, red, 0, (int)p.T, (int)(dv ? p.D : p.D8), dx, p.D, pieces, nullptr,
+      Product q{a.dz, a.w, a.ldz, a.ldw, (int)p.T, (int)p.D, red, 0, (int)p.T, (int)(dv ? p.D : p.ldx), dx, p.D, pieces, nullptr,
                 p.ld_dx, v0 > 0, p.dx.pieces == 1 && final, alpha};
       if (!dv) q.missing = red - a.cols;
       if (!(only && p.dx.pieces == 1)) q.acc = (float*)(ws + p.acc_dx);
@@ -507,18 +588,27 @@ static int backward(const Plan& p, const float* g, const float* count, const voi
       if (rc == MTX_OK && final && p.dx.pieces > 1) rc = join(p.f32, q.acc, p.dx.pieces, p.T, p.D, p.ld_dx, dx, p.D, alpha, st);
       if (rc != MTX_OK) return rc;
     }
-    if (dw) {
-      char* out = (char*)dw + (dv ? v0 : v0 * p.D) * size;
-      const int64_t ldo = dv ? p.V : p.D;
+    if (dw && rc == MTX_OK) {
+      // where the weight's rows are no whole chunks, the product goes to the place of their copy, which is done with
+      void* out = (char*)dw + (dv ? v0 : v0 * p.D) * size;
+      void* to = p.copy_w ? ws + p.w : out;
+      const int64_t ldo = dv ? p.V : p.D, ldt = p.copy_w ? a.ldw : ldo;
       Product q{};
-      if (dv) q = Product{a.x, a.dz, a.ldx, a.ldz, (int)p.D, a.cols, (int)p.T, 0, (int)p.D8, (int)p.piece, out, ldo, p.dw.pieces};
-      else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, (int)p.T, 0, (int)p.piece, (int)p.D8, out, ldo, p.dw.pieces};
+      if (dv) q = Product{a.x, a.dz, a.ldx, a.ldz, (int)p.D, a.cols, (int)p.T, 0, (int)p.ldx, (int)p.piece, to, ldt, p.dw.pieces};
+      else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, (int)p.T, 0, (int)p.piece, (int)p.ldx, to, ldt, p.dw.pieces};
+      const int64_t rows = q.rows, cols = q.cols;
+      if (p.copy_w) q.cols = (int)round_up(cols, 8);  // whole chunks; what lies behind the columns is not taken
       q.ldacc = p.ld_dw;
       q.last = p.dw.pieces == 1;
       q.alpha = alpha;
       if (p.dw.pieces > 1) q.acc = (float*)(ws + p.acc_dw);
       rc = product(p, q, true, true, p.dw, st);
-      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, q.rows, q.cols, p.ld_dw, out, ldo, alpha, st);
+      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, rows, q.cols, p.ld_dw, to, ldt, alpha, st);
+      if (rc == MTX_OK && p.copy_w) {
+        hipLaunchKernelGGL(unpad_kernel, dim3((unsigned)ceil_div(rows * (cols / 8 + 2), 256)), dim3(256), 0, st, (const uint16_t*)to,
+                           ldt, rows, cols, (uint16_t*)out, ldo);
+        rc = check_launch();
+      }
     }
   }
   return rc;
@@ -587,7 +677,9 @@ extern "C" int mtx_linear_cross_entropy_bwd(const float* g, const float* count, 
   const int rc = check_sizes(dtype, T, D, V, order);
   if (rc != MTX_OK) return rc;
   if (T == 0 || (!dx && !dw)) return MTX_OK;
-  if (!g || !x || !w || !targets || !lse || !state || !chosen || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  if (!g || !x || !w || !targets || !lse || !state || !chosen || !aligned16(x) || !aligned16(w) || !aligned16(dx) ||
+      !aligned16(dw))
+    return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, true);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
   const Entries e{targets, targets_64, nullptr, nullptr, nullptr, 0, 1};
@@ -641,7 +733,9 @@ extern "C" int mtx_linear_distillation_bwd(const float* g, const float* count, c
   if (K <= 0 || !(temperature > 0.0f && temperature < INFINITY)) return MTX_ERR_ARG;
   if (K > kMaxEntries) return MTX_ERR_UNSUPPORTED;
   if (T == 0 || (!dx && !dw)) return MTX_OK;
-  if (!g || !x || !w || !entries_buffer || !lse || !state || !chosen || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  if (!g || !x || !w || !entries_buffer || !lse || !state || !chosen || !aligned16(x) || !aligned16(w) || !aligned16(dx) ||
+      !aligned16(dw))
+    return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, true);
   const Saved s = saved(T, V, K);
   if (!aligned16(entries_buffer) || entries_bytes < s.total) return MTX_ERR_WORKSPACE;

@@ -82,9 +82,15 @@ __device__ __forceinline__ void forward_out(const Logits& p, dense::f32x16 (&acc
     if (p.e.targets) {
       if (hi[i] && half == 0) p.chosen[row] = *in_lds<T>(mine, lane & 31, lo[i]);
     } else {
-      for (int e = lo[i] + half; e < hi[i]; e += 2) {
-        const int c = p.e.idx[(int64_t)row * p.e.K + e] - p.v0 - c0;
-        if ((unsigned)c < (unsigned)BC) p.chosen[(int64_t)row * p.e.K + e] = *in_lds<T>(mine, lane & 31, c);
+      // eight at a time, so that a row whose entries all lie here (1531 x 1001 x 50257 with 100 of them) waits for few loads
+      for (int e = lo[i] + half; e < hi[i]; e += 16) {
+        const int64_t at = (int64_t)row * p.e.K;
+        int c[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) c[q] = p.e.idx[at + min(e + 2 * q, hi[i] - 1)] - p.v0 - c0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (e + 2 * q < hi[i] && (unsigned)c[q] < (unsigned)BC) p.chosen[at + e + 2 * q] = *in_lds<T>(mine, lane & 31, c[q]);
       }
     }
     asm volatile("" ::: "memory");
@@ -168,6 +174,17 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logit
 template <bool A_COLS, bool B_COLS, bool TAIL> using GradBig = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, A_COLS, B_COLS, TAIL>;
 template <bool A_COLS, bool B_COLS, bool TAIL> using GradSmall = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, A_COLS, B_COLS, TAIL>;
 
+// whole: rows of whole 16-byte chunks; left: columns that exist
+__device__ __forceinline__ void store_part(uint16_t* o, const float v[8], bool whole, int left) {
+  if (whole) {
+    dense::store8(o, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < left) o[q] = f32_to_bf16(v[q]);
+  }
+}
+
 template <class T>
 __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void product_kernel(Product p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
@@ -188,41 +205,50 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   __syncthreads();
   const int wave = threadIdx.x >> 6;
   char* mine = T::out_lds(lds);
-  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c = n0 + (wave % T::WN) * (T::TN * 32) + T::out_col(0);
+  const int wr = m0 + (wave / T::WN) * (T::TM * 32), c0 = n0 + (wave % T::WN) * (T::TN * 32);
   float* sums = p.acc ? p.acc + (int64_t)piece * p.rows * p.ldacc : nullptr;
   const float alpha = p.alpha && (!sums || p.last) ? *p.alpha : 1.0f;
   const bool whole = p.ldo % 8 == 0 && p.cols % 8 == 0 && (uintptr_t)p.out % 16 == 0;
+  if (sums) {
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i) {
-    T::put(acc[i], mine);
-#pragma unroll
-    for (int it = 0; it < T::OUT_STEPS; ++it) {
-      const int r = wr + i * 32 + T::out_row(it);
-      if (r >= p.rows || c >= p.cols) continue;
-      float v[8];
-      T::get(mine, it, v);
-      if (sums) {
+    for (int i = 0; i < T::TM; ++i) {
+      T::put(acc[i], mine);
+#pragma unroll 4
+      for (int it = 0; it < T::OUT_STEPS; ++it) {
+        const int r = wr + i * 32 + T::out_row(it), c = c0 + T::out_col(it);
+        if (r >= p.rows || c >= p.cols) continue;
+        float v[8];
+        T::get(mine, it, v);
         float* s = sums + (int64_t)r * p.ldacc + c;
         if (p.add) {
-          float o[8];
-          ld8(s, 0, o);
+          float x[8];
+          ld8(s, 0, x);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] += o[q];
+          for (int q = 0; q < 8; ++q) v[q] += x[q];
         }
         if (!p.last) {
           st8(s, 0, v);
           continue;
         }
+        uint16_t* out = (uint16_t*)p.out + (int64_t)r * p.ldo + c;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] *= alpha;
+        store_part(out, v, whole, p.cols - c);
       }
+    }
+  } else {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] *= alpha;
-      uint16_t* o = (uint16_t*)p.out + (int64_t)r * p.ldo + c;
-      if (whole) {
-        dense::store8(o, v);
-      } else {
+    for (int i = 0; i < T::TM; ++i) {
+      T::put(acc[i], mine);
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (c + q < p.cols) o[q] = f32_to_bf16(v[q]);
+      for (int it = 0; it < T::OUT_STEPS; ++it) {
+        const int r = wr + i * 32 + T::out_row(it), c = c0 + T::out_col(it);
+        if (r >= p.rows || c >= p.cols) continue;
+        float v[8];
+        T::get(mine, it, v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] *= alpha;
+        store_part((uint16_t*)p.out + (int64_t)r * p.ldo + c, v, whole, p.cols - c);
       }
     }
   }

@@ -9,6 +9,7 @@
 #include "common.h"
 #include "f32_tile.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace mtx {
 namespace norm {
@@ -73,6 +74,24 @@ __device__ __forceinline__ void load_row(const T* p, int D, float (&v)[kPer]) {
       v[i] = c < D ? gld<T>(p, c) : 0.0f;
     }
   }
+}
+// The same in two steps, so that bf16 rows can be on their way while another is worked on, in half the registers.
+template <int WPR>
+__device__ __forceinline__ void fetch_row(const uint16_t* p, int D, v4u32 (&raw)[kPer / 8]) {
+#pragma unroll
+  for (int i = 0; i < kPer / 8; ++i) {
+    const int c = column<8, WPR>(i);
+    raw[i] = c < D ? *(const v4u32*)(p + c) : v4u32{0u, 0u, 0u, 0u};
+  }
+}
+__device__ __forceinline__ void unpack_row(const v4u32 (&raw)[kPer / 8], float (&v)[kPer]) {
+#pragma unroll
+  for (int i = 0; i < kPer / 8; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[i * 8 + 2 * q] = __uint_as_float(raw[i][q] << 16);
+      v[i * 8 + 2 * q + 1] = __uint_as_float(raw[i][q] & 0xffff0000u);
+    }
 }
 template <typename T, int VEC, int WPR>
 __device__ __forceinline__ void store_row(T* p, int D, const float (&v)[kPer]) {
@@ -157,11 +176,13 @@ struct BwdArgs {
   bool w32, bias;
 };
 
-// A workgroup of 16 waves takes every gridDim.x-th set of 16 / WPR rows; a lane's columns are the same in all of them, so
-// its share of dw and db stays in registers until the end.
+// A workgroup of one row's waves, eight at least, takes every gridDim.x-th set of rows; a lane's columns are the same in all
+// of them, so its share of dw and db stays in registers until the end.  Eight waves leave registers for the next row's
+// values on their way.
+constexpr int backward_waves(int wpr) { return wpr > 8 ? wpr : 8; }
 template <typename T, bool RMS, int VEC, int WPR>
-__global__ __launch_bounds__(1024) void backward_kernel(BwdArgs p) {
-  constexpr int GROUPS = 16 / WPR;
+__global__ __launch_bounds__(backward_waves(WPR) * 64) void backward_kernel(BwdArgs p) {
+  constexpr int GROUPS = backward_waves(WPR) / WPR;
   __shared__ float s[2][16][2];
   __shared__ float sums[GROUPS > 1 ? WPR * 64 * kPer : 1];
   const int group = row_of_wave<WPR>();
@@ -169,14 +190,36 @@ __global__ __launch_bounds__(1024) void backward_kernel(BwdArgs p) {
   load_param<T, VEC, WPR>(p.weight, p.w32, p.D, w);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) dw[i] = db[i] = 0.0f;
+  // AHEAD: the next row's values are loaded before this one's are worked on
+  constexpr bool AHEAD = std::is_same<T, uint16_t>::value && VEC == 8 && WPR <= 8;
+  v4u32 next_h[kPer / 8], next_dy[kPer / 8], next_dh[kPer / 8];
+  auto fetch = [&](int64_t base) {
+    if constexpr (AHEAD) {
+      const int64_t at = min(base + group, p.T - 1) * p.D;
+      fetch_row<WPR>((const uint16_t*)p.h + at, p.D, next_h);
+      fetch_row<WPR>((const uint16_t*)p.dy + at, p.D, next_dy);
+      if (p.dh) fetch_row<WPR>((const uint16_t*)p.dh + at, p.D, next_dh);
+    }
+  };
   int turn = 0;
-  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.T; base += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  fetch((int64_t)blockIdx.x * GROUPS);
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.T; base += step, turn ^= 1) {
     const int64_t row = base + group;
     const bool live = row < p.T;
     const int64_t r = live ? row : p.T - 1, at = r * p.D;
     float n[kPer], u[kPer];
-    load_row<T, VEC, WPR>((const T*)p.h + at, p.D, n);
-    load_row<T, VEC, WPR>((const T*)p.dy + at, p.D, u);
+    v4u32 dh[kPer / 8];
+    if constexpr (AHEAD) {
+      unpack_row(next_h, n);
+      unpack_row(next_dy, u);
+#pragma unroll
+      for (int i = 0; i < kPer / 8; ++i) dh[i] = next_dh[i];
+      if (base + step < p.T) fetch(base + step);
+    } else {
+      load_row<T, VEC, WPR>((const T*)p.h + at, p.D, n);
+      load_row<T, VEC, WPR>((const T*)p.dy + at, p.D, u);
+    }
     const float rstd = p.rstd[r], mean = RMS ? 0.0f : p.mean[r];
     float t[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -184,7 +227,7 @@ __global__ __launch_bounds__(1024) void backward_kernel(BwdArgs p) {
       n[i] = (n[i] - mean) * rstd;  // past the row's end u is 0, which keeps it out of the sums
       if (live) {
         dw[i] += n[i] * u[i];
-        db[i] += u[i];
+        if (!RMS) db[i] += u[i];
       }
       u[i] *= w[i];
       t[0] += u[i] * n[i];
@@ -196,7 +239,8 @@ __global__ __launch_bounds__(1024) void backward_kernel(BwdArgs p) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) u[i] = (u[i] - m - n[i] * c) * rstd;
     if (p.dh) {
-      load_row<T, VEC, WPR>((const T*)p.dh + at, p.D, n);
+      if constexpr (AHEAD) unpack_row(dh, n);
+      else load_row<T, VEC, WPR>((const T*)p.dh + at, p.D, n);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) u[i] += n[i];
     }
@@ -207,7 +251,7 @@ __global__ __launch_bounds__(1024) void backward_kernel(BwdArgs p) {
   const int kinds = p.bias ? 2 : 1;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    if (k >= kinds) break;
+    if (k >= kinds || (RMS && k > 0)) break;
     float* v = k ? db : dw;
     if constexpr (GROUPS > 1) {  // the groups' sums in order
       for (int g = 0; g < GROUPS; ++g) {
@@ -254,7 +298,7 @@ static int waves(int D) {  // of a row
   return w;
 }
 static int groups(int64_t T, int D) {  // workgroups of the backward pass: one a CU
-  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(T, 16 / waves(D)), 256));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(T, backward_waves(waves(D)) / waves(D)), 256));
 }
 static int check_sizes(int dtype, int weight_dtype, int64_t T, int64_t D) {
   if (dtype != MTX_F32 && dtype != MTX_BF16) return MTX_ERR_ARG;
@@ -341,7 +385,7 @@ extern "C" int mtx_norm_bwd(const void* dy, const void* dh, const void* h, const
                     dbias != nullptr};
     const bool vec = D % 8 == 0 && aligned16(dy) && aligned16(dh) && aligned16(h) && aligned16(weight) && aligned16(dx);
 #define MTX_GRID(W) dim3((unsigned)n)
-#define MTX_THREADS(W) dim3(1024)
+#define MTX_THREADS(W) dim3(backward_waves(W) * 64)
     MTX_KINDS(backward_kernel, rms, dtype, vec, (int)D, MTX_GRID, MTX_THREADS, st, p)
 #undef MTX_GRID
 #undef MTX_THREADS

@@ -42,49 +42,69 @@ def _forward(x, residual, weight, bias, rms, eps, keep):
     D = x.shape[-1]
     T = x.numel() // D
     x, weight = x.contiguous(), weight.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    bias = None if bias is None else bias.contiguous()
     y = torch.empty_like(x)
-    h = None if residual is None else torch.empty_like(x)
-    stats = torch.empty((1 if rms else 2, T), dtype=torch.float32, device=dev) if keep else None
-    rstd = stats[0] if keep else None
-    mean = stats[1] if keep and not rms else None
+    r = b = h = m = s = mean = rstd = None  # the letters: addresses
+    if residual is not None:
+        residual = residual.contiguous()
+        hidden = torch.empty_like(x)
+        r, h = residual.data_ptr(), hidden.data_ptr()
+    else:
+        hidden = x
+    if bias is not None:
+        bias = bias.contiguous()
+        b = bias.data_ptr()
+    if keep:
+        rstd = torch.empty(T, dtype=torch.float32, device=dev)
+        s = rstd.data_ptr()
+        if not rms:
+            mean = torch.empty(T, dtype=torch.float32, device=dev)
+            m = mean.data_ptr()
     with L.on_device(dev):
-        L.call("mtx_norm", x.data_ptr(), L.ptr(residual), weight.data_ptr(), L.ptr(bias), L.dtype_code(x.dtype),
-               L.dtype_code(weight.dtype), int(rms), T, D, eps, y.data_ptr(), L.ptr(h), L.ptr(mean), L.ptr(rstd), L.stream(dev))
-    return y, (x if h is None else h), stats
+        L.call("mtx_norm", x.data_ptr(), r, weight.data_ptr(), b, L.dtype_code(x.dtype), L.dtype_code(weight.dtype), rms, T, D,
+               eps, y.data_ptr(), h, m, s, L.stream(dev))
+    return y, hidden, mean, rstd
 
 
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, rms, eps):
-        y, h, stats = _forward(x, residual, weight, bias, rms, eps, True)
-        ctx.save_for_backward(h, weight, stats)
-        ctx.rms, ctx.has_bias, ctx.has_residual = rms, bias is not None, residual is not None
+        y, h, mean, rstd = _forward(x, residual, weight, bias, rms, eps, True)
+        ctx.save_for_backward(h, weight, mean, rstd)
+        ctx.rms = rms
         ctx.set_materialize_grads(False)
         return (y, h) if residual is not None else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, stats = ctx.saved_tensors
+        h, weight, mean, rstd = ctx.saved_tensors
         need_x, need_r, need_w, need_b, _, _ = ctx.needs_input_grad
         if dy is None:  # the sum alone is used
             return (dh if need_x else None, dh if need_r else None, None, None, None, None)
+        rms = ctx.rms
         dev = L.require_device(dy, dh, h, weight)
         dy, weight = dy.contiguous(), weight.contiguous()
-        dh = None if dh is None else dh.contiguous()
         D = h.shape[-1]
         T = h.numel() // D
-        dx = torch.empty_like(h) if need_x or need_r else None
-        dw = torch.empty_like(weight) if need_w or need_b else None
-        db = torch.empty_like(weight) if need_b else None
-        ws = L.workspace(L.query("mtx_norm_bwd_workspace_size", T, D) if need_w or need_b else 0, dev)
-        mean = None if ctx.rms else stats[1]
+        dx = dw = db = None
+        dhp = dxp = dwp = dbp = wsp = None
+        nbytes = 0
+        if dh is not None:
+            dh = dh.contiguous()
+            dhp = dh.data_ptr()
+        if need_x or need_r:
+            dx = torch.empty_like(h)
+            dxp = dx.data_ptr()
+        if need_w or need_b:
+            dw = torch.empty_like(weight)
+            ws = L.workspace(L.query("mtx_norm_bwd_workspace_size", T, D), dev)
+            dwp, wsp, nbytes = dw.data_ptr(), ws.data_ptr(), ws.numel()
+        if need_b:
+            db = torch.empty_like(weight)
+            dbp = db.data_ptr()
         with L.on_device(dev):
-            L.call("mtx_norm_bwd", dy.data_ptr(), L.ptr(dh), h.data_ptr(), weight.data_ptr(), L.ptr(mean), stats.data_ptr(),
-                   L.dtype_code(h.dtype), L.dtype_code(weight.dtype), int(ctx.rms), T, D, L.ptr(dx), L.ptr(dw), L.ptr(db),
-                   ws.data_ptr(), ws.numel(), L.stream(dev))
+            L.call("mtx_norm_bwd", dy.data_ptr(), dhp, h.data_ptr(), weight.data_ptr(), L.ptr(mean), rstd.data_ptr(),
+                   L.dtype_code(h.dtype), L.dtype_code(weight.dtype), rms, T, D, dxp, dwp, dbp, wsp, nbytes, L.stream(dev))
         return dx if need_x else None, dx if need_r else None, dw if need_w else None, db, None, None
 
 
@@ -92,7 +112,7 @@ def _norm(name, x, weight, bias, rms, eps, residual):
     eps = float(eps)
     _check(name, x, weight, bias, residual, eps)
     if L.plain_forward(x, weight, bias, residual):
-        y, h, _ = _forward(x, residual, weight, bias, rms, eps, False)
+        y, h, _, _ = _forward(x, residual, weight, bias, rms, eps, False)
         return y if residual is None else (y, h)
     return _Norm.apply(x, residual, weight, bias, rms, eps)
 
