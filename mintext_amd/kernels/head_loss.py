@@ -68,62 +68,66 @@ class _Loss:
     def __init__(self, reduction, z_loss=0.0, ignore_index=0, temperature=1.0):
         self.reduction, self.z_loss, self.ignore_index, self.temperature = reduction, z_loss, ignore_index, temperature
 
+    @staticmethod
+    def rows(buffer, T, K):
+        """Addresses in the float32 buffer of log sum exp [T], state [T], the named logits [T, K], the count, the losses [T].
+        (Numbers, also where a jit trace has sizes of its own: it calls the Function again for other tensors.)"""
+        at = buffer.data_ptr()
+        return at, at + 4 * T, at + 8 * T, at + 4 * (2 + K) * T, at + 4 * (2 + K) * T + 4
+
     def forward(self, x, weight, classes, teacher):
         dev = L.require_device(x, weight, classes, teacher)
-        (D, V), shape = weight.shape, x.shape[:-1]
-        T = x.numel() // D
+        D, V = weight.shape
+        T, K = int(x.numel() // D), 1 if teacher is None else int(classes.shape[-1])
         x, weight, order = _dense(x, weight)
         classes = classes.contiguous()
         dt, wide = L.dtype_code(x.dtype), _index64("classes", classes)
-        # the results are tensors of their own, which a caller may change in place
-        loss = torch.empty(shape, dtype=torch.float32, device=dev)
-        rows = torch.empty((2, T), dtype=torch.float32, device=dev)  # log of the sum of exponentials, state
-        lse, state = rows.unbind(0)
-        total = count = None
-        if self.reduction != "none":
-            total, count = torch.empty((), dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
-        ends = (L.ptr(total), L.ptr(count))
+        # the result is a tensor of its own, which a caller may change in place
+        one = self.reduction != "none"
+        out = torch.empty(() if one else x.shape[:-1], dtype=torch.float32, device=dev)
+        buffer = torch.empty((2 + K + one) * T + 1, dtype=torch.float32, device=dev)
+        lse, state, chosen, count, loss = self.rows(buffer, T, K)
+        total = out.data_ptr() if one else None
+        if not one:
+            count, loss = None, out.data_ptr()
         mean = int(self.reduction == "mean")
         ws = L.workspace(L.query("mtx_head_loss_workspace_size", dt, T, D, V, order, 0), dev)
         kept = classes
         with L.on_device(dev):
             if teacher is None:
-                chosen = torch.empty(T, dtype=torch.float32, device=dev)
                 L.call("mtx_linear_cross_entropy", x.data_ptr(), weight.data_ptr(), classes.data_ptr(), wide, dt, T, D, V, order,
-                       self.ignore_index, self.z_loss, mean, loss.data_ptr(), lse.data_ptr(), state.data_ptr(), *ends,
-                       chosen.data_ptr(), ws.data_ptr(), ws.numel(), L.stream(dev))
+                       self.ignore_index, self.z_loss, mean, loss, lse, state, total, count, chosen, ws.data_ptr(), ws.numel(),
+                       L.stream(dev))
             else:
-                K = classes.shape[-1]
                 teacher = teacher.contiguous()
-                chosen = torch.empty((T, K), dtype=torch.float32, device=dev)
                 kept = L.workspace(L.query("mtx_distillation_entries_size", T, V, K), dev)
                 L.call("mtx_linear_distillation", x.data_ptr(), weight.data_ptr(), classes.data_ptr(), wide, teacher.data_ptr(),
-                       L.dtype_code(teacher.dtype), dt, T, D, V, K, order, self.temperature, mean, loss.data_ptr(),
-                       lse.data_ptr(), state.data_ptr(), *ends, chosen.data_ptr(), kept.data_ptr(), kept.numel(), ws.data_ptr(),
-                       ws.numel(), L.stream(dev))
-        return (loss if total is None else total), (x, weight, kept, rows, chosen, count)
+                       L.dtype_code(teacher.dtype), dt, T, D, V, K, order, self.temperature, mean, loss, lse, state, total, count,
+                       chosen, kept.data_ptr(), kept.numel(), ws.data_ptr(), ws.numel(), L.stream(dev))
+        return out, (x, weight, kept, buffer)
 
-    def backward(self, g, x, weight, kept, rows, chosen, count, K, need_x, need_w):
+    def backward(self, g, x, weight, kept, buffer, K, need_x, need_w):
         dev = L.require_device(g, x, weight)
         D, V = weight.shape
-        T = x.numel() // D
+        T = int(x.numel() // D)
         order = L.MTX_HEAD_DV if weight.is_contiguous() else L.MTX_HEAD_VD
         g = g.contiguous()
-        lse, state = rows.unbind(0)
+        lse, state, chosen, count, _ = self.rows(buffer, T, K or 1)
+        if self.reduction == "none":
+            count = None
         dt = L.dtype_code(x.dtype)
         dx = torch.empty_like(x) if need_x else None
         dw = (torch.empty_like(weight) if T else torch.zeros_like(weight)) if need_w else None  # with the weight's strides
         ws = L.workspace(L.query("mtx_head_loss_workspace_size", dt, T, D, V, order, 1), dev)
         with L.on_device(dev):
             if K is None:
-                L.call("mtx_linear_cross_entropy_bwd", g.data_ptr(), L.ptr(count), x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
-                       _index64("classes", kept), lse.data_ptr(), state.data_ptr(), chosen.data_ptr(), dt, T, D, V, order, self.z_loss, L.ptr(dx),
-                       L.ptr(dw), ws.data_ptr(), ws.numel(), L.stream(dev))
+                L.call("mtx_linear_cross_entropy_bwd", g.data_ptr(), count, x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
+                       _index64("classes", kept), lse, state, chosen, dt, T, D, V, order, self.z_loss, L.ptr(dx), L.ptr(dw),
+                       ws.data_ptr(), ws.numel(), L.stream(dev))
             else:
-                L.call("mtx_linear_distillation_bwd", g.data_ptr(), L.ptr(count), x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
-                       kept.numel(), lse.data_ptr(), state.data_ptr(), chosen.data_ptr(), dt, T, D, V, K, order, self.temperature,
-                       L.ptr(dx),
-                       L.ptr(dw), ws.data_ptr(), ws.numel(), L.stream(dev))
+                L.call("mtx_linear_distillation_bwd", g.data_ptr(), count, x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
+                       kept.numel(), lse, state, chosen, dt, T, D, V, K, order, self.temperature, L.ptr(dx), L.ptr(dw),
+                       ws.data_ptr(), ws.numel(), L.stream(dev))
         return dx, dw
 
 
@@ -132,7 +136,7 @@ class _HeadLoss(torch.autograd.Function):
     def forward(ctx, x, weight, classes, teacher, how):
         out, saved = how.forward(x, weight, classes, teacher)
         ctx.save_for_backward(*saved)
-        ctx.how, ctx.K = how, None if teacher is None else classes.shape[-1]
+        ctx.how, ctx.K = how, None if teacher is None else int(classes.shape[-1])
         return out
 
     @staticmethod
