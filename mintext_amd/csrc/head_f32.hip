@@ -71,7 +71,8 @@ __global__ __launch_bounds__(NT) void logits_f32_kernel(Logits p) {
     }
   } else {
     if (!live) return;
-    const float a = p.a[r], l2 = p.l2[r];
+    float l2;
+    const float a = p.f.a(r, p.f.b(r), l2);
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = a == 0.0f || e >= left ? 0.0f : a * exp2f(__builtin_fmaf(v[e], p.scale, -l2));
     float* dz = (float*)p.dz + (int64_t)row * p.ldz + c0;
@@ -100,6 +101,7 @@ __global__ __launch_bounds__(NT) void product_f32_kernel(Product p) {
   const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) >> 1, wn = (threadIdx.x >> 6) & 1;
   const int64_t n = n0 + wn * 32 + (lane & 31);
   if (n >= p.cols) return;
+  const float alpha = p.f.alpha();
 #pragma unroll
   for (int v = 0; v < 16; ++v) {
     const int64_t r = m0 + wm * 32 + 8 * (v / 4) + 4 * (lane >> 5) + v % 4;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(NT) void product_f32_kernel(Product p) {
         continue;
       }
     }
-    ((float*)p.out)[r * p.ldo + n] = p.alpha ? y * *p.alpha : y;
+    ((float*)p.out)[r * p.ldo + n] = y * alpha;
   }
 }
 

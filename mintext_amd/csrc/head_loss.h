@@ -34,6 +34,24 @@ __device__ __forceinline__ int64_t target(const Entries& e, int64_t row) {
   return e.wide ? ((const int64_t*)e.targets)[row] : ((const int32_t*)e.targets)[row];
 }
 
+// A row's factors in the backward pass, dz = a softmax - b share, and the one of all rows that is left to the products' results.
+struct Factors {
+  const float *g, *count;    // the gradient of the one loss and what its sum was divided by; or of each row's, and nullptr
+  const float *lse, *state;  // [T]
+  float unit, z_loss;
+  __device__ __forceinline__ float b(int64_t row) const {
+    const float s = state[row];
+    return s == 0.0f ? 0.0f : count ? s : s * unit * g[row];
+  }
+  // `l2`: log2 of sum exp(z / tau)
+  __device__ __forceinline__ float a(int64_t row, float b, float& l2) const {
+    const float l = lse[row];
+    l2 = l * 1.4426950408889634f;
+    return b == 0.0f ? 0.0f : b * (1.0f + 2.0f * z_loss * l);
+  }
+  __device__ __forceinline__ float alpha() const { return count ? unit * (g[0] / *count) : 1.0f; }
+};
+
 struct Logits {
   const void *x, *w;  // w: at column v0
   int64_t ldx, ldw;
@@ -46,7 +64,7 @@ struct Logits {
   float2* part;         // [block][T]: maximum of z, sum of exp2((z - maximum) scale)
   float* chosen;        // [T][K]: z of the entries
   // backward
-  const float *a, *l2;  // [T]: factor of the softmax; log2 of sum exp(z / tau)
+  Factors f;
   void* dz;             // [T][ldz], zeros behind the piece's columns
   int64_t ldz;
 };
@@ -64,14 +82,16 @@ struct Product {
   int64_t ldacc;
   int add;                       // acc holds sums of earlier calls
   int last;                      // pieces == 1: the result goes to out
-  const float* alpha;            // factor of the result, or nullptr
+  Factors f;                     // of which alpha
+  int group;                     // rows of tiles that go together
 };
 
 int launch_logits(const Logits& p, bool dz, int order, int path, hipStream_t st);  // bf16
-int launch_product(const Product& p, bool a_cols, bool b_cols, bool small, hipStream_t st);
+int launch_product(const Product& p, bool a_cols, bool b_cols, int size, hipStream_t st);
 int launch_logits_f32(const Logits& p, bool dz, int order, hipStream_t st);
 int launch_product_f32(const Product& p, bool a_cols, bool b_cols, hipStream_t st);
 
+enum { SIZE_BIG, SIZE_SMALL };  // tiles of launch_product: 256 x 256, 128 x 128
 // tiles of the logits: 256 x 256, 128 x 128, 64 x 128 (few rows); f32 64 x 64
 enum { PATH_BIG, PATH_SMALL, PATH_THIN, PATH_F32 };
 inline int tile_rows(int path) { return path == PATH_BIG ? 256 : path == PATH_SMALL ? 128 : 64; }

@@ -16,7 +16,7 @@ namespace mtx {
 namespace head {
 
 constexpr int kMaxEntries = 1024;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- a teacher's entries: shares, in the order of their classes ------------------------------------------------
 // A wave takes a row.  The place of an entry is the number of those before it (K^2 comparisons in LDS: 0.1 ms for 8192
@@ -239,26 +239,13 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* loss, const fl
   *count = (float)n;
 }
 
-// ---- backward: a row's factors ----------------------------------------------------------------------------------
-// b of the shares and a of the softmax; `count`: the factor that all rows share goes to *alpha, else it is in them
-__global__ __launch_bounds__(256) void factors_kernel(const float* g, const float* count, const float* lse, const float* state,
-                                                      int64_t T, float unit, float z_loss, float* a, float* b, float* l2,
-                                                      float* alpha) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t == 0) *alpha = count ? unit * (g[0] / *count) : 1.0f;
-  if (t >= T) return;
-  const float st = state[t], l = lse[t];
-  const float w = st == 0.0f ? 0.0f : count ? st : st * unit * g[t];
-  b[t] = w;
-  a[t] = w == 0.0f ? 0.0f : w * (1.0f + 2.0f * z_loss * l);
-  l2[t] = l * kLog2e;
-}
-
+// ---- backward -----------------------------------------------------------------------------------------------------
 // dz of the entries among columns v0 .. v0 + cols, from their logits: a softmax - b (the shares of one class), in the place
 // of what the tile left there.  A thread an entry; the first of several of one class takes them all.
 struct Named {
   Entries e;
-  const float *chosen, *a, *b, *l2;
+  Factors f;
+  const float* chosen;
   float scale;
   int64_t T;
   int v0, cols;
@@ -270,7 +257,7 @@ __global__ __launch_bounds__(256) void named_kernel(Named p) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= p.T * p.e.K) return;
   const int64_t t = at / p.e.K;
-  const float a = p.a[t], b = p.b[t];
+  const float b = p.f.b(t);
   if (b == 0.0f) return;
   int64_t c;
   float share = 1.0f;
@@ -285,7 +272,8 @@ __global__ __launch_bounds__(256) void named_kernel(Named p) {
   if (c < 0 || c >= p.cols) return;
   if (!p.e.targets)
     for (int64_t k = at + 1; k < (t + 1) * p.e.K && p.e.idx[k] == c + p.v0; ++k) share += p.e.share[k];
-  const float v = a * exp2f(__builtin_fmaf(p.chosen[at], p.scale, -p.l2[t])) - b * share;
+  float l2;
+  const float a = p.f.a(t, b, l2), v = a * exp2f(__builtin_fmaf(p.chosen[at], p.scale, -l2)) - b * share;
   if (p.f32) ((float*)p.dz)[t * p.ldz + c] = v;
   else ((uint16_t*)p.dz)[t * p.ldz + c] = f32_to_bf16(v);
 }
@@ -357,8 +345,8 @@ __global__ __launch_bounds__(256) void unpad_kernel(const uint16_t* __restrict__
 template <typename T, int V>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc, int pieces, int64_t rows, int64_t cols,
                                                    int64_t ldacc, T* __restrict__ out, int64_t ldo,
-                                                   const float* __restrict__ alpha) {
-  const float f = *alpha;
+                                                   Factors factors) {
+  const float f = factors.alpha();
   const int64_t per = (cols + V - 1) / V, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * per) return;
   const int64_t r = i / per, c = i % per * V, at = r * ldacc + c, n = rows * ldacc;
@@ -384,17 +372,18 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc
 // ---- how a call runs, by its sizes alone --------------------------------------------------------------------------
 constexpr int64_t kPiece = (int64_t)1 << 30;  // bytes of dz held at a time, at most
 constexpr int64_t kCopy = (int64_t)256 << 20;  // bytes of a padded copy of the weight's columns held at a time, at most
+constexpr int kTurn = 64;  // elements more than a piece in a row of dz, so that rows are no power of two apart in memory
 constexpr int kMostPieces = 16;
 
 struct Split {
-  bool small;  // bf16: tiles of 128 x 128, else of 256 x 256
+  int size;  // bf16: of the tiles
   int pieces;
 };
 // A product's tiles and pieces by an estimate of its time in us: rounds of the chip by what a stage of 32 takes, and what the
 // pieces' sums take to write, read and join.
 static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
   const int64_t stages = ceil_div(red, 32);
-  Split best{false, 1};
+  Split best{SIZE_BIG, 1};
   double least = 1e30;
   for (int kind = 0; kind < (f32 ? 1 : 2); ++kind) {
     const int64_t side = f32 ? 64 : kind ? 128 : 256, slots = f32 ? 512 : kind ? 512 : 256;
@@ -406,7 +395,7 @@ static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
                        (s > 1 ? s * rows * cols * 8 / 4e6 + 6.0 : 0.0);
       if (t < least) {
         least = t;
-        best = {kind == 1, s};
+        best = {kind, s};
       }
     }
   }
@@ -423,7 +412,7 @@ struct Plan {
   Split dx, dw;
   int64_t ld_dx, ld_dw, rows_dw;
   // bytes from the workspace's start
-  int64_t x, w, part, factors, dz, acc_dx, acc_dw, total;
+  int64_t x, w, part, dz, acc_dx, acc_dw, total;
 };
 static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool backward) {
   Plan p{};
@@ -438,7 +427,7 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
   p.red = !p.copy_x ? D : round_up(D, order == ORDER_VD ? 32 : 8);
   int64_t most = all;
   if (p.copy_w) most = std::min(most, std::max<int64_t>(kCopy / (p.ldx * 2) / 256 * 256, 256));
-  if (backward) most = std::min(most, std::max<int64_t>(kPiece / (T * size) / 256 * 256, 256));
+  if (backward) most = std::min(most, std::max<int64_t>((kPiece / (T * size) - kTurn) / 256 * 256, 256));
   p.piece = round_up(ceil_div(V, ceil_div(all, most)), 256);
   const int64_t big = ceil_div(T, 256) * ceil_div(p.piece, 256);
   p.path = p.f32 ? PATH_F32 : T <= 64 ? PATH_THIN : big >= 192 ? PATH_BIG : PATH_SMALL;
@@ -453,8 +442,7 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
   if (!backward) {
     p.part = take(round_up(V, tile_cols(p.path)) / block_cols(p.path) * T * 8);
   } else {
-    p.factors = take((3 * T + 1) * 4);
-    p.dz = take(T * p.piece * size);
+    p.dz = take(T * (p.piece + kTurn) * size);
     p.dx = split(p.f32, T, D, std::min(p.piece, V));
     p.ld_dx = round_up(D, 8);
     p.acc_dx = take(p.dx.pieces > 1 || p.piece < V ? p.dx.pieces * T * p.ld_dx * 4 : 0);
@@ -511,13 +499,13 @@ static int logits(const Plan& p, const Logits& a, bool dz, hipStream_t st) {
   return p.f32 ? launch_logits_f32(a, dz, p.order, st) : launch_logits(a, dz, p.order, p.path, st);
 }
 static int product(const Plan& p, const Product& a, bool a_cols, bool b_cols, const Split& s, hipStream_t st) {
-  return p.f32 ? launch_product_f32(a, a_cols, b_cols, st) : launch_product(a, a_cols, b_cols, s.small, st);
+  return p.f32 ? launch_product_f32(a, a_cols, b_cols, st) : launch_product(a, a_cols, b_cols, s.size, st);
 }
 static int join(bool f32, const float* acc, int pieces, int64_t rows, int64_t cols, int64_t ldacc, void* out, int64_t ldo,
-                const float* alpha, hipStream_t st) {
+                const Factors& f, hipStream_t st) {
   const bool vec = cols % 8 == 0 && ldo % 8 == 0 && aligned16(out);
   const dim3 grid((unsigned)ceil_div(rows * (vec ? cols / 8 : cols), 256));
-#define MTX_JOIN(T, V) hipLaunchKernelGGL((join_kernel<T, V>), grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (T*)out, ldo, alpha)
+#define MTX_JOIN(T, V) hipLaunchKernelGGL((join_kernel<T, V>), grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (T*)out, ldo, f)
   if (f32) {
     if (vec) MTX_JOIN(float, 8);
     else MTX_JOIN(float, 1);
@@ -553,27 +541,22 @@ static int forward(const Plan& p, const void* x, const void* w, Merge m, float* 
   return check_launch();
 }
 
-static int backward(const Plan& p, const float* g, const float* count, const void* x, const void* w, const float* lse,
-                    const float* state, const float* chosen, const Entries& e, float scale, float unit, float z_loss, void* dx, void* dw, char* ws,
-                    hipStream_t st) {
+static int backward(const Plan& p, const Factors& f, const void* x, const void* w, const float* chosen, const Entries& e,
+                    float scale, void* dx, void* dw, char* ws, hipStream_t st) {
   const int64_t size = p.f32 ? 4 : 2;
   const bool dv = p.order == ORDER_DV;
-  float* f = (float*)(ws + p.factors);
-  hipLaunchKernelGGL(factors_kernel, dim3((unsigned)ceil_div(p.T, 256)), dim3(256), 0, st, g, count, lse, state, p.T, unit, z_loss,
-                     f, f + p.T, f + 2 * p.T, f + 3 * p.T);
-  int rc = check_launch();
+  int rc = MTX_OK;
   Logits a{};
+  a.f = f;
   a.e = e;
   a.scale = scale;
-  a.a = f, a.l2 = f + 2 * p.T;
-  const float* alpha = f + 3 * p.T;
   a.dz = ws + p.dz;
-  a.ldz = p.piece;
+  a.ldz = p.piece + kTurn;
   for (int64_t v0 = 0; v0 < p.V && rc == MTX_OK; v0 += p.piece) {
     rc = operands(p, x, w, v0, ws, a, st);
     if (rc == MTX_OK) rc = logits(p, a, true, st);
     if (rc != MTX_OK) return rc;
-    const Named named{e, chosen, f, f + p.T, f + 2 * p.T, scale, p.T, a.v0, a.cols, a.dz, a.ldz, p.f32};
+    const Named named{e, f, chosen, scale, p.T, a.v0, a.cols, a.dz, a.ldz, p.f32};
     hipLaunchKernelGGL(named_kernel, dim3((unsigned)ceil_div(p.T * e.K, 256)), dim3(256), 0, st, named);
     if (dx) {
       const int red = p.f32 ? a.cols : (int)round_up(a.cols, 8);  // dz holds zeros behind its columns
@@ -581,11 +564,11 @@ static int backward(const Plan& p, const float* g, const float* count, const voi
       // the last piece of the vocabulary may be shorter than what the split was made for
       const int pieces = (int)std::min<int64_t>(p.dx.pieces, ceil_div(red, 32));
       Product q{a.dz, a.w, a.ldz, a.ldw, (int)p.T, (int)p.D, red, 0, (int)p.T, (int)(dv ? p.D : p.ldx), dx, p.D, pieces, nullptr,
-                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final, alpha};
+                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final, f, 8};
       if (!dv) q.missing = red - a.cols;
       if (!(only && p.dx.pieces == 1)) q.acc = (float*)(ws + p.acc_dx);
       rc = product(p, q, false, !dv, p.dx, st);
-      if (rc == MTX_OK && final && p.dx.pieces > 1) rc = join(p.f32, q.acc, p.dx.pieces, p.T, p.D, p.ld_dx, dx, p.D, alpha, st);
+      if (rc == MTX_OK && final && p.dx.pieces > 1) rc = join(p.f32, q.acc, p.dx.pieces, p.T, p.D, p.ld_dx, dx, p.D, f, st);
       if (rc != MTX_OK) return rc;
     }
     if (dw && rc == MTX_OK) {
@@ -600,10 +583,11 @@ static int backward(const Plan& p, const float* g, const float* count, const voi
       if (p.copy_w) q.cols = (int)round_up(cols, 8);  // whole chunks; what lies behind the columns is not taken
       q.ldacc = p.ld_dw;
       q.last = p.dw.pieces == 1;
-      q.alpha = alpha;
+      q.f = f;
+      q.group = p.T <= 256 ? 1 : 8;
       if (p.dw.pieces > 1) q.acc = (float*)(ws + p.acc_dw);
       rc = product(p, q, true, true, p.dw, st);
-      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, rows, q.cols, p.ld_dw, to, ldt, alpha, st);
+      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, rows, q.cols, p.ld_dw, to, ldt, f, st);
       if (rc == MTX_OK && p.copy_w) {
         hipLaunchKernelGGL(unpad_kernel, dim3((unsigned)ceil_div(rows * (cols / 8 + 2), 256)), dim3(256), 0, st, (const uint16_t*)to,
                            ldt, rows, cols, (uint16_t*)out, ldo);
@@ -683,7 +667,8 @@ extern "C" int mtx_linear_cross_entropy_bwd(const float* g, const float* count, 
   const Plan p = plan(dtype, T, D, V, order, true);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
   const Entries e{targets, targets_64, nullptr, nullptr, nullptr, 0, 1};
-  return backward(p, g, count, x, w, lse, state, chosen, e, kLog2e, 1.0f, z_loss, dx, dw, (char*)workspace, (hipStream_t)stream);
+  return backward(p, Factors{g, count, lse, state, 1.0f, z_loss}, x, w, chosen, e, kLog2e, dx, dw, (char*)workspace,
+                  (hipStream_t)stream);
 }
 
 extern "C" int mtx_linear_distillation(const void* x, const void* w, const void* teacher_idx, int idx_64,
@@ -740,6 +725,7 @@ extern "C" int mtx_linear_distillation_bwd(const float* g, const float* count, c
   const Saved s = saved(T, V, K);
   if (!aligned16(entries_buffer) || entries_bytes < s.total) return MTX_ERR_WORKSPACE;
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
-  return backward(p, g, count, x, w, lse, state, chosen, entries((char*)const_cast<void*>(entries_buffer), s, K), kLog2e / temperature,
-                  temperature, 0.0f, dx, dw, (char*)workspace, (hipStream_t)stream);
+  return backward(p, Factors{g, count, lse, state, temperature, 0.0f}, x, w, chosen,
+                  entries((char*)const_cast<void*>(entries_buffer), s, K), kLog2e / temperature, dx, dw, (char*)workspace,
+                  (hipStream_t)stream);
 }

@@ -14,9 +14,9 @@ template <bool VD, bool TAIL> using Thin = dense::Tile<dense::Bf16, 1, 2, 2, 2, 
 // Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2.
 constexpr int kGroup = 8;
 template <class T>
-__device__ __forceinline__ void tile_at(int t, int nm, int nn, int& m0, int& n0) {
-  const int g = t / (kGroup * nn), gs = min(kGroup, nm - g * kGroup), in = t - g * kGroup * nn;
-  m0 = (g * kGroup + in % gs) * T::BM;
+__device__ __forceinline__ void tile_at(int t, int nm, int nn, int group, int& m0, int& n0) {
+  const int g = t / (group * nn), gs = min(group, nm - g * group), in = t - g * group * nn;
+  m0 = (g * group + in % gs) * T::BM;
   n0 = in / gs * T::BN;
 }
 // where the way out of a wave (Tile::put) keeps column c of row r
@@ -109,8 +109,8 @@ __device__ __forceinline__ void gradient_out(const Logits& p, dense::f32x16 (&ac
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
     const int row = min(wr + i * 32 + r, p.T - 1);
-    a[i] = p.a[row];
-    off[i] = -p.l2[row];
+    a[i] = p.f.a(row, p.f.b(row), off[i]);
+    off[i] = -off[i];
   }
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) care |= a[i] == 0.0f;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logit
   const int t = dense::tile_of(blockIdx.x, nm * nn);
   if (t < 0) return;
   int m0, n0;
-  tile_at<T>(t, nm, nn, m0, n0);
+  tile_at<T>(t, nm, nn, kGroup, m0, n0);
   const uint16_t *x = (const uint16_t*)p.x + (int64_t)m0 * p.ldx, *w = (const uint16_t*)p.w;
   w += T::b_cols ? (int64_t)n0 : (int64_t)n0 * p.ldw;
   const Operand ox{{x, x}, p.ldx, p.T - m0}, ow{{w, w}, p.ldw, p.w_left - n0, p.missing};
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   const int k0 = (int)((int64_t)piece * stages / p.pieces) * dense::BKS;
   const int k1 = min((int)((int64_t)(piece + 1) * stages / p.pieces) * dense::BKS, p.red);
   int m0, n0;
-  tile_at<T>(t, nm, nn, m0, n0);
+  tile_at<T>(t, nm, nn, p.group, m0, n0);
   const uint16_t *a = (const uint16_t*)p.a, *b = (const uint16_t*)p.b;
   a += T::cols ? (int64_t)k0 * p.lda + m0 : (int64_t)m0 * p.lda + k0;
   b += T::b_cols ? (int64_t)k0 * p.ldb + n0 : (int64_t)n0 * p.ldb + k0;
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   char* mine = T::out_lds(lds);
   const int wr = m0 + (wave / T::WN) * (T::TM * 32), c0 = n0 + (wave % T::WN) * (T::TN * 32);
   float* sums = p.acc ? p.acc + (int64_t)piece * p.rows * p.ldacc : nullptr;
-  const float alpha = p.alpha && (!sums || p.last) ? *p.alpha : 1.0f;
+  const float alpha = p.f.alpha();
   const bool whole = p.ldo % 8 == 0 && p.cols % 8 == 0 && (uintptr_t)p.out % 16 == 0;
   if (sums) {
 #pragma unroll
@@ -280,15 +280,15 @@ static int go_product(const Product& p, hipStream_t st) {
   return check_launch();
 }
 template <bool A_COLS, bool B_COLS, bool TAIL>
-static int go_size(const Product& p, bool small, hipStream_t st) {
-  return small ? go_product<GradSmall<A_COLS, B_COLS, TAIL>>(p, st) : go_product<GradBig<A_COLS, B_COLS, TAIL>>(p, st);
+static int go_size(const Product& p, int size, hipStream_t st) {
+  return size == SIZE_BIG ? go_product<GradBig<A_COLS, B_COLS, TAIL>>(p, st) : go_product<GradSmall<A_COLS, B_COLS, TAIL>>(p, st);
 }
 // A dz [T][piece] or x^T, B W^T in either order or dz: (rows, rows), (rows, cols) and (cols, cols)
-int launch_product(const Product& p, bool a_cols, bool b_cols, bool small, hipStream_t st) {
+int launch_product(const Product& p, bool a_cols, bool b_cols, int size, hipStream_t st) {
   const bool tail = p.red % dense::BKS != 0 || p.missing > 0;
-  if (a_cols) return tail ? go_size<true, true, true>(p, small, st) : go_size<true, true, false>(p, small, st);
-  if (b_cols) return tail ? go_size<false, true, true>(p, small, st) : go_size<false, true, false>(p, small, st);
-  return tail ? go_size<false, false, true>(p, small, st) : go_size<false, false, false>(p, small, st);
+  if (a_cols) return tail ? go_size<true, true, true>(p, size, st) : go_size<true, true, false>(p, size, st);
+  if (b_cols) return tail ? go_size<false, true, true>(p, size, st) : go_size<false, true, false>(p, size, st);
+  return tail ? go_size<false, false, true>(p, size, st) : go_size<false, false, false>(p, size, st);
 }
 
 }  // namespace head
