@@ -173,6 +173,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets must be {tuple(x.shape[:-1])}, got {tuple(targets.shape)}")
     _index64("targets", targets)
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError(f"ignore_index must fit 64 bits, got {ignore_index}")
     if not 0.0 <= z_loss < math.inf:
         raise ValueError(f"z_loss must be finite and not negative, got {z_loss}")
     return _loss(x, weight, targets, None, _Loss(reduction, z_loss=z_loss, ignore_index=int(ignore_index)))

@@ -295,6 +295,35 @@ def test_rows_without_a_class(dev, dtype):
     assert torch.isnan(bad).tolist() == [True, False, False, False, False, False]
 
 
+@pytest.mark.parametrize("tau", [0.5, 1.0, 4.0])
+@pytest.mark.parametrize("tdtype", [F32, BF])
+def test_teacher_logits_of_the_lowest_value(dev, tau, tdtype):
+    """They are left out beside others, as their share is 0, and alone are all alike."""
+    from mintext_amd.kernels import linear_distillation
+
+    x, w, g = operands(dev, 3, 40, 300, F32, "dv")
+    low = torch.finfo(tdtype).min
+    idx = torch.tensor([[5, 9, 77, 250], [1, 2, 3, 4], [8, 299, 0, -1]], device=dev)
+    t = torch.tensor([[low] * 4, [low, 2.0, low, 1.0], [low] * 4], device=dev).to(tdtype)
+    same = torch.tensor([[0.0] * 4, [-float("inf"), 2.0, -float("inf"), 1.0], [0.0] * 4], device=dev)
+    a = linear_distillation(x, w, idx, t, temperature=tau, reduction="none")
+    assert torch.isfinite(a).all() and torch.equal(a, linear_distillation(x, w, idx, same, temperature=tau, reduction="none"))
+
+
+def test_backward_twice(dev):
+    from mintext_amd.kernels import linear_cross_entropy, linear_distillation
+
+    x, w, g = operands(dev, 70, 64, 500, BF, "vd")
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = torch.randint(0, 500, (70,), device=dev, generator=g)
+    idx, t = teacher(dev, 70, 500, 9, g)
+    for loss in (linear_cross_entropy(x, w, y), linear_distillation(x, w, idx, t)):
+        first = torch.autograd.grad(loss, [x, w], retain_graph=True)
+        half = torch.autograd.grad(loss / 2, [x, w], retain_graph=True)
+        again = torch.autograd.grad(loss, [x, w])
+        assert all(torch.equal(a, b) and torch.equal(a, 2 * c) for a, b, c in zip(first, again, half))
+
+
 def test_one_entry_is_cross_entropy(dev):
     from mintext_amd.kernels import linear_cross_entropy, linear_distillation
 

@@ -192,6 +192,21 @@ def test_only_what_is_asked_for(dev):
         torch.autograd.grad(gx.sum(), [leaves[0]])
 
 
+def test_a_tensor_beside_itself(dev):
+    """x as its own residual gets both gradients; a weight used twice the sum of its two."""
+    x, _, w, b, dy, dh = inputs(dev, 20, 72, F32, F32, True, True)
+    other = x.detach().clone().requires_grad_(True)
+    x.requires_grad_(True), w.requires_grad_(True)
+    (gx,) = torch.autograd.grad(list(call(x, x, w, b, False, 1e-5)), [x], [dy, dh])
+    parts = torch.autograd.grad(list(call(x, other, w, b, False, 1e-5)), [x, other], [dy, dh])
+    assert torch.equal(gx, parts[0] + parts[1])
+    y1, y2 = call(x, None, w, b, False, 1e-5), call(dh, None, w, b, False, 1e-5)
+    (gw,) = torch.autograd.grad([y1, y2], [w], [dy, dy], retain_graph=True)
+    (g1,) = torch.autograd.grad(y1, [w], dy)
+    (g2,) = torch.autograd.grad(y2, [w], dy)
+    assert torch.equal(gw, g1 + g2)
+
+
 @pytest.mark.parametrize("rms", [False, True])
 def test_gradient_against_differences(dev, rms):
     """The slope along a random direction, of the formula in 64 bits: a step of 1e-5 leaves 1e-10 of third derivatives (values

@@ -30,6 +30,7 @@ def i(*shape, dtype=torch.int64):
     ((z(4, 8), z(8, 16), i(4)), dict(reduction="batchmean"), ValueError),
     ((z(4, 8), z(8, 16), i(4)), dict(z_loss=-1e-4), ValueError),
     ((z(4, 8), z(8, 16), i(4)), dict(z_loss=float("nan")), ValueError),
+    ((z(4, 8), z(8, 16), i(4)), dict(ignore_index=1 << 63), ValueError),
     ((z(4, 8), z(8, 16, dtype=F32), i(4)), {}, TypeError),                   # mixed types
     ((z(4, 8, dtype=torch.float16), z(8, 16, dtype=torch.float16), i(4)), {}, TypeError),
     ((z(4, 8), z(8, 16), z(4, dtype=F32)), {}, TypeError),                   # targets that are no integers
