@@ -8,7 +8,6 @@
 //
 // A row's state is 1, 0 (left out: the ignored class, no entry; its loss is 0 and its gradient too) or NaN (a class
 // that is none), which its loss and its gradient become.
-#include "f32_tile.h"
 #include "head_loss.h"
 #include <algorithm>
 
@@ -323,63 +322,25 @@ __global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ i
   *(v4u32*)(out + i) = o;
 }
 
-// The way back: rows of `ld` elements to rows of any length.  A thread writes what lies between two 16-byte boundaries of `out`
-// (at a row's ends the part of it that is the row's), from the words that hold it.  The gradient of a weight of 704 x 50257
-// written by the tiles themselves, element by element: 199 us instead of 115 and 25.
-__global__ __launch_bounds__(256) void unpad_kernel(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols,
-                                                    uint16_t* __restrict__ out, int64_t ldo) {
-  struct __attribute__((aligned(4))) Words {
-    uint32_t v[4];
-  };
-  const int64_t per = cols / 8 + 2, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * per) return;
-  const int64_t r = i / per;
-  uint16_t* row = out + r * ldo;
-  const int head = (int)((16 - (uintptr_t)row % 16) % 16 / 2);  // columns before the first boundary
-  const int64_t c = head + (i - r * per - 1) * 8;
-  if (c >= cols || c + 8 <= 0) return;
-  const uint16_t* from = in + r * ld;
-  if (c >= 0 && c + 8 <= cols) {
-    const uint32_t* p = (const uint32_t*)from + (c >> 1);
-    const Words w = *(const Words*)p;
-    const uint32_t odd = (c & 1) * 16, next = odd ? p[4] : 0u;  // odd: column c + 8 or zeros behind the last one
-    v4u32 o;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = __builtin_amdgcn_alignbit(q < 3 ? w.v[q < 3 ? q + 1 : 3] : next, w.v[q], odd);
-    *(v4u32*)(row + c) = o;
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (c + q >= 0 && c + q < cols) row[c + q] = from[c + q];
-  }
-}
-
-// out = the pieces' sums, in order.  V columns a thread.
-template <typename T, int V>
+// out = the pieces' sums, in order.  Eight columns a thread; rows of acc are whole eights.
+template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc, int pieces, int64_t rows, int64_t cols,
-                                                   int64_t ldacc, T* __restrict__ out, int64_t ldo,
-                                                   Factors factors) {
+                                                   int64_t ldacc, T* __restrict__ out, int64_t ldo, Factors factors) {
   const float f = factors.alpha();
-  const int64_t per = (cols + V - 1) / V, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t per = (cols + 7) / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * per) return;
-  const int64_t r = i / per, c = i % per * V, at = r * ldacc + c, n = rows * ldacc;
-  if constexpr (V == 8) {
-    float v[8];
-    ld8(acc, at, v);
-    for (int s = 1; s < pieces; ++s) {
-      float o[8];
-      ld8(acc + s * n, at, o);
+  const int64_t r = i / per, c = i % per * 8, at = r * ldacc + c, n = rows * ldacc;
+  float v[8];
+  ld8(acc, at, v);
+  for (int s = 1; s < pieces; ++s) {
+    float o[8];
+    ld8(acc + s * n, at, o);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] += o[q];
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] *= f;
-    st8(out, r * ldo + c, v);
-  } else {
-    float v = acc[at];
-    for (int s = 1; s < pieces; ++s) v += acc[s * n + at];
-    gst<T>(out, r * ldo + c, v * f);
+    for (int q = 0; q < 8; ++q) v[q] += o[q];
   }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] *= f;
+  store_part(out + r * ldo + c, v, (int)min(cols - c, (int64_t)8));
 }
 
 // ---- how a call runs, by its sizes alone --------------------------------------------------------------------------
@@ -516,17 +477,9 @@ static int product(const Plan& p, const Product& a, bool a_cols, bool b_cols, co
 }
 static int join(bool f32, const float* acc, int pieces, int64_t rows, int64_t cols, int64_t ldacc, void* out, int64_t ldo,
                 const Factors& f, hipStream_t st) {
-  const bool vec = cols % 8 == 0 && ldo % 8 == 0 && aligned16(out);
-  const dim3 grid((unsigned)ceil_div(rows * (vec ? cols / 8 : cols), 256));
-#define MTX_JOIN(T, V) hipLaunchKernelGGL((join_kernel<T, V>), grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (T*)out, ldo, f)
-  if (f32) {
-    if (vec) MTX_JOIN(float, 8);
-    else MTX_JOIN(float, 1);
-  } else {
-    if (vec) MTX_JOIN(uint16_t, 8);
-    else MTX_JOIN(uint16_t, 1);
-  }
-#undef MTX_JOIN
+  const dim3 grid((unsigned)ceil_div(rows * ceil_div(cols, 8), 256));
+  if (f32) hipLaunchKernelGGL(join_kernel<float>, grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (float*)out, ldo, f);
+  else hipLaunchKernelGGL(join_kernel<uint16_t>, grid, dim3(256), 0, st, acc, pieces, rows, cols, ldacc, (uint16_t*)out, ldo, f);
   return check_launch();
 }
 
@@ -577,7 +530,7 @@ static int backward(const Plan& p, const Factors& f, const void* x, const void* 
       // the last piece of the vocabulary may be shorter than what the split was made for
       const int pieces = (int)std::min<int64_t>(p.dx.pieces, ceil_div(red, 32));
       Product q{a.dz, a.w, a.ldz, a.ldw, (int)p.T, (int)p.D, red, 0, (int)p.T, (int)(dv ? p.D : p.ldx), dx, p.D, pieces, nullptr,
-                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final, f, 8};
+                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final, f};
       if (!dv) q.missing = red - a.cols;
       if (!(only && p.dx.pieces == 1)) q.acc = (float*)(ws + p.acc_dx);
       rc = product(p, q, false, !dv, p.dx, st);
@@ -585,27 +538,17 @@ static int backward(const Plan& p, const Factors& f, const void* x, const void* 
       if (rc != MTX_OK) return rc;
     }
     if (dw && rc == MTX_OK) {
-      // where the weight's rows are no whole chunks, the product goes to the place of their copy, which is done with
       void* out = (char*)dw + (dv ? v0 : v0 * p.D) * size;
-      void* to = p.copy_w ? ws + p.w : out;
-      const int64_t ldo = dv ? p.V : p.D, ldt = p.copy_w ? a.ldw : ldo;
+      const int64_t ldo = dv ? p.V : p.D;
       Product q{};
-      if (dv) q = Product{a.x, a.dz, a.ldx, a.ldz, (int)p.D, a.cols, (int)p.T, 0, (int)p.ldx, (int)p.piece, to, ldt, p.dw.pieces};
-      else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, (int)p.T, 0, (int)p.piece, (int)p.ldx, to, ldt, p.dw.pieces};
-      const int64_t rows = q.rows, cols = q.cols;
-      if (p.copy_w) q.cols = (int)round_up(cols, 8);  // whole chunks; what lies behind the columns is not taken
+      if (dv) q = Product{a.x, a.dz, a.ldx, a.ldz, (int)p.D, a.cols, (int)p.T, 0, (int)p.ldx, (int)p.piece, out, ldo, p.dw.pieces};
+      else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, (int)p.T, 0, (int)p.piece, (int)p.ldx, out, ldo, p.dw.pieces};
       q.ldacc = p.ld_dw;
       q.last = p.dw.pieces == 1;
       q.f = f;
-      q.group = p.T <= 256 ? 1 : 8;
       if (p.dw.pieces > 1) q.acc = (float*)(ws + p.acc_dw);
       rc = product(p, q, true, true, p.dw, st);
-      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, rows, q.cols, p.ld_dw, to, ldt, f, st);
-      if (rc == MTX_OK && p.copy_w) {
-        hipLaunchKernelGGL(unpad_kernel, dim3((unsigned)ceil_div(rows * (cols / 8 + 2), 256)), dim3(256), 0, st, (const uint16_t*)to,
-                           ldt, rows, cols, (uint16_t*)out, ldo);
-        rc = check_launch();
-      }
+      if (rc == MTX_OK && p.dw.pieces > 1) rc = join(p.f32, q.acc, p.dw.pieces, q.rows, q.cols, p.ld_dw, out, ldo, f, st);
     }
   }
   return rc;

@@ -14,9 +14,9 @@ template <bool VD, bool TAIL> using Thin = dense::Tile<dense::Bf16, 1, 2, 2, 2, 
 // Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2.
 constexpr int kGroup = 8;
 template <class T>
-__device__ __forceinline__ void tile_at(int t, int nm, int nn, int group, int& m0, int& n0) {
-  const int g = t / (group * nn), gs = min(group, nm - g * group), in = t - g * group * nn;
-  m0 = (g * group + in % gs) * T::BM;
+__device__ __forceinline__ void tile_at(int t, int nm, int nn, int& m0, int& n0) {
+  const int g = t / (kGroup * nn), gs = min(kGroup, nm - g * kGroup), in = t - g * kGroup * nn;
+  m0 = (g * kGroup + in % gs) * T::BM;
   n0 = in / gs * T::BN;
 }
 // where the way out of a wave (Tile::put) keeps column c of row r
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logit
   const int t = dense::tile_of(blockIdx.x, nm * nn);
   if (t < 0) return;
   int m0, n0;
-  tile_at<T>(t, nm, nn, kGroup, m0, n0);
+  tile_at<T>(t, nm, nn, m0, n0);
   const uint16_t *x = (const uint16_t*)p.x + (int64_t)m0 * p.ldx, *w = (const uint16_t*)p.w;
   w += T::b_cols ? (int64_t)n0 : (int64_t)n0 * p.ldw;
   const Operand ox{{x, x}, p.ldx, p.T - m0}, ow{{w, w}, p.ldw, p.w_left - n0, p.missing};
@@ -174,17 +174,6 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logit
 template <bool A_COLS, bool B_COLS, bool TAIL> using GradBig = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, A_COLS, B_COLS, TAIL>;
 template <bool A_COLS, bool B_COLS, bool TAIL> using GradSmall = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, A_COLS, B_COLS, TAIL>;
 
-// whole: rows of whole 16-byte chunks; left: columns that exist
-__device__ __forceinline__ void store_part(uint16_t* o, const float v[8], bool whole, int left) {
-  if (whole) {
-    dense::store8(o, v);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (q < left) o[q] = f32_to_bf16(v[q]);
-  }
-}
-
 template <class T>
 __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void product_kernel(Product p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
@@ -195,7 +184,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   const int k0 = (int)((int64_t)piece * stages / p.pieces) * dense::BKS;
   const int k1 = min((int)((int64_t)(piece + 1) * stages / p.pieces) * dense::BKS, p.red);
   int m0, n0;
-  tile_at<T>(t, nm, nn, p.group, m0, n0);
+  tile_at<T>(t, nm, nn, m0, n0);
   const uint16_t *a = (const uint16_t*)p.a, *b = (const uint16_t*)p.b;
   a += T::cols ? (int64_t)k0 * p.lda + m0 : (int64_t)m0 * p.lda + k0;
   b += T::b_cols ? (int64_t)k0 * p.ldb + n0 : (int64_t)n0 * p.ldb + k0;
@@ -208,7 +197,6 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   const int wr = m0 + (wave / T::WN) * (T::TM * 32), c0 = n0 + (wave % T::WN) * (T::TN * 32);
   float* sums = p.acc ? p.acc + (int64_t)piece * p.rows * p.ldacc : nullptr;
   const float alpha = p.f.alpha();
-  const bool whole = p.ldo % 8 == 0 && p.cols % 8 == 0 && (uintptr_t)p.out % 16 == 0;
   if (sums) {
 #pragma unroll
     for (int i = 0; i < T::TM; ++i) {
@@ -233,7 +221,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
         uint16_t* out = (uint16_t*)p.out + (int64_t)r * p.ldo + c;
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] *= alpha;
-        store_part(out, v, whole, p.cols - c);
+        store_part(out, v, p.cols - c);
       }
     }
   } else {
@@ -248,7 +236,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
         T::get(mine, it, v);
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] *= alpha;
-        store_part((uint16_t*)p.out + (int64_t)r * p.ldo + c, v, whole, p.cols - c);
+        store_part((uint16_t*)p.out + (int64_t)r * p.ldo + c, v, p.cols - c);
       }
     }
   }
