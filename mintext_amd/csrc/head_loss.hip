@@ -353,8 +353,13 @@ struct Split {
   int size;  // bf16: of the tiles
   int pieces;
 };
-// A product's tiles and pieces by an estimate of its time in us: rounds of the chip by what a stage of 32 takes, and what the
-// pieces' sums take to write, read and join.
+// A product's tiles and pieces by an estimate of its time in us: rounds of the chip by what a stage of 32 takes and a tile's way
+// in and out, and what the pieces' sums take to write, read and join.  dx by itself, with dz before it (us):
+//   61 x 1536 x 32000    128 x 128 in 16 pieces 52, in 8 65, in 4 90; 256 x 256 in 16 67
+//   256 x 2048 x 32000   128 x 128 in 8 pieces 100, in 16 111, in 4 129; 256 x 256 in 16 102
+//   1531 x 704 x 50256   256 x 256 in 14 pieces 274, in 8 294, in 1 1058; 128 x 128 in 8 380
+//   4093 x 2048 x 131072 256 x 256 in 2 pieces 3826, in 4 3958, in 1 5000; 128 x 128 in 1 4783
+// and dW of 8000 x 512 x 4000 128 x 128 in 4 pieces 97, in 1 119, in 16 154; 256 x 256 in 8 107, in 1 203.
 static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
   const int64_t stages = ceil_div(red, 32);
   Split best{SIZE_BIG, 1};
@@ -362,8 +367,8 @@ static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
   for (int kind = 0; kind < (f32 ? 1 : 2); ++kind) {
     const int64_t side = f32 ? 64 : kind ? 128 : 256, slots = f32 ? 512 : kind ? 512 : 256;
     const int64_t tiles = ceil_div(rows, side) * ceil_div(cols, side);
-    const double stage = f32 ? 0.9 : kind ? 0.6 : 0.85;
     for (int s = 1; s <= kMostPieces && (s == 1 || stages / s >= 8); ++s) {
+      const double stage = f32 ? 0.9 : kind == 0 ? 0.7 : tiles * s > 256 ? 0.6 : 0.35;  // two small tiles a CU, or one
       const double out = f32 ? 4.0 : kind ? 5.0 : 12.0;
       const double t = ceil_div(tiles * s, slots) * (ceil_div(stages, s) * stage + out) +
                        (s > 1 ? s * rows * cols * 8 / 4e6 + 6.0 : 0.0);
@@ -395,15 +400,18 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
   const int64_t size = p.f32 ? 4 : 2, all = round_up(V, 256);
   p.copy_x = !p.f32 && D % 8 != 0;
   p.copy_w = !p.f32 && (order == ORDER_DV ? V : D) % 8 != 0;
-  // Copies have rows of whole 128-byte lines: 1531 x 1001 x 50257, whose rows of 1008 began inside lines, took 241 to 249 us for
-  // the logits.  x's zeros end whole stages where the weight is copied too.
+  // Copies have rows of whole 128-byte lines: 4000 x 1001 x 50257 takes 438 us forward and 1230 backward, with rows of 1008
+  // elements, which begin inside lines, 485 and 1335.  x's zeros end whole stages where the weight is copied too.
   p.ldx = p.copy_x ? round_up(D, 64) : D;
   p.red = !p.copy_x ? D : round_up(D, order == ORDER_VD ? 32 : 8);
-  int64_t most = all;
+  int64_t most = std::min(all, std::max<int64_t>(((int64_t)1 << 38) / T / 256 * 256, 256));  // threads of a grid: 2^30
   if (p.copy_w) most = std::min(most, std::max<int64_t>(kCopy / (p.ldx * 2) / 256 * 256, 256));
   if (backward) most = std::min(most, std::max<int64_t>((kPiece / (T * size) - kTurn) / 256 * 256, 256));
   p.piece = round_up(ceil_div(V, ceil_div(all, most)), 256);
   const int64_t big = ceil_div(T, 256) * ceil_div(p.piece, 256);
+  // Forward in 256 x 256, 128 x 128 and 64 x 128 tiles (us): 48 x 2048 x 32000 54.3, 31.2, 30.2; 65 rows 52.9, 31.2, 37.6; 256 rows
+  // 54.1, 47.2, 58.2; 512 x 2048 x 16384 (128 large tiles) 51.5, 44.4, 53.3; 1024 x 2048 x 12288 (192) 57.3, 62.6; 1024 x 2048 x
+  // 32000 (500) 120, 147.
   p.path = p.f32 ? PATH_F32 : T <= 64 ? PATH_THIN : big >= 192 ? PATH_BIG : PATH_SMALL;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -501,6 +509,7 @@ static int forward(const Plan& p, const void* x, const void* w, Merge m, float* 
   m.T = p.T;
   m.V = p.V;
   m.chosen = chosen;
+  // forward of 4096 x 64 x 32000: 81 us with neighbouring rows together, 87 with a wave a row; 1024 x 64 x 32000 31.6, 29.9
   if (p.T > 2048) hipLaunchKernelGGL(merge_kernel, dim3((unsigned)ceil_div(p.T, 32)), dim3(256), 0, st, m);
   else hipLaunchKernelGGL(merge_wave_kernel, dim3((unsigned)ceil_div(p.T, 4)), dim3(256), 0, st, m);
   if (total) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, m.loss, m.state, p.T, mean, total, count);
