@@ -452,31 +452,32 @@ int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre
  *   loss[t] = temperature^2 sum_k p_k (log p_k - z[t, i_k] / temperature + lse[t]).  A row without such an entry has loss
  *   0 and no gradient, one with an index of V or more, or a NaN, has NaN; an index that is there twice is two entries.
  *   entries (mtx_distillation_entries_size bytes, 16-byte aligned) is filled for the backward call.
- * Both write loss, lse, state[T] (1, 0 for rows left out, NaN) and chosen[T] (distillation: [T,K]), the named logits.  total
- *   and count (both or none) receive the sum of the losses and, with `mean`, what it was divided by: the rows that
- *   are not left out, 1 at least.
+ * Both write loss, stats[T][2] (the largest logit m and sum exp((z - m) / temperature)), state[T] (1, 0 for rows
+ *   left out, NaN) and chosen[T] (distillation: [T,K]), the named logits.  total and count (both or none) receive the
+ *   sum of the losses and, with `mean`, what it was divided by: the rows that are not left out, 1 at least.
  * The _bwd calls: g is the gradient of total (count as written) or, with count NULL, of loss[T]; dx[T,D] and dw (W's
- *   order) in dtype and 16-byte aligned, either may be NULL.  dz is rounded to dtype for the products; its columns go through in pieces of 1 GiB
- *   at most, over which dx is summed in float32.  No two calls that can run at the same time may share a workspace. */
+ *   order) in dtype and 16-byte aligned, either may be NULL.  dz is rounded to dtype for the products (up to 64 rows
+ *   in two planes, with what the rounding took); its columns go through in pieces of 1 GiB at most, over which dx is
+ *   summed in float32.  No two calls that can run at the same time may share a workspace. */
 #define MTX_HEAD_DV 0  /* W[D,V] */
 #define MTX_HEAD_VD 1  /* W[V,D] */
 int64_t mtx_head_loss_workspace_size(int dtype, int64_t T, int64_t D, int64_t V, int order, int backward);
 int64_t mtx_distillation_entries_size(int64_t T, int64_t V, int64_t K);
 int mtx_linear_cross_entropy(const void* x, const void* w, const void* targets, int targets_64, int dtype,
                              int64_t T, int64_t D, int64_t V, int order, int64_t ignore_index, float z_loss,
-                             int mean, float* loss, float* lse, float* state, float* total, float* count,
+                             int mean, float* loss, float* stats, float* state, float* total, float* count,
                              float* chosen, void* workspace, int64_t workspace_bytes, void* stream);
 int mtx_linear_cross_entropy_bwd(const float* g, const float* count, const void* x, const void* w,
-                                 const void* targets, int targets_64, const float* lse, const float* state,
+                                 const void* targets, int targets_64, const float* stats, const float* state,
                                  const float* chosen, int dtype, int64_t T, int64_t D, int64_t V, int order, float z_loss, void* dx,
                                  void* dw, void* workspace, int64_t workspace_bytes, void* stream);
 int mtx_linear_distillation(const void* x, const void* w, const void* teacher_idx, int idx_64,
                             const void* teacher_logits, int logits_dtype, int dtype, int64_t T, int64_t D,
-                            int64_t V, int64_t K, int order, float temperature, int mean, float* loss, float* lse,
+                            int64_t V, int64_t K, int order, float temperature, int mean, float* loss, float* stats,
                             float* state, float* total, float* count, float* chosen, void* entries,
                             int64_t entries_bytes, void* workspace, int64_t workspace_bytes, void* stream);
 int mtx_linear_distillation_bwd(const float* g, const float* count, const void* x, const void* w,
-                                const void* entries, int64_t entries_bytes, const float* lse, const float* state,
+                                const void* entries, int64_t entries_bytes, const float* stats, const float* state,
                                 const float* chosen, int dtype, int64_t T, int64_t D, int64_t V, int64_t K, int order,
                                 float temperature, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
                                 void* stream);

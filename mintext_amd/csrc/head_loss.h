@@ -16,6 +16,11 @@ namespace mtx {
 namespace head {
 
 enum { ORDER_DV = 0, ORDER_VD = 1 };  // of the weight in memory
+// Rows up to which precision comes first: bf16 dz in two planes, logits in several sums.  A gradient of few rows hangs on
+// few values of dz, whose roundings do not even out: 1 x 64 x 32768 bf16 3.4e-3 off with one plane and 1.5e-3, the result's own
+// rounding, with two; 300 x 2000 x 3000 2.4e-3 of 1.7e-3 with one.  Both directions of 48 x 2048 x 32000 take 147 us, with one
+// plane 132; 128 rows 197 and 159.
+constexpr int kTwoRows = 64;
 constexpr int kBlock = 128;           // columns an entry of Entries::bounds stands for
 
 // The classes of a row that its loss names.  Cross entropy: targets[row], int32 or int64.  Distillation: idx and share of
@@ -36,17 +41,19 @@ __device__ __forceinline__ int64_t target(const Entries& e, int64_t row) {
 // A row's factors in the backward pass, dz = a softmax - b share, and the one of all rows that is left to the products' results.
 struct Factors {
   const float *g, *count;    // the gradient of the one loss and what its sum was divided by; or of each row's, and nullptr
-  const float *lse, *state;  // [T]
+  const float *stats, *state;  // [T][2]: the row's largest logit m and sum exp((z - m) / tau); [T]
   float unit, z_loss;
   __device__ __forceinline__ float b(int64_t row) const {
     const float s = state[row];
     return s == 0.0f ? 0.0f : count ? s : s * unit * g[row];
   }
-  // `l2`: log2 of sum exp(z / tau)
-  __device__ __forceinline__ float a(int64_t row, float b, float& l2) const {
-    const float l = lse[row];
-    l2 = l * 1.4426950408889634f;
-    return b == 0.0f ? 0.0f : b * (1.0f + 2.0f * z_loss * l);
+  // a / sum, so that a softmax is that times exp((z - m) / tau).  Not exp(z / tau - lse): where lse is 15, its rounding alone is
+  // 4e-7 of every value of the row, and f32 gradients of 4 x 1324 x 10624 were 8e-6 off.
+  __device__ __forceinline__ float a(int64_t row, float b, float& m) const {
+    const float s = stats[2 * row + 1];
+    m = stats[2 * row];
+    if (b == 0.0f) return 0.0f;
+    return (z_loss == 0.0f ? b : b * (1.0f + 2.0f * z_loss * (m + logf(s)))) / s;  // z_loss: tau is 1
   }
   __device__ __forceinline__ float alpha() const { return count ? unit * (g[0] / *count) : 1.0f; }
 };
@@ -64,7 +71,8 @@ struct Logits {
   float* chosen;        // [T][K]: z of the entries
   // backward
   Factors f;
-  void* dz;             // [T][ldz], zeros behind the piece's columns
+  void* dz;             // [planes][T][ldz], zeros behind the piece's columns
+  int planes;           // 2: what the rounding took, rounded itself, stands behind dz
   int64_t ldz;
 };
 

@@ -125,7 +125,7 @@ struct Merge {
   const float* chosen;
   int64_t ignore;
   float scale, inv_tau, unit, z_loss;  // unit: tau^2
-  float *loss, *lse, *state;           // loss: [T]
+  float *loss, *stats, *state;         // loss: [T]
 };
 struct Sum {  // of exp2((z - m) scale)
   float m, s;
@@ -178,7 +178,8 @@ __device__ __forceinline__ void finish_row(const Merge& p, int64_t row, const Su
   float loss = p.unit * (konst + below + log_sum);
   if (p.z_loss != 0.0f) loss += p.z_loss * lse * lse;
   p.loss[row] = state == 0.0f ? 0.0f : state * loss;
-  p.lse[row] = lse;
+  p.stats[2 * row] = a.m;
+  p.stats[2 * row + 1] = a.s;
   p.state[row] = state;
 }
 // 32 rows a workgroup, eight threads a row, joined in order: neighbours read neighbouring rows' blocks.  4096 rows of 250
@@ -263,7 +264,7 @@ struct Named {
   int v0, cols;
   void* dz;
   int64_t ldz;
-  int f32;
+  int f32, planes;
 };
 __global__ __launch_bounds__(256) void named_kernel(Named p) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -284,22 +285,28 @@ __global__ __launch_bounds__(256) void named_kernel(Named p) {
   if (c < 0 || c >= p.cols) return;
   if (!p.e.targets)
     for (int64_t k = at + 1; k < (t + 1) * p.e.K && p.e.idx[k] == c + p.v0; ++k) share += p.e.share[k];
-  float l2;
-  const float a = p.f.a(t, b, l2), v = a * exp2f(__builtin_fmaf(p.chosen[at], p.scale, -l2)) - b * share;
-  if (p.f32) ((float*)p.dz)[t * p.ldz + c] = v;
-  else ((uint16_t*)p.dz)[t * p.ldz + c] = f32_to_bf16(v);
+  float m;
+  const float a = p.f.a(t, b, m), v = a * exp2f((p.chosen[at] - m) * p.scale) - b * share;
+  if (p.f32) {
+    ((float*)p.dz)[t * p.ldz + c] = v;
+    return;
+  }
+  uint16_t* dz = (uint16_t*)p.dz + t * p.ldz + c;
+  *dz = f32_to_bf16(v);
+  if (p.planes == 2) dz[p.T * p.ldz] = f32_to_bf16(v - bf16_to_f32(*dz));
 }
 
 // rows x cols of a bf16 matrix into one with rows of `ld` (a multiple of 8), zeros behind the columns.  `in` lies on a 4-byte
 // boundary and has rows of any length: eight elements come as the words that hold them, shifted by one where the first is odd.
+// `times` such matrices, one behind the other.
 __global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ in, int64_t ldi, int64_t rows, int64_t cols,
-                                                  uint16_t* __restrict__ out, int64_t ld) {
+                                                  uint16_t* __restrict__ out, int64_t ld, int times) {
   struct __attribute__((aligned(4))) Words {
     uint32_t v[4];
   };
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (i >= rows * ld) return;
-  const int64_t r = i / ld, c = i - r * ld, e = r * ldi + c, end = (rows - 1) * ldi + cols;
+  if (i >= times * rows * ld) return;
+  const int64_t at = i / ld, r = at % rows, c = i - at * ld, e = r * ldi + c, end = (rows - 1) * ldi + cols;
   v4u32 o = {0u, 0u, 0u, 0u};
   if (c < cols) {
     if (e + 9 < end) {  // all the words lie inside
@@ -386,9 +393,11 @@ struct Plan {
   int64_t T, D, V, ldx, red;  // ldx: x's row length in use; red: reduction elements of the logits
   int order;
   bool copy_x, copy_w;
+  int planes;                // of dz, and copies of x behind one another
   int64_t piece;             // columns of a piece, a multiple of 256
   int path;
   Split dx, dw;
+  int join_dx;               // sums of dx to be joined: the reduction's pieces, of each plane
   int64_t ld_dx, ld_dw, rows_dw;
   // bytes from the workspace's start
   int64_t x, w, part, dz, acc_dx, acc_dw, total;
@@ -398,40 +407,44 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
   p.f32 = dtype == MTX_F32;
   p.T = T, p.D = D, p.V = V, p.order = order;
   const int64_t size = p.f32 ? 4 : 2, all = round_up(V, 256);
-  p.copy_x = !p.f32 && D % 8 != 0;
+  p.planes = !p.f32 && backward && T <= kTwoRows ? 2 : 1;
+  const bool odd = !p.f32 && D % 8 != 0;
+  p.copy_x = odd || p.planes == 2;
   p.copy_w = !p.f32 && (order == ORDER_DV ? V : D) % 8 != 0;
   // Copies have rows of whole 128-byte lines: 4000 x 1001 x 50257 takes 438 us forward and 1230 backward, with rows of 1008
   // elements, which begin inside lines, 485 and 1335.  x's zeros end whole stages where the weight is copied too.
-  p.ldx = p.copy_x ? round_up(D, 64) : D;
-  p.red = !p.copy_x ? D : round_up(D, order == ORDER_VD ? 32 : 8);
+  p.ldx = odd ? round_up(D, 64) : D;
+  p.red = odd ? round_up(D, order == ORDER_VD ? 32 : 8) : D;
   int64_t most = std::min(all, std::max<int64_t>(((int64_t)1 << 38) / T / 256 * 256, 256));  // threads of a grid: 2^30
   if (p.copy_w) most = std::min(most, std::max<int64_t>(kCopy / (p.ldx * 2) / 256 * 256, 256));
-  if (backward) most = std::min(most, std::max<int64_t>((kPiece / (T * size) - kTurn) / 256 * 256, 256));
+  if (backward) most = std::min(most, std::max<int64_t>((kPiece / (p.planes * T * size) - kTurn) / 256 * 256, 256));
   p.piece = round_up(ceil_div(V, ceil_div(all, most)), 256);
   const int64_t big = ceil_div(T, 256) * ceil_div(p.piece, 256);
   // Forward in 256 x 256, 128 x 128 and 64 x 128 tiles (us): 48 x 2048 x 32000 54.3, 31.2, 30.2; 65 rows 52.9, 31.2, 37.6; 256 rows
   // 54.1, 47.2, 58.2; 512 x 2048 x 16384 (128 large tiles) 51.5, 44.4, 53.3; 1024 x 2048 x 12288 (192) 57.3, 62.6; 1024 x 2048 x
-  // 32000 (500) 120, 147.
-  p.path = p.f32 ? PATH_F32 : T <= 64 ? PATH_THIN : big >= 192 ? PATH_BIG : PATH_SMALL;
+  // 32000 (500) 120, 147.  Both directions of 128 x 4096 x 131072 take 1242 with large tiles, 1199 with small ones.
+  p.path = p.f32 ? PATH_F32 : T <= 64 ? PATH_THIN : big >= 192 && T > 128 ? PATH_BIG : PATH_SMALL;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
     at += round_up(bytes, 256);
     return here;
   };
-  p.x = take(p.copy_x ? T * p.ldx * 2 : 0);
+  p.x = take(p.copy_x ? p.planes * T * p.ldx * 2 : 0);
   p.w = take(p.copy_w ? p.piece * (order == ORDER_DV ? D : p.ldx) * 2 : 0);
   if (!backward) {
     p.part = take(round_up(V, tile_cols(p.path)) / block_cols(p.path) * T * 8);
   } else {
-    p.dz = take(T * (p.piece + kTurn) * size);
-    p.dx = split(p.f32, T, D, std::min(p.piece, V));
+    const int64_t rows = p.planes * T;
+    p.dz = take(rows * (p.piece + kTurn) * size);
+    p.dx = split(p.f32, rows, D, std::min(p.piece, V));
     p.ld_dx = round_up(D, 8);
-    p.acc_dx = take(p.dx.pieces > 1 || p.piece < V ? p.dx.pieces * T * p.ld_dx * 4 : 0);
+    p.join_dx = p.dx.pieces * p.planes;
+    p.acc_dx = take(p.join_dx > 1 || p.piece < V ? p.join_dx * T * p.ld_dx * 4 : 0);
     const int64_t n = std::min(p.piece, V);
     p.rows_dw = order == ORDER_DV ? D : n;
     p.ld_dw = round_up(order == ORDER_DV ? n : D, 8);
-    p.dw = split(p.f32, p.rows_dw, order == ORDER_DV ? n : D, T);
+    p.dw = split(p.f32, p.rows_dw, order == ORDER_DV ? n : D, rows);
     p.acc_dw = take(p.dw.pieces > 1 ? p.dw.pieces * p.rows_dw * p.ld_dw * 4 : 0);
   }
   p.total = std::max<int64_t>(at, 256);
@@ -448,9 +461,9 @@ static int check_sizes(int dtype, int64_t T, int64_t D, int64_t V, int order) {
 }
 static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
-static int pad(const void* in, int64_t ldi, int64_t rows, int64_t cols, char* out, int64_t ld, hipStream_t st) {
-  hipLaunchKernelGGL(pad_kernel, dim3((unsigned)ceil_div(rows * ld, 2048)), dim3(256), 0, st, (const uint16_t*)in, ldi, rows, cols,
-                     (uint16_t*)out, ld);
+static int pad(const void* in, int64_t ldi, int64_t rows, int64_t cols, char* out, int64_t ld, int times, hipStream_t st) {
+  hipLaunchKernelGGL(pad_kernel, dim3((unsigned)ceil_div(times * rows * ld, 2048)), dim3(256), 0, st, (const uint16_t*)in, ldi,
+                     rows, cols, (uint16_t*)out, ld, times);
   return check_launch();
 }
 // The operands of the logits of columns v0 ..: x and w where they are, or copies with rows of whole 16-byte chunks
@@ -458,14 +471,14 @@ static int operands(const Plan& p, const void* x, const void* w, int64_t v0, cha
   const int64_t size = p.f32 ? 4 : 2, n = std::min(p.piece, p.V - v0);
   int rc = MTX_OK;
   a.x = p.copy_x ? ws + p.x : x;
-  if (p.copy_x && v0 == 0) rc = pad(x, p.D, p.T, p.D, ws + p.x, p.ldx, st);
+  if (p.copy_x && v0 == 0) rc = pad(x, p.D, p.T, p.D, ws + p.x, p.ldx, p.planes, st);
   a.ldx = p.ldx;
   a.w = (const char*)w + (p.order == ORDER_DV ? v0 : v0 * p.D) * size;
   a.ldw = p.order == ORDER_DV ? p.V : p.D;
   a.w_left = (int)n;
   if (p.copy_w && rc == MTX_OK) {
     const bool dv = p.order == ORDER_DV;
-    rc = pad(a.w, a.ldw, dv ? p.D : n, dv ? n : p.D, ws + p.w, dv ? p.piece : p.ldx, st);
+    rc = pad(a.w, a.ldw, dv ? p.D : n, dv ? n : p.D, ws + p.w, dv ? p.piece : p.ldx, 1, st);
     a.w = ws + p.w;
     a.ldw = dv ? p.piece : p.ldx;
     if (dv) a.w_left = (int)p.piece;
@@ -527,31 +540,33 @@ static int backward(const Plan& p, const Factors& f, const void* x, const void* 
   a.scale = scale;
   a.dz = ws + p.dz;
   a.ldz = p.piece + kTurn;
+  a.planes = p.planes;
+  const int rows = (int)(p.planes * p.T);
   for (int64_t v0 = 0; v0 < p.V && rc == MTX_OK; v0 += p.piece) {
     rc = operands(p, x, w, v0, ws, a, st);
     if (rc == MTX_OK) rc = logits(p, a, true, st);
     if (rc != MTX_OK) return rc;
-    const Named named{e, f, chosen, scale, p.T, a.v0, a.cols, a.dz, a.ldz, p.f32};
+    const Named named{e, f, chosen, scale, p.T, a.v0, a.cols, a.dz, a.ldz, p.f32, p.planes};
     hipLaunchKernelGGL(named_kernel, dim3((unsigned)ceil_div(p.T * e.K, 256)), dim3(256), 0, st, named);
     if (dx) {
       const int red = p.f32 ? a.cols : (int)round_up(a.cols, 8);  // dz holds zeros behind its columns
       const bool only = p.piece >= p.V, final = v0 + p.piece >= p.V;
       // the last piece of the vocabulary may be shorter than what the split was made for
       const int pieces = (int)std::min<int64_t>(p.dx.pieces, ceil_div(red, 32));
-      Product q{a.dz, a.w, a.ldz, a.ldw, (int)p.T, (int)p.D, red, 0, (int)p.T, (int)(dv ? p.D : p.ldx), dx, p.D, pieces, nullptr,
-                p.ld_dx, v0 > 0, p.dx.pieces == 1 && final, f};
+      Product q{a.dz, a.w, a.ldz, a.ldw, rows, (int)p.D, red, 0, rows, (int)(dv ? p.D : p.ldx), dx, p.D, pieces, nullptr,
+                p.ld_dx, v0 > 0, p.join_dx == 1 && final, f};
       if (!dv) q.missing = red - a.cols;
-      if (!(only && p.dx.pieces == 1)) q.acc = (float*)(ws + p.acc_dx);
+      if (!(only && p.join_dx == 1)) q.acc = (float*)(ws + p.acc_dx);
       rc = product(p, q, false, !dv, p.dx, st);
-      if (rc == MTX_OK && final && p.dx.pieces > 1) rc = join(p.f32, q.acc, p.dx.pieces, p.T, p.D, p.ld_dx, dx, p.D, f, st);
+      if (rc == MTX_OK && final && p.join_dx > 1) rc = join(p.f32, q.acc, p.join_dx, p.T, p.D, p.ld_dx, dx, p.D, f, st);
       if (rc != MTX_OK) return rc;
     }
     if (dw && rc == MTX_OK) {
       void* out = (char*)dw + (dv ? v0 : v0 * p.D) * size;
       const int64_t ldo = dv ? p.V : p.D;
       Product q{};
-      if (dv) q = Product{a.x, a.dz, a.ldx, a.ldz, (int)p.D, a.cols, (int)p.T, 0, (int)p.ldx, (int)p.piece, out, ldo, p.dw.pieces};
-      else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, (int)p.T, 0, (int)p.piece, (int)p.ldx, out, ldo, p.dw.pieces};
+      if (dv) q = Product{a.x, a.dz, a.ldx, a.ldz, (int)p.D, a.cols, rows, 0, (int)p.ldx, (int)p.piece, out, ldo, p.dw.pieces};
+      else q = Product{a.dz, a.x, a.ldz, a.ldx, a.cols, (int)p.D, rows, 0, (int)p.piece, (int)p.ldx, out, ldo, p.dw.pieces};
       q.ldacc = p.ld_dw;
       q.last = p.dw.pieces == 1;
       q.f = f;
@@ -596,7 +611,7 @@ extern "C" int64_t mtx_distillation_entries_size(int64_t T, int64_t V, int64_t K
 
 extern "C" int mtx_linear_cross_entropy(const void* x, const void* w, const void* targets, int targets_64, int dtype, int64_t T,
                                         int64_t D, int64_t V, int order, int64_t ignore_index, float z_loss, int mean,
-                                        float* loss, float* lse, float* state, float* total, float* count, float* chosen,
+                                        float* loss, float* stats, float* state, float* total, float* count, float* chosen,
                                         void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace head;
   const int rc = check_sizes(dtype, T, D, V, order);
@@ -607,38 +622,38 @@ extern "C" int mtx_linear_cross_entropy(const void* x, const void* w, const void
     if (total) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, state, (int64_t)0, mean, total, count);
     return check_launch();
   }
-  if (!x || !w || !targets || !loss || !lse || !state || !chosen || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
+  if (!x || !w || !targets || !loss || !stats || !state || !chosen || !aligned16(x) || !aligned16(w)) return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, false);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
   Merge m{};
   m.e = Entries{targets, targets_64, nullptr, nullptr, nullptr, 0, 1};
   m.ignore = ignore_index;
   m.scale = kLog2e, m.inv_tau = 1.0f, m.unit = 1.0f, m.z_loss = z_loss;
-  m.loss = loss, m.lse = lse, m.state = state;
+  m.loss = loss, m.stats = stats, m.state = state;
   return forward(p, x, w, m, chosen, total, count, mean, (char*)workspace, st);
 }
 
 extern "C" int mtx_linear_cross_entropy_bwd(const float* g, const float* count, const void* x, const void* w, const void* targets,
-                                            int targets_64, const float* lse, const float* state, const float* chosen, int dtype, int64_t T, int64_t D,
-                                            int64_t V, int order, float z_loss, void* dx, void* dw, void* workspace,
+                                            int targets_64, const float* stats, const float* state, const float* chosen, int dtype,
+                                            int64_t T, int64_t D, int64_t V, int order, float z_loss, void* dx, void* dw, void* workspace,
                                             int64_t workspace_bytes, void* stream) {
   using namespace head;
   const int rc = check_sizes(dtype, T, D, V, order);
   if (rc != MTX_OK) return rc;
   if (T == 0 || (!dx && !dw)) return MTX_OK;
-  if (!g || !x || !w || !targets || !lse || !state || !chosen || !aligned16(x) || !aligned16(w) || !aligned16(dx) ||
+  if (!g || !x || !w || !targets || !stats || !state || !chosen || !aligned16(x) || !aligned16(w) || !aligned16(dx) ||
       !aligned16(dw))
     return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, true);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
   const Entries e{targets, targets_64, nullptr, nullptr, nullptr, 0, 1};
-  return backward(p, Factors{g, count, lse, state, 1.0f, z_loss}, x, w, chosen, e, kLog2e, dx, dw, (char*)workspace,
+  return backward(p, Factors{g, count, stats, state, 1.0f, z_loss}, x, w, chosen, e, kLog2e, dx, dw, (char*)workspace,
                   (hipStream_t)stream);
 }
 
 extern "C" int mtx_linear_distillation(const void* x, const void* w, const void* teacher_idx, int idx_64,
                                        const void* teacher_logits, int logits_dtype, int dtype, int64_t T, int64_t D, int64_t V,
-                                       int64_t K, int order, float temperature, int mean, float* loss, float* lse, float* state,
+                                       int64_t K, int order, float temperature, int mean, float* loss, float* stats, float* state,
                                        float* total, float* count, float* chosen, void* entries_buffer, int64_t entries_bytes,
                                        void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace head;
@@ -653,7 +668,7 @@ extern "C" int mtx_linear_distillation(const void* x, const void* w, const void*
     if (total) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, state, (int64_t)0, mean, total, count);
     return check_launch();
   }
-  if (!x || !w || !teacher_idx || !teacher_logits || !loss || !lse || !state || !chosen || !entries_buffer || !aligned16(x) ||
+  if (!x || !w || !teacher_idx || !teacher_logits || !loss || !stats || !state || !chosen || !entries_buffer || !aligned16(x) ||
       !aligned16(w))
     return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, false);
@@ -668,29 +683,29 @@ extern "C" int mtx_linear_distillation(const void* x, const void* w, const void*
   m.e = entries(buf, s, K);
   m.row = prep.row;
   m.scale = kLog2e * inv, m.inv_tau = inv, m.unit = temperature * temperature;
-  m.loss = loss, m.lse = lse, m.state = state;
+  m.loss = loss, m.stats = stats, m.state = state;
   return forward(p, x, w, m, chosen, total, count, mean, (char*)workspace, st);
 }
 
 extern "C" int mtx_linear_distillation_bwd(const float* g, const float* count, const void* x, const void* w,
-                                           const void* entries_buffer, int64_t entries_bytes, const float* lse,
+                                           const void* entries_buffer, int64_t entries_bytes, const float* stats,
                                            const float* state, const float* chosen, int dtype, int64_t T, int64_t D, int64_t V,
-                                           int64_t K, int order, float temperature, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
-                                           void* stream) {
+                                           int64_t K, int order, float temperature, void* dx, void* dw, void* workspace,
+                                           int64_t workspace_bytes, void* stream) {
   using namespace head;
   const int rc = check_sizes(dtype, T, D, V, order);
   if (rc != MTX_OK) return rc;
   if (K <= 0 || !(temperature > 0.0f && temperature < INFINITY)) return MTX_ERR_ARG;
   if (K > kMaxEntries) return MTX_ERR_UNSUPPORTED;
   if (T == 0 || (!dx && !dw)) return MTX_OK;
-  if (!g || !x || !w || !entries_buffer || !lse || !state || !chosen || !aligned16(x) || !aligned16(w) || !aligned16(dx) ||
+  if (!g || !x || !w || !entries_buffer || !stats || !state || !chosen || !aligned16(x) || !aligned16(w) || !aligned16(dx) ||
       !aligned16(dw))
     return MTX_ERR_ARG;
   const Plan p = plan(dtype, T, D, V, order, true);
   const Saved s = saved(T, V, K);
   if (!aligned16(entries_buffer) || entries_bytes < s.total) return MTX_ERR_WORKSPACE;
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.total) return MTX_ERR_WORKSPACE;
-  return backward(p, Factors{g, count, lse, state, temperature, 0.0f}, x, w, chosen,
+  return backward(p, Factors{g, count, stats, state, temperature, 0.0f}, x, w, chosen,
                   entries((char*)const_cast<void*>(entries_buffer), s, K), kLog2e / temperature, dx, dw, (char*)workspace,
                   (hipStream_t)stream);
 }

@@ -9,7 +9,7 @@ namespace head {
 using dense::Operand;
 template <bool VD, bool TAIL> using Big = dense::Tile<dense::Bf16, 4, 4, 2, 2, 4, false, !VD, TAIL>;
 template <bool VD, bool TAIL> using Small = dense::Tile<dense::Bf16, 2, 2, 2, 2, 4, false, !VD, TAIL>;
-template <bool VD, bool TAIL> using Thin = dense::Tile<dense::Bf16, 1, 2, 2, 2, 6, false, !VD, TAIL>;
+template <bool VD, bool TAIL> using Thin = dense::Tile<dense::Bf16, 1, 2, 2, 2, 6, false, !VD, TAIL, false, dense::DIAG_NONE, 4>;
 
 // Tiles go row by row within groups of kGroup rows of tiles, so that neighbours share both operands' strips in L2.
 constexpr int kGroup = 8;
@@ -98,8 +98,9 @@ __device__ __forceinline__ void forward_out(const Logits& p, dense::f32x16 (&acc
 }
 
 // dz = a softmax, rounded, 32 rows at a time into LDS (16-byte chunk c of a row at chunk c ^ (row % chunks)) and out in whole
-// lines.  What a row's entries take from it is entries_kernel's, which knows their logits.
-template <class T>
+// lines; with two planes what the rounding left goes the same way after it.  What a row's entries take from it is
+// named_kernel's, which knows their logits.
+template <class T, int PLANES>
 __device__ __forceinline__ void gradient_out(const Logits& p, dense::f32x16 (&acc)[T::TM][T::TN], char* mine, int wr, int c0) {
   constexpr int BC = T::TN * 32, CH = T::TN * 4, BYTES = 32 * T::TN * 64;  // chunks of a row; bytes of 32 rows
   typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
@@ -110,7 +111,7 @@ __device__ __forceinline__ void gradient_out(const Logits& p, dense::f32x16 (&ac
   for (int i = 0; i < T::TM; ++i) {
     const int row = min(wr + i * 32 + r, p.T - 1);
     a[i] = p.f.a(row, p.f.b(row), off[i]);
-    off[i] = -off[i];
+    off[i] *= -p.scale;
   }
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) care |= a[i] == 0.0f;
@@ -131,27 +132,47 @@ __device__ __forceinline__ void gradient_out(const Logits& p, dense::f32x16 (&ac
           for (int q = 0; q < 4; ++q)
             if (a[i] == 0.0f || 32 * j + 8 * g + 4 * half + q >= left) d[q] = 0.0f;
         }
-        *(bf16x4*)(mine + i * BYTES + r * (CH * 16) + (((j * 4 + g) ^ (r & (CH - 1))) << 4) + half * 8) =
-            bf16x4{(__bf16)d[0], (__bf16)d[1], (__bf16)d[2], (__bf16)d[3]};
+        const bf16x4 y{(__bf16)d[0], (__bf16)d[1], (__bf16)d[2], (__bf16)d[3]};
+        *(bf16x4*)(mine + i * BYTES + r * (CH * 16) + (((j * 4 + g) ^ (r & (CH - 1))) << 4) + half * 8) = y;
+        if constexpr (PLANES == 2)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[i][j][4 * g + q] = d[q] - (float)y[q];
       }
   }
-  __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
-  asm volatile("" ::: "memory");
+  auto leave = [&](uint16_t* dz) {
+    __builtin_amdgcn_s_waitcnt(MTX_LGKMCNT0);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+      for (int it = 0; it < T::TN * 2; ++it) {
+        const int at = it * 64 + lane, o = at / CH, c = at % CH, row = wr + i * 32 + o;
+        const v4u32 v = *(const v4u32*)(mine + i * BYTES + o * (CH * 16) + ((c ^ (o & (CH - 1))) << 4));
+        if (row < p.T) *(v4u32*)(dz + (int64_t)row * p.ldz + c * 8) = v;
+      }
+  };
   uint16_t* dz = (uint16_t*)p.dz + c0;
+  leave(dz);
+  if constexpr (PLANES == 2) {
+    asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i)
+    for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-    for (int it = 0; it < T::TN * 2; ++it) {
-      const int at = it * 64 + lane, o = at / CH, c = at % CH, row = wr + i * 32 + o;
-      const v4u32 v = *(const v4u32*)(mine + i * BYTES + o * (CH * 16) + ((c ^ (o & (CH - 1))) << 4));
-      if (row < p.T) *(v4u32*)(dz + (int64_t)row * p.ldz + c * 8) = v;
-    }
+      for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(bf16x4*)(mine + i * BYTES + r * (CH * 16) + (((j * 4 + g) ^ (r & (CH - 1))) << 4) + half * 8) =
+              bf16x4{(__bf16)acc[i][j][4 * g], (__bf16)acc[i][j][4 * g + 1], (__bf16)acc[i][j][4 * g + 2],
+                     (__bf16)acc[i][j][4 * g + 3]};
+    leave(dz + (int64_t)p.T * p.ldz);
+  }
 }
 
-template <class T, bool DZ>
+// PLANES: of dz; 0 for the forward pass
+template <class T, int PLANES>
 __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logits_kernel(Logits p) {
   __shared__ __attribute__((aligned(1024))) char lds[T::LDS_BYTES];
-  constexpr int OUT = DZ ? T::TM * 32 * T::TN * 64 : T::OUT_BYTES;  // of a wave
+  constexpr int OUT = PLANES ? T::TM * 32 * T::TN * 64 : T::OUT_BYTES;  // of a wave
   static_assert(T::NW * OUT <= T::LDS_BYTES, "the way out fits the ring");
   const int nm = (p.T + T::BM - 1) / T::BM, nn = (p.cols + T::BN - 1) / T::BN;
   const int t = dense::tile_of(blockIdx.x, nm * nn);
@@ -166,7 +187,7 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void logit
   __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = m0 + (wave / T::WN) * (T::TM * 32), c0 = n0 + (wave % T::WN) * (T::TN * 32);
-  if constexpr (DZ) gradient_out<T>(p, acc, lds + wave * OUT, wr, c0);
+  if constexpr (PLANES) gradient_out<T, PLANES>(p, acc, lds + wave * OUT, wr, c0);
   else forward_out<T>(p, acc, lds + wave * OUT, wr, c0);
 }
 
@@ -242,18 +263,27 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   }
 }
 
-template <class T>
+template <class T, bool TWO>
 static int go_logits(const Logits& p, bool dz, hipStream_t st) {
   const dim3 grid((unsigned)dense::tiles_grid(ceil_div(p.T, T::BM) * ceil_div(p.cols, T::BN)));
-  if (dz) hipLaunchKernelGGL((logits_kernel<T, true>), grid, dim3(T::NT), 0, st, p);
-  else hipLaunchKernelGGL((logits_kernel<T, false>), grid, dim3(T::NT), 0, st, p);
+  if (!dz) {
+    hipLaunchKernelGGL((logits_kernel<T, 0>), grid, dim3(T::NT), 0, st, p);
+    return check_launch();
+  }
+  if constexpr (TWO) {
+    if (p.planes == 2) {
+      hipLaunchKernelGGL((logits_kernel<T, 2>), grid, dim3(T::NT), 0, st, p);
+      return check_launch();
+    }
+  }
+  hipLaunchKernelGGL((logits_kernel<T, 1>), grid, dim3(T::NT), 0, st, p);
   return check_launch();
 }
 template <bool VD, bool TAIL>
 static int go_path(const Logits& p, bool dz, int path, hipStream_t st) {
-  if (path == PATH_BIG) return go_logits<Big<VD, TAIL>>(p, dz, st);
-  if (path == PATH_SMALL) return go_logits<Small<VD, TAIL>>(p, dz, st);
-  return go_logits<Thin<VD, TAIL>>(p, dz, st);
+  if (path == PATH_BIG) return go_logits<Big<VD, TAIL>, false>(p, dz, st);
+  if (path == PATH_SMALL) return go_logits<Small<VD, TAIL>, false>(p, dz, st);
+  return go_logits<Thin<VD, TAIL>, true>(p, dz, st);
 }
 int launch_logits(const Logits& p, bool dz, int order, int path, hipStream_t st) {
   const bool tail = p.red % dense::BKS != 0 || p.missing > 0;

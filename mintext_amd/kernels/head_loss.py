@@ -6,7 +6,8 @@ makes the logits tile by tile on the matrix cores and leaves each tile's maxima,
 names; the [T, V] logits are not stored, in neither direction.  The backward makes them again in pieces of the
 vocabulary whose gradient takes 1 GiB at most, and runs the two products of each piece; over the pieces the gradient of
 ``x`` is summed in float32.  The gradient of the logits is rounded to the operands' type for the products (bfloat16:
-as in ``linear``'s backward, the results end 2.4e-3 off where their own rounding is 1.7e-3).  Every sum has a fixed order.
+as in ``linear``'s backward, the results end 2.4e-3 off where their own rounding is 1.7e-3; up to 64 tokens keep what that
+rounding took as well, and end at their own).  Every sum has a fixed order.
 
 The weight is [D, V] as it lies in memory, or an embedding table [V, D] passed as ``table.t()``: both are read in place, and
 the weight's gradient has the weight's strides.  In bfloat16 a vocabulary (or, for a table, a width) that is no multiple of 8
@@ -70,10 +71,10 @@ class _Loss:
 
     @staticmethod
     def rows(buffer, T, K):
-        """Addresses in the float32 buffer of log sum exp [T], state [T], the named logits [T, K], the count, the losses [T].
+        """Addresses in the float32 buffer of maxima and sums [T, 2], state [T], the named logits [T, K], the count, the losses [T].
         (Numbers, also where a jit trace has sizes of its own: it calls the Function again for other tensors.)"""
         at = buffer.data_ptr()
-        return at, at + 4 * T, at + 8 * T, at + 4 * (2 + K) * T, at + 4 * (2 + K) * T + 4
+        return at, at + 8 * T, at + 12 * T, at + 4 * (3 + K) * T, at + 4 * (3 + K) * T + 4
 
     def forward(self, x, weight, classes, teacher):
         dev = L.require_device(x, weight, classes, teacher)
@@ -85,8 +86,8 @@ class _Loss:
         # the result is a tensor of its own, which a caller may change in place
         one = self.reduction != "none"
         out = torch.empty(() if one else x.shape[:-1], dtype=torch.float32, device=dev)
-        buffer = torch.empty((2 + K + one) * T + 1, dtype=torch.float32, device=dev)
-        lse, state, chosen, count, loss = self.rows(buffer, T, K)
+        buffer = torch.empty((3 + K + one) * T + 1, dtype=torch.float32, device=dev)
+        stats, state, chosen, count, loss = self.rows(buffer, T, K)
         total = out.data_ptr() if one else None
         if not one:
             count, loss = None, out.data_ptr()
@@ -96,13 +97,13 @@ class _Loss:
         with L.on_device(dev):
             if teacher is None:
                 L.call("mtx_linear_cross_entropy", x.data_ptr(), weight.data_ptr(), classes.data_ptr(), wide, dt, T, D, V, order,
-                       self.ignore_index, self.z_loss, mean, loss, lse, state, total, count, chosen, ws.data_ptr(), ws.numel(),
+                       self.ignore_index, self.z_loss, mean, loss, stats, state, total, count, chosen, ws.data_ptr(), ws.numel(),
                        L.stream(dev))
             else:
                 teacher = teacher.contiguous()
                 kept = L.workspace(L.query("mtx_distillation_entries_size", T, V, K), dev)
                 L.call("mtx_linear_distillation", x.data_ptr(), weight.data_ptr(), classes.data_ptr(), wide, teacher.data_ptr(),
-                       L.dtype_code(teacher.dtype), dt, T, D, V, K, order, self.temperature, mean, loss, lse, state, total, count,
+                       L.dtype_code(teacher.dtype), dt, T, D, V, K, order, self.temperature, mean, loss, stats, state, total, count,
                        chosen, kept.data_ptr(), kept.numel(), ws.data_ptr(), ws.numel(), L.stream(dev))
         return out, (x, weight, kept, buffer)
 
@@ -112,7 +113,7 @@ class _Loss:
         T = int(x.numel() // D)
         order = L.MTX_HEAD_DV if weight.is_contiguous() else L.MTX_HEAD_VD
         g = g.contiguous()
-        lse, state, chosen, count, _ = self.rows(buffer, T, K or 1)
+        stats, state, chosen, count, _ = self.rows(buffer, T, K or 1)
         if self.reduction == "none":
             count = None
         dt = L.dtype_code(x.dtype)
@@ -122,11 +123,11 @@ class _Loss:
         with L.on_device(dev):
             if K is None:
                 L.call("mtx_linear_cross_entropy_bwd", g.data_ptr(), count, x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
-                       _index64("classes", kept), lse, state, chosen, dt, T, D, V, order, self.z_loss, L.ptr(dx), L.ptr(dw),
+                       _index64("classes", kept), stats, state, chosen, dt, T, D, V, order, self.z_loss, L.ptr(dx), L.ptr(dw),
                        ws.data_ptr(), ws.numel(), L.stream(dev))
             else:
                 L.call("mtx_linear_distillation_bwd", g.data_ptr(), count, x.data_ptr(), weight.data_ptr(), kept.data_ptr(),
-                       kept.numel(), lse, state, chosen, dt, T, D, V, K, order, self.temperature, L.ptr(dx), L.ptr(dw),
+                       kept.numel(), stats, state, chosen, dt, T, D, V, K, order, self.temperature, L.ptr(dx), L.ptr(dw),
                        ws.data_ptr(), ws.numel(), L.stream(dev))
         return dx, dw
 

@@ -57,8 +57,8 @@ def rows_of(idx, t, tau, V):
     return share, const, live
 
 
-def reference(x, w, share, const, live, tau, z_loss, g, K):
-    """The rows' losses, dx and dW in 64 bits with their tolerances; g: the gradient of each row's loss."""
+def reference(x, w, share, const, live, tau, z_loss, g, K, half=None):
+    """The rows' losses, dx and dW in 64 bits with their tolerances; g: the gradient of each row's loss, half: dz's half step."""
     T, D = x.shape
     V = w.shape[1]
     X, W = x.detach().double(), w.detach().double()
@@ -81,7 +81,7 @@ def reference(x, w, share, const, live, tau, z_loss, g, K):
     dz = unit * (front * q - share)
     ed = unit.abs() * (front * q * (ez + el[:, None] + 16 * V_ * (1 + z.abs() + lse.abs()[:, None])) + (K + 16) * V_ * share)
     ed = ed + 4 * V_ * dz.abs()
-    er = ed + u * dz.abs()
+    er = ed + (u if half is None else half) * dz.abs()
     dx, dw = torch.mm(dz, W.t()), torch.mm(X.t(), dz)
     tx = u * dx.abs() + torch.mm(er + (V + 8) * V_ * dz.abs(), W.abs().t().contiguous())
     tw = u * dw.abs() + torch.mm(X.abs().t().contiguous(), er + (T + 8) * V_ * dz.abs())
@@ -147,6 +147,59 @@ def check_kd(dev, T, D, V, K, dtype, order, tau=1.0, wide=False, tdtype=F32, see
     i = idx.to(torch.int64 if wide else torch.int32)
     call = lambda a, b, reduction: linear_distillation(a, b, i, t, temperature=tau, reduction=reduction)
     check(dev, call, x, w, share, const, live, tau, 0.0, K)
+
+
+@pytest.mark.parametrize("order", ["dv", "vd"])
+@pytest.mark.parametrize("T,D,V,K", [(1, 72, 1408, 1), (1, 65, 5003, 90), (4, 264, 2056, 1), (20, 1001, 999, 33), (64, 128, 4100, 1),
+                                     (50, 130, 3001, 7), (63, 512, 777, 1)])
+def test_few_rows_dz_in_two_planes(dev, T, D, V, K, order):
+    """dz of few rows is held as its rounding and the rounded rest: what is left is u times at most u |dz|, u = 2^-8."""
+    from mintext_amd.kernels import linear_cross_entropy, linear_distillation
+
+    x, w, gen = operands(dev, T, D, V, BF, order, 11)
+    g = torch.rand(T, device=dev, generator=gen) + 0.5
+    if K == 1:
+        y = torch.randint(0, V, (T,), device=dev, generator=gen)
+        live = torch.arange(T, device=dev) % 5 != 3
+        share = torch.zeros(T, V, dtype=torch.float64, device=dev).scatter_(1, y[:, None], 1.0)
+        const, tau = torch.zeros(T, dtype=torch.float64, device=dev), 1.0
+        call = lambda a, b: linear_cross_entropy(a, b, torch.where(live, y, -100), z_loss=1e-3, reduction="none")
+    else:
+        idx, t = teacher(dev, T, V, K, gen, F32)
+        tau = 0.5
+        share, const, live = rows_of(idx, t, tau, V)
+        call = lambda a, b: linear_distillation(a, b, idx, t, temperature=tau, reduction="none")
+    _, dx, dw = reference(x, w, share, const, live, tau, 1e-3 if K == 1 else 0.0, g, K, half=2.0 ** -16)
+    gx, gw = torch.autograd.grad(call(x.requires_grad_(True), w.requires_grad_(True)), [x, w], g)
+    close(gx, dx, "dx")
+    close(gw, dw, "dw")
+
+
+@pytest.mark.parametrize("order", ["dv", "vd"])
+def test_gradient_of_logits_far_from_zero(dev, order):
+    """f32 logits of 4096 + n / 128 are exact here, and what softmax has to do with is their distance from the largest alone:
+    q is off by 16 v (1 + that) and the sum's v (blocks + 64), however large they are."""
+    from mintext_amd.kernels import linear_cross_entropy
+
+    T, V = 3, 1000
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.tensor([[64.0, 1.0], [64.0, 0.5], [64.0, -1.0]], device=dev)
+    n = torch.randint(-256, 256, (V,), device=dev, generator=g) / 64
+    w = torch.stack([torch.full_like(n, 64.0), n])
+    w = w.t().contiguous().t() if order == "vd" else w
+    y = torch.tensor([1, V - 1, 500], device=dev)
+    z = torch.mm(x.double(), w.double())
+    far = z.amax(1, keepdim=True) - z
+    q = torch.softmax(z, 1)
+    dz = q - torch.zeros_like(q).scatter_(1, y[:, None], 1.0)
+    ed = q * V_ * (16 * (1 + far) + V / 64 + 64) + 4 * V_ * dz.abs()
+    for t in range(T):
+        x1, w1 = x[t:t + 1].clone().requires_grad_(True), w.detach().requires_grad_(True)
+        gx, gw = torch.autograd.grad(linear_cross_entropy(x1, w1, y[t:t + 1], reduction="sum"), [x1, w1])
+        X, W = x1.detach().double(), w1.detach().double()
+        close(gw, (torch.mm(X.t(), dz[t:t + 1]), torch.mm(X.abs().t(), ed[t:t + 1] + 4 * V_ * dz[t:t + 1].abs())), "dw")
+        close(gx, (torch.mm(dz[t:t + 1], W.t()),
+                   torch.mm(ed[t:t + 1] + (V + 8) * V_ * dz[t:t + 1].abs(), W.abs().t().contiguous())), "dx")
 
 
 # few rows; small tiles that hang over; large tiles (more than 192 of them) with whole and cut stages; odd widths and vocabularies
