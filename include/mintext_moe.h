@@ -484,7 +484,8 @@ int mtx_linear_distillation_bwd(const float* g, const float* count, const void* 
 
 /* ---- norms ---------------------------------------------------------------------------------
  * RMSNorm (mintext/modules/norm.py:10) and layer norm of T rows of D values, dense, of one dtype (F32 or
- * BF16); weight[D] and bias[D] in that or in F32.  1 <= D <= 16384, any alignment; sums in float32.
+ * BF16); weight[D] and bias[D] in that or in F32.  1 <= D <= 16384, T <= 2^30, any alignment; sums in
+ * float32.
  * mtx_norm:     h = x + residual, rounded to dtype (residual and h may both be NULL: h is x);
  *               rms == 0: y = (h - mean) rstd weight + bias (bias may be NULL), rms != 0: y = h rstd weight.
  *               mean[T] and rstd[T] may be NULL (mean always with rms).

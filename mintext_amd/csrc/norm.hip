@@ -451,9 +451,14 @@ extern "C" int mtx_norm(const void* x, const void* residual, const void* weight,
   if ((rms && bias) || !(eps >= 0.0f)) return MTX_ERR_ARG;
   if (T == 0) return MTX_OK;
   if (!x || !weight || !y || (residual && !h) || (rstd && !rms && !mean)) return MTX_ERR_ARG;
-  const Args p{x, residual, weight, bias, y, h, mean, rstd, T, (int)D, eps};
-  if (rms) { MTX_TYPES(go_forward, true, dtype, weight_dtype, p, (hipStream_t)stream) }
-  else { MTX_TYPES(go_forward, false, dtype, weight_dtype, p, (hipStream_t)stream) }
+  const int64_t most = ((int64_t)1 << 31) / lanes((int)D), bytes = D * (dtype == MTX_F32 ? 4 : 2);  // a grid's threads: 32 bits
+  for (int64_t t = 0; t < T; t += most) {
+    auto from = [&](auto* v, int64_t each) { return v ? (decltype(v))((char*)v + t * each) : nullptr; };
+    const Args p{from(x, bytes), from(residual, bytes), weight, bias, from(y, bytes), from(h, bytes), from(mean, 4), from(rstd, 4),
+                 std::min(most, T - t), (int)D, eps};
+    if (rms) { MTX_TYPES(go_forward, true, dtype, weight_dtype, p, (hipStream_t)stream) }
+    else { MTX_TYPES(go_forward, false, dtype, weight_dtype, p, (hipStream_t)stream) }
+  }
   return check_launch();
 }
 

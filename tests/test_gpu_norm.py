@@ -116,6 +116,24 @@ def test_many_rows(dev, rms):
     check(dev, 9001, 4096, BF, F32, rms, True, True)
 
 
+def test_more_rows_than_a_grid_holds(dev):
+    """D = 1: rms_norm(x) = x / sqrt(x^2 + eps) w, to be within a few roundings of float32 and one of bfloat16."""
+    from mintext_amd.kernels import rms_norm
+
+    T = 2 ** 28 + 2 ** 20 + 3
+    x = torch.empty(T, 1, device=dev, dtype=torch.bfloat16)
+    x.view(-1)[::2], x.view(-1)[1::2] = 0.75, -1.5
+    x[0], x[2 ** 28 - 1], x[2 ** 28], x[T - 1] = 3.0, 0.0, 0.01, -7.0
+    w = torch.full((1,), 1.25, device=dev, dtype=torch.bfloat16)
+    y = rms_norm(x, w, eps=1e-3)
+    for at in (slice(0, 4), slice(2 ** 28 - 4, 2 ** 28 + 4), slice(T - 4, T)):
+        X = x[at].double()
+        want = X / (X * X + 1e-3).sqrt() * 1.25
+        assert ((y[at].double() - want).abs() <= (2.0 ** -8 + 8 * 2.0 ** -24) * want.abs()).all()
+    # 1.25 and -1.25 in bfloat16, of 3 and -7 too
+    assert int((y == 1.25).sum() + (y == -1.25).sum()) == T - 2
+
+
 @pytest.mark.parametrize("eps", [0.0, 1e-12, 1.0])
 def test_eps_and_constant_rows(dev, eps):
     check(dev, 10, 64, F32, F32, False, True, False, eps=eps)
