@@ -366,7 +366,9 @@ struct Split {
 //   256 x 2048 x 32000   128 x 128 in 8 pieces 100, in 16 111, in 4 129; 256 x 256 in 16 102
 //   1531 x 704 x 50256   256 x 256 in 14 pieces 274, in 8 294, in 1 1058; 128 x 128 in 8 380
 //   4093 x 2048 x 131072 256 x 256 in 2 pieces 3826, in 4 3958, in 1 5000; 128 x 128 in 1 4783
-// and dW of 8000 x 512 x 4000 128 x 128 in 4 pieces 97, in 1 119, in 16 154; 256 x 256 in 8 107, in 1 203.
+// and dW of 8000 x 512 x 4000 128 x 128 in 4 pieces 97, in 1 119, in 16 154; 256 x 256 in 8 107, in 1 203.  Where a tile has few
+// stages, as dW of few rows, the ways out decide: 128 x 2048 x 32000 in both directions 149 with 128 x 128 tiles of dW, 160 with
+// 256 x 256; 128 x 4096 x 131072 1155 and 1198, 128 x 2048 x 65536 354 and 343.
 static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
   const int64_t stages = ceil_div(red, 32);
   Split best{SIZE_BIG, 1};
@@ -376,7 +378,7 @@ static Split split(bool f32, int64_t rows, int64_t cols, int64_t red) {
     const int64_t tiles = ceil_div(rows, side) * ceil_div(cols, side);
     for (int s = 1; s <= kMostPieces && (s == 1 || stages / s >= 8); ++s) {
       const double stage = f32 ? 0.9 : kind == 0 ? 0.7 : tiles * s > 256 ? 0.6 : 0.35;  // two small tiles a CU, or one
-      const double out = f32 ? 4.0 : kind ? 5.0 : 12.0;
+      const double out = f32 ? 4.0 : kind ? 4.5 : 12.0;
       const double t = ceil_div(tiles * s, slots) * (ceil_div(stages, s) * stage + out) +
                        (s > 1 ? s * rows * cols * 8 / 4e6 + 6.0 : 0.0);
       if (t < least) {
