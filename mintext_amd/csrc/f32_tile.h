@@ -97,9 +97,8 @@ __device__ __forceinline__ void fragment(const float* lds, int x0, int lane, flo
   }
 }
 // acc of lane l, element v: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32 of the wave's 32x32 tile.
-// nred: reduction elements; any_a, any_b: valid addresses of the operands (for nred > 0).  PART > 0: every PART stages make a
-// sum of their own: logits around 10 of 1324 products end 0.4e-6 off with 4, 0.5e-6 with 8, 1.7e-6 with one sum.
-template <typename T, bool ACOLS, bool BCOLS, int VEC, int PART = 0, typename AtA, typename AtB>
+// nred: reduction elements; any_a, any_b: valid addresses of the operands (for nred > 0).
+template <typename T, bool ACOLS, bool BCOLS, int VEC, typename AtA, typename AtB>
 __device__ __forceinline__ void mainloop(f32x16& acc, int nred, float* as, float* bs, AtA at_a, AtB at_b, const T* any_a,
                                          const T* any_b) {
   constexpr bool BF16 = std::is_same<T, uint16_t>::value;
@@ -117,38 +116,22 @@ __device__ __forceinline__ void mainloop(f32x16& acc, int nred, float* as, float
   };
   if (nk > 0) load(0);
   // one LDS buffer: a second one saves a barrier a stage but halves the workgroups per CU (5-9 % slower)
-  auto stages = [&](int s, int end) {
-    for (; s < end; ++s) {
-      const int left = elements(s);
-      a.store(as, left, tid);
-      b.store(bs, left, tid);
-      __syncthreads();
-      if (s + 1 < nk) load(s + 1);
-      float fa[16], fb[16];
-      fragment<ACOLS>(as, wm * 32, lane, fa);
-      fragment<BCOLS>(bs, wn * 32, lane, fb);
+  for (int s = 0; s < nk; ++s) {
+    const int left = elements(s);
+    a.store(as, left, tid);
+    b.store(bs, left, tid);
+    __syncthreads();
+    if (s + 1 < nk) load(s + 1);
+    float fa[16], fb[16];
+    fragment<ACOLS>(as, wm * 32, lane, fa);
+    fragment<BCOLS>(bs, wn * 32, lane, fb);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (BF16 && 8 * q >= left) continue;
+    for (int q = 0; q < 4; ++q) {
+      if (BF16 && 8 * q >= left) continue;
 #pragma unroll
-        for (int m = 4 * q; m < 4 * q + 4; ++m) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[m], fb[m], acc, 0, 0, 0);
-      }
-      __syncthreads();
+      for (int m = 4 * q; m < 4 * q + 4; ++m) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[m], fb[m], acc, 0, 0, 0);
     }
-  };
-  if constexpr (PART == 0) {
-    stages(0, nk);
-  } else {
-    f32x16 sum = acc;
-    for (int s = 0; s < nk; s += PART) {
-      stages(s, min(s + PART, nk));
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        sum[v] += acc[v];
-        acc[v] = 0.0f;
-      }
-    }
-    acc = sum;
+    __syncthreads();
   }
 }
 

@@ -22,7 +22,7 @@ __device__ __forceinline__ void to_rows(const f32mm::f32x16& acc, float* lds, fl
   for (int e = 0; e < 16; ++e) v[e] = row[e];
 }
 
-// PART: of mainloop
+// PART > 0: every PART stages of the reduction make a sum of their own.
 template <bool VD, bool DZ, int VEC, int PART>
 __global__ __launch_bounds__(NT) void logits_f32_kernel(Logits p) {
   __shared__ __attribute__((aligned(16))) float lds[2 * f32mm::TILE];
@@ -38,7 +38,21 @@ __global__ __launch_bounds__(NT) void logits_f32_kernel(Logits p) {
     return n < p.cols && k < p.red ? W + (VD ? (int64_t)n * p.ldw + k : (int64_t)k * p.ldw + n) : nullptr;
   };
   f32mm::f32x16 acc;
-  f32mm::mainloop<float, false, !VD, VEC, PART>(acc, p.red, lds, lds + f32mm::TILE, at_x, at_w, X, W);
+  if constexpr (PART == 0) {
+    f32mm::mainloop<float, false, !VD, VEC>(acc, p.red, lds, lds + f32mm::TILE, at_x, at_w, X, W);
+  } else {
+    f32mm::f32x16 sum;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
+    for (int s0 = 0; s0 * KS < p.red; s0 += PART) {
+      f32mm::mainloop<float, false, !VD, VEC>(
+          acc, min(PART * KS, p.red - s0 * KS), lds, lds + f32mm::TILE, [&](int r, int c, int s) { return at_x(r, c, s0 + s); },
+          [&](int r, int c, int s) { return at_w(r, c, s0 + s); }, X, W);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum[e] += acc[e];
+    }
+    acc = sum;
+  }
   float v[16];
   to_rows(acc, lds, v);
   const int row = m0 + (threadIdx.x >> 2), quarter = threadIdx.x & 3, c0 = n0 + quarter * 16, left = p.cols - c0;
@@ -128,8 +142,8 @@ static int go_logits(const Logits& p, hipStream_t st) {
   // a whole row of four is inside or outside: of the reduction in x (and W [V][D]), of the columns in W [D][V]
   const bool vec = quads(p.x, p.ldx) && quads(p.w, p.ldw) && p.red % 4 == 0 && (VD || p.cols % 4 == 0);
   // Few rows' gradients are as far off as their few large logits, 7e-6 for 4 x 1324 x 10624 in one run of sums and 0.7e-6 this
-  // way.  Over many rows it evens out: 100 x 1000 x 3000 1.3e-6 and 0.5e-6; the logits' products take 6 % longer for it (forward
-  // and backward of 1009 x 1000 x 5003 240 and 255 us).
+  // way.  Over many rows it evens out: 100 x 1000 x 3000 1.3e-6 and 0.5e-6.  64 x 2048 x 32000 takes 385 us in both directions
+  // in one run of sums, 401 this way.
   const bool parts = p.T <= kTwoRows;
   if (vec && parts) hipLaunchKernelGGL((logits_f32_kernel<VD, DZ, 4, 4>), grid, dim3(NT), 0, st, p);
   else if (vec) hipLaunchKernelGGL((logits_f32_kernel<VD, DZ, 4, 0>), grid, dim3(NT), 0, st, p);
