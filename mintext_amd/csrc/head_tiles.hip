@@ -25,6 +25,10 @@ __device__ __forceinline__ float* in_lds(char* mine, int r, int c) {
   return (float*)(mine + r * (T::TN * 128) + (((c >> 2) ^ (r & (T::TN * 8 - 1))) << 4) + (c & 3) * 4);
 }
 
+// exp((z - m) / tau).  The difference first: of z scale - m scale, whose second product is rounded, all terms of a row are off by a
+// common factor, by 4e-5 where m / tau is 1000, and the largest logit's own term is not 1.
+__device__ __forceinline__ float exp_of(float z, float m, float scale) { return __builtin_amdgcn_exp2f((z - m) * scale); }
+
 // A lane holds, of 32 rows at a time, one row's 16 TN values in columns 32 j + 8 g + 4 (lane / 32) + q (accumulator j, element
 // 4 g + q): the row's maximum and sum are taken in the lane and joined with that of lane ^ 32.  Entries are looked up in LDS,
 // where the 32 rows are put for that only if one of them has an entry among the wave's columns.
@@ -68,12 +72,12 @@ __device__ __forceinline__ void forward_out(const Logits& p, dense::f32x16 (&acc
 #pragma unroll
       for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[i][j][v]);
     m = fmaxf(m, lane_xchg<5>(m));
-    const float off = m == -INFINITY ? 0.0f : -m * p.scale;  // nothing but -inf: a sum of 0
+    const float off = m == -INFINITY ? 0.0f : m;  // nothing but -inf: a sum of 0
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) s[v & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], p.scale, off));
+      for (int v = 0; v < 16; ++v) s[v & 3] += exp_of(acc[i][j][v], off, p.scale);
     float sum = (s[0] + s[1]) + (s[2] + s[3]);
     sum += lane_xchg<5>(sum);
     if (row < p.T && half == 0) p.part[(int64_t)((p.v0 + c0) / BC) * p.T + row] = make_float2(m, sum);
@@ -105,13 +109,12 @@ __device__ __forceinline__ void gradient_out(const Logits& p, dense::f32x16 (&ac
   constexpr int BC = T::TN * 32, CH = T::TN * 4, BYTES = 32 * T::TN * 64;  // chunks of a row; bytes of 32 rows
   typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
   const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31, left = p.cols - c0;
-  float a[T::TM], off[T::TM];
+  float a[T::TM], m[T::TM];
   bool care = left < BC;
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
     const int row = min(wr + i * 32 + r, p.T - 1);
-    a[i] = p.f.a(row, p.f.b(row), off[i]);
-    off[i] *= -p.scale;
+    a[i] = p.f.a(row, p.f.b(row), m[i]);
   }
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) care |= a[i] == 0.0f;
@@ -126,7 +129,7 @@ __device__ __forceinline__ void gradient_out(const Logits& p, dense::f32x16 (&ac
         float d[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          d[q] = a[i] * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][4 * g + q], p.scale, off[i]));
+          d[q] = a[i] * exp_of(acc[i][j][4 * g + q], m[i], p.scale);
         if (care) {  // zeros behind the columns, and in rows that are left out, whatever their logits are
 #pragma unroll
           for (int q = 0; q < 4; ++q)
