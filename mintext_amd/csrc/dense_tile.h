@@ -51,8 +51,8 @@ constexpr int BKS = 32;  // reduction elements per ring stage
 
 // One operand of a tile: `p[0]` at the tile's first row (or column) of reduction element 0, uniform; `p[1]` the lo
 // plane of it; `ld` its row stride in elements; `left` the rows (rows) or columns (cols) from there that exist.
-// `missing` (cols, TAIL, below 8): lines at the reduction's end that this operand does not have, for which it re-reads its
-// last one; the other operand holds zeros there.
+// `missing` (cols, TAIL, below 8): lines at the reduction's end that this operand does not have and that the product leaves out;
+// what the other operand has there can be read.
 struct Operand {
   const void* p[2];
   int64_t ld;
@@ -135,6 +135,7 @@ struct Tile {
     const int wm = wave / WN, wn = wave % WN;
     const int nk1 = (K + BKS - 1) / BKS, nk = TWO ? 3 * nk1 : nk1;
     const int tail = K - (nk1 - 1) * BKS, a_tail = tail - (A_COLS ? a.missing : 0), b_tail = tail - (B_COLS ? b.missing : 0);
+    const int both_tail = min(a_tail, b_tail);  // what lies behind it is masked: a last line read again, times 0, may be no number
     uint32_t aoff[A_INSTR], boff[B_INSTR], atail[TAIL ? A_INSTR : 1], btail[TAIL ? B_INSTR : 1];
 #pragma unroll
     for (int i = 0; i < A_INSTR; ++i) {
@@ -213,7 +214,7 @@ struct Tile {
                                    wn * (TN * 32) + (r - TM) * 32, kk);
     };
     auto mask = [&](int buf, int kk) {
-      const int nv = min(max(tail - kk * 16 - 8 * fhalf, 0), 8);
+      const int nv = min(max(both_tail - kk * 16 - 8 * fhalf, 0), 8);
       u32x4 m;
 #pragma unroll
       for (int d = 0; d < 4; ++d) m[d] = (2 * d + 1 < nv) ? 0xFFFFFFFFu : ((2 * d < nv) ? 0xFFFFu : 0u);
@@ -323,7 +324,7 @@ struct Tile {
     constexpr int S = TM * TN;
     auto half = [&](auto which, int kt) {
       constexpr int sub = decltype(which)::value;
-      if (TAIL && kt == nk - 1 && tail < BKS) mask(sub, sub);
+      if (TAIL && kt == nk - 1 && both_tail < BKS) mask(sub, sub);
 #pragma unroll
       for (int qq = 0; qq < S; ++qq) {
         const int i = qq / TN, j = qq % TN;

@@ -87,3 +87,40 @@ def test_logits_far_from_zero(dev, T, V, dtype, order, kind):
     dx, dw = torch.mm(dz, W.t()), torch.mm(X.t(), dz)
     close(gx, dx, u * dx.abs() + torch.mm(er + (V + 8) * V_ * dz.abs(), W.abs().t().contiguous()) + LEAST * (V + 1), "dx")
     close(gw, dw, u * dw.abs() + torch.mm(X.abs().t().contiguous(), er + (2 * T + 8) * V_ * dz.abs()) + LEAST * (T + 1), "dw")
+
+
+@pytest.mark.parametrize("order", ["dv", "vd"])
+@pytest.mark.parametrize("T,D,V", [(20, 33, 301), (20, 31, 304), (64, 1, 300), (130, 39, 301), (300, 65, 512), (2048, 97, 6401)])
+def test_weight_of_minus_infinity_takes_a_class_out(dev, T, D, V, order):
+    """A weight of -inf in the last row, where the row's x are positive: the class's logit is -inf, its probability 0.  The losses and
+    the gradients are those without it, but for that row's share of dx, 0 times -inf.  Widths end a stage or 1 to 7 before an
+    eight; the bounds are the logits' (D + 2) v |x| |W|, twice, with those at the file's head for logits of 16 at most."""
+    from mintext_amd.kernels import linear_cross_entropy
+
+    gen = torch.Generator(device=dev).manual_seed(T + D)
+    x = torch.randn(T, D, device=dev, generator=gen)
+    x[:, -1] = x[:, -1].abs() + 0.5
+    x = x.to(BF)
+    w = (torch.randn(D, V, device=dev, generator=gen) * D ** -0.5).to(BF)
+    w[-1, 0] = -float("inf")
+    w = w.t().contiguous().t() if order == "vd" else w
+    y = torch.randint(1, V, (T,), device=dev, generator=gen)
+    X, W = x.double(), w[:, 1:].double()
+    z = torch.mm(X, W)
+    assert z.abs().max() <= 16
+    ez = (D + 2) * V_ * torch.mm(X.abs(), W.abs())
+    lse = torch.logsumexp(z, 1)
+    want = lse - z.gather(1, y[:, None] - 1)[:, 0]
+    el = ez.amax(1) + V_ * (16 * 33 + V / 64 + 64)
+    loss = linear_cross_entropy(x.requires_grad_(True), w.requires_grad_(True), y, reduction="none")
+    close(loss.detach(), want, 2 * el + 8 * V_ * (16 + want), "loss")
+    gx, gw = torch.autograd.grad(loss, [x, w], torch.ones(T, device=dev))
+    q = torch.softmax(z, 1)
+    dz = q.scatter_add(1, y[:, None] - 1, -torch.ones(T, 1, device=dev).double())
+    u = 2.0 ** -8
+    er = q * (ez + el[:, None] + 16 * V_ * 33) + 32 * V_ + (u + 4 * V_) * dz.abs()
+    dx, dw = torch.mm(dz, W.t()), torch.mm(X.t(), dz)
+    tx = u * dx.abs() + torch.mm(er + (V + 8) * V_ * dz.abs(), W.abs().t().contiguous())
+    close(gx[:, :-1], dx[:, :-1], tx[:, :-1], "dx")
+    close(gw[:, 1:], dw, u * dw.abs() + torch.mm(X.abs().t().contiguous(), er + (2 * T + 8) * V_ * dz.abs()), "dw")
+    assert not gw[:, 0].any()
