@@ -128,9 +128,8 @@ int launch_logits_f32(const Logits& p, bool dz, int order, hipStream_t st);
 int launch_product_f32(const Product& p, bool a_cols, bool b_cols, hipStream_t st);
 
 enum { SIZE_BIG, SIZE_SMALL };  // tiles of launch_product: 256 x 256, 128 x 128
-// tiles of the logits: 256 x 256, 128 x 128, 64 x 128 (few rows); f32 64 x 64
+// tiles of the logits: 256 x 256, 128 x 128, 64 x 128 (up to kTwoRows, the ones that write two planes of dz); f32 64 x 64
 enum { PATH_BIG, PATH_SMALL, PATH_THIN, PATH_F32 };
-inline int tile_rows(int path) { return path == PATH_BIG ? 256 : path == PATH_SMALL ? 128 : 64; }
 inline int tile_cols(int path) { return path == PATH_BIG ? 256 : path == PATH_F32 ? 64 : 128; }
 inline int block_cols(int path) { return path == PATH_BIG ? 128 : 64; }  // of a partial maximum and sum
 

@@ -436,7 +436,7 @@ static Plan plan(int dtype, int64_t T, int64_t D, int64_t V, int order, bool bac
   // Forward in 256 x 256, 128 x 128 and 64 x 128 tiles (us): 48 x 2048 x 32000 54.3, 31.2, 30.2; 65 rows 52.9, 31.2, 37.6; 256 rows
   // 54.1, 47.2, 58.2; 512 x 2048 x 16384 (128 large tiles) 51.5, 44.4, 53.3; 1024 x 2048 x 12288 (192) 57.3, 62.6; 1024 x 2048 x
   // 32000 (500) 120, 147.  Both directions of 128 x 4096 x 131072 take 1242 with large tiles, 1199 with small ones.
-  p.path = p.f32 ? PATH_F32 : T <= 64 ? PATH_THIN : big >= 192 && T > 128 ? PATH_BIG : PATH_SMALL;
+  p.path = p.f32 ? PATH_F32 : T <= kTwoRows ? PATH_THIN : big >= 192 && T > 128 ? PATH_BIG : PATH_SMALL;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;

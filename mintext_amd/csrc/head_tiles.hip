@@ -266,27 +266,20 @@ __global__ __launch_bounds__(T::NT, T::LDS_BYTES > 80 * 1024 ? 1 : 2) void produ
   }
 }
 
-template <class T, bool TWO>
+// PLANES: that a tile writes of dz
+template <class T, int PLANES>
 static int go_logits(const Logits& p, bool dz, hipStream_t st) {
+  if (dz && p.planes != PLANES) return MTX_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)dense::tiles_grid(ceil_div(p.T, T::BM) * ceil_div(p.cols, T::BN)));
-  if (!dz) {
-    hipLaunchKernelGGL((logits_kernel<T, 0>), grid, dim3(T::NT), 0, st, p);
-    return check_launch();
-  }
-  if constexpr (TWO) {
-    if (p.planes == 2) {
-      hipLaunchKernelGGL((logits_kernel<T, 2>), grid, dim3(T::NT), 0, st, p);
-      return check_launch();
-    }
-  }
-  hipLaunchKernelGGL((logits_kernel<T, 1>), grid, dim3(T::NT), 0, st, p);
+  if (dz) hipLaunchKernelGGL((logits_kernel<T, PLANES>), grid, dim3(T::NT), 0, st, p);
+  else hipLaunchKernelGGL((logits_kernel<T, 0>), grid, dim3(T::NT), 0, st, p);
   return check_launch();
 }
 template <bool VD, bool TAIL>
 static int go_path(const Logits& p, bool dz, int path, hipStream_t st) {
-  if (path == PATH_BIG) return go_logits<Big<VD, TAIL>, false>(p, dz, st);
-  if (path == PATH_SMALL) return go_logits<Small<VD, TAIL>, false>(p, dz, st);
-  return go_logits<Thin<VD, TAIL>, true>(p, dz, st);
+  if (path == PATH_BIG) return go_logits<Big<VD, TAIL>, 1>(p, dz, st);
+  if (path == PATH_SMALL) return go_logits<Small<VD, TAIL>, 1>(p, dz, st);
+  return go_logits<Thin<VD, TAIL>, 2>(p, dz, st);
 }
 int launch_logits(const Logits& p, bool dz, int order, int path, hipStream_t st) {
   const bool tail = p.red % dense::BKS != 0 || p.missing > 0;
