@@ -457,8 +457,9 @@ int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre
  *   sum of the losses and, with `mean`, what it was divided by: the rows that are not left out, 1 at least.
  * The _bwd calls: g is the gradient of total (count as written) or, with count NULL, of loss[T]; dx[T,D] and dw (W's
  *   order) in dtype and 16-byte aligned, either may be NULL.  dz is rounded to dtype for the products (up to 64 rows
- *   in two planes, with what the rounding took); its columns go through in pieces of 1 GiB at most, over which dx is
- *   summed in float32.  No two calls that can run at the same time may share a workspace. */
+ *   in two planes, with what the rounding took); its columns go through in pieces of 1 GiB at most (320 columns
+ *   of T rows where that is more), over which dx is summed in float32.  No two calls that can run at the same time
+ *   may share a workspace. */
 #define MTX_HEAD_DV 0  /* W[D,V] */
 #define MTX_HEAD_VD 1  /* W[V,D] */
 int64_t mtx_head_loss_workspace_size(int dtype, int64_t T, int64_t D, int64_t V, int order, int backward);

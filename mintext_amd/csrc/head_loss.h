@@ -8,7 +8,8 @@
 //             dx += dz W^T (in f32) and dW of the piece = x^T dz.  A factor that all rows share (1 / count, the gradient of
 //             the one loss) is left to the products' results: with it in dz, every row's -1 + q is rounded alike where q is
 //             small, and the gradients of 4096 x 4096 x 32000 were 2.8e-3 off instead of 2.0e-3.
-// So a step computes 8 T D V operations, 2 of them for the logits made again, and holds kPiece bytes of dz at most.
+// So a step computes 8 T D V operations, 2 of them for the logits made again, and holds kPiece bytes of dz at most, or 320 columns
+// of it where T is so large that those are more.
 #pragma once
 #include "common.h"
 

@@ -362,8 +362,8 @@ __global__ __launch_bounds__(64) void join_kernel(const float* __restrict__ acc,
 }
 
 // ---- how a call runs, by its sizes alone --------------------------------------------------------------------------
-constexpr int64_t kPiece = (int64_t)1 << 30;  // bytes of dz held at a time, at most
-constexpr int64_t kCopy = (int64_t)256 << 20;  // bytes of a padded copy of the weight's columns held at a time, at most
+// Bytes of dz held at a time, at most (or those of 256 columns and kTurn), and of a padded copy of the weight's columns (or of 256).
+constexpr int64_t kPiece = (int64_t)1 << 30, kCopy = (int64_t)256 << 20;
 constexpr int kTurn = 64;  // elements more than a piece in a row of dz, so that rows are no power of two apart in memory
 constexpr int kMostPieces = 16;
 

@@ -4,10 +4,10 @@
 ``linear_distillation`` is the same against a teacher's top logits.  Both take the head's input and its weight: one kernel
 makes the logits tile by tile on the matrix cores and leaves each tile's maxima, sums and the logits that the loss
 names; the [T, V] logits are not stored, in neither direction.  The backward makes them again in pieces of the
-vocabulary whose gradient takes 1 GiB at most, and runs the two products of each piece; over the pieces the gradient of
-``x`` is summed in float32.  The gradient of the logits is rounded to the operands' type for the products (bfloat16:
-as in ``linear``'s backward, the results end 2.4e-3 off where their own rounding is 1.7e-3; up to 64 tokens keep what that
-rounding took as well, and end at their own).  Every sum has a fixed order.
+vocabulary whose gradient takes 1 GiB at most (or 320 columns of it, where the tokens are so many that those take more), and runs
+the two products of each piece; over the pieces the gradient of ``x`` is summed in float32.  The gradient of the logits is rounded
+to the operands' type for the products (bfloat16: as in ``linear``'s backward, the results end 2.4e-3 off where their own rounding
+is 1.7e-3; up to 64 tokens keep what that rounding took as well, and end at their own).  Every sum has a fixed order.
 
 The weight is [D, V] as it lies in memory, or an embedding table [V, D] passed as ``table.t()``: both are read in place, and
 the weight's gradient has the weight's strides.  In bfloat16 a vocabulary (or, for a table, a width) that is no multiple of 8
