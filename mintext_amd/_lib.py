@@ -229,6 +229,18 @@ def plain_forward(*tensors) -> bool:
     return getattr(torch.autograd.forward_ad, "_current_level", 0) < 0 and _functorch_level() is None
 
 
+def once_differentiable(backward):
+    """torch's decorator of that name, in whose place the function itself runs where no second derivative is asked for: its
+    switch of the grad mode is 1.5 to 3 us of the 55 to 110 that a small norm with its gradients takes."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
 def refuse_watched(name: str, *tensors) -> None:
     """Raise for an op without an autograd Function where something would have to see it: a jit trace, which
     records none of the kernels it launches, or a forward-mode tangent, which its result would not have."""

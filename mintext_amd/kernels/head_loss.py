@@ -18,7 +18,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib as L
 
@@ -141,7 +140,7 @@ class _HeadLoss(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @L.once_differentiable
     def backward(ctx, g):
         need_x, need_w = ctx.needs_input_grad[:2]
         return (*ctx.how.backward(g, *ctx.saved_tensors, ctx.K, need_x, need_w), None, None, None)

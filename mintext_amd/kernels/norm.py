@@ -8,7 +8,6 @@ gradients and a sum of its workgroups' shares of the weight's and bias's gradien
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib as L
 
@@ -38,12 +37,13 @@ def _check(name, x, weight, bias, residual, eps):
 
 
 def _forward(x, residual, weight, bias, rms, eps, keep):
+    """y, h, what the backward needs of each row (1 / sqrt(variance + eps), behind it the means), and its sizes and type codes."""
     dev = L.require_device(x, residual, weight, bias)
-    D = x.shape[-1]
-    T = x.numel() // D
+    D = int(x.shape[-1])  # numbers, also where a jit trace has sizes of its own: it calls the Function again for other tensors
+    T = int(x.numel() // D)
     x, weight = x.contiguous(), weight.contiguous()
     y = torch.empty_like(x)
-    r = b = h = m = s = mean = rstd = None  # the letters: addresses
+    r = b = h = m = s = stats = None  # the letters: addresses
     if residual is not None:
         residual = residual.contiguous()
         hidden = torch.empty_like(x)
@@ -54,41 +54,39 @@ def _forward(x, residual, weight, bias, rms, eps, keep):
         bias = bias.contiguous()
         b = bias.data_ptr()
     if keep:
-        rstd = torch.empty(T, dtype=torch.float32, device=dev)
-        s = rstd.data_ptr()
+        stats = torch.empty(T if rms else 2 * T, dtype=torch.float32, device=dev)
+        s = stats.data_ptr()
         if not rms:
-            mean = torch.empty(T, dtype=torch.float32, device=dev)
-            m = mean.data_ptr()
+            m = s + 4 * T
+    how = (L.dtype_code(x.dtype), L.dtype_code(weight.dtype), rms, T, D)
     with L.on_device(dev):
-        L.call("mtx_norm", x.data_ptr(), r, weight.data_ptr(), b, L.dtype_code(x.dtype), L.dtype_code(weight.dtype), rms, T, D,
-               eps, y.data_ptr(), h, m, s, L.stream(dev))
-    return y, hidden, mean, rstd
+        L.call("mtx_norm", x.data_ptr(), r, weight.data_ptr(), b, *how, eps, y.data_ptr(), h, m, s, L.stream(dev))
+    return y, hidden, stats, how
 
 
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, rms, eps):
-        y, h, mean, rstd = _forward(x, residual, weight, bias, rms, eps, True)
-        ctx.save_for_backward(h, weight, mean, rstd)
-        ctx.rms = rms
+        y, h, stats, how = _forward(x, residual, weight, bias, rms, eps, True)
+        ctx.save_for_backward(h, weight, stats)
+        # worked out here: the backward runs in a thread of its own, where each step may cost two to three times as much
+        ctx.how = how, L.query("mtx_norm_bwd_workspace_size", *how[3:])
         ctx.set_materialize_grads(False)
         return (y, h) if residual is not None else y
 
     @staticmethod
-    @once_differentiable
+    @L.once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, mean, rstd = ctx.saved_tensors
+        h, weight, stats = ctx.saved_tensors
         need_x, need_r, need_w, need_b, _, _ = ctx.needs_input_grad
         if dy is None:  # the sum alone is used
             return (dh if need_x else None, dh if need_r else None, None, None, None, None)
-        rms = ctx.rms
-        dev = L.require_device(dy, dh, h, weight)
+        how, nbytes = ctx.how
+        rms, T = how[2:4]
+        dev = L.require_device(dy, dh, h)
         dy, weight = dy.contiguous(), weight.contiguous()
-        D = h.shape[-1]
-        T = h.numel() // D
         dx = dw = db = None
         dhp = dxp = dwp = dbp = wsp = None
-        nbytes = 0
         if dh is not None:
             dh = dh.contiguous()
             dhp = dh.data_ptr()
@@ -97,14 +95,15 @@ class _Norm(torch.autograd.Function):
             dxp = dx.data_ptr()
         if need_w or need_b:
             dw = torch.empty_like(weight)
-            ws = L.workspace(L.query("mtx_norm_bwd_workspace_size", T, D), dev)
-            dwp, wsp, nbytes = dw.data_ptr(), ws.data_ptr(), ws.numel()
+            ws = L.workspace(nbytes, dev)
+            dwp, wsp = dw.data_ptr(), ws.data_ptr()
         if need_b:
             db = torch.empty_like(weight)
             dbp = db.data_ptr()
+        rstd = stats.data_ptr()
         with L.on_device(dev):
-            L.call("mtx_norm_bwd", dy.data_ptr(), dhp, h.data_ptr(), weight.data_ptr(), L.ptr(mean), rstd.data_ptr(),
-                   L.dtype_code(h.dtype), L.dtype_code(weight.dtype), rms, T, D, dxp, dwp, dbp, wsp, nbytes, L.stream(dev))
+            L.call("mtx_norm_bwd", dy.data_ptr(), dhp, h.data_ptr(), weight.data_ptr(), None if rms else rstd + 4 * T, rstd, *how,
+                   dxp, dwp, dbp, wsp, nbytes, L.stream(dev))
         return dx if need_x else None, dx if need_r else None, dw if need_w else None, db, None, None
 
 
