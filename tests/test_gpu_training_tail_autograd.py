@@ -1,5 +1,5 @@
-"""What autograd and traces see of the norms and the head's losses: second derivatives are refused, and a trace holds for other
-numbers of tokens."""
+"""What autograd, its transforms and traces see of the norms and the head's losses: second derivatives, vmap, torch.func.grad and
+forward-mode tangents are refused, and a trace holds for other numbers of tokens."""
 from __future__ import annotations
 
 import pytest
@@ -37,6 +37,21 @@ def test_second_derivative_is_refused(dev, op):
     assert torch.equal(plain, g)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), [x])
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_transforms_are_refused(dev, op):
+    f, x = build(dev, op)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: f(a).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(f)(x)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(f, (x,), (torch.ones_like(x),))
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises(RuntimeError):
+        f(fwd.make_dual(x, torch.ones_like(x)))
+    assert torch.isfinite(f(x)).all()  # and leave the operator as it was
 
 
 @pytest.mark.parametrize("op", ["layer_norm", "layer_norm_residual", "rms_norm"])
