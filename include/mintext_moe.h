@@ -450,7 +450,8 @@ int mtx_linear_bwd(const void* dy, const void* x, const void* w, const void* pre
  * mtx_linear_distillation: p = softmax(teacher_logits[t] / temperature) over the entries of a row (K of
  *   them, K <= 1024) whose index is not negative and whose logit is not -inf; lse[t] = log sum exp(z[t] / temperature);
  *   loss[t] = temperature^2 sum_k p_k (log p_k - z[t, i_k] / temperature + lse[t]).  A row without such an entry has loss
- *   0 and no gradient, one with an index of V or more, or a NaN, has NaN; an index that is there twice is two entries.
+ *   0 and no gradient, one with an index of V or more, or an entry of NaN or +inf, has NaN; an index that is there
+ *   twice is two entries.
  *   entries (mtx_distillation_entries_size bytes, 16-byte aligned) is filled for the backward call.
  * Both write loss, stats[T][2] (the largest logit m and sum exp((z - m) / temperature)), state[T] (1, 0 for rows
  *   left out, NaN) and chosen[T] (distillation: [T,K]), the named logits.  total and count (both or none) receive the

@@ -60,8 +60,8 @@ __global__ __launch_bounds__(64) void entries_kernel(Prep p) {
   for (int k = lane; k < p.K; k += 64) {
     const int64_t i = p.wide ? ((const int64_t*)p.idx)[base + k] : ((const int32_t*)p.idx)[base + k];
     const float t = p.f32 ? ((const float*)p.logits)[base + k] : bf16_to_f32(((const uint16_t*)p.logits)[base + k]);
-    const bool live = i >= 0 && !(t == -INFINITY);  // NaN counts, and makes the row's shares NaN
-    bad |= i >= p.V || (live && t != t);
+    const bool live = i >= 0 && !(t == -INFINITY);  // NaN and +inf count, and leave the row no shares
+    bad |= i >= p.V || (live && !(t < INFINITY));
     key[k] = (live && i < p.V ? (uint32_t)i : kNoClass) << 10 | (uint32_t)k;
     val[k] = t;
     if (live) m = fmaxf(m, t);

@@ -191,7 +191,7 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_indices: 
             negative ones are empty places.  A class that is there twice is two entries of the sum; one of V or more
             makes its token's loss and gradient NaN.
         teacher_logits: [..., K] float32 or bfloat16; p is their softmax over the token's entries (those of -inf left
-            out).  The teacher gets no gradient.
+            out; one of +inf or NaN makes the token's loss and gradient NaN).  The teacher gets no gradient.
         temperature: of both distributions.
         reduction: "mean" over the tokens that have an entry (0 if none has), "sum", or "none".
 

@@ -124,3 +124,29 @@ def test_weight_of_minus_infinity_takes_a_class_out(dev, T, D, V, order):
     close(gx[:, :-1], dx[:, :-1], tx[:, :-1], "dx")
     close(gw[:, 1:], dw, u * dw.abs() + torch.mm(X.abs().t().contiguous(), er + (2 * T + 8) * V_ * dz.abs()), "dw")
     assert not gw[:, 0].any()
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("T", [5, 70])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_teacher_logit_without_a_softmax(dev, dtype, T, value):
+    """An entry of +inf leaves a token no softmax, as one of NaN does: its loss and its whole gradient are NaN, the weight's too,
+    and no other token's.  In an empty place it is not looked at."""
+    from mintext_amd.kernels import linear_distillation
+
+    gen = torch.Generator(device=dev).manual_seed(T)
+    x = torch.randn(T, 40, device=dev, generator=gen).to(dtype).requires_grad_(True)
+    w = (torch.randn(40, 300, device=dev, generator=gen) * 0.1).to(dtype).requires_grad_(True)
+    idx = torch.randint(0, 300, (T, 3), device=dev, generator=gen)
+    idx[1, 2] = -1
+    t = torch.randn(T, 3, device=dev, generator=gen)
+    clean = linear_distillation(x, w, idx, t, reduction="none")
+    (cx,) = torch.autograd.grad(clean.sum(), [x])
+    t[1, 2] = value
+    assert torch.equal(linear_distillation(x, w, idx, t, reduction="none"), clean)
+    t[2, 0] = value
+    loss = linear_distillation(x, w, idx, t, reduction="none")
+    gx, gw = torch.autograd.grad(loss.sum(), [x, w])
+    keep = torch.arange(T, device=dev) != 2
+    assert torch.isnan(loss[2]) and torch.isnan(gx[2]).all() and torch.isnan(gw).all()
+    assert torch.equal(loss[keep], clean[keep]) and torch.equal(gx[keep], cx[keep])
