@@ -29,6 +29,8 @@ __device__ __forceinline__ float* in_lds(char* mine, int r, int c) {
 // common factor, by 4e-5 where m / tau is 1000, and the largest logit's own term is not 1.
 __device__ __forceinline__ float exp_of(float z, float m, float scale) { return __builtin_amdgcn_exp2f((z - m) * scale); }
 
+// The 256 x 256 tiles' way out of the forward pass spills 23 VGPRs, each written once and read once or twice; their product's
+// loop has no spill.
 // A lane holds, of 32 rows at a time, one row's 16 TN values in columns 32 j + 8 g + 4 (lane / 32) + q (accumulator j, element
 // 4 g + q): the row's maximum and sum are taken in the lane and joined with that of lane ^ 32.  Entries are looked up in LDS,
 // where the 32 rows are put for that only if one of them has an entry among the wave's columns.

@@ -12,6 +12,10 @@ is 1.7e-3; up to 64 tokens keep what that rounding took as well, and end at thei
 The weight is [D, V] as it lies in memory, or an embedding table [V, D] passed as ``table.t()``: both are read in place, and
 the weight's gradient has the weight's strides.  In bfloat16 a vocabulary (or, for a table, a width) that is no multiple of 8
 costs a padded copy of the weight, piece by piece, in each direction.
+
+In float32 a loss with its gradients takes 1.4 to 1.7 times as long as with the logits in memory where both the tokens (more than 64)
+and the vocabulary are many: four products in tiles that reach half to three quarters of a library's rate, for three.  What it
+saves there is memory.
 """
 from __future__ import annotations
 
